@@ -526,6 +526,85 @@ int mimg_attention_dev(const float *q, const void *kcache, const void *vcache, c
                        const int64_t *kstart, int64_t T, int heads, int kv_heads, int d, int64_t context,
                        int64_t max_keys, int f16, float *out, void *ws, uint64_t ws_bytes, void *stream);
 
+/* ---- the 8-bit key-value cache -------------------------------------------
+ * A cache of half the bytes of an f16 one: int8 values, with one float32
+ * scale for each block of 32 entries and kv head, for keys and for values. One
+ * buffer of mimg_cache_q8_bytes holds the keys and values of a layer; it must
+ * be zeroed before its first use. No reference counterpart (its caches are f32
+ * or f16, importer/llama.go:489-503).
+ *
+ * Layout, with DP = d rounded up to a multiple of 64 and NB =
+ * ceil(context/32): [kv_heads][NB] records of 64*DP bytes, then
+ * [kv_heads][NB] of {float key scale, float value scale, uint32 entries that
+ * are not finite, uint32 0}. Value = (byte - 128) * scale. In a record, of
+ * entry e (0..31) and dim i:
+ *   key   byte (((e/16)*(DP/64) + i/64)*64 + (i/16%4)*16 + e%16)*16 + i%16
+ *   value byte 32*DP + ((i/32)*64 + (e/4%4)*16 + i%16)*16 + (i/16%2)*8 +
+ *         (e/16)*4 + e%4
+ * (operands of the matrix cores in lane order). Dims past d hold 128 or 0. */
+
+/* Bytes of such a cache; 0 for shapes that have none: kv_heads 1..16384,
+ * context 1..2^30, d a multiple of 8 up to 256. */
+uint64_t mimg_cache_q8_bytes(int kv_heads, int64_t context, int d);
+
+/* k, v [T, kv_heads, d] into the cache entries cache_index[t] (T <= 65535). For
+ * each block and kv head that the rows touch: scale = max(old scale, largest
+ * |value| of the new rows / 127, rounded to float32 and at least 2^-96 unless
+ * all are zero), entries rint(x / scale), ties to even; where the scale grew, the
+ * block's other entries are requantized to it. A store that includes a block's
+ * first entry begins the block anew: old scale 0, its other entries zeros. So
+ * sequences start at multiples of 32 and append in order; a store into the
+ * middle of a block keeps the others. Rows whose index is outside
+ * 0..context-1 are not stored; of two rows with one index the later is. A row
+ * with a value that is not finite in a kv head marks the entry: its values
+ * that are not finite count as zeros in the scale, and what sees the entry
+ * there gets NaN. */
+int mimg_kv_store_q8_dev(const float *k, const float *v, const int64_t *cache_index, int64_t T, int kv_heads, int d,
+                         int64_t context, void *cache, void *stream);
+
+/* mimg_rope_dev on q [T, heads, d] (in place) and k, and mimg_kv_store_q8_dev of
+ * the rotated k and of v, in one launch, bit for bit those calls; k is left as
+ * it was (the form of mimg_rope_kv_dev for this cache). */
+int mimg_rope_kv_q8_dev(float *q, const float *k, const float *v, const int64_t *pos, const int64_t *cache_index,
+                        const double *inv_freq, int64_t T, int heads, int kv_heads, int d, int rotary, int interleaved,
+                        int64_t context, void *cache, void *stream);
+
+/* The cache entries cache_index[t] as float32 k, v [T, kv_heads, d]; zeros for
+ * an index outside 0..context-1, NaN for an entry that is marked not finite. */
+int mimg_kv_load_q8_dev(const void *cache, const int64_t *cache_index, int64_t T, int kv_heads, int d, int64_t context,
+                        float *k, float *v, void *stream);
+
+/* mimg_attention_dev over an 8-bit cache: query t of head h sees the entries
+ * kstart[t]..kend[t] (kstart may be NULL for 0) of kv head h / (heads /
+ * kv_heads), clipped to the cache and to the first max_keys (1..2^30: no limit
+ * of 8192 here); scale 1/sqrt(d); q, out [T, heads, d], out not overlapping q.
+ * Float32 accuracy (products of 22-bit parts summed in float32; the softmax in
+ * one pass), not the reference's float order. A query that sees nothing gets
+ * zeros; one that sees an entry marked not finite, or is not finite itself, or
+ * whose largest score is not finite, NaN. ws: device scratch of
+ * mimg_attention_q8_workspace_bytes (which may be 0, then ws may be NULL),
+ * 16-byte aligned. */
+uint64_t mimg_attention_q8_workspace_bytes(int64_t T, int heads, int kv_heads, int d, int64_t max_keys);
+int mimg_attention_q8_dev(const float *q, const void *cache, const int64_t *kend, const int64_t *kstart, int64_t T,
+                          int heads, int kv_heads, int d, int64_t context, int64_t max_keys, float *out, void *ws,
+                          uint64_t ws_bytes, void *stream);
+
+/* Log probabilities of rows of logits [rows, n], ld >= n elements apart (no
+ * reference counterpart: its only choice is the greedy one, mimg_argmax_dev):
+ *   logprob[r]      = log softmax(row r)[targets[r]]; 0 for a target outside
+ *                     0..n-1 (a padded row)
+ *   entropy[r]      = -sum_i p_i log p_i, in nats
+ *   top_ids[r, j], top_logprobs[r, j], j < top: the largest logits in
+ *                     falling order, equal ones by the lowest index, NaN never
+ *                     (-1 and NaN past the last), with their log probabilities
+ * Any output may be NULL (targets too, without logprob), not all. A row with a
+ * NaN or +inf, or of -inf alone, has NaN results (top_ids apart). n up to 2^21,
+ * top 0..64 and at most n. ws: mimg_logprobs_workspace_bytes, 16-byte aligned. */
+uint64_t mimg_logprobs_workspace_bytes(int64_t rows, int64_t n, int top);
+int mimg_logprobs_dev(const float *logits, int64_t rows, int64_t n, int64_t ld, const int32_t *targets, int top,
+                      float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs, void *ws, uint64_t ws_bytes,
+                      void *stream);
+
 /* One step of the greedy loop on the device (reference cmd/mim-run/main.go
  * generate, 184-257), for n sequences: ids[i] = chosen[i], out[count*n+i] =
  * chosen[i] while count < cap (out holds cap*n ids), pos[i] += 1,

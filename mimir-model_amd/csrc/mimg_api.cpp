@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/mimg.h"
+#include "cache_q8.hpp"
 #include "mimg_device.hpp"
 #include "mimg_kernels.hpp"
 
@@ -1526,6 +1527,126 @@ int mimg_attention_dev(const float* q, const void* kcache, const void* vcache, c
                     (unsigned long long)mimg_attention_workspace_bytes(T, heads, max_keys));
     HIP_TRY(launch_attention(q, kcache, vcache, kend, kstart, (int)T, heads, kv_heads, d, context, max_keys, f16, out,
                              (float*)ws, (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+// ---- the 8-bit key-value cache ------------------------------------------------
+
+constexpr int64_t Q8_MAX_CONTEXT = 1ll << 30;  // cache entries: indices and blocks are ints in the kernels
+constexpr int Q8_MAX_HEADS = 16384;
+
+static int check_cache_q8(const char* what, int64_t T, int kv_heads, int d, int64_t context, const void* cache) {
+    if (T < 0 || T > 65535 || kv_heads < 1 || kv_heads > Q8_MAX_HEADS || d < 8 || d > Q8C_MAX_D || d % 8 || context < 1 ||
+        context > Q8_MAX_CONTEXT)
+        return fail(MIMG_ERR_ARG, "%s: T %lld, kv heads %d, D %d, context %lld (T <= 65535, D a multiple of 8, <= %d)", what,
+                    (long long)T, kv_heads, d, (long long)context, Q8C_MAX_D);
+    if (T > 0 && !cache) return fail(MIMG_ERR_ARG, "null pointer");
+    if (cache && !aligned(cache, 16)) return fail(MIMG_ERR_ARG, "%s: the cache must be 16-byte aligned", what);
+    return MIMG_OK;
+}
+
+uint64_t mimg_cache_q8_bytes(int kv_heads, int64_t context, int d) {
+    if (kv_heads < 1 || kv_heads > Q8_MAX_HEADS || d < 8 || d > Q8C_MAX_D || d % 8 || context < 1 || context > Q8_MAX_CONTEXT)
+        return 0;
+    return (uint64_t)q8c_bytes(kv_heads, context, q8c_dp(d));
+}
+
+int mimg_kv_store_q8_dev(const float* k, const float* v, const int64_t* cache_index, int64_t T, int kv_heads, int d,
+                         int64_t context, void* cache, void* stream) {
+    int rc;
+    if ((rc = check_cache_q8("kv_store_q8", T, kv_heads, d, context, cache))) return rc;
+    if (T > 0 && (!k || !v || !cache_index)) return fail(MIMG_ERR_ARG, "null pointer");
+    if ((rc = ensure_device()) || T == 0) return rc;
+    HIP_TRY(launch_kv_store_q8(k, v, cache_index, (int)T, kv_heads, d, context, cache, (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+int mimg_rope_kv_q8_dev(float* q, const float* k, const float* v, const int64_t* pos, const int64_t* cache_index,
+                        const double* inv_freq, int64_t T, int heads, int kv_heads, int d, int rotary, int interleaved,
+                        int64_t context, void* cache, void* stream) {
+    int rc;
+    if ((rc = check_cache_q8("rope_kv_q8", T, kv_heads, d, context, cache))) return rc;
+    if (heads < 1 || heads > Q8_MAX_HEADS || rotary <= 0 || rotary % 2 || rotary > d)
+        return fail(MIMG_ERR_ARG, "rope_kv_q8: heads %d, D %d, rotary %d", heads, d, rotary);
+    if (T > 0 && (!q || !k || !v || !pos || !cache_index || !inv_freq)) return fail(MIMG_ERR_ARG, "null pointer");
+    if ((rc = ensure_device()) || T == 0) return rc;
+    HIP_TRY(launch_rope_kv_q8(q, k, v, pos, cache_index, inv_freq, (int)T, heads, kv_heads, d, rotary, interleaved, context,
+                              cache, (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+int mimg_kv_load_q8_dev(const void* cache, const int64_t* cache_index, int64_t T, int kv_heads, int d, int64_t context,
+                        float* k, float* v, void* stream) {
+    int rc;
+    if ((rc = check_cache_q8("kv_load_q8", T, kv_heads, d, context, cache))) return rc;
+    if (T > 0 && (!k || !v || !cache_index)) return fail(MIMG_ERR_ARG, "null pointer");
+    if ((rc = ensure_device()) || T == 0) return rc;
+    HIP_TRY(launch_kv_load_q8(cache, cache_index, (int)T, kv_heads, d, context, k, v, (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+static bool attention_q8_shape(int64_t T, int heads, int kv_heads, int d, int64_t max_keys) {
+    return T >= 0 && T <= 65535 && heads >= 1 && heads <= Q8_MAX_HEADS && kv_heads >= 1 && heads % kv_heads == 0 && d >= 8 &&
+           d <= Q8C_MAX_D && d % 8 == 0 && max_keys >= 1 && max_keys <= Q8_MAX_CONTEXT;
+}
+
+uint64_t mimg_attention_q8_workspace_bytes(int64_t T, int heads, int kv_heads, int d, int64_t max_keys) {
+    if (T == 0 || !attention_q8_shape(T, heads, kv_heads, d, max_keys)) return 0;
+    return attention_q8_ws_bytes(T, heads, kv_heads, d, max_keys);
+}
+
+int mimg_attention_q8_dev(const float* q, const void* cache, const int64_t* kend, const int64_t* kstart, int64_t T, int heads,
+                          int kv_heads, int d, int64_t context, int64_t max_keys, float* out, void* ws, uint64_t ws_bytes,
+                          void* stream) {
+    int rc;
+    if (!attention_q8_shape(T, heads, kv_heads, d, max_keys))
+        return fail(MIMG_ERR_ARG, "attention_q8: T %lld, heads %d, kv heads %d, D %d, max_keys %lld (T <= 65535, D a multiple of 8, <= %d)",
+                    (long long)T, heads, kv_heads, d, (long long)max_keys, Q8C_MAX_D);
+    if ((rc = check_cache_q8("attention_q8", T, kv_heads, d, context, cache))) return rc;
+    if (T == 0) return ensure_device();
+    if (!q || !kend || !out) return fail(MIMG_ERR_ARG, "null pointer");
+    const uint64_t rb = (uint64_t)T * heads * d * 4, need = attention_q8_ws_bytes(T, heads, kv_heads, d, max_keys);
+    if ((uintptr_t)q < (uintptr_t)out + rb && (uintptr_t)out < (uintptr_t)q + rb)
+        return fail(MIMG_ERR_ARG, "attention_q8: out overlaps q");
+    if (need && !ws) return fail(MIMG_ERR_ARG, "null pointer");
+    if (need && !aligned(ws, 16)) return fail(MIMG_ERR_ARG, "attention_q8: the workspace must be 16-byte aligned");
+    if (ws_bytes < need)
+        return fail(MIMG_ERR_WORKSPACE, "attention_q8 workspace %llu < %llu bytes", (unsigned long long)ws_bytes,
+                    (unsigned long long)need);
+    if ((rc = ensure_device())) return rc;
+    HIP_TRY(launch_attention_q8(q, cache, kend, kstart, (int)T, heads, kv_heads, d, context, max_keys, out, (float*)ws,
+                                (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+// ---- log probabilities ----------------------------------------------------------
+
+static bool logprobs_shape(int64_t rows, int64_t n, int top) {
+    return rows >= 0 && rows <= (1 << 22) && n >= 1 && n <= logprobs_max_n() && top >= 0 && top <= 64 && top <= n;
+}
+
+uint64_t mimg_logprobs_workspace_bytes(int64_t rows, int64_t n, int top) {
+    return logprobs_shape(rows, n, top) ? logprobs_ws_bytes(rows, n, top) : 0;
+}
+
+int mimg_logprobs_dev(const float* logits, int64_t rows, int64_t n, int64_t ld, const int32_t* targets, int top,
+                      float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* ws, uint64_t ws_bytes,
+                      void* stream) {
+    if (!logprobs_shape(rows, n, top) || ld < n || ld > (1ll << 31))
+        return fail(MIMG_ERR_ARG, "logprobs: rows %lld, n %lld, ld %lld, top %d (rows <= 2^22, n <= %d, n <= ld, top <= 64 and n)",
+                    (long long)rows, (long long)n, (long long)ld, top, logprobs_max_n());
+    if (rows == 0) return ensure_device();
+    if (!logits || !ws || (logprob && !targets)) return fail(MIMG_ERR_ARG, "null pointer");
+    if (!logprob && !entropy && !(top > 0 && (top_ids || top_logprobs)))
+        return fail(MIMG_ERR_ARG, "logprobs: no output is asked for");
+    if (!aligned(ws, 16)) return fail(MIMG_ERR_ARG, "logprobs: the workspace must be 16-byte aligned");
+    const uint64_t need = logprobs_ws_bytes(rows, n, top);
+    if (ws_bytes < need)
+        return fail(MIMG_ERR_WORKSPACE, "logprobs workspace %llu < %llu bytes", (unsigned long long)ws_bytes,
+                    (unsigned long long)need);
+    if (int rc = ensure_device()) return rc;
+    HIP_TRY(launch_logprobs(logits, rows, n, ld, targets, top, logprob, entropy, top_ids, top_logprobs, ws,
+                            (hipStream_t)stream));
     return MIMG_OK;
 }
 

@@ -222,6 +222,23 @@ hipError_t launch_att_scores_mfma(const float* q, const void* kc, const int64_t*
 hipError_t launch_attention(const float* q, const void* kc, const void* vc, const int64_t* kend, const int64_t* kstart,
                             int T, int H, int Hkv, int D, int64_t C, int64_t maxk, int f16, float* out, float* ws,
                             hipStream_t s);
+// The 8-bit key-value cache (cache_q8.hip) and attention over it
+// (attention_q8.hip). d a multiple of 8, at most 256.
+hipError_t launch_kv_store_q8(const float* k, const float* v, const int64_t* index, int T, int Hkv, int d, int64_t C,
+                              void* cache, hipStream_t s);
+hipError_t launch_rope_kv_q8(float* q, const float* k, const float* v, const int64_t* pos, const int64_t* index,
+                             const double* inv_freq, int T, int H, int Hkv, int d, int rotary, int interleaved,
+                             int64_t C, void* cache, hipStream_t s);
+hipError_t launch_kv_load_q8(const void* cache, const int64_t* index, int T, int Hkv, int d, int64_t C, float* k, float* v,
+                             hipStream_t s);
+uint64_t attention_q8_ws_bytes(int64_t T, int H, int Hkv, int d, int64_t maxk);
+hipError_t launch_attention_q8(const float* q, const void* cache, const int64_t* kend, const int64_t* kstart, int T, int H,
+                               int Hkv, int d, int64_t C, int64_t maxk, float* out, float* ws, hipStream_t s);
+// Log probabilities (logprobs.hip): n at most logprobs_max_n(), top at most 64.
+int logprobs_max_n();
+uint64_t logprobs_ws_bytes(int64_t rows, int64_t n, int top);
+hipError_t launch_logprobs(const float* x, int64_t rows, int64_t n, int64_t ld, const int32_t* targets, int top,
+                           float* logprob, float* entropy, int32_t* top_ids, float* top_lp, void* ws, hipStream_t s);
 hipError_t launch_greedy_advance(const int32_t* chosen, int32_t* ids, int64_t* pos, int64_t* cidx, int32_t* out,
                                  int32_t* count, int cap, int n, hipStream_t s);
 hipError_t launch_swiglu(const float* g, const float* u, float* out, int64_t n, int64_t chunk, hipStream_t s);

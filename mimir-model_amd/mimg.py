@@ -83,6 +83,14 @@ SIGNATURES = {
     "mimg_kv_store_dev": (_I, [_P, _P, _P, _I64, _I, _I, _I64, _P, _P, _I, _P]),
     "mimg_attention_workspace_bytes": (_U64, [_I64, _I, _I64]),
     "mimg_attention_dev": (_I, [_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I64, _I64, _I, _P, _P, _U64, _P]),
+    "mimg_cache_q8_bytes": (_U64, [_I, _I64, _I]),
+    "mimg_kv_store_q8_dev": (_I, [_P, _P, _P, _I64, _I, _I, _I64, _P, _P]),
+    "mimg_rope_kv_q8_dev": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I64, _P, _P]),
+    "mimg_kv_load_q8_dev": (_I, [_P, _P, _I64, _I, _I, _I64, _P, _P, _P]),
+    "mimg_attention_q8_workspace_bytes": (_U64, [_I64, _I, _I, _I, _I64]),
+    "mimg_attention_q8_dev": (_I, [_P, _P, _P, _P, _I64, _I, _I, _I, _I64, _I64, _P, _P, _U64, _P]),
+    "mimg_logprobs_workspace_bytes": (_U64, [_I64, _I64, _I]),
+    "mimg_logprobs_dev": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _P, _P, _P, _P, _U64, _P]),
     "mimg_greedy_advance_dev": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _P]),
     "mimg_swiglu_dev": (_I, [_P, _P, _P, _I64, _I, _P]),
     "mimg_argmax_dev": (_I, [_P, _I64, _I64, _P, _P]),
@@ -533,6 +541,90 @@ def attention_dev(q_ptr, kc_ptr, vc_ptr, kend_ptr, kstart_ptr, T, heads, kv_head
     _check(load().mimg_attention_dev(_P(q_ptr), _P(kc_ptr), _P(vc_ptr), _P(kend_ptr), _o(kstart_ptr), T, heads,
                                      kv_heads, d, context, max_keys, int(f16), _P(out_ptr), _o(ws_ptr), ws_bytes,
                                      _P(stream)))
+
+
+Q8_CACHE_BLOCK = 32  # entries of an 8-bit cache that share a scale
+
+
+def cache_q8_bytes(kv_heads, context, d):
+    """Bytes of an 8-bit key-value cache of one layer (mimg_cache_q8_bytes)."""
+    return int(load().mimg_cache_q8_bytes(kv_heads, context, d))
+
+
+def pack_cache_q8(k, k_scale, v, v_scale, bad=None):
+    """int8 k, v [kv_heads, context, d] and float32 scales [kv_heads,
+    ceil(context/32)] (and uint32 masks of the entries that are not finite) as
+    the bytes of an 8-bit cache (include/mimg.h)."""
+    hk, c, d = k.shape
+    nb, dp = (c + 31) // 32, (d + 63) // 64 * 64
+
+    def padded(a):
+        p = np.full((hk, nb * 32, dp), 128, np.uint8)
+        p[:, :c, :d] = (a.astype(np.int16) + 128).astype(np.uint8)
+        return p
+
+    kb = padded(k).reshape(hk, nb, 2, 16, dp // 64, 4, 16).transpose(0, 1, 2, 4, 5, 3, 6).reshape(hk, nb, 32 * dp)
+    vb = padded(v).reshape(hk, nb, 2, 4, 4, dp // 32, 2, 16).transpose(0, 1, 5, 3, 7, 6, 2, 4).reshape(hk, nb, 32 * dp)
+    meta = np.zeros((hk, nb, 4), np.uint32)
+    meta[..., 0] = np.ascontiguousarray(k_scale, np.float32).view(np.uint32)
+    meta[..., 1] = np.ascontiguousarray(v_scale, np.float32).view(np.uint32)
+    if bad is not None:
+        meta[..., 2] = bad
+    return np.concatenate([np.concatenate([kb, vb], -1).reshape(-1), meta.reshape(-1).view(np.uint8)])
+
+
+def unpack_cache_q8(raw, kv_heads, context, d):
+    """The inverse of pack_cache_q8: (k, k_scale, v, v_scale, bad)."""
+    nb, dp = (context + 31) // 32, (d + 63) // 64 * 64
+    split = kv_heads * nb * 64 * dp
+    rec = raw[:split].reshape(kv_heads, nb, 64 * dp)
+    meta = raw[split:].view(np.uint32).reshape(kv_heads, nb, 4)
+    kb = rec[..., :32 * dp].reshape(kv_heads, nb, 2, dp // 64, 4, 16, 16).transpose(0, 1, 2, 5, 3, 4, 6)
+    vb = rec[..., 32 * dp:].reshape(kv_heads, nb, dp // 32, 4, 16, 2, 2, 4).transpose(0, 1, 6, 3, 7, 2, 5, 4)
+    k, v = (np.ascontiguousarray((b.reshape(kv_heads, nb * 32, dp)[:, :context, :d].astype(np.int16) - 128).astype(np.int8))
+            for b in (kb, vb))
+    scales = np.ascontiguousarray(meta).view(np.float32)
+    return k, scales[..., 0].copy(), v, scales[..., 1].copy(), meta[..., 2].copy()
+
+
+def kv_store_q8_dev(k_ptr, v_ptr, cidx_ptr, T, kv_heads, d, context, cache_ptr, stream):
+    _check(load().mimg_kv_store_q8_dev(_P(k_ptr), _P(v_ptr), _P(cidx_ptr), T, kv_heads, d, context, _P(cache_ptr),
+                                       _P(stream)))
+
+
+def rope_kv_q8_dev(q_ptr, k_ptr, v_ptr, pos_ptr, cidx_ptr, inv_freq_ptr, T, heads, kv_heads, d, rotary, interleaved,
+                   context, cache_ptr, stream):
+    _check(load().mimg_rope_kv_q8_dev(_P(q_ptr), _P(k_ptr), _P(v_ptr), _P(pos_ptr), _P(cidx_ptr), _P(inv_freq_ptr), T,
+                                      heads, kv_heads, d, rotary, int(interleaved), context, _P(cache_ptr), _P(stream)))
+
+
+def kv_load_q8_dev(cache_ptr, cidx_ptr, T, kv_heads, d, context, k_ptr, v_ptr, stream):
+    _check(load().mimg_kv_load_q8_dev(_P(cache_ptr), _P(cidx_ptr), T, kv_heads, d, context, _P(k_ptr), _P(v_ptr),
+                                      _P(stream)))
+
+
+def attention_q8_workspace_bytes(T, heads, kv_heads, d, max_keys):
+    return int(load().mimg_attention_q8_workspace_bytes(T, heads, kv_heads, d, max_keys))
+
+
+def attention_q8_dev(q_ptr, cache_ptr, kend_ptr, kstart_ptr, T, heads, kv_heads, d, context, max_keys, out_ptr, ws_ptr,
+                     ws_bytes, stream):
+    """Attention over an 8-bit cache, to float32 accuracy (mimg_attention_q8_dev)."""
+    _check(load().mimg_attention_q8_dev(_P(q_ptr), _P(cache_ptr), _P(kend_ptr), _o(kstart_ptr), T, heads, kv_heads, d,
+                                        context, max_keys, _P(out_ptr), _o(ws_ptr), ws_bytes, _P(stream)))
+
+
+def logprobs_workspace_bytes(rows, n, top):
+    return int(load().mimg_logprobs_workspace_bytes(rows, n, top))
+
+
+def logprobs_dev(x_ptr, rows, n, ld, targets_ptr, top, logprob_ptr, entropy_ptr, top_ids_ptr, top_logprobs_ptr, ws_ptr,
+                 ws_bytes, stream):
+    """Log probabilities of the targets, the entropy and the `top` largest
+    alternatives of each row of logits (mimg_logprobs_dev); outputs that are
+    None are not written."""
+    _check(load().mimg_logprobs_dev(_P(x_ptr), rows, n, ld, _o(targets_ptr), top, _o(logprob_ptr), _o(entropy_ptr),
+                                    _o(top_ids_ptr), _o(top_logprobs_ptr), _o(ws_ptr), ws_bytes, _P(stream)))
 
 
 def greedy_advance_dev(chosen_ptr, ids_ptr, pos_ptr, cidx_ptr, out_ptr, count_ptr, cap, n, stream):
