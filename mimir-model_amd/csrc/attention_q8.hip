@@ -19,6 +19,8 @@
 // needs no scaling by block. M moves only when a column's new maximum passes
 // it by 2^7 (weights are taken 2^8 up, so they stay below 2^15): the rescaling
 // of O is rare, and no maximum crosses lanes otherwise.
+#include <algorithm>
+
 #include "cache_q8.hpp"
 #include "decoder_math.hpp"
 #include "mimg_device.hpp"
@@ -32,6 +34,16 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
+// In the present group of instructions: n times a product and then v vector ones.
+template <int N, int V>
+__device__ __forceinline__ void alternate() {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, V, 0);
+    }
+}
+
 constexpr float M_NONE = -3.0e38f;  // a column's M before its first key
 constexpr int COLS = 16;            // (token, head) pairs of a tile
 
@@ -43,19 +55,12 @@ struct Args {
     int64_t C, maxk, nb;
     float* out;      // [T][H][d]
     float* part;     // [splits][T * H][DP] sums, then [splits][T * H] of {M, l}
-    int splits, cpt;  // cpt: columns a tile takes
+    int splits;      // of the keys, in the workspace
+    int few_splits;  // those that few_kernel cuts its rows into
+    int tpt, fan;    // tokens a tile of many_kernel; workgroups of few_kernel that share one
+    int choose;      // both kernels run: takes_many() says whose a tile is
+    int least;       // blocks that many_kernel's tiles span at least
 };
-
-__device__ __forceinline__ int wave_min_i32(int v) {
-    v = min(v, lane_xor<32>(v));
-    v = min(v, lane_xor<16>(v));
-    v = min(v, lane_xor<8>(v));
-    v = min(v, lane_xor<4>(v));
-    v = min(v, lane_xor<2>(v));
-    v = min(v, lane_xor<1>(v));
-    return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ int wave_max_i32(int v) { return -wave_min_i32(-v); }
 
 // Eight cache bytes as f16: 0x6400 | byte is 1024 + value + 128.
 __device__ __forceinline__ v8h widen(uint32_t a, uint32_t b) {
@@ -70,79 +75,55 @@ __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdg
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The blocks that the columns of a tile see, as disjoint rising ranges.
-struct Ranges {
-    int2 iv[COLS];
-    int n, total;
+// Step s of a lane's query row: dims 64 (s / 2) + 16 g + 8 (s % 2) .. +7, the
+// key operand's order.
+struct Eight {
+    float x[8];
 };
-// By one wave; each lane gives the blocks [sb, eb) of a column (eb = 0: none).
-__device__ __forceinline__ void join_ranges(int sb, int eb, Ranges& r) {
-    int done = 0, n = 0, total = 0;
-    for (;;) {
-        const int s = wave_min_i32(eb > done ? max(sb, done) : 0x7fffffff);
-        if (s == 0x7fffffff) break;
-        int e = s;
-        for (;;) {
-            const int e2 = wave_max_i32(sb <= e && eb > e ? eb : e);
-            if (e2 == e) break;
-            e = e2;
-        }
-        if ((threadIdx.x & 63) == 0) r.iv[n] = make_int2(s, e);
-        n++;
-        total += e - s;
-        done = e;
+__device__ __forceinline__ Eight query_step(const float* row, int d, int s, int g) {
+    const int d0 = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+    f32x4a4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+    if (d0 < d) {  // d is a multiple of 8
+        a = *(const f32x4a4*)(row + d0);
+        b = *(const f32x4a4*)(row + d0 + 4);
     }
-    if ((threadIdx.x & 63) == 0) {
-        r.n = n;
-        r.total = total;
-    }
+    return Eight{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
-
-// A column's query, its two parts as operands and the factor of its scores
-// (log2, without the block's key scale; NaN where q is not finite).
-template <int DP>
-struct Query {
-    v8h hi[DP / 32], lo[DP / 32];
+// A row's exponent e, amax * 2^e in [2^14, 2^15), and the factor of its scores
+// (log2, without the block's key scale; NaN where the row is not finite).
+struct RowScale {
+    int e;
     float scale;
 };
 template <int DP>
-__device__ __forceinline__ void load_query(Query<DP>& Q, const float* row, int d, int g) {
+__device__ __forceinline__ RowScale row_scale(const Eight* x, int d) {
     float amax = 0.f;
-    bool fin = true;
-    float x[DP / 32][8];
-#pragma unroll
-    for (int s = 0; s < DP / 32; s++) {
-        const int d0 = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-        f32x4a4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-        if (d0 < d) {  // d is a multiple of 8
-            a = *(const f32x4a4*)(row + d0);
-            b = *(const f32x4a4*)(row + d0 + 4);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x[s][j] = j < 4 ? a[j & 3] : b[j & 3];
-            fin &= (__float_as_uint(x[s][j]) & 0x7f800000u) != 0x7f800000u;
-            amax = fmaxf(amax, __builtin_fabsf(x[s][j]));
-        }
-    }
-    amax = fmaxf(amax, lane_xor_f32<16>(amax));
-    amax = fmaxf(amax, lane_xor_f32<32>(amax));
-    int f = fin ? 1 : 0;
-    f &= lane_xor<16>(f);
-    f &= lane_xor<32>(f);
-    // amax * 2^e in [2^14, 2^15)
-    const int e = amax > 0.f && f ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
-    const float k = (float)(1.4426950408889634 / sqrt((double)d));
-    Q.scale = f ? __builtin_ldexpf(k, -e) : __builtin_nanf("");
+    int f = 1;
 #pragma unroll
     for (int s = 0; s < DP / 32; s++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float v = f ? __builtin_ldexpf(x[s][j], e) : 0.f;
-            const _Float16 h = (_Float16)v;
-            Q.hi[s][j] = h;
-            Q.lo[s][j] = (_Float16)(v - (float)h);
+            f &= (__float_as_uint(x[s].x[j]) & 0x7f800000u) != 0x7f800000u ? 1 : 0;
+            amax = fmaxf(amax, __builtin_fabsf(x[s].x[j]));
         }
+    amax = fmaxf(amax, lane_xor_f32<16>(amax));
+    amax = fmaxf(amax, lane_xor_f32<32>(amax));
+    f &= lane_xor<16>(f);
+    f &= lane_xor<32>(f);
+    RowScale r;
+    r.e = amax > 0.f && f ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
+    const float k = (float)(1.4426950408889634 / sqrt((double)d));
+    r.scale = f ? __builtin_ldexpf(k, -r.e) : __builtin_nanf("");
+    return r;
+}
+__device__ __forceinline__ void two_parts(const Eight& x, const RowScale& r, v8h& hi, v8h& lo) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float v = r.scale == r.scale ? __builtin_ldexpf(x.x[j], r.e) : 0.f;
+        const _Float16 h = (_Float16)v;
+        hi[j] = h;
+        lo[j] = (_Float16)(v - (float)h);
+    }
 }
 
 // A column's running state: O^T tiles (dims 16 i + 4 g .. +3), M (the same in
@@ -153,239 +134,638 @@ struct State {
     float M, l;
 };
 
-// The eight weights of a lane from its scores (key 16 kt + 4 g + i of block
-// blk), M moved where needed, and the operands of the second product.
-struct Weights {
-    v8h hi, lo;
+// A block's value scale for the exponents: log2 and reciprocal (of a block of
+// zeros the floor's; its weights are left out below).
+struct Scale {
+    float lv, iv;
 };
-template <int DP>
-__device__ __forceinline__ Weights weigh(v4f s0, v4f s1, const Q8Meta& m, float scale, int blk, int g, int k0, int n,
-                                         bool all_seen, State<DP>& S) {
+__device__ __forceinline__ Scale value_scale(const Q8Meta& m) {
     const float vs = m.vs > 0.f ? m.vs : Q8C_FLOOR;
-    const float lv = __builtin_amdgcn_logf(vs), cs = scale * m.ks;
-    float iv = __builtin_amdgcn_rcpf(vs);
-    float y[8];
+    return {__builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+}
+// The factor of a block's scores; at least float32's smallest normal number, so
+// that -inf times it is -inf (a NaN stays).
+__device__ __forceinline__ float key_scale(float scale, const Q8Meta& m) {
+    const float c = scale * m.ks;
+    return c < 1.17549435e-38f ? 1.17549435e-38f : c;
+}
+__device__ __forceinline__ float largest(v4f s0, v4f s1) {
+    return fmaxf(fmaxf(fmaxf(s0.x, s0.y), fmaxf(s0.z, s0.w)), fmaxf(fmaxf(s1.x, s1.y), fmaxf(s1.z, s1.w)));
+}
+// Whether a lane's scores need no more than weights() of them: M is near
+// enough, and no weight so small that the scale in it could matter. (NaN: no.)
+__device__ __forceinline__ bool near_enough(float top, float M) { return top <= M + 7.f && top >= M - 60.f; }
+
+// What a block may need before its weights, in lanes or as a whole: entries
+// that a column does not see (-inf) or that are not finite (NaN), M moved, and
+// weights left out. Returns the exponents' offset.
+template <int DP>
+__device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Q8Meta& m, float cs, Scale v, int blk, int g, int k0, int n,
+                                         State<DP>& S) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) y[j] = (j < 4 ? s0[j & 3] : s1[j & 3]) * cs;
-    if (!all_seen || m.bad) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int e = 16 * (j >> 2) + 4 * g + (j & 3);
-            if ((m.bad >> e) & 1) y[j] = __builtin_nanf("");
-            if ((unsigned)(Q8C_BLOCK * blk + e - k0) >= (unsigned)n) y[j] = -__builtin_inff();
-        }
+    for (int j = 0; j < 8; j++) {
+        float& x = j < 4 ? ((float*)&s0)[j] : ((float*)&s1)[j - 4];
+        const int e = 16 * (j >> 2) + 4 * g + (j & 3);
+        if ((m.bad >> e) & 1) x = __builtin_nanf("");
+        if ((unsigned)(Q8C_BLOCK * blk + e - k0) >= (unsigned)n) x = -__builtin_inff();
     }
-    float mx = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-    mx += lv;
+    const float mx = largest(s0, s1) * cs + v.lv;
     if (__any(mx > S.M + 7.f)) {
         float cm = fmaxf(mx, lane_xor_f32<16>(mx));
         cm = fmaxf(cm, lane_xor_f32<32>(cm));
         const float M = fmaxf(S.M, cm), a = exp2_hw(0.5f * (S.M - M));
         S.M = M;
-        S.l = S.l * a * a;
+        S.l = S.l * a * a;  // (in two factors: l may be large where M is small)
 #pragma unroll
         for (int i = 0; i < DP / 16; i++) S.o[i] *= a * a;
     }
-    float base = lv - S.M + 8.f;
-    // Where a lane's w are all below 2^-60 of the largest (a block of zeros or
-    // nearly beside large values) they count in the sum alone, as p: with the
-    // scale in them they could pass float32's range.
-    const bool deep = mx < S.M - 60.f;
-    if (__any(deep)) {
-        base = deep ? 8.f - S.M : base;
-        iv = deep ? 1.f : iv;
-    }
-    Weights w;
-    float sum = 0.f;
+    // A block of zeros, and lanes whose w are all below 2^-60 of the largest,
+    // count in the sum alone, as p: with the scale in them they could pass
+    // float32's range.
+    const bool zeros = !(m.vs > 0.f), out = zeros || mx < S.M - 60.f;
+    if (!__any(out)) return v.lv - S.M + 8.f;
+    // (p beside w: at most 2^8 * 2^96, where the block's floor set M)
+    const float base = zeros && !(mx < S.M - 60.f) ? v.lv - S.M + 8.f : 8.f - S.M, iv = base == 8.f - S.M ? 1.f : v.iv;
+    if (out) {
+        float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float p = exp2_hw(y[j] + base);
-        sum += p;
-        const _Float16 h = (_Float16)p;
-        w.hi[j] = h;
-        w.lo[j] = (_Float16)(p - (float)h);
+        for (int j = 0; j < 8; j++) sum += exp2_hw(__builtin_fmaf(j < 4 ? s0[j & 3] : s1[j & 3], cs, base));
+        S.l = __builtin_fmaf(sum, iv, S.l);
     }
-    S.l = __builtin_fmaf(sum, iv, S.l);
-    if (!(m.vs > 0.f) || __any(deep)) {  // a block of zeros, whatever its integers
-        const bool none = deep || !(m.vs > 0.f);
-        w.hi = none ? v8h{} : w.hi;
-        w.lo = none ? v8h{} : w.lo;
-    }
-    return w;
+    return out ? -__builtin_inff() : v.lv - S.M + 8.f;
 }
 
-// Few columns: a workgroup per (tile of 16 columns, kv head, split of the
-// keys); its four waves take blocks in turn, straight from memory, each with
-// a state of its own, joined at the end.
-template <int DP>
-__global__ __launch_bounds__(256) void few_kernel(Args A) {
-    __shared__ Ranges R;
-    __shared__ float ml[4][2][COLS];
-    __shared__ __align__(16) float os[2][COLS][DP];
-    const int tid = threadIdx.x, l = tid & 63, g = l >> 4, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x % (unsigned)A.Hkv, c0 = (blockIdx.x / (unsigned)A.Hkv) * A.cpt;
-    const int ncol = min(A.cpt, A.T * A.G - c0), col = l & 15;
-    const int c = c0 + min(col, ncol - 1), t = c / A.G;
-    const int head = t * A.H + hk * A.G + (c - t * A.G);
+// The eight weights of a lane in two parts, rounded towards zero: 22 bits.
+struct Weights {
+    uint32_t hi[4], lo[4];
+    __device__ __forceinline__ v8h h() const { return __builtin_bit_cast(v8h, (u32x4){hi[0], hi[1], hi[2], hi[3]}); }
+    __device__ __forceinline__ v8h r() const { return __builtin_bit_cast(v8h, (u32x4){lo[0], lo[1], lo[2], lo[3]}); }
+};
+// Those of one key tile: two words of each part; their sum.
+__device__ __forceinline__ float weigh_tile(v4f s, float cs, float base, uint32_t* hi, uint32_t* lo) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) y[j] = exp2_hw(__builtin_fmaf(s[j], cs, base));
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const v2h h = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(y[2 * j], y[2 * j + 1]));
+        const float r0 = __builtin_fmaf((float)h.x, -1.f, y[2 * j]), r1 = __builtin_fmaf((float)h.y, -1.f, y[2 * j + 1]);
+        hi[j] = __builtin_bit_cast(uint32_t, h);
+        lo[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+    }
+    return (y[0] + y[1]) + (y[2] + y[3]);
+}
+
+__device__ __forceinline__ int wave_min_i32(int v) {
+    v = min(v, lane_xor<32>(v));
+    v = min(v, lane_xor<16>(v));
+    v = min(v, lane_xor<8>(v));
+    v = min(v, lane_xor<4>(v));
+    v = min(v, lane_xor<2>(v));
+    v = min(v, lane_xor<1>(v));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i32(int v) { return -wave_min_i32(-v); }
+
+__device__ __forceinline__ int wave_sum_i32(int v) {
+    v += lane_xor<32>(v);
+    v += lane_xor<16>(v);
+    v += lane_xor<8>(v);
+    v += lane_xor<4>(v);
+    v += lane_xor<2>(v);
+    v += lane_xor<1>(v);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+constexpr int MAX_COLS = 128;  // columns of a tile of many_kernel, and so tokens
+
+// The blocks that a workgroup's columns see, as disjoint rising ranges.
+struct Ranges {
+    int2 iv[MAX_COLS];
+    int2 kn[MAX_COLS];  // each column's first key and number of keys
+    int total;
+};
+// The blocks [s0, e0) and [s1, e1) of the tokens l and 64 + l of a tile (e = 0:
+// none).
+struct Spans {
+    int s0, e0, s1, e1;
+};
+__device__ __forceinline__ int2 span_of(const Args& A, int t) {
     const AttRange r = att_range(A.kend, A.kstart, t, A.C, A.maxk);
-    const int k0 = (int)r.k0, n = (int)r.n;
-    if (w == 0) join_ranges(k0 >> 5, n > 0 ? (k0 + n + 31) >> 5 : 0, R);
-    Query<DP> Q;
-    load_query<DP>(Q, A.q + (int64_t)head * A.d, A.d, g);
+    return r.n > 0 ? make_int2((int)(r.k0 >> 5), (int)((r.k0 + r.n + 31) >> 5)) : make_int2(0, 0);
+}
+__device__ __forceinline__ Spans spans_of(const Args& A, int tile) {
+    const int l = threadIdx.x & 63, t = tile * A.tpt + l, last = min(A.T, (tile + 1) * A.tpt);
+    const int2 a = t < last ? span_of(A, t) : make_int2(0, 0), b = t + 64 < last ? span_of(A, t + 64) : make_int2(0, 0);
+    return {a.x, a.y, b.x, b.y};
+}
+// Whether many_kernel takes a tile: its tokens see the same blocks (a prompt),
+// not each its own (a decode batch). many_kernel reads a block once for the
+// tile, at 6 ns (128 columns; MI355X, all CUs busy), few_kernel once for each
+// token and 16 heads, at 0.7 ns from the caches. By a whole wave.
+__device__ __forceinline__ bool takes_many(const Args& A, const Spans& p, int cols) {
+    const int span = wave_max_i32(max(p.e0, p.e1)) - wave_min_i32(min(p.e0 ? p.s0 : 0x7fffffff, p.e1 ? p.s1 : 0x7fffffff));
+    const int64_t sum = (int64_t)wave_sum_i32(p.e0 - p.s0 + (p.e1 - p.s1)) * ((A.G + COLS - 1) / COLS);
+    return sum > 0 && span >= A.least && sum >= (int64_t)(cols / 16) * span;
+}
+// By one wave.
+__device__ __forceinline__ void join_ranges(const Spans& p, Ranges& r) {
+    const int s0 = p.s0, e0 = p.e0, s1 = p.s1, e1 = p.e1;
+    int done = 0, n = 0, total = 0;
+    for (;;) {
+        const int s = wave_min_i32(min(e0 > done ? max(s0, done) : 0x7fffffff, e1 > done ? max(s1, done) : 0x7fffffff));
+        if (s == 0x7fffffff) break;
+        int e = s;
+        for (;;) {
+            const int e2 = wave_max_i32(max(s0 <= e && e0 > e ? e0 : e, s1 <= e && e1 > e ? e1 : e));
+            if (e2 == e) break;
+            e = e2;
+        }
+        if ((threadIdx.x & 63) == 0) r.iv[n] = make_int2(s, e);
+        n++;
+        total += e - s;
+        done = e;
+    }
+    if ((threadIdx.x & 63) == 0) r.total = total;
+}
+
+template <int DP>
+constexpr int MANY_COLS = DP <= 128 ? MAX_COLS : MAX_COLS / 2;
+
+// Few rows: a workgroup per (token, kv head, split of the keys) and up to 16
+// query heads (beside many_kernel: for every fan-th token of a tile); its NW
+// waves take the token's blocks in turn, straight from
+// memory, each with a state of its own, joined at the end. A wave has its next
+// block's keys in flight while it works on one, and the values during the
+// score product. The query's parts lie in LDS (for the registers).
+constexpr int NW = 4;
+template <int DP>
+struct FewLds {
+    union {
+        v8h q[2][DP / 32][64];
+        float o[NW][COLS][DP + 4];  // rows four banks apart
+    };
+    float ml[NW][2][COLS];
+};
+template <int DP>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A) {
+    __shared__ FewLds<DP> S_;
+    const int tid = threadIdx.x, l = tid & 63, g = l >> 4, col = l & 15, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int subs = (A.G + COLS - 1) / COLS, hk = blockIdx.x % (unsigned)A.Hkv, sub = blockIdx.x / (unsigned)A.Hkv % subs;
+    const int unit = blockIdx.x / (unsigned)(A.Hkv * subs), tile = unit / A.fan, g0 = sub * COLS, ncol = min(COLS, A.G - g0);
+    if (A.choose && takes_many(A, spans_of(A, tile), MANY_COLS<DP>)) return;
+    const int last = min(A.T, (tile + 1) * A.tpt);
+    for (int t = tile * A.tpt + (unit - tile * A.fan); t < last; t += A.fan) {
+    const int head0 = t * A.H + hk * A.G + g0;
+    const AttRange r = att_range(A.kend, A.kstart, t, A.C, A.maxk);
+    Eight x[DP / 32];
+    const float* row = A.q + (int64_t)(head0 + min(col, ncol - 1)) * A.d;
+#pragma unroll
+    for (int s = 0; s < DP / 32; s++) x[s] = query_step(row, A.d, s, g);
+    const int k0 = __builtin_amdgcn_readfirstlane((int)r.k0), n = __builtin_amdgcn_readfirstlane((int)r.n);
+    const int b0 = k0 >> 5, total = n > 0 ? ((k0 + n + 31) >> 5) - b0 : 0;
+    const int per = max((total + A.few_splits - 1) / A.few_splits, NW);
+    int b = b0 + (int)blockIdx.y * per + w;
+    const int b1 = min(b0 + total, b0 + ((int)blockIdx.y + 1) * per);
+    const u32x4* rec = (const u32x4*)A.cache + l;
+    constexpr int64_t REC = 2 * Q8C_BLOCK * DP / 16;
+    const int64_t first = (int64_t)hk * A.nb;
+    const Q8Meta* meta = (const Q8Meta*)(A.cache + q8c_meta(A.nb, A.Hkv, hk, 0, DP));
+    u32x4 kb[DP / 32], vb[DP / 32];
+    Q8Meta m;
+    auto fetch_k = [&](int blk) {
+        const u32x4* p = rec + (first + blk) * REC;
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) kb[i] = __builtin_nontemporal_load(p + 64 * i);
+        m = meta[blk];
+    };
+    if (b < b1) fetch_k(b);
+    const RowScale rs = row_scale<DP>(x, A.d);
+    __syncthreads();  // (the last token's sums are read)
+#pragma unroll
+    for (int s = 0; s < DP / 32; s++)
+        if (s % NW == w) two_parts(x[s], rs, S_.q[0][s][l], S_.q[1][s][l]);
     __syncthreads();
-    const int total = R.total, per = max((total + A.splits - 1) / A.splits, 4);
-    const int p0 = (int)blockIdx.y * per, p1 = min(total, p0 + per);
     State<DP> S;
 #pragma unroll
     for (int i = 0; i < DP / 16; i++) S.o[i] = v4f{0.f, 0.f, 0.f, 0.f};
     S.M = M_NONE;
     S.l = 0.f;
-    int i = 0, below = 0;  // blocks of the ranges before range i
-    for (int p = p0 + w; p < p1; p += 4) {
-        int2 iv = R.iv[i];
-        while (p - below >= iv.y - iv.x) {
-            below += iv.y - iv.x;
-            iv = R.iv[++i];
+    while (b < b1) {
+        {
+            const u32x4* p = rec + (first + b) * REC + 64 * (DP / 32);
+#pragma unroll
+            for (int i = 0; i < DP / 32; i++) vb[i] = __builtin_nontemporal_load(p + 64 * i);
         }
-        const int blk = __builtin_amdgcn_readfirstlane(iv.x + p - below);
-        const u32x4* rec = (const u32x4*)(A.cache + q8c_record(A.nb, hk, blk, DP)) + l;
-        const Q8Meta m = *(const Q8Meta*)(A.cache + q8c_meta(A.nb, A.Hkv, hk, blk, DP));
-        v4f s[2];
+        v4f s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-            s[kt] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < DP / 64; i++)
 #pragma unroll
-            for (int x = 0; x < DP / 64; x++) {
-                const u32x4 u = rec[(kt * (DP / 64) + x) * 64];
-                const v8h a = widen(u.x, u.y), b = widen(u.z, u.w);
-                s[kt] = mfma(a, Q.lo[2 * x], s[kt]);
-                s[kt] = mfma(b, Q.lo[2 * x + 1], s[kt]);
-                s[kt] = mfma(a, Q.hi[2 * x], s[kt]);
-                s[kt] = mfma(b, Q.hi[2 * x + 1], s[kt]);
+            for (int kt = 0; kt < 2; kt++) {
+                const u32x4 u = kb[kt * (DP / 64) + i];
+                const v8h ka = widen(u.x, u.y), kc = widen(u.z, u.w);
+                s[kt] = mfma(ka, S_.q[1][2 * i][l], s[kt]);
+                s[kt] = mfma(kc, S_.q[1][2 * i + 1][l], s[kt]);
+                s[kt] = mfma(ka, S_.q[0][2 * i][l], s[kt]);
+                s[kt] = mfma(kc, S_.q[0][2 * i + 1][l], s[kt]);
             }
-        }
-        const bool all_seen = __all(k0 <= Q8C_BLOCK * blk && k0 + n >= Q8C_BLOCK * (blk + 1));
-        const Weights W = weigh<DP>(s[0], s[1], m, Q.scale, blk, g, k0, n, all_seen, S);
+        const Q8Meta mb = m;
+        const int blk = b;
+        b += NW;
+        if (b < b1) fetch_k(b);
+        const bool all_seen = k0 <= Q8C_BLOCK * blk && k0 + n >= Q8C_BLOCK * (blk + 1);
+        const Scale v = value_scale(mb);
+        const float cs = key_scale(rs.scale, mb);
+        float base = v.lv - S.M + 8.f;
+        if (!all_seen || mb.bad || !(mb.vs > 0.f) || !__all(near_enough(largest(s[0], s[1]) * cs + v.lv, S.M)))
+            base = correct<DP>(s[0], s[1], mb, cs, v, blk, g, k0, n, S);
+        Weights W;
+        const float sum = weigh_tile(s[0], cs, base, W.hi, W.lo) + weigh_tile(s[1], cs, base, W.hi + 2, W.lo + 2);
+        S.l = __builtin_fmaf(sum, v.iv, S.l);
 #pragma unroll
-        for (int x = 0; x < DP / 32; x++) {
-            const u32x4 u = rec[(DP / 32 + x) * 64];
-            const v8h a = widen(u.x, u.y), b = widen(u.z, u.w);
-            S.o[2 * x] = mfma(a, W.lo, S.o[2 * x]);
-            S.o[2 * x + 1] = mfma(b, W.lo, S.o[2 * x + 1]);
-            S.o[2 * x] = mfma(a, W.hi, S.o[2 * x]);
-            S.o[2 * x + 1] = mfma(b, W.hi, S.o[2 * x + 1]);
+        for (int i = 0; i < DP / 32; i++) {
+            __builtin_amdgcn_sched_barrier(0);
+            const v8h va = widen(vb[i].x, vb[i].y), vc = widen(vb[i].z, vb[i].w);
+            S.o[2 * i] = mfma(va, W.r(), S.o[2 * i]);
+            S.o[2 * i + 1] = mfma(vc, W.r(), S.o[2 * i + 1]);
+            S.o[2 * i] = mfma(va, W.h(), S.o[2 * i]);
+            S.o[2 * i + 1] = mfma(vc, W.h(), S.o[2 * i + 1]);
         }
     }
-    // join: every wave's O to the largest M, then waves 2, 3 into 0, 1 and 1 into 0
+    // join the waves' states
     S.l += lane_xor_f32<16>(S.l);
     S.l += lane_xor_f32<32>(S.l);
     if (l < COLS) {
-        ml[w][0][l] = S.M;
-        ml[w][1][l] = S.l;
+        S_.ml[w][0][l] = S.M;
+        S_.ml[w][1][l] = S.l;
+    }
+    __syncthreads();  // (every wave has read its query for the last time)
+    if (col < ncol)
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) *(v4f*)&S_.o[w][col][16 * i + 4 * g] = S.o[i];
+    __syncthreads();
+    const int64_t rows = (int64_t)A.T * A.H;
+    const bool none = (int)blockIdx.y * per >= total;
+    for (int i = tid; i < ncol * (DP / 4); i += 64 * NW) {
+        const int c = i / (DP / 4), d4 = (i - c * (DP / 4)) * 4;
+        float M = S_.ml[0][0][c];
+#pragma unroll
+        for (int j = 1; j < NW; j++) M = fmaxf(M, S_.ml[j][0][c]);
+        float L = 0.f;
+        v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NW; j++) {  // (in two factors: l may be large where M is small)
+            const float f = exp2_hw(0.5f * (S_.ml[j][0][c] - M));
+            L += S_.ml[j][1][c] * f * f;
+            o += *(const v4f*)&S_.o[j][c][d4] * (f * f);
+        }
+        const int64_t head = head0 + c;
+        if (A.splits > 1) {
+            const int64_t at = (int64_t)blockIdx.y * rows + head;
+            if (d4 == 0)
+                ((float2*)(A.part + (int64_t)A.splits * rows * DP))[at] = make_float2(none ? -__builtin_inff() : M, L);
+            if (!none) *(v4f*)(A.part + at * DP + d4) = o;
+            if (d4 == 0 && blockIdx.y == 0)  // (splits that few_kernel does not use)
+                for (int y = A.few_splits; y < A.splits; y++)
+                    ((float2*)(A.part + (int64_t)A.splits * rows * DP))[y * rows + head] = make_float2(-__builtin_inff(), 0.f);
+        } else if (d4 < A.d) {
+            // a row that sees no key gives zeros, one whose weights are all zero NaN
+            *(f32x4a4*)(A.out + head * A.d + d4) = none ? v4f{0.f, 0.f, 0.f, 0.f} : o * (L > 0.f ? 1.f / L : __builtin_nanf(""));
+        }
+    }
+    }
+}
+
+// Many rows: a workgroup per (tile of whole tokens, at most 64 NCT columns, kv
+// head, split of the keys), 16 NCT columns a wave. A block's record is widened once for the four
+// waves into LDS, in operand order (two buffers: the next block is written and
+// the one after it in flight while a block is worked on), and an operand read
+// from there serves 2 NCT products.
+template <int DP, int NCT>
+__global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
+    constexpr int WC = 16 * NCT, PIECES = DP / 64;  // columns a wave; 16-byte pieces of a record a thread
+    __shared__ v8h buf[3][DP / 8][64];
+    __shared__ Ranges R;
+    const int tid = threadIdx.x, l = tid & 63, g = l >> 4, col = l & 15, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x % (unsigned)A.Hkv;
+    // The last columns (the most keys of a prompt) first, but every other 256
+    // workgroups rising: a CU's two share it, and get as many keys in all as
+    // another's two.
+    const int tiles = gridDim.x / (unsigned)A.Hkv, turn = max(256 / A.Hkv, 1), ti = blockIdx.x / (unsigned)A.Hkv;
+    const int r0 = ti / turn * turn, tile = (ti / turn) & 1 ? r0 + min(turn, tiles - r0) - 1 - (ti - r0) : ti;
+    const int t0 = (tiles - 1 - tile) * A.tpt, cols = min(A.tpt, A.T - t0) * A.G;
+    const Spans spans = spans_of(A, tiles - 1 - tile);
+    if (A.choose && !takes_many(A, spans, MANY_COLS<DP>)) return;
+    if (w == 0) join_ranges(spans, R);
+    float scale[NCT];
+    v8h qhi[NCT][DP / 32], qlo[NCT][DP / 32];
+    State<DP> S[NCT];
+    int from = 0, to = 0x7fffffff;  // keys that all of the wave's columns see
+#pragma unroll
+    for (int ct = 0; ct < NCT; ct++) {
+        const int c = min(WC * w + 16 * ct + col, cols - 1), t = t0 + c / A.G, head = t * A.H + hk * A.G + c % A.G;
+        const AttRange r = att_range(A.kend, A.kstart, t, A.C, A.maxk);
+        if (g == 0) R.kn[WC * w + 16 * ct + col] = make_int2((int)r.k0, (int)r.n);
+        from = max(from, (int)r.k0);
+        to = min(to, r.n > 0 ? (int)(r.k0 + r.n) : 0);
+        Eight x[DP / 32];
+#pragma unroll
+        for (int s = 0; s < DP / 32; s++) x[s] = query_step(A.q + (int64_t)head * A.d, A.d, s, g);
+        const RowScale rs = row_scale<DP>(x, A.d);
+        scale[ct] = rs.scale;
+#pragma unroll
+        for (int s = 0; s < DP / 32; s++) two_parts(x[s], rs, qhi[ct][s], qlo[ct][s]);
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) S[ct].o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        S[ct].M = M_NONE;
+        S[ct].l = 0.f;
+    }
+    from = wave_max_i32(from);
+    to = wave_min_i32(to);
+    __syncthreads();
+    const int total = R.total, per = max((total + A.splits - 1) / A.splits, 2);
+    const int p0 = (int)blockIdx.y * per, p1 = min(total, p0 + per);
+    // The block of position p (rising): ranges [.., end) lie `shift` above theirs.
+    int i = -1, end = 0, shift = 0;
+    auto block_at = [&](int p) {
+        while (p >= end) {
+            const int2 iv = R.iv[++i];
+            shift = __builtin_amdgcn_readfirstlane(iv.x) - end;
+            end += __builtin_amdgcn_readfirstlane(iv.y) - __builtin_amdgcn_readfirstlane(iv.x);
+        }
+        return p + shift;
+    };
+    const Q8Meta* meta = (const Q8Meta*)(A.cache + q8c_meta(A.nb, A.Hkv, hk, 0, DP));
+    u32x4 raw[PIECES];
+    auto fetch = [&](u32x4 (&r)[PIECES], int blk) {
+        const u32x4* p = (const u32x4*)(A.cache + q8c_record(A.nb, hk, blk, DP)) + tid;
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) r[j] = p[256 * j];
+    };
+    // Half h of the thread's pieces: 0 .. DP / 32 - 1.
+    auto put = [&](v8h (*b)[64], const u32x4 (&q)[PIECES], int h) {
+        const u32x4 r = q[h >> 1];
+        b[2 * (w + 4 * (h >> 1)) + (h & 1)][l] = h & 1 ? widen(r.z, r.w) : widen(r.x, r.y);
+    };
+    constexpr int NS = DP / 32;  // steps of a score product, and pairs of dim tiles
+    int here = 0, next = 0, after = 0;  // blocks of positions p, p + 1 (in LDS), p + 2 (in flight)
+    Q8Meta mh{}, mn{};
+    v4f sa[NCT][2], sb[NCT][2];
+    float top[NCT];  // the largest of a lane's scores
+    if (p0 < p1) {
+        u32x4 raw0[PIECES], raw1[PIECES];
+        here = next = after = block_at(p0);
+        fetch(raw0, here);
+        if (p0 + 1 < p1) next = after = block_at(p0 + 1);
+        fetch(raw1, next);
+        if (p0 + 2 < p1) after = block_at(p0 + 2);
+        fetch(raw, after);
+#pragma unroll
+        for (int h = 0; h < NS; h++) put(buf[0], raw0, h);
+#pragma unroll
+        for (int h = 0; h < NS; h++) put(buf[1], raw1, h);
+        mh = meta[here];
+        mn = meta[next];
     }
     __syncthreads();
-    const float M = fmaxf(fmaxf(ml[0][0][col], ml[1][0][col]), fmaxf(ml[2][0][col], ml[3][0][col]));
-    float L = 0.f;
+    if (p0 < p1) {
 #pragma unroll
-    for (int x = 0; x < 4; x++) {  // (in two factors: l may be large where M is small)
-        const float f = exp2_hw(0.5f * (ml[x][0][col] - M));
-        L += ml[x][1][col] * f * f;
+        for (int ct = 0; ct < NCT; ct++) sa[ct][0] = sa[ct][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < NS; x++)
+#pragma unroll
+            for (int ct = 0; ct < NCT; ct++)
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) {
+                    sa[ct][kt] = mfma(buf[0][kt * NS + x][l], qlo[ct][x], sa[ct][kt]);
+                    sa[ct][kt] = mfma(buf[0][kt * NS + x][l], qhi[ct][x], sa[ct][kt]);
+                }
+#pragma unroll
+        for (int ct = 0; ct < NCT; ct++) top[ct] = largest(sa[ct][0], sa[ct][1]);
     }
-    const float a = exp2_hw(S.M - M);
+    int bi = 0;
+    // One block: its weights beside the next block's score product, then the
+    // second product beside the record after that (past the last block: what
+    // the buffers hold, unused). In groups of 4 NCT products, a dozen or two
+    // vector instructions between them: a wave's matrix and vector
+    // instructions overlap when they alternate, those of two waves hardly do.
+    // Operands are read from LDS a group ahead.
+    auto step = [&](int p, v4f (&s)[NCT][2], v4f (&sn)[NCT][2]) {
+        const int b1 = bi == 2 ? 0 : bi + 1, b2 = b1 == 2 ? 0 : b1 + 1;
+        v8h (*kb)[64] = buf[b1], (*vb)[64] = buf[bi] + DP / 16, (*pb)[64] = buf[b2];
+        v8h k0 = kb[0][l], k1 = kb[NS][l];
+        const Q8Meta m = mh;
+        const Scale v = value_scale(m);
+        float cs[NCT], base[NCT];
+        bool fine = true;
 #pragma unroll
-    for (int x = 0; x < DP / 16; x++) S.o[x] *= a;
+        for (int ct = 0; ct < NCT; ct++) {
+            cs[ct] = key_scale(scale[ct], m);
+            fine &= near_enough(top[ct] * cs[ct] + v.lv, S[ct].M);
+            base[ct] = v.lv - S[ct].M + 8.f;
+        }
+        if (!(Q8C_BLOCK * here >= from && Q8C_BLOCK * (here + 1) <= to && m.bad == 0 && m.vs > 0.f && __all(fine))) {
 #pragma unroll
-    for (int step = 2; step >= 1; step >>= 1) {
-        if (w >= step && w < 2 * step)
+            for (int ct = 0; ct < NCT; ct++) {
+                const int2 k = R.kn[WC * w + 16 * ct + col];
+                base[ct] = correct<DP>(s[ct][0], s[ct][1], m, cs[ct], v, here, g, k.x, k.y, S[ct]);
+            }
+        }
+        here = next;
+        next = after;
+        mh = mn;
+        mn = meta[next];
+        Weights W[NCT];
+        float sum[NCT][2];
+        v8h v0, v1;
 #pragma unroll
-            for (int x = 0; x < DP / 16; x++) *(v4f*)&os[w - step][col][16 * x + 4 * g] = S.o[x];
+        for (int ct = 0; ct < NCT; ct++) sn[ct][0] = sn[ct][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+            __builtin_amdgcn_sched_barrier(0);
+            v8h n0, n1;
+            if (x + 1 < NS) {
+                n0 = kb[x + 1][l];
+                n1 = kb[NS + x + 1][l];
+            } else {
+                v0 = vb[0][l];
+                v1 = vb[1][l];
+            }
+#pragma unroll
+            for (int j = x * 2 * NCT / NS; j < (x + 1) * 2 * NCT / NS; j++)
+                sum[j >> 1][j & 1] = weigh_tile(s[j >> 1][j & 1], cs[j >> 1], base[j >> 1], W[j >> 1].hi + 2 * (j & 1),
+                                                W[j >> 1].lo + 2 * (j & 1));
+#pragma unroll
+            for (int ct = 0; ct < NCT; ct++) {
+                sn[ct][0] = mfma(k0, qlo[ct][x], sn[ct][0]);
+                sn[ct][1] = mfma(k1, qlo[ct][x], sn[ct][1]);
+            }
+#pragma unroll
+            for (int ct = 0; ct < NCT; ct++) {
+                sn[ct][0] = mfma(k0, qhi[ct][x], sn[ct][0]);
+                sn[ct][1] = mfma(k1, qhi[ct][x], sn[ct][1]);
+            }
+            alternate<4 * NCT, 3>();
+            k0 = n0;
+            k1 = n1;
+        }
+#pragma unroll
+        for (int ct = 0; ct < NCT; ct++) S[ct].l = __builtin_fmaf(sum[ct][0] + sum[ct][1], v.iv, S[ct].l);
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+            __builtin_amdgcn_sched_barrier(0);
+            v8h n0, n1;
+            if (x + 1 < NS) {
+                n0 = vb[2 * x + 2][l];
+                n1 = vb[2 * x + 3][l];
+            }
+            put(pb, raw, x);
+            if (x == NS - 1)
+#pragma unroll
+                for (int ct = 0; ct < NCT; ct++) top[ct] = largest(sn[ct][0], sn[ct][1]);
+#pragma unroll
+            for (int ct = 0; ct < NCT; ct++) {
+                S[ct].o[2 * x] = mfma(v0, W[ct].r(), S[ct].o[2 * x]);
+                S[ct].o[2 * x + 1] = mfma(v1, W[ct].r(), S[ct].o[2 * x + 1]);
+            }
+#pragma unroll
+            for (int ct = 0; ct < NCT; ct++) {
+                S[ct].o[2 * x] = mfma(v0, W[ct].h(), S[ct].o[2 * x]);
+                S[ct].o[2 * x + 1] = mfma(v1, W[ct].h(), S[ct].o[2 * x + 1]);
+            }
+            alternate<4 * NCT, 1>();
+            v0 = n0;
+            v1 = n1;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (p + 3 < p1) after = block_at(p + 3);
+        fetch(raw, after);
+        bi = b1;
         __syncthreads();
-        if (w < step)
-#pragma unroll
-            for (int x = 0; x < DP / 16; x++) S.o[x] += *(const v4f*)&os[w][col][16 * x + 4 * g];
-        __syncthreads();
+    };
+    for (int p = p0; p < p1; p += 2) {
+        step(p, sa, sb);
+        if (p + 1 < p1) step(p + 1, sb, sa);
     }
-    if (w != 0 || col >= ncol) return;
-    if (A.splits > 1) {
-        const int64_t rows = (int64_t)A.T * A.H, at = (int64_t)blockIdx.y * rows + head;
-        float2* pml = (float2*)(A.part + (int64_t)A.splits * rows * DP);
-        const bool none = p0 >= p1 || n == 0;
-        if (g == 0) pml[at] = make_float2(none ? -__builtin_inff() : M, L);
-        if (none) return;
+    const int64_t rows = (int64_t)A.T * A.H;
 #pragma unroll
-        for (int x = 0; x < DP / 16; x++) *(v4f*)(A.part + at * DP + 16 * x + 4 * g) = S.o[x];
-        return;
-    }
-    // a row that sees no key gives zeros, one whose weights are all zero NaN
-    const float inv = n == 0 ? 0.f : (L > 0.f ? 1.f / L : __builtin_nanf(""));
+    for (int ct = 0; ct < NCT; ct++) {
+        float L = S[ct].l + lane_xor_f32<16>(S[ct].l);
+        L += lane_xor_f32<32>(L);
+        const int c = WC * w + 16 * ct + col, head = (t0 + c / A.G) * A.H + hk * A.G + c % A.G;
+        if (c >= cols) continue;
+        const bool none = p0 >= p1 || R.kn[WC * w + 16 * ct + col].y <= 0;
+        if (A.splits > 1) {
+            const int64_t at = (int64_t)blockIdx.y * rows + head;
+            if (g == 0)
+                ((float2*)(A.part + (int64_t)A.splits * rows * DP))[at] = make_float2(none ? -__builtin_inff() : S[ct].M, L);
+            if (none) continue;
 #pragma unroll
-    for (int x = 0; x < DP / 16; x++) {
-        const int d0 = 16 * x + 4 * g;
-        if (d0 < A.d) *(f32x4a4*)(A.out + (int64_t)head * A.d + d0) = n == 0 ? v4f{0.f, 0.f, 0.f, 0.f} : S.o[x] * inv;
+            for (int x = 0; x < DP / 16; x++) *(v4f*)(A.part + at * DP + 16 * x + 4 * g) = S[ct].o[x];
+        } else {
+            const float inv = L > 0.f ? 1.f / L : __builtin_nanf("");
+#pragma unroll
+            for (int x = 0; x < DP / 16; x++) {
+                const int d0 = 16 * x + 4 * g;
+                if (d0 < A.d) *(f32x4a4*)(A.out + (int64_t)head * A.d + d0) = none ? v4f{0.f, 0.f, 0.f, 0.f} : S[ct].o[x] * inv;
+            }
+        }
     }
 }
 
-// The splits of a row joined: a wave per (token, head).
+// The splits of a row joined: a workgroup per (token, head), DP / 4 threads a
+// split, so 1024 / DP splits at a time.
 template <int DP>
 __global__ __launch_bounds__(256) void join_kernel(Args A) {
-    const int64_t rows = (int64_t)A.T * A.H, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int l = threadIdx.x & 63;
-    if (row >= rows) return;
+    constexpr int LANES = DP / 4, AT_ONCE = 256 / LANES;
+    __shared__ __align__(16) float os[AT_ONCE][DP];
+    const int64_t rows = (int64_t)A.T * A.H, row = blockIdx.x;
+    const int tid = threadIdx.x, l = tid & 63, u = tid / LANES, d4 = (tid - u * LANES) * 4;
     const float2* pml = (const float2*)(A.part + (int64_t)A.splits * rows * DP);
     const float2 x = l < A.splits ? pml[l * rows + row] : make_float2(-__builtin_inff(), 0.f);  // at most 64 splits
+    const bool none = x.x == -__builtin_inff();
     const float M = wave_max_f32(x.x);
-    const float wl = x.x == -__builtin_inff() ? 0.f : exp2_hw(x.x - M);
-    const float wh = exp2_hw(0.5f * (x.x - M));
-    const float L = wave_sum_f32(x.x == -__builtin_inff() ? 0.f : x.y * wh * wh);
-    const unsigned long long used = __ballot(x.x != -__builtin_inff());
-    float o[DP / 64];
-#pragma unroll
-    for (int j = 0; j < DP / 64; j++) o[j] = 0.f;
-    for (unsigned long long m = used; m; m &= m - 1) {
-        const int s = __builtin_ctzll(m);
-        const float f = __shfl(wl, s);
-        const float* p = A.part + ((int64_t)s * rows + row) * DP + l;
-#pragma unroll
-        for (int j = 0; j < DP / 64; j++) o[j] = __builtin_fmaf(f, p[64 * j], o[j]);
+    const float wh = none ? 0.f : exp2_hw(0.5f * (x.x - M));
+    const float L = wave_sum_f32(none ? 0.f : x.y * wh * wh);
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s0 = 0; s0 < A.splits; s0 += AT_ONCE) {
+        const int s = s0 + u;
+        const float f = __shfl(wh, s & 63);  // 0 where a split holds nothing: its sums are not read
+        if (u < AT_ONCE && s < A.splits && f != 0.f) o += *(const v4f*)(A.part + ((int64_t)s * rows + row) * DP + d4) * (f * f);
     }
-    const float inv = L > 0.f ? 1.f / L : __builtin_nanf("");
+    if (u < AT_ONCE) *(v4f*)&os[u][d4] = o;
+    __syncthreads();
+    if (tid >= A.d) return;
+    float v = 0.f;
 #pragma unroll
-    for (int j = 0; j < DP / 64; j++)
-        if (64 * j + l < A.d) A.out[row * A.d + 64 * j + l] = used ? o[j] * inv : 0.f;
+    for (int j = 0; j < AT_ONCE; j++) v += os[j][tid];
+    A.out[row * A.d + tid] = M == -__builtin_inff() ? 0.f : (L > 0.f ? v / L : __builtin_nanf(""));
 }
 
-// How a call is cut: columns a tile and splits of the keys.
+// How a call is cut.
 struct Cut {
-    int cpt, tiles, splits;
+    bool many;
+    int tpt, fan, least;
+    int64_t few_wgs, many_wgs;
+    int splits, few_splits;
 };
-Cut cut(int64_t T, int H, int Hkv, int64_t maxk) {
-    const int64_t G = H / Hkv, cols = T * G;
-    Cut c;
-    // few tokens: a tile per token, each with its own range of keys (a decode
-    // batch's sequences have none in common)
-    c.cpt = G <= COLS && T < 64 ? (int)G : COLS;
-    c.tiles = (int)((cols + c.cpt - 1) / c.cpt);
-    const int64_t wgs = (int64_t)c.tiles * Hkv, blocks = (maxk + Q8C_BLOCK - 1) / Q8C_BLOCK;
-    int64_t s = (1024 + wgs - 1) / wgs;
-    if (s > blocks / 8) s = blocks / 8;
-    c.splits = (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
+    const int64_t G = H / Hkv, subs = (G + COLS - 1) / COLS, blocks = (maxk + Q8C_BLOCK - 1) / Q8C_BLOCK;
+    const int64_t cols = d <= 128 ? MAX_COLS : MAX_COLS / 2;
+    // splits that give about 512 workgroups, of eight blocks and more
+    auto splits = [&](int64_t wgs) {
+        int64_t s = (512 + wgs - 1) / wgs;
+        if (s > blocks / 8) s = blocks / 8;
+        return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+    };
+    Cut c{};
+    // Prompts of many tokens are many_kernel's, a decode batch of as many
+    // sequences few_kernel's: the ranges, on the device, tell them apart, so
+    // both are launched, and each leaves the other's tiles (3 to 4 us). Alone,
+    // few_kernel is ahead below 96 tokens (d = 64 and 128, 8 kv heads, 64
+    // tokens: 22 and 30 us behind 2000 cached ones, many_kernel the same; 128
+    // tokens: 35 and 51 us against 27 and 33) and where the keys are few (512
+    // tokens, nothing cached: 30 and 44 us against 34 and 40; 1024: 79 and 122
+    // against 57 and 73). Below 192 tokens many_kernel is left the tiles that
+    // span 24 blocks and more (128 tokens, nothing cached: 7 and 10 us against
+    // 13 and 17).
+    c.least = T < 192 ? 24 : 0;
+    c.many = T >= 96 && G <= cols && blocks >= c.least && T * Hkv * subs * blocks * (d <= 64 ? 1 : 2) >= 1 << 17;
+    c.tpt = c.many ? (int)(cols / G) : 1;
+    const int64_t tiles = (T + c.tpt - 1) / c.tpt;
+    c.many_wgs = tiles * Hkv;
+    c.fan = 1;
+    if (c.many) {
+        const int64_t f = (512 + c.many_wgs * subs - 1) / (c.many_wgs * subs);
+        c.fan = (int)(f < c.tpt ? f : c.tpt);
+    }
+    c.few_wgs = tiles * c.fan * subs * Hkv;
+    c.few_splits = splits(T * subs * Hkv);
+    c.splits = c.many ? std::max(splits(c.many_wgs), c.few_splits) : c.few_splits;
     return c;
 }
 
 template <int DP>
 hipError_t launch(Args A, const Cut& c, hipStream_t s) {
-    A.cpt = c.cpt;
     A.splits = c.splits;
-    hipLaunchKernelGGL(few_kernel<DP>, dim3((unsigned)(c.tiles * A.Hkv), (unsigned)c.splits), dim3(256), 0, s, A);
+    A.few_splits = c.few_splits;
+    A.tpt = c.tpt;
+    A.fan = c.fan;
+    A.least = c.least;
+    A.choose = c.many ? 1 : 0;
+    hipLaunchKernelGGL(few_kernel<DP>, dim3((unsigned)c.few_wgs, (unsigned)c.few_splits), dim3(64 * NW), 0, s, A);
+    if (c.many)
+        hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.splits), dim3(256), 0, s, A);
     if (c.splits > 1)
-        hipLaunchKernelGGL(join_kernel<DP>, dim3((unsigned)(((int64_t)A.T * A.H + 3) / 4)), dim3(256), 0, s, A);
+        hipLaunchKernelGGL(join_kernel<DP>, dim3((unsigned)(A.T * A.H)), dim3(256), 0, s, A);
     return hipGetLastError();
 }
 
 }  // namespace aq
 
 uint64_t attention_q8_ws_bytes(int64_t T, int H, int Hkv, int d, int64_t maxk) {
-    const aq::Cut c = aq::cut(T, H, Hkv, maxk);
+    const aq::Cut c = aq::cut(T, H, Hkv, d, maxk);
     return c.splits > 1 ? (uint64_t)c.splits * (uint64_t)T * (uint64_t)H * (q8c_dp(d) + 2) * 4 : 0;
 }
 
@@ -406,7 +786,7 @@ hipError_t launch_attention_q8(const float* q, const void* cache, const int64_t*
     A.nb = q8c_blocks(C);
     A.out = out;
     A.part = ws;
-    const aq::Cut c = aq::cut(T, H, Hkv, maxk);
+    const aq::Cut c = aq::cut(T, H, Hkv, d, maxk);
     switch (q8c_dp(d)) {
     case 64: return aq::launch<64>(A, c, s);
     case 128: return aq::launch<128>(A, c, s);
