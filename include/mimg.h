@@ -535,8 +535,9 @@ int mimg_attention_dev(const float *q, const void *kcache, const void *vcache, c
  *
  * Layout, with DP = d rounded up to a multiple of 64 and NB =
  * ceil(context/32): [kv_heads][NB] records of 64*DP bytes, then
- * [kv_heads][NB] of {float key scale, float value scale, uint32 entries that
- * are not finite, uint32 0}. Value = (byte - 128) * scale. In a record, of
+ * [kv_heads][NB] of {float key scale, float value scale, uint32 keys that are
+ * not finite, uint32 values that are not}, bit e for entry e. Value = (byte -
+ * 128) * scale. In a record, of
  * entry e (0..31) and dim i:
  *   key   byte (((e/16)*(DP/64) + i/64)*64 + (i/16%4)*16 + e%16)*16 + i%16
  *   value byte 32*DP + ((i/32)*64 + (e/4%4)*16 + i%16)*16 + (i/16%2)*8 +

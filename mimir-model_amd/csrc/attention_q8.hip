@@ -162,11 +162,12 @@ __device__ __forceinline__ bool near_enough(float top, float M) { return top <= 
 template <int DP>
 __device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Q8Meta& m, float cs, Scale v, int blk, int g, int k0, int n,
                                          State<DP>& S) {
+    const uint32_t bad = m.bad();
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         float& x = j < 4 ? ((float*)&s0)[j] : ((float*)&s1)[j - 4];
         const int e = 16 * (j >> 2) + 4 * g + (j & 3);
-        if ((m.bad >> e) & 1) x = __builtin_nanf("");
+        if ((bad >> e) & 1) x = __builtin_nanf("");
         if ((unsigned)(Q8C_BLOCK * blk + e - k0) >= (unsigned)n) x = -__builtin_inff();
     }
     const float mx = largest(s0, s1) * cs + v.lv;
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         const Scale v = value_scale(mb);
         const float cs = key_scale(rs.scale, mb);
         float base = v.lv - S.M + 8.f;
-        if (!all_seen || mb.bad || !(mb.vs > 0.f) || !__all(near_enough(largest(s[0], s[1]) * cs + v.lv, S.M)))
+        if (!all_seen || mb.bad() || !(mb.vs > 0.f) || !__all(near_enough(largest(s[0], s[1]) * cs + v.lv, S.M)))
             base = correct<DP>(s[0], s[1], mb, cs, v, blk, g, k0, n, S);
         Weights W;
         const float sum = weigh_tile(s[0], cs, base, W.hi, W.lo) + weigh_tile(s[1], cs, base, W.hi + 2, W.lo + 2);
@@ -564,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
             fine &= near_enough(top[ct] * cs[ct] + v.lv, S[ct].M);
             base[ct] = v.lv - S[ct].M + 8.f;
         }
-        if (!(Q8C_BLOCK * here >= from && Q8C_BLOCK * (here + 1) <= to && m.bad == 0 && m.vs > 0.f && __all(fine))) {
+        if (!(Q8C_BLOCK * here >= from && Q8C_BLOCK * (here + 1) <= to && m.bad() == 0 && m.vs > 0.f && __all(fine))) {
 #pragma unroll
             for (int ct = 0; ct < NCT; ct++) {
                 const int2 k = R.kn[WC * w + 16 * ct + col];

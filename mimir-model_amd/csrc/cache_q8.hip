@@ -3,13 +3,14 @@
 // A store of T rows touches some blocks; the new scale of a block and kv head
 // is s = max(s_old, amax / 127) over the finite new values (s_old = 0 where
 // the block's first entry is among the rows: the block begins anew), and an
-// entry is rint(x / s), ties to even, decided in 64 bits. Where s grew, the
+// entry is rint(x / s), ties to even, of the exact quotient. Where s grew, the
 // entries that stay are requantized, rint(q * s_old / s).
 //
-// A workgroup per (row, kv head) looks through the rows' indices; that of a
-// block's first row takes all of the block's rows (of two with one index the
-// last), the others end at once, mostly on their left neighbour's index. So a
-// block is written by one workgroup and the result does not depend on order.
+// A workgroup per (row or a few, kv head, keys or values) looks through the
+// rows' indices; that of a block's first row takes all of the block's rows (of
+// two with one index the last), the others end at once, mostly on their left
+// neighbour's index. So a block is written by one workgroup and the result
+// does not depend on order.
 #include "cache_q8.hpp"
 #include "mimg_device.hpp"
 #include "decoder_math.hpp"
@@ -27,6 +28,7 @@ struct StoreArgs {
     const int64_t *index, *pos;
     const double* inv_freq;
     int T, H, Hkv, d, rotary, interleaved;
+    int each;  // rows a workgroup looks at
     int64_t C, nb;
     uint8_t* cache;
 };
@@ -51,156 +53,216 @@ __device__ __forceinline__ void turn(float& xa, float& xb, int64_t pos, double i
 
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// rint(x / s) + 128 for |x / s| <= 127 but for the scale's rounding; s = 0: zero.
-__device__ __forceinline__ uint32_t q8_byte(double x, double s) {
-    const double r = s > 0.0 ? __builtin_rint(x / s) : 0.0;
-    return (uint32_t)((int)fmin(fmax(r, -127.0), 127.0) + 128);
+// rint(x / s) + 128, ties to even, of the exact quotient, for |x / s| < 128:
+// r is x times s's float32 reciprocal, within 2^-15 of the quotient (three
+// roundings of 2^-24, |r| < 128), so with f = floor(r) the quotient rounds to f
+// or f + 1, and the sign of x - (f + 1/2) s says which: a fused multiply-add's
+// sign is exact (x and s are whole multiples of 2^-149).
+__device__ __forceinline__ uint32_t q8_round(float f, float sign) {
+    const float h = f + 0.5f;
+    const float n = sign > 0.f ? f + 1.f : (sign < 0.f ? f : __builtin_rintf(h));
+    return (uint32_t)((int)fminf(fmaxf(n, -127.f), 127.f) + 128);
+}
+__device__ __forceinline__ uint32_t q8_new(float x, float inv, float s) {
+    const float f = __builtin_floorf(x * inv);
+    return q8_round(f, __builtin_fmaf(-(f + 0.5f), s, x));
+}
+// The same for x = q * was, an integer times the old scale. (f + 1/2) s = p + e;
+// near p the difference q * was - p is exact (32-bit products, above 2^-25 of
+// them), farther off its sign is plain.
+__device__ __forceinline__ uint32_t q8_again(float q, float was, float ratio, float s) {
+    const float f = __builtin_floorf(q * ratio), h = f + 0.5f;
+    const float p = h * s, e = __builtin_fmaf(h, s, -p);
+    return q8_round(f, __builtin_fmaf(q, was, -p) - e);
 }
 
 template <int DP, bool ROPE>
 __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
-    constexpr int NP = DP / 16;  // pairs of a row that one of its eight threads holds
-    constexpr int HALF = Q8C_BLOCK * DP;
+    constexpr int NP = DP / 16;  // pairs of dims that a thread holds
+    constexpr int HALF = Q8C_BLOCK * DP, WORDS = (HALF / 16 + 255) / 256;
     __shared__ __align__(16) uint8_t image[HALF];
     __shared__ int rows[Q8C_BLOCK];
-    __shared__ float part[2][4];
+    __shared__ int2 list[Q8C_BLOCK];  // the entries to store and their rows
+    __shared__ float part[4];
     __shared__ uint32_t newbad;
     __shared__ int earlier;
-    const int t = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x;
+    const int tid = threadIdx.x, y = blockIdx.y, hk = y >> 1, half = y & 1;
+    int np = A.d / 2;
+    const int t0 = blockIdx.x * A.each;
     if constexpr (ROPE) {
-        if (hk >= A.Hkv) {  // the workgroups behind the kv heads' turn q
-            const int n = A.H * (A.d / 2);
-            for (int j = (hk - A.Hkv) * 256 + tid; j < n; j += ((int)gridDim.y - A.Hkv) * 256) {
-                const int h = j / (A.d / 2);
-                const Pair p = pair_of(j - h * (A.d / 2), A.rotary, A.interleaved);
-                if (!p.rot) continue;
-                float* r = A.q + ((int64_t)t * A.H + h) * A.d;
-                float xa = r[p.a], xb = r[p.b];
-                turn(xa, xb, A.pos[t], A.inv_freq[A.interleaved ? p.a / 2 : p.a]);
-                r[p.a] = xa;
-                r[p.b] = xb;
-            }
+        if (y >= 2 * A.Hkv) {  // the workgroups behind the kv heads' turn q
+            const int n = A.H * np, qw = (int)gridDim.y - 2 * A.Hkv;
+            for (int t = t0; t < min(A.T, t0 + A.each); t++)
+                for (int j = (y - 2 * A.Hkv) * 256 + tid; j < n; j += qw * 256) {
+                    const int h = j / np;
+                    const Pair p = pair_of(j - h * np, A.rotary, A.interleaved);
+                    if (!p.rot) continue;
+                    float* r = A.q + ((int64_t)t * A.H + h) * A.d;
+                    float xa = r[p.a], xb = r[p.b];
+                    turn(xa, xb, A.pos[t], A.inv_freq[A.interleaved ? p.a / 2 : p.a]);
+                    r[p.a] = xa;
+                    r[p.b] = xb;
+                }
             return;
         }
     }
-    const int64_t at = A.index[t];
-    if (at < 0 || at >= A.C) return;  // outside the cache: not stored
-    const int64_t blk = at >> 5;
-    // (an index outside the cache may lie in its last, partial block)
-    auto in_block = [&](int64_t i) { return i >= 0 && i < A.C && (i >> 5) == blk; };
-    if (t > 0 && in_block(A.index[t - 1])) return;
-    if (tid < Q8C_BLOCK) rows[tid] = -1;
-    if (tid == 0) {
-        newbad = 0;
-        earlier = 0;
-    }
-    __syncthreads();
-    for (int i = tid; i < A.T; i += 256) {
-        const int64_t x = A.index[i];
-        if (!in_block(x)) continue;
-        if (i < t) earlier = 1;
-        else atomicMax(&rows[x & (Q8C_BLOCK - 1)], i);
-    }
-    __syncthreads();
-    if (earlier) return;
-
-    // eight threads an entry: thread c holds its pairs c, c + 8, ...
-    const int e = tid >> 3, c = tid & 7, row = rows[e], np = A.d / 2;
-    const bool fresh = rows[0] >= 0;
-    float kx[2 * NP], vx[2 * NP];
-    float kmax = 0.f, vmax = 0.f;
-    bool bad = false;
+    const int64_t first = tid < A.T ? A.index[tid] : -1;
+    // Lane j: row t0 + j and the one before it. The rows that may be a block's
+    // first (outside the cache: not stored).
+    const int tl = t0 + (tid & 63);
+    const bool look_at = tl < A.T && (tid & 63) < A.each;
+    const int64_t mine = look_at ? A.index[tl] : -1, left = look_at && tl > 0 ? A.index[tl - 1] : -1;
+    const bool inside = mine >= 0 && mine < A.C;
+    unsigned long long todo = __ballot(inside && !(left >= 0 && left < A.C && (left >> 5) == (mine >> 5)));
+    for (; todo; todo &= todo - 1) {
+        const int j0 = __builtin_ctzll(todo), t = t0 + j0;
+        const int64_t at = __shfl(mine, j0), blk = at >> 5;
+        // (an index outside the cache may lie in its last, partial block)
+        auto in_block = [&](int64_t i) { return i >= 0 && i < A.C && (i >> 5) == blk; };
+        uint8_t* dst = A.cache + q8c_record(A.nb, hk, blk, DP) + half * HALF;
+        Q8Meta* mp = (Q8Meta*)(A.cache + q8c_meta(A.nb, A.Hkv, hk, blk, DP));
+        // what is held, on its way unless this row begins the block anew
+        u32x4 held[WORDS];
+        float was = 0.f;
+        uint32_t wasbad = 0;
+        if ((at & 31) != 0) {
 #pragma unroll
-    for (int j = 0; j < NP; j++) {
-        const int i = c + 8 * j;
-        kx[2 * j] = kx[2 * j + 1] = vx[2 * j] = vx[2 * j + 1] = 0.f;
-        if (row < 0 || i >= np) continue;
-        const float* kr = A.k + ((int64_t)row * A.Hkv + hk) * A.d;
-        const f32x2a4 v = *(const f32x2a4*)(A.v + ((int64_t)row * A.Hkv + hk) * A.d + 2 * i);
-        float ka, kb;
-        if constexpr (ROPE) {
-            const Pair p = pair_of(i, A.rotary, A.interleaved);
-            ka = kr[p.a];
-            kb = kr[p.b];
-            if (p.rot) turn(ka, kb, A.pos[row], A.inv_freq[i]);
-        } else {
-            ka = kr[2 * i];
-            kb = kr[2 * i + 1];
+            for (int i = 0; i < WORDS; i++)
+                if (tid + 256 * i < HALF / 16) held[i] = ((const u32x4*)dst)[tid + 256 * i];
+            was = half ? mp->vs : mp->ks;
+            wasbad = half ? mp->vbad : mp->kbad;
         }
-        bad |= !(finite_bits(ka) && finite_bits(kb) && finite_bits(v.x) && finite_bits(v.y));
-        kx[2 * j] = finite_bits(ka) ? ka : 0.f;
-        kx[2 * j + 1] = finite_bits(kb) ? kb : 0.f;
-        vx[2 * j] = finite_bits(v.x) ? v.x : 0.f;
-        vx[2 * j + 1] = finite_bits(v.y) ? v.y : 0.f;
-        kmax = fmaxf(kmax, fmaxf(__builtin_fabsf(kx[2 * j]), __builtin_fabsf(kx[2 * j + 1])));
-        vmax = fmaxf(vmax, fmaxf(__builtin_fabsf(vx[2 * j]), __builtin_fabsf(vx[2 * j + 1])));
-    }
-    if (bad) atomicOr(&newbad, 1u << e);
-    kmax = wave_max_f32(kmax);
-    vmax = wave_max_f32(vmax);
-    if ((tid & 63) == 0) {
-        part[0][tid >> 6] = kmax;
-        part[1][tid >> 6] = vmax;
-    }
-    __syncthreads();
-    const int dp = DP;
-    Q8Meta* mp = (Q8Meta*)(A.cache + q8c_meta(A.nb, A.Hkv, hk, blk, dp));
-    const Q8Meta old = *mp;
-    uint32_t stored = 0;
-    for (int i = 0; i < Q8C_BLOCK; i++) stored |= rows[i] >= 0 ? 1u << i : 0u;
-    Q8Meta now;
-    now.bad = (fresh ? 0u : old.bad & ~stored) | newbad;
-    now.zero = 0;
-    uint8_t* rec = A.cache + q8c_record(A.nb, hk, blk, dp);
+        __syncthreads();  // (the last block is done)
+        if (tid < Q8C_BLOCK) rows[tid] = -1;
+        if (tid == 0) {
+            newbad = 0;
+            earlier = 0;
+        }
+        __syncthreads();
+        auto look = [&](int i, int64_t x) {
+            if (!in_block(x)) return;
+            if (i < t) earlier = 1;
+            else atomicMax(&rows[x & (Q8C_BLOCK - 1)], i);
+        };
+        if (tid < A.T) look(tid, first);
+        for (int i = tid + 256; i < A.T; i += 8 * 256) {
+            int64_t x[8];
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-        const float* pm = part[half];
-        const float amax = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
-        const float was = fresh ? 0.f : (half ? old.vs : old.ks);
-        const float need = amax > 0.f ? fmaxf(amax / 127.f, Q8C_FLOOR) : 0.f;
-        const float s = fmaxf(was, need);
-        (half ? now.vs : now.ks) = s;
-        uint8_t* dst = rec + half * HALF;
+            for (int j = 0; j < 8; j++) x[j] = i + 256 * j < A.T ? A.index[i + 256 * j] : -1;
+#pragma unroll
+            for (int j = 0; j < 8; j++) look(i + 256 * j, x[j]);
+        }
+        __syncthreads();
+        if (earlier) continue;
+        const bool used = (tid & 63) < Q8C_BLOCK && rows[tid & 31] >= 0;
+        const uint32_t stored = (uint32_t)__ballot(used);
+        if (tid < 64 && used) list[__popc(stored & ((1u << tid) - 1))] = make_int2(tid, rows[tid]);
+        __syncthreads();
+        const bool fresh = stored & 1;
+        asm volatile("" : "+s"(np));  // (the items' places are not kept in registers over the blocks)
+        const int items = __popc(stored) * np;
+        uint32_t inv_np = ((1u << 20) + np - 1) / np;  // items / np: at most 4096 items
+        float xs[2 * NP];
+        float amax = 0.f;
+        // (all loads on their way before the first is used)
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+            const int it = tid + 256 * j;
+            xs[2 * j] = xs[2 * j + 1] = 0.f;
+            if (it < items) {
+                const int u = (int)(((uint32_t)it * inv_np) >> 20), i = it - u * np;
+                const int64_t row = ((int64_t)list[u].y * A.Hkv + hk) * A.d;
+                if (ROPE && half == 0) {
+                    const Pair p = pair_of(i, A.rotary, A.interleaved);
+                    xs[2 * j] = A.k[row + p.a];
+                    xs[2 * j + 1] = A.k[row + p.b];
+                } else {
+                    const f32x2a4 v = *(const f32x2a4*)((half ? A.v : A.k) + row + 2 * i);
+                    xs[2 * j] = v.x;
+                    xs[2 * j + 1] = v.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+            const int it = tid + 256 * j;
+            if (it >= items) continue;
+            float &xa = xs[2 * j], &xb = xs[2 * j + 1];
+            if (ROPE && half == 0) {
+                const int u = (int)(((uint32_t)it * inv_np) >> 20), i = it - u * np;
+                if (pair_of(i, A.rotary, A.interleaved).rot) turn(xa, xb, A.pos[list[u].y], A.inv_freq[i]);
+            }
+            if (!(finite_bits(xa) && finite_bits(xb))) {
+                atomicOr(&newbad, 1u << list[(uint32_t)it * inv_np >> 20].x);
+                xa = finite_bits(xa) ? xa : 0.f;
+                xb = finite_bits(xb) ? xb : 0.f;
+            }
+            amax = fmaxf(amax, fmaxf(__builtin_fabsf(xa), __builtin_fabsf(xb)));
+        }
+        amax = wave_max_f32(amax);
+        if ((tid & 63) == 0) part[tid >> 6] = amax;
+        __syncthreads();
+        amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        if (fresh) was = 0.f;
+        const float need = amax > 0.f ? fmaxf(amax / 127.f, Q8C_FLOOR) : 0.f, s = fmaxf(was, need);
+        const float inv = s > 0.f ? 1.f / s : 0.f;
         const bool whole = fresh || need > was;  // the other entries change too
         if (whole) {
-            for (int i = tid; i < HALF / 16; i += 256) {
-                u32x4 w = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
-                if (!fresh) {
-                    w = ((const u32x4*)dst)[i];
+            const float ratio = was * inv;
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) {
+                if (tid + 256 * i >= HALF / 16) break;
+                u32x4 w4 = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+                if (!fresh && was > 0.f) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         uint32_t r = 0;
+#pragma unroll
                         for (int b = 0; b < 4; b++) {
-                            const int qv = (int)((w[j] >> (8 * b)) & 255u) - 128;
-                            r |= q8_byte((double)qv * (double)was, (double)s) << (8 * b);
+                            const float qv = (float)((held[i][j] >> (8 * b)) & 255u) - 128.f;
+                            r |= q8_again(qv, was, ratio, s) << (8 * b);
                         }
-                        w[j] = r;
+                        w4[j] = r;
                     }
                 }
-                ((u32x4*)image)[i] = w;
+                ((u32x4*)image)[tid + 256 * i] = w4;
             }
             __syncthreads();
         }
-        uint8_t* to = whole ? image : dst;
-        if (row >= 0) {
+        asm volatile("" : "+s"(inv_np));
+        // an item's two bytes into the image, or straight into the record
+        auto put = [&](uint8_t* to, int j) {
+            const int it = tid + 256 * j;
+            if (it >= items) return;
+            const int u = (int)(((uint32_t)it * inv_np) >> 20), i = it - u * np, e = list[u].x;
+            const Pair p = ROPE && half == 0 ? pair_of(i, A.rotary, A.interleaved) : Pair{2 * i, 2 * i + 1, false};
+            to[half ? q8c_vbyte(e, p.a) : q8c_kbyte(e, p.a, DP)] = (uint8_t)q8_new(xs[2 * j], inv, s);
+            to[half ? q8c_vbyte(e, p.b) : q8c_kbyte(e, p.b, DP)] = (uint8_t)q8_new(xs[2 * j + 1], inv, s);
+        };
+        if (whole) {
 #pragma unroll
-            for (int j = 0; j < NP; j++) {
-                const int i = c + 8 * j;
-                if (i >= np) continue;
-                Pair p = {2 * i, 2 * i + 1, false};
-                if (ROPE && half == 0) p = pair_of(i, A.rotary, A.interleaved);
-                const float xa = half ? vx[2 * j] : kx[2 * j], xb = half ? vx[2 * j + 1] : kx[2 * j + 1];
-                to[half ? q8c_vbyte(e, p.a) : q8c_kbyte(e, p.a, dp)] = (uint8_t)q8_byte((double)xa, (double)s);
-                to[half ? q8c_vbyte(e, p.b) : q8c_kbyte(e, p.b, dp)] = (uint8_t)q8_byte((double)xb, (double)s);
-            }
+            for (int j = 0; j < NP; j++) put(image, j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NP; j++) put(dst, j);
         }
         if (whole) {
             __syncthreads();
-            for (int i = tid; i < HALF / 16; i += 256) ((u32x4*)dst)[i] = ((const u32x4*)image)[i];
-            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WORDS; i++)
+                if (tid + 256 * i < HALF / 16) ((u32x4*)dst)[tid + 256 * i] = ((const u32x4*)image)[tid + 256 * i];
+        }
+        if (tid == 0) {
+            const uint32_t bad = (fresh ? 0u : wasbad & ~stored) | newbad;
+            if (half) {
+                mp->vs = s;
+                mp->vbad = bad;
+            } else {
+                mp->ks = s;
+                mp->kbad = bad;
+            }
         }
     }
-    if (tid == 0) *mp = now;
 }
 
 // Entries index[t] as float32 rows [T, Hkv, d]: value * scale; zeros outside
@@ -226,7 +288,7 @@ __global__ __launch_bounds__(256) void load_q8_kernel(const uint8_t* __restrict_
             for (int j = 0; j < 4; j++) {
                 ko[j] = (float)((int)((kw >> (8 * j)) & 255u) - 128) * m.ks;
                 vo[j] = (float)((int)vp[q8c_vbyte(e, dd + j)] - 128) * m.vs;
-                if ((m.bad >> e) & 1) ko[j] = vo[j] = __builtin_nanf("");
+                if ((m.bad() >> e) & 1) ko[j] = vo[j] = __builtin_nanf("");
             }
         }
         *(f32x4a4*)(k + i * 4) = ko;
@@ -235,10 +297,13 @@ __global__ __launch_bounds__(256) void load_q8_kernel(const uint8_t* __restrict_
 }
 
 template <bool ROPE>
-hipError_t launch_store(const StoreArgs& a, hipStream_t s) {
-    // q: a few hundred pairs a workgroup (each takes a 64-bit sine and cosine)
+hipError_t launch_store(StoreArgs a, hipStream_t s) {
+    // One row a workgroup for a decode batch, whose rows are a block each;
+    // several of a prompt, of which one in 32 begins a block.
+    a.each = a.T <= 128 ? 1 : (a.T <= 2048 ? 16 : 32);
+    // q: a pair a thread (each takes a 64-bit sine and cosine)
     const int qw = ROPE ? (a.H * (a.d / 2) + 255) / 256 : 0;
-    const dim3 grid((unsigned)a.T, (unsigned)(a.Hkv + qw));
+    const dim3 grid((unsigned)((a.T + a.each - 1) / a.each), (unsigned)(2 * a.Hkv + qw));
     switch (q8c_dp(a.d)) {
     case 64: hipLaunchKernelGGL((store_q8_kernel<64, ROPE>), grid, dim3(256), 0, s, a); break;
     case 128: hipLaunchKernelGGL((store_q8_kernel<128, ROPE>), grid, dim3(256), 0, s, a); break;

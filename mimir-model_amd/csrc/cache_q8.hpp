@@ -26,11 +26,12 @@ constexpr int Q8C_MAX_D = 256;
 // weights of 2^15 times it stay in float32's range.
 #define Q8C_FLOOR 0x1p-96f
 
-// A block's scales; bit e of bad: entry e had a key or value that is not
-// finite (stored as zeros; what sees it gets NaN).
+// A block's scales; bit e of kbad (vbad): entry e has a key (value) that is not
+// finite (stored as zero; what sees it gets NaN).
 struct __align__(16) Q8Meta {
     float ks, vs;
-    uint32_t bad, zero;
+    uint32_t kbad, vbad;
+    __device__ __forceinline__ uint32_t bad() const { return kbad | vbad; }
 };
 
 __host__ __device__ __forceinline__ int q8c_dp(int d) { return (d + 63) & ~63; }

@@ -584,23 +584,33 @@ def unpack_cache_q8(raw, kv_heads, context, d):
     k, v = (np.ascontiguousarray((b.reshape(kv_heads, nb * 32, dp)[:, :context, :d].astype(np.int16) - 128).astype(np.int8))
             for b in (kb, vb))
     scales = np.ascontiguousarray(meta).view(np.float32)
-    return k, scales[..., 0].copy(), v, scales[..., 1].copy(), meta[..., 2].copy()
+    return k, scales[..., 0].copy(), v, scales[..., 1].copy(), meta[..., 2] | meta[..., 3]
 
+
+# (These take addresses as they are, ints or None: argtypes convert them.)
 
 def kv_store_q8_dev(k_ptr, v_ptr, cidx_ptr, T, kv_heads, d, context, cache_ptr, stream):
-    _check(load().mimg_kv_store_q8_dev(_P(k_ptr), _P(v_ptr), _P(cidx_ptr), T, kv_heads, d, context, _P(cache_ptr),
-                                       _P(stream)))
+    """float32 rows k, v [T, kv_heads, d] into the entries cidx of an 8-bit
+    cache (mimg_kv_store_q8_dev)."""
+    rc = load().mimg_kv_store_q8_dev(k_ptr, v_ptr, cidx_ptr, T, kv_heads, d, context, cache_ptr, stream)
+    if rc:
+        _check(rc)
 
 
 def rope_kv_q8_dev(q_ptr, k_ptr, v_ptr, pos_ptr, cidx_ptr, inv_freq_ptr, T, heads, kv_heads, d, rotary, interleaved,
                    context, cache_ptr, stream):
-    _check(load().mimg_rope_kv_q8_dev(_P(q_ptr), _P(k_ptr), _P(v_ptr), _P(pos_ptr), _P(cidx_ptr), _P(inv_freq_ptr), T,
-                                      heads, kv_heads, d, rotary, int(interleaved), context, _P(cache_ptr), _P(stream)))
+    """rope_dev on q and k and kv_store_q8_dev, in one launch, bit for bit."""
+    rc = load().mimg_rope_kv_q8_dev(q_ptr, k_ptr, v_ptr, pos_ptr, cidx_ptr, inv_freq_ptr, T, heads, kv_heads, d, rotary,
+                                    int(interleaved), context, cache_ptr, stream)
+    if rc:
+        _check(rc)
 
 
 def kv_load_q8_dev(cache_ptr, cidx_ptr, T, kv_heads, d, context, k_ptr, v_ptr, stream):
-    _check(load().mimg_kv_load_q8_dev(_P(cache_ptr), _P(cidx_ptr), T, kv_heads, d, context, _P(k_ptr), _P(v_ptr),
-                                      _P(stream)))
+    """Entries cidx of an 8-bit cache as float32 rows (mimg_kv_load_q8_dev)."""
+    rc = load().mimg_kv_load_q8_dev(cache_ptr, cidx_ptr, T, kv_heads, d, context, k_ptr, v_ptr, stream)
+    if rc:
+        _check(rc)
 
 
 def attention_q8_workspace_bytes(T, heads, kv_heads, d, max_keys):
@@ -610,8 +620,10 @@ def attention_q8_workspace_bytes(T, heads, kv_heads, d, max_keys):
 def attention_q8_dev(q_ptr, cache_ptr, kend_ptr, kstart_ptr, T, heads, kv_heads, d, context, max_keys, out_ptr, ws_ptr,
                      ws_bytes, stream):
     """Attention over an 8-bit cache, to float32 accuracy (mimg_attention_q8_dev)."""
-    _check(load().mimg_attention_q8_dev(_P(q_ptr), _P(cache_ptr), _P(kend_ptr), _o(kstart_ptr), T, heads, kv_heads, d,
-                                        context, max_keys, _P(out_ptr), _o(ws_ptr), ws_bytes, _P(stream)))
+    rc = load().mimg_attention_q8_dev(q_ptr, cache_ptr, kend_ptr, kstart_ptr, T, heads, kv_heads, d, context, max_keys,
+                                      out_ptr, ws_ptr, ws_bytes, stream)
+    if rc:
+        _check(rc)
 
 
 def logprobs_workspace_bytes(rows, n, top):
@@ -623,8 +635,10 @@ def logprobs_dev(x_ptr, rows, n, ld, targets_ptr, top, logprob_ptr, entropy_ptr,
     """Log probabilities of the targets, the entropy and the `top` largest
     alternatives of each row of logits (mimg_logprobs_dev); outputs that are
     None are not written."""
-    _check(load().mimg_logprobs_dev(_P(x_ptr), rows, n, ld, _o(targets_ptr), top, _o(logprob_ptr), _o(entropy_ptr),
-                                    _o(top_ids_ptr), _o(top_logprobs_ptr), _o(ws_ptr), ws_bytes, _P(stream)))
+    rc = load().mimg_logprobs_dev(x_ptr, rows, n, ld, targets_ptr, top, logprob_ptr, entropy_ptr, top_ids_ptr,
+                                  top_logprobs_ptr, ws_ptr, ws_bytes, stream)
+    if rc:
+        _check(rc)
 
 
 def greedy_advance_dev(chosen_ptr, ids_ptr, pos_ptr, cidx_ptr, out_ptr, count_ptr, cap, n, stream):
