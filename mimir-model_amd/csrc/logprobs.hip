@@ -8,7 +8,7 @@
 // chunk_kernel: a workgroup holds CHUNK logits of a row in registers, so the
 // maximum, the sums and the alternatives take one read. The alternatives: of
 // the 256 threads' maxima the k-th largest, tau, is at most the k-th largest
-// value, and only the fewer than k threads above it hold larger ones: the
+// value, and only the at most k threads not below it hold larger ones: the
 // values above tau, and as many equal to it as are missing (lowest indices),
 // go to LDS as 64-bit keys (value, ~index) and are ranked by counting.
 // merge_kernel: a workgroup a row joins the chunks.
@@ -50,12 +50,21 @@ struct Args {
     uint64_t* keys;  // [rows][chunks][top], largest first, 0 past the last
 };
 
-// Keys cand[0..c) in LDS: the `top` largest, in order, into out (0 past c).
-__device__ __forceinline__ void ranked(const uint64_t* cand, int c, int top, uint64_t* out) {
+// Keys cand[0..c) in LDS: the `top` largest, in order, into out (0 past c). Eight
+// are read at a time; cand has room for seven more than c.
+__device__ __forceinline__ void ranked(uint64_t* cand, int c, int top, uint64_t* out) {
+    if (threadIdx.x < 7) cand[c + threadIdx.x] = 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < c; i += 256) {
         const uint64_t k = cand[i];
         int r = 0;
-        for (int j = 0; j < c; j++) r += cand[j] > k ? 1 : 0;
+        for (int j = 0; j < c; j += 8) {
+            uint64_t o[8];
+#pragma unroll
+            for (int b = 0; b < 8; b++) o[b] = cand[j + b];
+#pragma unroll
+            for (int b = 0; b < 8; b++) r += o[b] > k ? 1 : 0;
+        }
         if (r < top) out[r] = k;
     }
     for (int i = c + (int)threadIdx.x; i < top; i += 256) out[i] = 0;
@@ -64,10 +73,10 @@ __device__ __forceinline__ void ranked(const uint64_t* cand, int c, int top, uin
 __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
     __shared__ float red[3][4];
     __shared__ uint32_t tmax[256];
-    __shared__ uint64_t cand[(KMAX - 1) * 4 * VEC + KMAX];
-    __shared__ int cnt[4];
+    __shared__ uint64_t cand[KMAX * 4 * VEC + KMAX + 7];
+    __shared__ int cnt[4], steps[VEC];
     __shared__ uint32_t tau_s;
-    __shared__ int ncand;
+    __shared__ int ncand, nequal;
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63;
     const int row = blockIdx.x / (unsigned)A.chunks, chunk = blockIdx.x - row * A.chunks;
     const float* xr = A.x + (int64_t)row * A.ld;
@@ -77,7 +86,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
     for (int j = 0; j < VEC; j++) {
         const int i = i0 + 1024 * j;
         if (i + 4 <= A.n) {
-            const f32x4a4 v = *(const f32x4a4*)(xr + i);
+            const f32x4a4 v = __builtin_nontemporal_load((const f32x4a4*)(xr + i));
 #pragma unroll
             for (int b = 0; b < 4; b++) x[4 * j + b] = v[b];
         } else {
@@ -90,7 +99,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
     for (int j = 0; j < 4 * VEC; j++) mx = fmaxf(mx, x[j]);
     const float wm = wave_max_f32(mx);
     if (l == 0) red[0][w] = wm;
-    if (tid == 0) ncand = 0;
+    if (tid == 0) ncand = nequal = 0;
     // the thread's largest value as a number; 0 where it holds no logit
     tmax[tid] = i0 < A.n ? order_of(mx) : 0u;
     __syncthreads();
@@ -110,7 +119,8 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
         red[2][w] = t;
     }
     if (A.top > 0 && w == 0) {
-        // tau: the k-th largest of the threads' maxima, bit by bit
+        // tau: the k-th largest of the threads' maxima, bit by bit, or as soon as
+        // k of them are not below it
         const uint32_t a = tmax[l], b = tmax[64 + l], c = tmax[128 + l], d = tmax[192 + l];
         uint32_t tau = 0;
         for (int bit = 31; bit >= 0; bit--) {
@@ -118,6 +128,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
             const int n = __popcll(__ballot(a >= y)) + __popcll(__ballot(b >= y)) + __popcll(__ballot(c >= y)) +
                           __popcll(__ballot(d >= y));
             if (n >= A.top) tau = y;
+            if (n == A.top) break;
         }
         if (l == 0) tau_s = tau;
     }
@@ -138,59 +149,62 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
     auto key = [&](int j) {
         return (uint64_t)order_of(x[j]) << 32 | (uint32_t)~(uint32_t)(i0 + 1024 * (j >> 2) + (j & 3));
     };
-    int eq = 0;
+    int mine = 0, eq = 0;
     if (mx >= tf) {
 #pragma unroll
         for (int j = 0; j < 4 * VEC; j++) {
-            if (x[j] > tf) cand[atomicAdd(&ncand, 1)] = key(j);
-            else if (x[j] == tf && i0 + 1024 * (j >> 2) + (j & 3) < A.n) eq++;
+            mine += x[j] > tf ? 1 : 0;
+            eq += x[j] == tf && i0 + 1024 * (j >> 2) + (j & 3) < A.n ? 1 : 0;
         }
-    }
-    // how many equal tau over the workgroup
-    int v = eq;
-    v += lane_xor<32>(v);
-    v += lane_xor<16>(v);
-    v += lane_xor<8>(v);
-    v += lane_xor<4>(v);
-    v += lane_xor<2>(v);
-    v += lane_xor<1>(v);
-    if (l == 0) cnt[w] = v;
-    __syncthreads();
-    const int need = A.top - ncand, have = cnt[0] + cnt[1] + cnt[2] + cnt[3];
-    __syncthreads();
-    if (need > 0 && have > 0) {
-        // those equal to tau up to index `upto`: all, or the lowest `need`
-        int upto = 0x7fffffff;
-        if (have > need) {
-            upto = chunk * CHUNK - 1;
-            for (int step = CHUNK; step >= 1; step >>= 1) {
-                const int y = upto + step;  // are fewer than `need` at or below y?
-                int q = 0;
-                if (eq)
+        if (mine) {
+            int at = atomicAdd(&ncand, mine);
 #pragma unroll
-                    for (int j = 0; j < 4 * VEC; j++) {
-                        const int i = i0 + 1024 * (j >> 2) + (j & 3);
-                        q += x[j] == tf && i < A.n && i <= y ? 1 : 0;
-                    }
-                q += lane_xor<32>(q);
-                q += lane_xor<16>(q);
-                q += lane_xor<8>(q);
-                q += lane_xor<4>(q);
-                q += lane_xor<2>(q);
-                q += lane_xor<1>(q);
-                if (l == 0) cnt[w] = q;
-                __syncthreads();
-                if (cnt[0] + cnt[1] + cnt[2] + cnt[3] < need) upto = y;
-                __syncthreads();
-            }
-            upto++;  // the index of the need-th
+            for (int j = 0; j < 4 * VEC; j++)
+                if (x[j] > tf) cand[at++] = key(j);
         }
+        if (eq) atomicAdd(&nequal, eq);
+    }
+    __syncthreads();
+    const int above = ncand, have = nequal;
+    __syncthreads();
+    const int need = A.top - above;
+    if (need > 0 && have > 0) {
+        // Those equal to tau of the lowest indices, 1024 j + 4 thread + b: all of
+        // the first steps j, and of the one where `need` is reached the first
+        // threads'.
+        uint32_t same = 0;
         if (eq)
 #pragma unroll
-            for (int j = 0; j < 4 * VEC; j++) {
-                const int i = i0 + 1024 * (j >> 2) + (j & 3);
-                if (x[j] == tf && i < A.n && i <= upto) cand[atomicAdd(&ncand, 1)] = key(j);
-            }
+            for (int j = 0; j < 4 * VEC; j++) same |= x[j] == tf && i0 + 1024 * (j >> 2) + (j & 3) < A.n ? 1u << j : 0u;
+        if (tid < VEC) steps[tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            int n = 0;
+#pragma unroll
+            for (int b = 0; b < 4; b++) n += __popcll(__ballot((same >> (4 * j + b)) & 1));
+            if (l == 0 && n) atomicAdd(&steps[j], n);
+        }
+        __syncthreads();
+        int left = need, last = 0;  // the step where `need` is reached, and what is left for it
+        while (last < VEC - 1 && steps[last] < left) left -= steps[last++];
+        const int here = __popc((same >> (4 * last)) & 15u);
+        int before = here;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(before, o);
+            before += l >= o ? v : 0;
+        }
+        if (l == 63) cnt[w] = before;
+        __syncthreads();
+        before -= here;
+        for (int j = 0; j < w; j++) before += cnt[j];
+#pragma unroll
+        for (int j = 0; j < 4 * VEC; j++) {
+            if (!((same >> j) & 1)) continue;
+            const int step = j >> 2;
+            if (step < last || (step == last && before++ < left)) cand[atomicAdd(&ncand, 1)] = key(j);
+        }
         __syncthreads();
     }
     ranked(cand, ncand, A.top, A.keys + ((int64_t)row * A.chunks + chunk) * A.top);
@@ -198,22 +212,50 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
 
 constexpr int MAX_CHUNKS = 256;
 
+// Keys of a row that merge_kernel ranks as they are (of more it first drops what
+// a bound excludes: 320 keys 8.7 us as they are, 5.5 with the bound), and that
+// it reads ahead.
+constexpr int AS_THEY_ARE = 128, HELD = 1024;
+
 __global__ __launch_bounds__(256) void merge_kernel(Args A) {
     __shared__ float red[3][4];
-    __shared__ uint64_t cand[(KMAX - 1) * KMAX + 1];
+    __shared__ uint64_t cand[(KMAX - 1) * KMAX + 1 + 7];
+    __shared__ uint64_t held[HELD];
     __shared__ uint64_t heads[MAX_CHUNKS];
     __shared__ uint64_t best[KMAX];
     __shared__ uint64_t bound_s;
     __shared__ int ncand;
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, row = blockIdx.x;
     const Part* part = A.part + (int64_t)row * A.chunks;
+    const uint64_t* keys = A.keys + (int64_t)row * A.chunks * A.top;
+    const int nkeys = A.chunks * A.top;
+    const bool small = nkeys <= AS_THEY_ARE, ahead = nkeys <= HELD;
+    // all that is read, on its way at once
     Part p = {-__builtin_inff(), 0.f, 0.f, 0.f};
     if (tid < A.chunks) p = part[tid];
+    uint64_t mine[HELD / 256];
+    if (ahead) {
+#pragma unroll
+        for (int j = 0; j < HELD / 256; j++) mine[j] = tid + 256 * j < nkeys ? keys[tid + 256 * j] : 0;
+    }
+    float xt = 0.f;
+    bool given = false;
+    if (tid == 0 && A.logprob) {
+        const int id = A.targets[row];
+        given = id >= 0 && id < A.n;
+        if (given) xt = A.x[(int64_t)row * A.ld + id];
+    }
     const float wm = wave_max_f32(p.m);
     if (l == 0) red[0][w] = wm;
+    if (tid < KMAX) best[tid] = 0;  // what stays 0 has no key
     if (tid == 0) {
         ncand = 0;
         bound_s = ~0ull;
+    }
+    if (ahead) {
+#pragma unroll
+        for (int j = 0; j < HELD / 256; j++)
+            if (tid + 256 * j < nkeys) (small ? cand : held)[tid + 256 * j] = mine[j];
     }
     __syncthreads();
     const float m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
@@ -226,41 +268,38 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A) {
         red[1][w] = s1;
         red[2][w] = t1;
     }
+    // A bound that at least k keys reach: of each chunk's r-th key the least, r =
+    // ceil(k / chunks), or with k chunks and more the k-th largest first key.
+    const int r = (A.top + A.chunks - 1) / A.chunks;
+    if (!small && tid < A.chunks) heads[tid] = ahead ? held[tid * A.top + r - 1] : keys[tid * A.top + r - 1];
     __syncthreads();
     const float s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     const float t = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
     const float log_s = logf(s);
     if (tid == 0) {
         if (A.entropy) A.entropy[row] = log_s + t / s;
-        if (A.logprob) {
-            const int id = A.targets[row];
-            A.logprob[row] = id >= 0 && id < A.n ? (A.x[(int64_t)row * A.ld + id] - m) - log_s : 0.f;
-        }
+        if (A.logprob) A.logprob[row] = given ? (xt - m) - log_s : 0.f;
     }
     if (A.top == 0) return;
-    // a bound that at least k keys reach: of each chunk's r-th key the least,
-    // r = ceil(k / chunks), or with k chunks and more the k-th largest first key
-    const uint64_t* keys = A.keys + (int64_t)row * A.chunks * A.top;
-    const int r = (A.top + A.chunks - 1) / A.chunks;
-    if (tid < A.chunks) heads[tid] = keys[tid * A.top + r - 1];
-    __syncthreads();
-    if (A.chunks < A.top) {
-        if (tid < A.chunks) atomicMin((unsigned long long*)&bound_s, (unsigned long long)heads[tid]);
-    } else if (tid < A.chunks) {
-        const uint64_t k = heads[tid];
-        int above = 0;
-        for (int j = 0; j < A.chunks; j++) above += heads[j] > k ? 1 : 0;
-        // (first keys are distinct but for the zeros of chunks without any)
-        if (above < A.top) atomicMin((unsigned long long*)&bound_s, (unsigned long long)k);
+    if (!small) {
+        if (A.chunks < A.top) {
+            if (tid < A.chunks) atomicMin((unsigned long long*)&bound_s, (unsigned long long)heads[tid]);
+        } else if (tid < A.chunks) {
+            const uint64_t k = heads[tid];
+            int above = 0;
+            for (int j = 0; j < A.chunks; j++) above += heads[j] > k ? 1 : 0;
+            // (first keys are distinct but for the zeros of chunks without any)
+            if (above < A.top) atomicMin((unsigned long long*)&bound_s, (unsigned long long)k);
+        }
+        __syncthreads();
+        const uint64_t bound = bound_s;
+        for (int i = tid; i < nkeys; i += 256) {
+            const uint64_t k = ahead ? held[i] : keys[i];
+            if (k != 0 && k >= bound) cand[atomicAdd(&ncand, 1)] = k;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    const uint64_t bound = bound_s;
-    for (int i = tid; i < A.chunks * A.top; i += 256) {
-        const uint64_t k = keys[i];
-        if (k != 0 && k >= bound) cand[atomicAdd(&ncand, 1)] = k;
-    }
-    __syncthreads();
-    ranked(cand, ncand, A.top, best);
+    ranked(cand, small ? nkeys : ncand, A.top, best);
     __syncthreads();
     if (tid < A.top) {
         const uint64_t k = best[tid];
