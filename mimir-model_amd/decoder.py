@@ -12,7 +12,8 @@ memory; a decode step is one HIP graph replay with no host round trip.
 Several sequences ("slots", reference LlamaOptions.Slots,
 importer/llama.go:306-310) share one cache of slots * context positions:
 the token at position p of slot s goes to cache index s*context + p and sees
-the keys s*context .. s*context + p.
+the keys s*context .. s*context + p. With an 8-bit cache a slot takes context
+rounded up to a multiple of 32 entries, which share their scales.
 
 There is no CPU fallback: every op is a libmimg call, which raises if the
 library or a gfx950 GPU is missing.
@@ -109,13 +110,20 @@ class Decoder:
     f32_tile_rows (float32 activations only): products of at least this many
     rows run on the fp32 matrix cores (mimg_linear_f32_mfma_dev), within the
     spec's bound for dequant_matmul.v1 but not in the reference's float
-    order; 0 keeps the reference's order everywhere.
+    order; 0 keeps the reference's order everywhere. cache_q8: keys and values
+    in 8 bits (mimg_kv_store_q8_dev, mimg_attention_q8_dev), half the memory
+    and traffic of cache_f16, contexts past 8192; not the reference's bits.
     """
 
     def __init__(self, config, tensors, a8=True, cache_f16=False, max_rows=64, slots=1, procs=16, kquant_block=256,
-                 f32_tile_rows=0, fuse_rope=True, fuse_swiglu=True):
+                 f32_tile_rows=0, fuse_rope=True, fuse_swiglu=True, cache_q8=False):
         c = self.c = config if isinstance(config, Config) else Config(**config)
         self.a8, self.f16, self.slots = bool(a8), bool(cache_f16), int(slots)
+        self.q8 = bool(cache_q8)
+        if self.q8 and self.f16:
+            raise ValueError("cache_f16 and cache_q8: a cache has one type")
+        if self.q8 and (c.head_dim % 8 or c.head_dim > 256):
+            raise ValueError(f"head size {c.head_dim}: an 8-bit cache takes multiples of 8 up to 256")
         # activation blocks for Q4_K/Q6_K weights: 256 is dequant_matmul_a8.v2
         # as the importer writes it (importer/llama.go:264-280), 32 is .v1
         if kquant_block not in (32, 256):
@@ -137,18 +145,25 @@ class Decoder:
                 self.vec[name] = hiprt.DeviceBuffer.from_array(np.ascontiguousarray(data, np.float32))
             else:
                 self.w[name] = mimg.Weight(data, dt, int(shape[0]), int(shape[1]))
-        if c.context > 8192:
-            raise ValueError(f"context {c.context}: attention handles at most 8192 positions per sequence")
+        if c.context > (MAX_CONTEXT if self.q8 else 8192):
+            raise ValueError(f"context {c.context}: attention handles at most {MAX_CONTEXT if self.q8 else 8192} "
+                             "positions per sequence")
         self.head = self.w.get("output.weight") or self.w["token_embd.weight"]
         self.vocab = self.w["token_embd.weight"].n
         E, F, H, Hkv, D, R = c.embed, c.ffn, c.heads, c.kv_heads, c.head_dim, self.R
-        self.cache_len = self.slots * c.context
+        # cache entries of a slot: with 8 bits whole blocks
+        self.slot_len = -(-c.context // mimg.Q8_CACHE_BLOCK) * mimg.Q8_CACHE_BLOCK if self.q8 else c.context
+        self.cache_len = self.slots * self.slot_len
         esz = 2 if self.f16 else 4
         B = hiprt.DeviceBuffer
-        self.kc = [B(Hkv * self.cache_len * D * esz) for _ in range(c.layers)]
-        # the value cache is blocked by eight keys (include/mimg.h)
-        self.vc = [B(Hkv * mimg.vcache_len(self.cache_len) * D * esz) for _ in range(c.layers)]
-        for buf in self.kc + self.vc:
+        self.kc, self.vc, self.kv = [], [], []
+        if self.q8:  # keys and values of a layer in one buffer
+            self.kv = [B(mimg.cache_q8_bytes(Hkv, self.cache_len, D)) for _ in range(c.layers)]
+        else:
+            self.kc = [B(Hkv * self.cache_len * D * esz) for _ in range(c.layers)]
+            # the value cache is blocked by eight keys (include/mimg.h)
+            self.vc = [B(Hkv * mimg.vcache_len(self.cache_len) * D * esz) for _ in range(c.layers)]
+        for buf in self.kc + self.vc + self.kv:
             buf.zero()
         self.invf = B.from_array(inv_freq(c))
         self.x, self.h, self.ao = B(R * E * 4), B(R * E * 4), B(R * E * 4)
@@ -158,12 +173,13 @@ class Decoder:
         self.norm_fused = {}  # names -> whether the fused norm GEMV takes them
         # one row: norm, q/k/v, rope and the cache scatter in one launch
         # (until the library answers NotHandled for the shape)
-        self.rope_fused = bool(fuse_rope)
+        # (an 8-bit cache's store needs whole rows of k and v)
+        self.rope_fused = bool(fuse_rope) and not self.q8
         # one row, and 2..8 rows: gate/up products with swiglu in their epilogue
         self.swiglu_fused = bool(fuse_swiglu)
         self.swiglu_rows_fused = bool(fuse_swiglu)
         # 4..8 rows: q/k/v products with rope and the cache scatter
-        self.qkv_rows_fused = bool(fuse_rope)
+        self.qkv_rows_fused = bool(fuse_rope) and not self.q8
         self.q, self.o = B(R * H * D * 4), B(R * H * D * 4)
         self.k, self.v = B(R * Hkv * D * 4), B(R * Hkv * D * 4)
         self.g, self.u, self.sw = B(R * F * 4), B(R * F * 4), B(R * F * 4)
@@ -172,10 +188,14 @@ class Decoder:
         self.cidx, self.kstart = B(R * 8), B(R * 8)
         self.chosen, self.count = B(R * 4), B(4)
         self.out, self.out_cap = None, 0
+        self.targets, self.lp, self.lp_ws = None, None, None  # log probabilities, made when asked for
         kmax = max(E, H * D, F)
         self.ws_bytes = mimg.a8_workspace_bytes(R, kmax)
         self.ws = B(self.ws_bytes)
-        self.att_ws_bytes = mimg.attention_workspace_bytes(R, H, c.context)
+        if self.q8:  # (fewer rows are cut into more splits of the keys)
+            self.att_ws_bytes = max(mimg.attention_q8_workspace_bytes(r, H, Hkv, D, c.context) for r in range(1, R + 1))
+        else:
+            self.att_ws_bytes = mimg.attention_workspace_bytes(R, H, c.context)
         self.att_ws = B(self.att_ws_bytes)
         self.graphs = {}
 
@@ -322,6 +342,27 @@ class Decoder:
         self.x, self.x_alt = self.x_alt, self.x
         return True
 
+    def _rope_store(self, l, T, pos, cidx):
+        """rope of q and k, and k and v into layer l's cache."""
+        c, s = self.c, self.stream.handle
+        if self.q8:
+            mimg.rope_kv_q8_dev(self.q.ptr, self.k.ptr, self.v.ptr, pos, cidx, self.invf.ptr, T, c.heads, c.kv_heads,
+                                c.head_dim, c.rope_dims, c.interleaved, self.cache_len, self.kv[l].ptr, s)
+        else:
+            mimg.rope_kv_dev(self.q.ptr, self.k.ptr, self.v.ptr, pos, cidx, self.invf.ptr, T, c.heads, c.kv_heads,
+                             c.head_dim, c.rope_dims, c.interleaved, self.cache_len, self.kc[l].ptr, self.vc[l].ptr,
+                             self.f16, s)
+
+    def _attend(self, l, T, cidx, kstart):
+        c, s = self.c, self.stream.handle
+        if self.q8:
+            mimg.attention_q8_dev(self.q.ptr, self.kv[l].ptr, cidx, kstart, T, c.heads, c.kv_heads, c.head_dim,
+                                  self.cache_len, c.context, self.o.ptr, self.att_ws.ptr, self.att_ws_bytes, s)
+        else:
+            mimg.attention_dev(self.q.ptr, self.kc[l].ptr, self.vc[l].ptr, cidx, kstart, T, c.heads, c.kv_heads,
+                               c.head_dim, self.cache_len, c.context, self.f16, self.o.ptr, self.att_ws.ptr,
+                               self.att_ws_bytes, s)
+
     def _forward(self, T, ids=None, pos=None, cidx=None, kstart=None, head_rows=None):
         """Enqueues the forward pass of T rows (device arrays of token ids,
         positions, cache indices and slot starts; by default the decoder's
@@ -329,7 +370,7 @@ class Decoder:
         [(row, logits row)] only those rows (the head is the largest matrix;
         generation needs the last row of each prompt only)."""
         c, s = self.c, self.stream.handle
-        E, F, H, Hkv, D = c.embed, c.ffn, c.heads, c.kv_heads, c.head_dim
+        E, F = c.embed, c.ffn
         ids = ids or self.ids.ptr
         pos = pos or self.pos.ptr
         cidx = cidx or self.cidx.ptr
@@ -345,11 +386,8 @@ class Decoder:
                     not (4 <= T <= 8 and self._qkv_rope_rows(l, resid, qkv, qkv_b, T, pos, cidx)):
                 self._norm_linears(resid, p + "attn_norm.weight", T, qkv, [self.q.ptr, self.k.ptr, self.v.ptr], qkv_b,
                                    single_fused=True)
-                mimg.rope_kv_dev(self.q.ptr, self.k.ptr, self.v.ptr, pos, cidx, self.invf.ptr, T, H, Hkv, D,
-                                 c.rope_dims, c.interleaved, self.cache_len, self.kc[l].ptr, self.vc[l].ptr, self.f16,
-                                 s)
-            mimg.attention_dev(self.q.ptr, self.kc[l].ptr, self.vc[l].ptr, cidx, kstart, T, H, Hkv, D,
-                               self.cache_len, c.context, self.f16, self.o.ptr, self.att_ws.ptr, self.att_ws_bytes, s)
+                self._rope_store(l, T, pos, cidx)
+            self._attend(l, T, cidx, kstart)
             self._linears([p + "attn_output.weight"], self.o.ptr, T, [self.ao.ptr])
             down = self.w[p + "ffn_down.weight"]
             if T <= 8 and self._ffn_rows(l, T):
@@ -397,7 +435,7 @@ class Decoder:
             raise ValueError(f"slots {slots} (0..{self.slots - 1})")
         if positions.min() < 0 or positions.max() >= self.c.context:
             raise ValueError(f"positions outside 0..{self.c.context - 1}")
-        start = slots * self.c.context
+        start = slots * self.slot_len
         self.stream.sync()
         self.ids.upload(tokens)
         self.pos.upload(positions)
@@ -415,37 +453,98 @@ class Decoder:
         self.stream.sync()
         return self.logits.download(np.float32, T * self.vocab).reshape(T, self.vocab)
 
-    def _decode_step(self, n):
+    def _ensure_logprobs(self, rows, top):
+        """Buffers for the log probabilities of `rows` rows with `top`
+        alternatives: floats [rows] each of log probability and entropy,
+        [rows, top] log probabilities and ids of the alternatives."""
+        need, wsb = rows * (2 + 2 * top) * 4, mimg.logprobs_workspace_bytes(rows, self.vocab, top)
+        if wsb == 0:
+            raise ValueError(f"{top} alternatives of {self.vocab} tokens")
+        if self.lp is None or self.lp.nbytes < need or self.lp_ws.nbytes < wsb:
+            self._drop_graphs()  # captured with the old buffers
+            self.lp, self.lp_ws = hiprt.DeviceBuffer(need), hiprt.DeviceBuffer(wsb)
+        if self.targets is None:
+            self.targets = hiprt.DeviceBuffer(self.R * 4)
+
+    def _logprobs(self, rows, targets, top):
+        """Log probabilities of the targets and of the alternatives in the
+        logits, into self.lp."""
+        p, at = self.lp.ptr, rows * 8
+        mimg.logprobs_dev(self.logits.ptr, rows, self.vocab, self.vocab, targets, top, p, p + rows * 4,
+                          p + at + rows * top * 4 if top else None, p + at if top else None, self.lp_ws.ptr,
+                          self.lp_ws.nbytes, self.stream.handle)
+
+    @staticmethod
+    def _split_logprobs(flat, rows, top):
+        """self.lp's values [.., rows * (2 + 2 top)] as a dict."""
+        lead, at = flat.shape[:-1], rows * (2 + top)
+        return dict(logprobs=flat[..., :rows].copy(), entropy=flat[..., rows:2 * rows].copy(),
+                    top_logprobs=flat[..., 2 * rows:at].reshape(*lead, rows, top).copy(),
+                    top_ids=flat[..., at:].copy().view(np.int32).reshape(*lead, rows, top))
+
+    def score(self, tokens, top=0, slot=0):
+        """The log probability of each token after the first, given those
+        before it, and of `top` alternatives (up to 64) for every position:
+        dict(logprobs [P - 1], entropy [P], top_ids and top_logprobs [P, top]),
+        position i of the last three being the choice after tokens[i]. The mean
+        of -logprobs is the log of the perplexity. The tokens take the slot's
+        cache from its start."""
+        tokens = np.asarray(tokens, np.int32).ravel()
+        P, R = tokens.size, self.R
+        if P < 1 or P > self.c.context:
+            raise ValueError(f"{P} tokens (1..{self.c.context})")
+        self._ensure_logprobs(min(P, R), top)
+        parts = []
+        for c0 in range(0, P, R):
+            T = min(R, P - c0)
+            self._set_rows(tokens[c0:c0 + T], np.arange(c0, c0 + T), np.full(T, slot))
+            self.targets.upload(np.append(tokens[c0 + 1:c0 + T + 1], np.full(int(c0 + T == P), -1, np.int32)))
+            self._forward(T)
+            self._logprobs(T, self.targets.ptr, top)
+            self.stream.sync()
+            parts.append(self._split_logprobs(self.lp.download(np.float32, T * (2 + 2 * top)), T, top))
+        r = {k: np.concatenate([p[k] for p in parts]) for k in parts[0]}
+        return dict(r, logprobs=r["logprobs"][:P - 1])
+
+    def _decode_step(self, n, top=None):
         """One greedy step of n sequences: forward of the tokens in ids,
-        pick, append, advance."""
+        pick (its log probability too, with top), append, advance."""
         self._forward(n)
         mimg.argmax_dev(self.logits.ptr, n, self.vocab, self.chosen.ptr, self.stream.handle)
+        if top is not None:
+            self._logprobs(n, self.chosen.ptr, top)
         mimg.greedy_advance_dev(self.chosen.ptr, self.ids.ptr, self.pos.ptr, self.cidx.ptr, self.out.ptr,
                                 self.count.ptr, self.out_cap, n, self.stream.handle)
 
-    def _decode_graph(self, n):
-        g = self.graphs.get(n)
+    def _decode_graph(self, n, top=None):
+        g = self.graphs.get((n, top))
         if g is None:
-            g = self.graphs[n] = hiprt.Graph(self.stream, lambda: self._decode_step(n))
+            g = self.graphs[n, top] = hiprt.Graph(self.stream, lambda: self._decode_step(n, top))
         return g
+
+    def _drop_graphs(self):
+        self.stream.sync()
+        for g in self.graphs.values():
+            g.destroy()
+        self.graphs = {}
 
     def _ensure_out(self, cap, n):
         if self.out is None or self.out_cap < cap or self.out.nbytes < cap * n * 4:
-            self.stream.sync()
-            for g in self.graphs.values():  # captured with the old buffer
-                g.destroy()
-            self.graphs = {}
+            self._drop_graphs()  # captured with the old buffer
             self.out = hiprt.DeviceBuffer(cap * n * 4)
             self.out_cap = cap
 
-    def generate(self, prompts, n_new, slots=None, graph=True, timing=None):
+    def generate(self, prompts, n_new, slots=None, graph=True, timing=None, logprobs=None):
         """Greedy continuation of each prompt (one per slot, all of the same
         length): n_new tokens each, [len(prompts), n_new] (reference
         cmd/mim-run/main.go generate). The prompt rows run in batches of at
         most max_rows, the first pick is made on the device, and every
         decode step is one graph replay. With a dict as timing, it receives
         the device times of the prompt (to the first pick) and of the
-        decode steps."""
+        decode steps. With logprobs = the number of alternatives (0..64), the
+        result is (tokens, dict(logprobs and entropy [len(prompts), n_new],
+        top_ids and top_logprobs [len(prompts), n_new, logprobs])) of each
+        chosen token."""
         prompts = np.atleast_2d(np.asarray(prompts, np.int32))
         n, P = prompts.shape
         if n > self.slots or n > self.R:
@@ -457,7 +556,16 @@ class Decoder:
             raise ValueError(f"slots {slots}")
         self._ensure_out(max(n_new, 1), n)
         s = self.stream.handle
-        C = self.c.context
+        C = self.slot_len
+        if logprobs is not None:
+            self._ensure_logprobs(n, logprobs)
+            step_bytes = n * (2 + 2 * logprobs) * 4
+            history = hiprt.DeviceBuffer(step_bytes * max(n_new, 1))
+
+        def keep(i):  # step i's log probabilities, behind it on the stream
+            if logprobs is not None and i < n_new:
+                hiprt.copy_async(history.ptr + i * step_bytes, self.lp.ptr, step_bytes, self.stream)
+
         # every prompt row's inputs, and the state of the first decode step
         B = hiprt.DeviceBuffer
         rows_pos = np.tile(np.arange(P, dtype=np.int64), n)
@@ -477,26 +585,33 @@ class Decoder:
             self._forward(T, p_ids.ptr + 4 * c0, p_pos.ptr + 8 * c0, p_cidx.ptr + 8 * c0, p_start.ptr + 8 * c0,
                           head_rows=heads)
         mimg.argmax_dev(self.logits.ptr, n, self.vocab, self.chosen.ptr, s)
+        if logprobs is not None:
+            self._logprobs(n, self.chosen.ptr, logprobs)
+        keep(0)
         mimg.greedy_advance_dev(self.chosen.ptr, self.ids.ptr, self.pos.ptr, self.cidx.ptr, self.out.ptr,
                                 self.count.ptr, self.out_cap, n, s)
         ev[1].record(self.stream)
-        if graph and n_new > 1:
-            g = self._decode_graph(n)
-            for _ in range(n_new - 1):
+        g = self._decode_graph(n, logprobs) if graph and n_new > 1 else None
+        for i in range(1, n_new):
+            if g is not None:
                 g.launch(self.stream)
-        else:
-            for _ in range(n_new - 1):
-                self._decode_step(n)
+            else:
+                self._decode_step(n, logprobs)
+            keep(i)
         ev[2].record(self.stream)
         self.stream.sync()
         if timing is not None:
             timing["prompt_ms"] = ev[0].elapsed_ms(ev[1])
             timing["decode_ms"] = ev[1].elapsed_ms(ev[2])
             timing["prompt_rows"], timing["decode_steps"] = n * P, n_new - 1
-        return self.out.download(np.int32, n_new * n).reshape(n_new, n).T.copy()
+        ids = self.out.download(np.int32, n_new * n).reshape(n_new, n).T.copy()
+        if logprobs is None:
+            return ids
+        lp = self._split_logprobs(history.download(np.float32, n_new * step_bytes // 4).reshape(n_new, -1), n, logprobs)
+        return ids, {k: np.swapaxes(v, 0, 1).copy() for k, v in lp.items()}
 
     def reset(self):
         """Clears the cache (a new session)."""
         self.stream.sync()
-        for buf in self.kc + self.vc:
+        for buf in self.kc + self.vc + self.kv:
             buf.zero()

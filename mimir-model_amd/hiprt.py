@@ -108,6 +108,12 @@ class DeviceBuffer:
             pass
 
 
+def copy_async(dst, src, nbytes, stream):
+    """nbytes between two device addresses, in order on the stream."""
+    check(rt().hipMemcpyAsync(ctypes.c_void_p(dst), ctypes.c_void_p(src), nbytes, D2D, ctypes.c_void_p(stream.handle)),
+          "D2D")
+
+
 class Stream:
     def __init__(self):
         s = ctypes.c_void_p()
