@@ -28,7 +28,9 @@ struct StoreArgs {
     const int64_t *index, *pos;
     const double* inv_freq;
     int T, H, Hkv, d, rotary, interleaved;
-    int each;  // rows a workgroup looks at
+    int each;       // rows a workgroup looks at
+    int store_wgs;  // workgroups that store; those behind them turn q, qw a row
+    int qw;
     int64_t C, nb;
     uint8_t* cache;
 };
@@ -45,8 +47,9 @@ __device__ __forceinline__ Pair pair_of(int i, int rotary, int interleaved) {
     return {rotary + 2 * (i - h2), rotary + 2 * (i - h2) + 1, false};
 }
 __device__ __forceinline__ void turn(float& xa, float& xb, int64_t pos, double inv_freq) {
-    const double ang = (double)pos * inv_freq;
-    const float c = (float)cos(ang), sn = (float)sin(ang), x1 = xa, x2 = xb;
+    double c64, s64;
+    sincos((double)pos * inv_freq, &s64, &c64);
+    const float c = (float)c64, sn = (float)s64, x1 = xa, x2 = xb;
     xa = x1 * c - x2 * sn;
     xb = x2 * c + x1 * sn;
 }
@@ -86,26 +89,27 @@ __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
     __shared__ float part[4];
     __shared__ uint32_t newbad;
     __shared__ int earlier;
-    const int tid = threadIdx.x, y = blockIdx.y, hk = y >> 1, half = y & 1;
+    const int tid = threadIdx.x;
     int np = A.d / 2;
-    const int t0 = blockIdx.x * A.each;
     if constexpr (ROPE) {
-        if (y >= 2 * A.Hkv) {  // the workgroups behind the kv heads' turn q
-            const int n = A.H * np, qw = (int)gridDim.y - 2 * A.Hkv;
-            for (int t = t0; t < min(A.T, t0 + A.each); t++)
-                for (int j = (y - 2 * A.Hkv) * 256 + tid; j < n; j += qw * 256) {
-                    const int h = j / np;
-                    const Pair p = pair_of(j - h * np, A.rotary, A.interleaved);
-                    if (!p.rot) continue;
-                    float* r = A.q + ((int64_t)t * A.H + h) * A.d;
-                    float xa = r[p.a], xb = r[p.b];
-                    turn(xa, xb, A.pos[t], A.inv_freq[A.interleaved ? p.a / 2 : p.a]);
-                    r[p.a] = xa;
-                    r[p.b] = xb;
-                }
+        if ((int)blockIdx.x >= A.store_wgs) {  // the workgroups behind the stores' turn q
+            // a thread keeps to one pair, so one 64-bit sine and cosine serve its heads
+            const int u = (int)blockIdx.x - A.store_wgs, t = u / A.qw, per = 256 / np, sub = tid / np, i = tid - sub * np;
+            const Pair p = pair_of(i, A.rotary, A.interleaved);
+            if (sub >= per || !p.rot) return;
+            double c64, s64;
+            sincos((double)A.pos[t] * A.inv_freq[i], &s64, &c64);
+            const float c = (float)c64, sn = (float)s64;
+            for (int h = (u - t * A.qw) * per + sub; h < A.H; h += A.qw * per) {
+                float* r = A.q + ((int64_t)t * A.H + h) * A.d;
+                const float x1 = r[p.a], x2 = r[p.b];
+                r[p.a] = x1 * c - x2 * sn;
+                r[p.b] = x2 * c + x1 * sn;
+            }
             return;
         }
     }
+    const int y = blockIdx.x % (2u * A.Hkv), hk = y >> 1, half = y & 1, t0 = blockIdx.x / (2u * A.Hkv) * A.each;
     const int64_t first = tid < A.T ? A.index[tid] : -1;
     // Lane j: row t0 + j and the one before it. The rows that may be a block's
     // first (outside the cache: not stored).
@@ -301,9 +305,10 @@ hipError_t launch_store(StoreArgs a, hipStream_t s) {
     // One row a workgroup for a decode batch, whose rows are a block each;
     // several of a prompt, of which one in 32 begins a block.
     a.each = a.T <= 128 ? 1 : (a.T <= 2048 ? 16 : 32);
-    // q: a pair a thread (each takes a 64-bit sine and cosine)
-    const int qw = ROPE ? (a.H * (a.d / 2) + 255) / 256 : 0;
-    const dim3 grid((unsigned)((a.T + a.each - 1) / a.each), (unsigned)(2 * a.Hkv + qw));
+    a.store_wgs = (a.T + a.each - 1) / a.each * 2 * a.Hkv;
+    const int rounds = (a.H + 256 / (a.d / 2) - 1) / (256 / (a.d / 2));  // heads a thread turns alone in its row
+    a.qw = a.T <= 64 ? rounds : 1;
+    const dim3 grid((unsigned)(a.store_wgs + (ROPE ? a.T * a.qw : 0)));
     switch (q8c_dp(a.d)) {
     case 64: hipLaunchKernelGGL((store_q8_kernel<64, ROPE>), grid, dim3(256), 0, s, a); break;
     case 128: hipLaunchKernelGGL((store_q8_kernel<128, ROPE>), grid, dim3(256), 0, s, a); break;
