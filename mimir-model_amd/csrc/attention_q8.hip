@@ -73,6 +73,19 @@ __device__ __forceinline__ v8h widen(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// A block's scales in scalar registers, by scalar loads: the cache does not
+// change while these kernels run, and blk is uniform. (In vector registers they
+// cost many_kernel its last ones: 43 spilled, 34 us became 52 at 128 rows.)
+struct Scales {
+    float ks, vs;
+    uint32_t bad;
+};
+__device__ __forceinline__ Scales scales_of(const Q8Meta* meta, int blk) {
+    typedef const __attribute__((address_space(4))) u32x4* Constant;
+    const u32x4 v = *(Constant)(uintptr_t)(meta + blk);
+    return {__uint_as_float(v.x), __uint_as_float(v.y), v.z | v.w};
+}
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Step s of a lane's query row: dims 64 (s / 2) + 16 g + 8 (s % 2) .. +7, the
@@ -139,13 +152,13 @@ struct State {
 struct Scale {
     float lv, iv;
 };
-__device__ __forceinline__ Scale value_scale(const Q8Meta& m) {
+__device__ __forceinline__ Scale value_scale(const Scales& m) {
     const float vs = m.vs > 0.f ? m.vs : Q8C_FLOOR;
     return {__builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
 }
 // The factor of a block's scores; at least float32's smallest normal number, so
 // that -inf times it is -inf (a NaN stays).
-__device__ __forceinline__ float key_scale(float scale, const Q8Meta& m) {
+__device__ __forceinline__ float key_scale(float scale, const Scales& m) {
     const float c = scale * m.ks;
     return c < 1.17549435e-38f ? 1.17549435e-38f : c;
 }
@@ -160,14 +173,13 @@ __device__ __forceinline__ bool near_enough(float top, float M) { return top <= 
 // that a column does not see (-inf) or that are not finite (NaN), M moved, and
 // weights left out. Returns the exponents' offset.
 template <int DP>
-__device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Q8Meta& m, float cs, Scale v, int blk, int g, int k0, int n,
+__device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Scales& m, float cs, Scale v, int blk, int g, int k0, int n,
                                          State<DP>& S) {
-    const uint32_t bad = m.bad();
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         float& x = j < 4 ? ((float*)&s0)[j] : ((float*)&s1)[j - 4];
         const int e = 16 * (j >> 2) + 4 * g + (j & 3);
-        if ((bad >> e) & 1) x = __builtin_nanf("");
+        if ((m.bad >> e) & 1) x = __builtin_nanf("");
         if ((unsigned)(Q8C_BLOCK * blk + e - k0) >= (unsigned)n) x = -__builtin_inff();
     }
     const float mx = largest(s0, s1) * cs + v.lv;
@@ -333,12 +345,12 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
     const int64_t first = (int64_t)hk * A.nb;
     const Q8Meta* meta = (const Q8Meta*)(A.cache + q8c_meta(A.nb, A.Hkv, hk, 0, DP));
     u32x4 kb[DP / 32], vb[DP / 32];
-    Q8Meta m;
+    Scales m;
     auto fetch_k = [&](int blk) {
         const u32x4* p = rec + (first + blk) * REC;
 #pragma unroll
         for (int i = 0; i < DP / 32; i++) kb[i] = __builtin_nontemporal_load(p + 64 * i);
-        m = meta[blk];
+        m = scales_of(meta, blk);
     };
     if (b < b1) fetch_k(b);
     const RowScale rs = row_scale<DP>(x, A.d);
@@ -370,7 +382,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
                 s[kt] = mfma(ka, S_.q[0][2 * i][l], s[kt]);
                 s[kt] = mfma(kc, S_.q[0][2 * i + 1][l], s[kt]);
             }
-        const Q8Meta mb = m;
+        const Scales mb = m;
         const int blk = b;
         b += NW;
         if (b < b1) fetch_k(b);
@@ -378,7 +390,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         const Scale v = value_scale(mb);
         const float cs = key_scale(rs.scale, mb);
         float base = v.lv - S.M + 8.f;
-        if (!all_seen || mb.bad() || !(mb.vs > 0.f) || !__all(near_enough(largest(s[0], s[1]) * cs + v.lv, S.M)))
+        if (!all_seen || mb.bad || !(mb.vs > 0.f) || !__all(near_enough(largest(s[0], s[1]) * cs + v.lv, S.M)))
             base = correct<DP>(s[0], s[1], mb, cs, v, blk, g, k0, n, S);
         Weights W;
         const float sum = weigh_tile(s[0], cs, base, W.hi, W.lo) + weigh_tile(s[1], cs, base, W.hi + 2, W.lo + 2);
@@ -484,7 +496,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
     from = wave_max_i32(from);
     to = wave_min_i32(to);
     __syncthreads();
-    const int total = R.total, per = max((total + A.splits - 1) / A.splits, 2);
+    const int total = R.total, per = max((total + A.splits - 1) / A.splits, 8);
     const int p0 = (int)blockIdx.y * per, p1 = min(total, p0 + per);
     // The block of position p (rising): ranges [.., end) lie `shift` above theirs.
     int i = -1, end = 0, shift = 0;
@@ -510,7 +522,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
     };
     constexpr int NS = DP / 32;  // steps of a score product, and pairs of dim tiles
     int here = 0, next = 0, after = 0;  // blocks of positions p, p + 1 (in LDS), p + 2 (in flight)
-    Q8Meta mh{}, mn{};
+    Scales mh{}, mn{};
     v4f sa[NCT][2], sb[NCT][2];
     float top[NCT];  // the largest of a lane's scores
     if (p0 < p1) {
@@ -525,8 +537,8 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
         for (int h = 0; h < NS; h++) put(buf[0], raw0, h);
 #pragma unroll
         for (int h = 0; h < NS; h++) put(buf[1], raw1, h);
-        mh = meta[here];
-        mn = meta[next];
+        mh = scales_of(meta, here);
+        mn = scales_of(meta, next);
     }
     __syncthreads();
     if (p0 < p1) {
@@ -555,7 +567,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
         const int b1 = bi == 2 ? 0 : bi + 1, b2 = b1 == 2 ? 0 : b1 + 1;
         v8h (*kb)[64] = buf[b1], (*vb)[64] = buf[bi] + DP / 16, (*pb)[64] = buf[b2];
         v8h k0 = kb[0][l], k1 = kb[NS][l];
-        const Q8Meta m = mh;
+        const Scales m = mh;
         const Scale v = value_scale(m);
         float cs[NCT], base[NCT];
         bool fine = true;
@@ -565,7 +577,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
             fine &= near_enough(top[ct] * cs[ct] + v.lv, S[ct].M);
             base[ct] = v.lv - S[ct].M + 8.f;
         }
-        if (!(Q8C_BLOCK * here >= from && Q8C_BLOCK * (here + 1) <= to && m.bad() == 0 && m.vs > 0.f && __all(fine))) {
+        if (!(Q8C_BLOCK * here >= from && Q8C_BLOCK * (here + 1) <= to && m.bad == 0 && m.vs > 0.f && __all(fine))) {
 #pragma unroll
             for (int ct = 0; ct < NCT; ct++) {
                 const int2 k = R.kn[WC * w + 16 * ct + col];
@@ -575,7 +587,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
         here = next;
         next = after;
         mh = mn;
-        mn = meta[next];
+        mn = scales_of(meta, next);
         Weights W[NCT];
         float sum[NCT][2];
         v8h v0, v1;
@@ -674,34 +686,69 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
     }
 }
 
-// The splits of a row joined: a workgroup per (token, head), DP / 4 threads a
-// split, so 1024 / DP splits at a time.
-template <int DP>
+// The splits of a row joined, DP / 4 threads a row and split. WIDE: a workgroup
+// per row, 1024 / DP of its splits at a time (few rows, which many splits may
+// hold); else 1024 / DP rows a workgroup.
+template <int DP, bool WIDE>
 __global__ __launch_bounds__(256) void join_kernel(Args A) {
-    constexpr int LANES = DP / 4, AT_ONCE = 256 / LANES;
-    __shared__ __align__(16) float os[AT_ONCE][DP];
-    const int64_t rows = (int64_t)A.T * A.H, row = blockIdx.x;
-    const int tid = threadIdx.x, l = tid & 63, u = tid / LANES, d4 = (tid - u * LANES) * 4;
+    constexpr int LANES = DP / 4, GROUPS = 256 / LANES;
+    __shared__ __align__(16) float os[WIDE ? GROUPS : 1][DP];
+    const int64_t rows = (int64_t)A.T * A.H;
+    const int tid = threadIdx.x, u = tid / LANES, d4 = (tid - u * LANES) * 4;
+    const int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * GROUPS + u;
     const float2* pml = (const float2*)(A.part + (int64_t)A.splits * rows * DP);
-    const float2 x = l < A.splits ? pml[l * rows + row] : make_float2(-__builtin_inff(), 0.f);  // at most 64 splits
-    const bool none = x.x == -__builtin_inff();
-    const float M = wave_max_f32(x.x);
-    const float wh = none ? 0.f : exp2_hw(0.5f * (x.x - M));
-    const float L = wave_sum_f32(none ? 0.f : x.y * wh * wh);
     v4f o = {0.f, 0.f, 0.f, 0.f};
+    float M = -__builtin_inff(), L = 0.f;
+    if constexpr (WIDE) {
+        const int l = tid & 63;
+        const float2 x = l < A.splits ? pml[l * rows + row] : make_float2(-__builtin_inff(), 0.f);  // at most 64 splits
+        const bool none = x.x == -__builtin_inff();
+        M = wave_max_f32(x.x);
+        const float wh = none ? 0.f : exp2_hw(0.5f * (x.x - M));
+        L = wave_sum_f32(none ? 0.f : x.y * wh * wh);
 #pragma unroll 8
-    for (int s0 = 0; s0 < A.splits; s0 += AT_ONCE) {
-        const int s = s0 + u;
-        const float f = __shfl(wh, s & 63);  // 0 where a split holds nothing: its sums are not read
-        if (u < AT_ONCE && s < A.splits && f != 0.f) o += *(const v4f*)(A.part + ((int64_t)s * rows + row) * DP + d4) * (f * f);
-    }
-    if (u < AT_ONCE) *(v4f*)&os[u][d4] = o;
-    __syncthreads();
-    if (tid >= A.d) return;
-    float v = 0.f;
+        for (int s0 = 0; s0 < A.splits; s0 += GROUPS) {
+            const int s = s0 + u;
+            const float f = __shfl(wh, s & 63);  // 0 where a split holds nothing: its sums are not read
+            if (u < GROUPS && s < A.splits && f != 0.f) o += *(const v4f*)(A.part + ((int64_t)s * rows + row) * DP + d4) * (f * f);
+        }
+        if (u < GROUPS) *(v4f*)&os[u][d4] = o;
+        __syncthreads();
+        if (u != 0) return;
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; j++) v += os[j][tid];
-    A.out[row * A.d + tid] = M == -__builtin_inff() ? 0.f : (L > 0.f ? v / L : __builtin_nanf(""));
+        for (int j = 1; j < GROUPS; j++) o += *(const v4f*)&os[j][d4];
+    } else {
+        if (u >= GROUPS || row >= rows) return;
+        // in batches of eight splits, all loads of one on their way together
+        for (int s0 = 0; s0 < A.splits; s0 += 8) {
+            float2 x[8];
+            v4f v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = s0 + j < A.splits ? pml[(s0 + j) * rows + row] : make_float2(-__builtin_inff(), 0.f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int s = min(s0 + j, A.splits - 1);
+                v[j] = *(const v4f*)(A.part + ((int64_t)s * rows + row) * DP + d4);
+            }
+            float m = M;
+#pragma unroll
+            for (int j = 0; j < 8; j++) m = fmaxf(m, x[j].x);
+            if (m == -__builtin_inff()) continue;
+            const float a = M == -__builtin_inff() ? 0.f : exp2_hw(0.5f * (M - m));
+            M = m;
+            L = L * a * a;
+            o *= a * a;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (x[j].x == -__builtin_inff()) continue;  // (what was read of it means nothing)
+                const float wh = exp2_hw(0.5f * (x[j].x - M));
+                L += x[j].y * wh * wh;
+                o += v[j] * (wh * wh);
+            }
+        }
+    }
+    const float inv = M == -__builtin_inff() ? 0.f : (L > 0.f ? 1.f / L : __builtin_nanf(""));
+    if (d4 < A.d) *(f32x4a4*)(A.out + row * A.d + d4) = M == -__builtin_inff() ? v4f{0.f, 0.f, 0.f, 0.f} : o * inv;
 }
 
 // How a call is cut.
@@ -735,7 +782,7 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     // span 24 blocks and more (128 tokens, nothing cached: 7 and 10 us against
     // 13 and 17).
     c.least = T < 192 ? 24 : 0;
-    c.many = T >= 96 && G <= cols && blocks >= c.least && T * Hkv * subs * blocks * (d <= 64 ? 1 : 2) >= 1 << 17;
+    c.many = T >= 96 && G <= cols && blocks >= c.least && T * Hkv * subs * blocks >= 1 << 16;
     c.tpt = c.many ? (int)(cols / G) : 1;
     const int64_t tiles = (T + c.tpt - 1) / c.tpt;
     c.many_wgs = tiles * Hkv;
@@ -761,8 +808,11 @@ hipError_t launch(Args A, const Cut& c, hipStream_t s) {
     hipLaunchKernelGGL(few_kernel<DP>, dim3((unsigned)c.few_wgs, (unsigned)c.few_splits), dim3(64 * NW), 0, s, A);
     if (c.many)
         hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.splits), dim3(256), 0, s, A);
-    if (c.splits > 1)
-        hipLaunchKernelGGL(join_kernel<DP>, dim3((unsigned)(A.T * A.H)), dim3(256), 0, s, A);
+    const int rows = A.T * A.H, groups = 1024 / DP;
+    if (c.splits > 1 && rows <= 1024)
+        hipLaunchKernelGGL((join_kernel<DP, true>), dim3((unsigned)rows), dim3(256), 0, s, A);
+    else if (c.splits > 1)
+        hipLaunchKernelGGL((join_kernel<DP, false>), dim3((unsigned)((rows + groups - 1) / groups)), dim3(256), 0, s, A);
     return hipGetLastError();
 }
 

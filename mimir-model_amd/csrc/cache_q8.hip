@@ -46,12 +46,16 @@ __device__ __forceinline__ Pair pair_of(int i, int rotary, int interleaved) {
     if (i < h2) return {i, i + h2, true};
     return {rotary + 2 * (i - h2), rotary + 2 * (i - h2) + 1, false};
 }
-__device__ __forceinline__ void turn(float& xa, float& xb, int64_t pos, double inv_freq) {
-    double c64, s64;
-    sincos((double)pos * inv_freq, &s64, &c64);
-    const float c = (float)c64, sn = (float)s64, x1 = xa, x2 = xb;
-    xa = x1 * c - x2 * sn;
-    xb = x2 * c + x1 * sn;
+// Cosine and sine of a pair's angle, in 64 bits, rounded.
+__device__ __forceinline__ float2 turn_of(int64_t pos, double inv_freq) {
+    double c, s;
+    sincos((double)pos * inv_freq, &s, &c);
+    return make_float2((float)c, (float)s);
+}
+__device__ __forceinline__ void turn(float& xa, float& xb, float2 cs) {
+    const float x1 = xa, x2 = xb;
+    xa = x1 * cs.x - x2 * cs.y;
+    xb = x2 * cs.x + x1 * cs.y;
 }
 
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
@@ -84,6 +88,7 @@ __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
     constexpr int NP = DP / 16;  // pairs of dims that a thread holds
     constexpr int HALF = Q8C_BLOCK * DP, WORDS = (HALF / 16 + 255) / 256;
     __shared__ __align__(16) uint8_t image[HALF];
+    __shared__ float2 turns[ROPE ? Q8C_BLOCK * DP / 2 : 1];
     __shared__ int rows[Q8C_BLOCK];
     __shared__ int2 list[Q8C_BLOCK];  // the entries to store and their rows
     __shared__ float part[4];
@@ -97,14 +102,13 @@ __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
             const int u = (int)blockIdx.x - A.store_wgs, t = u / A.qw, per = 256 / np, sub = tid / np, i = tid - sub * np;
             const Pair p = pair_of(i, A.rotary, A.interleaved);
             if (sub >= per || !p.rot) return;
-            double c64, s64;
-            sincos((double)A.pos[t] * A.inv_freq[i], &s64, &c64);
-            const float c = (float)c64, sn = (float)s64;
+            const float2 cs = turn_of(A.pos[t], A.inv_freq[i]);
             for (int h = (u - t * A.qw) * per + sub; h < A.H; h += A.qw * per) {
                 float* r = A.q + ((int64_t)t * A.H + h) * A.d;
-                const float x1 = r[p.a], x2 = r[p.b];
-                r[p.a] = x1 * c - x2 * sn;
-                r[p.b] = x2 * c + x1 * sn;
+                float xa = r[p.a], xb = r[p.b];
+                turn(xa, xb, cs);
+                r[p.a] = xa;
+                r[p.b] = xb;
             }
             return;
         }
@@ -187,14 +191,24 @@ __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
                 }
             }
         }
+        if constexpr (ROPE) {
+            // meanwhile the thread's cosines and sines, into LDS so that their code
+            // (a kibibyte and more each) stands here once
+            if (half == 0)
+#pragma unroll 1
+                for (int it = tid; it < items; it += 256) {
+                    const int u = (int)(((uint32_t)it * inv_np) >> 20), i = it - u * np;
+                    if (pair_of(i, A.rotary, A.interleaved).rot) turns[it] = turn_of(A.pos[list[u].y], A.inv_freq[i]);
+                }
+        }
 #pragma unroll
         for (int j = 0; j < NP; j++) {
             const int it = tid + 256 * j;
             if (it >= items) continue;
             float &xa = xs[2 * j], &xb = xs[2 * j + 1];
             if (ROPE && half == 0) {
-                const int u = (int)(((uint32_t)it * inv_np) >> 20), i = it - u * np;
-                if (pair_of(i, A.rotary, A.interleaved).rot) turn(xa, xb, A.pos[list[u].y], A.inv_freq[i]);
+                const int i = it - (int)(((uint32_t)it * inv_np) >> 20) * np;
+                if (pair_of(i, A.rotary, A.interleaved).rot) turn(xa, xb, turns[it]);
             }
             if (!(finite_bits(xa) && finite_bits(xb))) {
                 atomicOr(&newbad, 1u << list[(uint32_t)it * inv_np >> 20].x);
@@ -292,7 +306,7 @@ __global__ __launch_bounds__(256) void load_q8_kernel(const uint8_t* __restrict_
             for (int j = 0; j < 4; j++) {
                 ko[j] = (float)((int)((kw >> (8 * j)) & 255u) - 128) * m.ks;
                 vo[j] = (float)((int)vp[q8c_vbyte(e, dd + j)] - 128) * m.vs;
-                if ((m.bad() >> e) & 1) ko[j] = vo[j] = __builtin_nanf("");
+                if (((m.kbad | m.vbad) >> e) & 1) ko[j] = vo[j] = __builtin_nanf("");
             }
         }
         *(f32x4a4*)(k + i * 4) = ko;

@@ -31,7 +31,6 @@ constexpr int Q8C_MAX_D = 256;
 struct __align__(16) Q8Meta {
     float ks, vs;
     uint32_t kbad, vbad;
-    __device__ __forceinline__ uint32_t bad() const { return kbad | vbad; }
 };
 
 __host__ __device__ __forceinline__ int q8c_dp(int d) { return (d + 63) & ~63; }
