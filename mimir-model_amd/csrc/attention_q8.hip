@@ -73,6 +73,14 @@ __device__ __forceinline__ v8h widen(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// att_range for a token of the whole wave: its ends by scalar loads (nothing
+// writes them while these kernels run).
+__device__ __forceinline__ AttRange range_of(const Args& A, int t) {
+    typedef const __attribute__((address_space(4))) int64_t* Constant;
+    int64_t end = *(Constant)(uintptr_t)(A.kend + t), start = A.kstart ? *(Constant)(uintptr_t)(A.kstart + t) : 0;
+    return att_range(&end, &start, 0, A.C, A.maxk);
+}
+
 // A block's scales in scalar registers, by scalar loads: the cache does not
 // change while these kernels run, and blk is uniform. (In vector registers they
 // cost many_kernel its last ones: 43 spilled, 34 us became 52 at 128 rows.)
@@ -324,22 +332,24 @@ template <int DP>
 __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A) {
     __shared__ FewLds<DP> S_;
     const int tid = threadIdx.x, l = tid & 63, g = l >> 4, col = l & 15, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int subs = (A.G + COLS - 1) / COLS, hk = blockIdx.x % (unsigned)A.Hkv, sub = blockIdx.x / (unsigned)A.Hkv % subs;
-    const int unit = blockIdx.x / (unsigned)(A.Hkv * subs), tile = unit / A.fan, g0 = sub * COLS, ncol = min(COLS, A.G - g0);
+    // (divisions only where there is something to divide: a dozen of them are
+    // most of a microsecond before the first load)
+    const int sub = A.G > COLS ? (int)blockIdx.x / A.Hkv : 0, hk = (int)blockIdx.x - sub * A.Hkv, g0 = sub * COLS;
+    const int ncol = min(COLS, A.G - g0), unit = blockIdx.y, split = blockIdx.z, tile = A.fan > 1 ? unit / A.fan : unit;
     if (A.choose && takes_many(A, spans_of(A, tile), MANY_COLS<DP>)) return;
     const int last = min(A.T, (tile + 1) * A.tpt);
     for (int t = tile * A.tpt + (unit - tile * A.fan); t < last; t += A.fan) {
     const int head0 = t * A.H + hk * A.G + g0;
-    const AttRange r = att_range(A.kend, A.kstart, t, A.C, A.maxk);
+    const AttRange r = range_of(A, t);
     Eight x[DP / 32];
     const float* row = A.q + (int64_t)(head0 + min(col, ncol - 1)) * A.d;
 #pragma unroll
     for (int s = 0; s < DP / 32; s++) x[s] = query_step(row, A.d, s, g);
-    const int k0 = __builtin_amdgcn_readfirstlane((int)r.k0), n = __builtin_amdgcn_readfirstlane((int)r.n);
+    const int k0 = (int)r.k0, n = (int)r.n;
     const int b0 = k0 >> 5, total = n > 0 ? ((k0 + n + 31) >> 5) - b0 : 0;
-    const int per = max((total + A.few_splits - 1) / A.few_splits, NW);
-    int b = b0 + (int)blockIdx.y * per + w;
-    const int b1 = min(b0 + total, b0 + ((int)blockIdx.y + 1) * per);
+    const int per = A.few_splits > 1 ? max((total + A.few_splits - 1) / A.few_splits, NW) : max(total, NW);
+    int b = b0 + split * per + w;
+    const int b1 = min(b0 + total, b0 + (split + 1) * per);
     const u32x4* rec = (const u32x4*)A.cache + l;
     constexpr int64_t REC = 2 * Q8C_BLOCK * DP / 16;
     const int64_t first = (int64_t)hk * A.nb;
@@ -418,7 +428,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         for (int i = 0; i < DP / 16; i++) *(v4f*)&S_.o[w][col][16 * i + 4 * g] = S.o[i];
     __syncthreads();
     const int64_t rows = (int64_t)A.T * A.H;
-    const bool none = (int)blockIdx.y * per >= total;
+    const bool none = split * per >= total;
     for (int i = tid; i < ncol * (DP / 4); i += 64 * NW) {
         const int c = i / (DP / 4), d4 = (i - c * (DP / 4)) * 4;
         float M = S_.ml[0][0][c];
@@ -434,11 +444,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         }
         const int64_t head = head0 + c;
         if (A.splits > 1) {
-            const int64_t at = (int64_t)blockIdx.y * rows + head;
+            const int64_t at = (int64_t)split * rows + head;
             if (d4 == 0)
                 ((float2*)(A.part + (int64_t)A.splits * rows * DP))[at] = make_float2(none ? -__builtin_inff() : M, L);
             if (!none) *(v4f*)(A.part + at * DP + d4) = o;
-            if (d4 == 0 && blockIdx.y == 0)  // (splits that few_kernel does not use)
+            if (d4 == 0 && split == 0)  // (splits that few_kernel does not use)
                 for (int y = A.few_splits; y < A.splits; y++)
                     ((float2*)(A.part + (int64_t)A.splits * rows * DP))[y * rows + head] = make_float2(-__builtin_inff(), 0.f);
         } else if (d4 < A.d) {
@@ -755,7 +765,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
 struct Cut {
     bool many;
     int tpt, fan, least;
-    int64_t few_wgs, many_wgs;
+    int64_t units, subs, many_wgs;
     int splits, few_splits;
 };
 Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
@@ -791,7 +801,8 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
         const int64_t f = (512 + c.many_wgs * subs - 1) / (c.many_wgs * subs);
         c.fan = (int)(f < c.tpt ? f : c.tpt);
     }
-    c.few_wgs = tiles * c.fan * subs * Hkv;
+    c.units = tiles * c.fan;
+    c.subs = subs;
     c.few_splits = splits(T * subs * Hkv);
     c.splits = c.many ? std::max(splits(c.many_wgs), c.few_splits) : c.few_splits;
     return c;
@@ -805,7 +816,7 @@ hipError_t launch(Args A, const Cut& c, hipStream_t s) {
     A.fan = c.fan;
     A.least = c.least;
     A.choose = c.many ? 1 : 0;
-    hipLaunchKernelGGL(few_kernel<DP>, dim3((unsigned)c.few_wgs, (unsigned)c.few_splits), dim3(64 * NW), 0, s, A);
+    hipLaunchKernelGGL(few_kernel<DP>, dim3((unsigned)(A.Hkv * c.subs), (unsigned)c.units, (unsigned)c.few_splits), dim3(64 * NW), 0, s, A);
     if (c.many)
         hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.splits), dim3(256), 0, s, A);
     const int rows = A.T * A.H, groups = 1024 / DP;
