@@ -607,7 +607,8 @@ class Decoder:
         ids = self.out.download(np.int32, n_new * n).reshape(n_new, n).T.copy()
         if logprobs is None:
             return ids
-        lp = self._split_logprobs(history.download(np.float32, n_new * step_bytes // 4).reshape(n_new, -1), n, logprobs)
+        lp = self._split_logprobs(history.download(np.float32, n_new * step_bytes // 4).reshape(n_new, step_bytes // 4),
+                                  n, logprobs)
         return ids, {k: np.swapaxes(v, 0, 1).copy() for k, v in lp.items()}
 
     def reset(self):

@@ -195,12 +195,16 @@ def check(got, ref, q, kend, kstart=None, maxk=None):
     assert (off <= np.nan_to_num(bound)[..., None] + 1e-37).all(), (off.max(), np.argwhere(off > bound[..., None])[:5])
 
 
+# `room`: max_keys, which with T, heads and kv heads decides on the kernels: the
+# cache's length, and far more than it (many splits; from 96 tokens the prompt
+# kernel beside the other)
+@pytest.mark.parametrize("room", [None, 1 << 18])
 @pytest.mark.parametrize("T,H,hk,d,slots,stride", [
-    (1, 1, 1, 64, 1, 32), (1, 4, 1, 8, 1, 1), (1, 32, 8, 64, 1, 181), (2, 16, 16, 128, 2, 33), (3, 14, 2, 64, 3, 500),
+    (100, 144, 1, 64, 1, 250), (97, 34, 1, 64, 2, 150), (260, 8, 8, 128, 1, 900), (120, 3, 1, 256, 1, 400), (1, 1, 1, 64, 1, 32), (1, 4, 1, 8, 1, 1), (1, 32, 8, 64, 1, 181), (2, 16, 16, 128, 2, 33), (3, 14, 2, 64, 3, 500),
     (8, 32, 8, 128, 8, 300), (5, 40, 2, 80, 5, 77), (1, 34, 2, 256, 1, 700), (4, 6, 3, 192, 2, 129), (1, 8, 2, 128, 1, 6000),
     (1, 3, 1, 64, 1, 20001), (64, 4, 2, 64, 16, 70), (70, 14, 2, 64, 7, 90), (200, 32, 8, 128, 1, 200), (133, 8, 8, 64, 1, 300),
     (130, 34, 2, 80, 3, 130), (181, 14, 2, 64, 1, 181), (65, 12, 4, 256, 2, 100), (150, 16, 2, 128, 150, 13), (300, 6, 2, 192, 2, 400)])
-def test_attention(gpu, rt, T, H, hk, d, slots, stride):
+def test_attention(gpu, rt, T, H, hk, d, slots, stride, room):
     """Prompts and decode batches, sequences that start inside a block, rows
     that see nothing, keys that no row sees marked as not finite."""
     rng = np.random.default_rng(T * 31 + H + stride)
@@ -220,10 +224,27 @@ def test_attention(gpu, rt, T, H, hk, d, slots, stride):
     for a, b in zip(start, end):
         used[a:b + 1] = True
     ref.bad[:] = (~used).reshape(-1, 32) @ (1 << np.arange(32, dtype=np.uint64))
-    check(run(gpu, rt, q, ref, end, start if slots > 1 else None), ref, q, end, start if slots > 1 else None)
+    check(run(gpu, rt, q, ref, end, start if slots > 1 else None, room), ref, q, end, start if slots > 1 else None)
 
 
-@pytest.mark.parametrize("T", [3, 80])
+def test_prompts_and_decode_rows_in_one_call(gpu, rt):
+    """Tiles of a prompt beside tiles of single rows of many sequences, and tiles
+    of both: each row comes from one of the kernels."""
+    rng = np.random.default_rng(11)
+    for hk, H, d in ((2, 8, 64), (1, 7, 128), (1, 2, 192)):
+        stride, singles = 96, 150
+        C = stride * singles + 2000
+        ref = random_cache(rng, hk, C, d)
+        start = [stride * i for i in range(singles)] + [stride * singles] * 333
+        end = [s + int(rng.integers(0, stride)) for s in start[:singles]] + [stride * singles + 1500 + i for i in range(333)]
+        start, end = np.array(start), np.array(end)
+        end[[3, 40, 41, 42, 300]] = start[[3, 40, 41, 42, 300]] - 1
+        q = rng.standard_normal((len(end), H, d)).astype(np.float32)
+        for room in (2000, 1 << 20):
+            check(run(gpu, rt, q, ref, end, start, room), ref, q, end, start, room)
+
+
+@pytest.mark.parametrize("T", [3, 80, 200])
 def test_ranges(gpu, rt, T):
     """Windows anywhere, negative and past the cache, max_keys inside a block."""
     rng = np.random.default_rng(T)
@@ -231,12 +252,12 @@ def test_ranges(gpu, rt, T):
     q = rng.standard_normal((T, 8, 64)).astype(np.float32)
     start = rng.integers(-50, C + 40, T)
     end = start + rng.integers(-20, 400, T)
-    for maxk in (1, 33, 250, C):
+    for maxk in (1, 33, 250, C, 1 << 19):
         check(run(gpu, rt, q, ref, end, start, maxk), ref, q, end, start, maxk)
 
 
 @pytest.mark.parametrize("T", [1, 100])
-@pytest.mark.parametrize("maxk", [256, 4096])
+@pytest.mark.parametrize("maxk", [256, 4096, 1 << 17])
 def test_values_at_the_ends(gpu, rt, T, maxk):
     """Blocks of zeros, value scales from 2^-96 to 1e30 beside each other,
     queries of zeros, tiny, large and with large outliers."""
@@ -255,7 +276,7 @@ def test_values_at_the_ends(gpu, rt, T, maxk):
     assert not run(gpu, rt, q, ref, *only_zeros, maxk).any()
 
 
-@pytest.mark.parametrize("T", [2, 90])
+@pytest.mark.parametrize("T", [2, 90, 130])
 def test_not_finite(gpu, rt, T):
     """A marked entry reaches the rows that see it alone; a query that is not
     finite its own row; scores past float32 give NaN."""
@@ -265,6 +286,7 @@ def test_not_finite(gpu, rt, T):
     q = rng.standard_normal((T, 4, 128)).astype(np.float32)
     kend = np.where(np.arange(T) % 2 == 0, 166, 250)
     check(run(gpu, rt, q, ref, kend), ref, q, kend)
+    check(run(gpu, rt, q, ref, kend, None, 1 << 20), ref, q, kend)
     q[0, 1, 3], q[0, 2, 100] = np.nan, np.inf
     got = run(gpu, rt, q, ref, kend)
     assert np.isnan(got[0, 1:3]).all() and np.isfinite(got[0, [0, 3]]).all() and (kend[0] == 166)
@@ -273,6 +295,26 @@ def test_not_finite(gpu, rt, T):
     big = random_cache(rng, 1, 64, 128)
     big.ks[:] = 1e36
     assert np.isnan(run(gpu, rt, np.full((T, 4, 128), 1e10, np.float32), big, np.full(T, 40))).all()
+
+
+@pytest.mark.parametrize("T,room", [(1, 1 << 16), (8, 3000), (200, 1 << 18)])
+def test_the_same_bits_every_time(gpu, rt, T, room):
+    """Nothing depends on the order of workgroups: two calls at once on two
+    streams, each with its workspace, give one call's bits; so does a call with
+    other rows beside these where the cut is the same."""
+    rng = np.random.default_rng(T)
+    ref = random_cache(rng, 2, 3000, 64)
+    q = rng.standard_normal((T, 8, 64)).astype(np.float32)
+    kend = 2999 - np.arange(T)[::-1]
+    want = run(gpu, rt, q, ref, kend, None, room)
+    calls = [Call(gpu, rt, q, ref, kend, None, room) for _ in range(2)]
+    streams = [rt.Stream(), rt.Stream()]
+    for _ in range(3):
+        for c, s in zip(calls, streams):
+            c.enqueue(s)
+        for c, s in zip(calls, streams):
+            s.sync()
+            assert np.array_equal(c.result(), want)
 
 
 def test_graphs_share_a_workspace(gpu, rt):
