@@ -28,7 +28,7 @@ struct StoreArgs {
     const int64_t *index, *pos;
     const double* inv_freq;
     int T, H, Hkv, d, rotary, interleaved;
-    int each;       // rows a workgroup looks at
+    int each, runs;  // rows a workgroup looks at; runs of 32 rows, a workgroup of each run in turn
     int store_wgs;  // workgroups that store; those behind them turn q, qw a row
     int qw;
     int64_t C, nb;
@@ -88,7 +88,6 @@ __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
     constexpr int NP = DP / 16;  // pairs of dims that a thread holds
     constexpr int HALF = Q8C_BLOCK * DP, WORDS = (HALF / 16 + 255) / 256;
     __shared__ __align__(16) uint8_t image[HALF];
-    __shared__ float2 turns[ROPE ? Q8C_BLOCK * DP / 2 : 1];
     __shared__ int rows[Q8C_BLOCK];
     __shared__ int2 list[Q8C_BLOCK];  // the entries to store and their rows
     __shared__ float part[4];
@@ -113,7 +112,8 @@ __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
             return;
         }
     }
-    const int y = blockIdx.x % (2u * A.Hkv), hk = y >> 1, half = y & 1, t0 = blockIdx.x / (2u * A.Hkv) * A.each;
+    const int y = blockIdx.x % (2u * A.Hkv), hk = y >> 1, half = y & 1;
+    const int g = blockIdx.x / (2u * A.Hkv), t0 = g % A.runs * 32 + g / A.runs * A.each;
     const int64_t first = tid < A.T ? A.index[tid] : -1;
     // Lane j: row t0 + j and the one before it. The rows that may be a block's
     // first (outside the cache: not stored).
@@ -191,24 +191,17 @@ __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
                 }
             }
         }
-        if constexpr (ROPE) {
-            // meanwhile the thread's cosines and sines, into LDS so that their code
-            // (a kibibyte and more each) stands here once
-            if (half == 0)
-#pragma unroll 1
-                for (int it = tid; it < items; it += 256) {
-                    const int u = (int)(((uint32_t)it * inv_np) >> 20), i = it - u * np;
-                    if (pair_of(i, A.rotary, A.interleaved).rot) turns[it] = turn_of(A.pos[list[u].y], A.inv_freq[i]);
-                }
-        }
 #pragma unroll
         for (int j = 0; j < NP; j++) {
             const int it = tid + 256 * j;
             if (it >= items) continue;
             float &xa = xs[2 * j], &xb = xs[2 * j + 1];
             if (ROPE && half == 0) {
-                const int i = it - (int)(((uint32_t)it * inv_np) >> 20) * np;
-                if (pair_of(i, A.rotary, A.interleaved).rot) turn(xa, xb, turns[it]);
+                // (unrolled, so that the pairs' sines overlap; a loop of one copy into
+                // LDS is 0.3 us faster where the code is cold, but 7.7 against 5.8 us
+                // for 64 rows of 8 heads of 128 dims and 47 against 38 us for 2048)
+                const int u = (int)(((uint32_t)it * inv_np) >> 20), i = it - u * np;
+                if (pair_of(i, A.rotary, A.interleaved).rot) turn(xa, xb, turn_of(A.pos[list[u].y], A.inv_freq[i]));
             }
             if (!(finite_bits(xa) && finite_bits(xb))) {
                 atomicOr(&newbad, 1u << list[(uint32_t)it * inv_np >> 20].x);
@@ -316,10 +309,20 @@ __global__ __launch_bounds__(256) void load_q8_kernel(const uint8_t* __restrict_
 
 template <bool ROPE>
 hipError_t launch_store(StoreArgs a, hipStream_t s) {
-    // One row a workgroup for a decode batch, whose rows are a block each;
-    // several of a prompt, of which one in 32 begins a block.
-    a.each = a.T <= 128 ? 1 : (a.T <= 2048 ? 16 : 32);
-    a.store_wgs = (a.T + a.each - 1) / a.each * 2 * a.Hkv;
+    // A decode batch's rows are a block each and want a workgroup each; of a
+    // prompt's, one in 32 begins a block. The workgroups of every 32nd row come
+    // one after another in the grid (then those of the rows behind these), so
+    // that a prompt's, which all have such a row or all the one at the same
+    // place, are spread over the compute units, and the rest end in their
+    // shadow: 10.8 us for a prompt of 2048 rows of 8 heads of 128 dims, in the
+    // rows' order 18.2. Rows a workgroup: prompts of 512 / 1024 / 2048 / 4000
+    // rows 7.4 / 8.4 / 15.8 / 30.5 us with 2, 7.3 / 8.2 / 10.8 / 19.8 with 8;
+    // decode batches of 128 / 256 / 512 / 1024 / 2048 rows 7.1 / 11.2 / 23 / 42 /
+    // 80 with 2, 15.6 / 17 / 26 / 47 / 79 with 8. 64 decode rows 4.9 us one by one
+    // in their order (as a prompt 6.9), 6.1 (6.5) by twos.
+    a.each = a.T <= 64 ? 1 : (a.T <= 1024 ? 2 : 8);
+    a.runs = a.T <= 64 ? 1 : (a.T + 31) / 32;
+    a.store_wgs = (a.T <= 64 ? a.T : a.runs * (32 / a.each)) * 2 * a.Hkv;
     const int rounds = (a.H + 256 / (a.d / 2) - 1) / (256 / (a.d / 2));  // heads a thread turns alone in its row
     a.qw = a.T <= 64 ? rounds : 1;
     const dim3 grid((unsigned)(a.store_wgs + (ROPE ? a.T * a.qw : 0)));
