@@ -318,9 +318,10 @@ hipError_t launch_store(StoreArgs a, hipStream_t s) {
     // rows' order 18.2. Rows a workgroup: prompts of 512 / 1024 / 2048 / 4000
     // rows 7.4 / 8.4 / 15.8 / 30.5 us with 2, 7.3 / 8.2 / 10.8 / 19.8 with 8;
     // decode batches of 128 / 256 / 512 / 1024 / 2048 rows 7.1 / 11.2 / 23 / 42 /
-    // 80 with 2, 15.6 / 17 / 26 / 47 / 79 with 8. 64 decode rows 4.9 us one by one
-    // in their order (as a prompt 6.9), 6.1 (6.5) by twos.
-    a.each = a.T <= 64 ? 1 : (a.T <= 1024 ? 2 : 8);
+    // 80 with 2, 15.6 / 17 / 26 / 47 / 79 with 8. 4 prompts of 1000 rows of 64 dims
+    // 18.4 us with 8, 15.9 with 32. 64 decode rows 4.9 us one by one in their
+    // order (as a prompt 6.9), 6.1 (6.5) by twos.
+    a.each = a.T <= 64 ? 1 : (a.T <= 1024 ? 2 : (a.T <= 2048 ? 8 : 32));
     a.runs = a.T <= 64 ? 1 : (a.T + 31) / 32;
     a.store_wgs = (a.T <= 64 ? a.T : a.runs * (32 / a.each)) * 2 * a.Hkv;
     const int rounds = (a.H + 256 / (a.d / 2) - 1) / (256 / (a.d / 2));  // heads a thread turns alone in its row

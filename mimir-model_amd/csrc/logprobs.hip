@@ -74,9 +74,9 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
     __shared__ float red[3][4];
     __shared__ uint32_t tmax[256];
     __shared__ uint64_t cand[KMAX * 4 * VEC + KMAX + 7];
-    __shared__ int cnt[4], steps[VEC];
+    __shared__ int cnt[2][4];
     __shared__ uint32_t tau_s;
-    __shared__ int ncand, nequal;
+    __shared__ int ncand;
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63;
     const int row = blockIdx.x / (unsigned)A.chunks, chunk = blockIdx.x - row * A.chunks;
     const float* xr = A.x + (int64_t)row * A.ld;
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
     for (int j = 0; j < 4 * VEC; j++) mx = fmaxf(mx, x[j]);
     const float wm = wave_max_f32(mx);
     if (l == 0) red[0][w] = wm;
-    if (tid == 0) ncand = nequal = 0;
+    if (tid == 0) ncand = 0;
     // the thread's largest value as a number; 0 where it holds no logit
     tmax[tid] = i0 < A.n ? order_of(mx) : 0u;
     __syncthreads();
@@ -149,12 +149,13 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
     auto key = [&](int j) {
         return (uint64_t)order_of(x[j]) << 32 | (uint32_t)~(uint32_t)(i0 + 1024 * (j >> 2) + (j & 3));
     };
-    int mine = 0, eq = 0;
+    uint32_t same = 0;  // the thread's values equal to tau
     if (mx >= tf) {
+        int mine = 0;
 #pragma unroll
         for (int j = 0; j < 4 * VEC; j++) {
             mine += x[j] > tf ? 1 : 0;
-            eq += x[j] == tf && i0 + 1024 * (j >> 2) + (j & 3) < A.n ? 1 : 0;
+            same |= x[j] == tf && i0 + 1024 * (j >> 2) + (j & 3) < A.n ? 1u << j : 0u;
         }
         if (mine) {
             int at = atomicAdd(&ncand, mine);
@@ -162,52 +163,35 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
             for (int j = 0; j < 4 * VEC; j++)
                 if (x[j] > tf) cand[at++] = key(j);
         }
-        if (eq) atomicAdd(&nequal, eq);
     }
     __syncthreads();
-    const int above = ncand, have = nequal;
-    __syncthreads();
-    const int need = A.top - above;
-    if (need > 0 && have > 0) {
-        // Those equal to tau of the lowest indices, 1024 j + 4 thread + b: all of
-        // the first steps j, and of the one where `need` is reached the first
-        // threads'.
-        uint32_t same = 0;
-        if (eq)
+    // Then those equal to tau of the lowest indices, 1024 j + 4 thread + b, step
+    // by step until there are k (mostly one step: they are one, or a mask's).
+    int c = ncand;
+    for (int j = 0; j < VEC && c < A.top; j++) {
+        const uint32_t four = (same >> (4 * j)) & 15u;
+        int n = 0, at = 0;
 #pragma unroll
-            for (int j = 0; j < 4 * VEC; j++) same |= x[j] == tf && i0 + 1024 * (j >> 2) + (j & 3) < A.n ? 1u << j : 0u;
-        if (tid < VEC) steps[tid] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            int n = 0;
-#pragma unroll
-            for (int b = 0; b < 4; b++) n += __popcll(__ballot((same >> (4 * j + b)) & 1));
-            if (l == 0 && n) atomicAdd(&steps[j], n);
+        for (int b = 0; b < 4; b++) {
+            const unsigned long long has = __ballot((four >> b) & 1);
+            n += __popcll(has);
+            at += __popcll(has & ((1ull << l) - 1));
         }
+        if (l == 0) cnt[j & 1][w] = n;
         __syncthreads();
-        int left = need, last = 0;  // the step where `need` is reached, and what is left for it
-        while (last < VEC - 1 && steps[last] < left) left -= steps[last++];
-        const int here = __popc((same >> (4 * last)) & 15u);
-        int before = here;
+        at += c;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(before, o);
-            before += l >= o ? v : 0;
+        for (int i = 0; i < 4; i++) {
+            const int v = cnt[j & 1][i];
+            at += i < w ? v : 0;
+            c += v;
         }
-        if (l == 63) cnt[w] = before;
-        __syncthreads();
-        before -= here;
-        for (int j = 0; j < w; j++) before += cnt[j];
 #pragma unroll
-        for (int j = 0; j < 4 * VEC; j++) {
-            if (!((same >> j) & 1)) continue;
-            const int step = j >> 2;
-            if (step < last || (step == last && before++ < left)) cand[atomicAdd(&ncand, 1)] = key(j);
-        }
-        __syncthreads();
+        for (int b = 0; b < 4; b++)
+            if (((four >> b) & 1) && at < A.top) cand[at++] = (uint64_t)order_of(tf) << 32 | (uint32_t)~(uint32_t)(i0 + 1024 * j + b);
     }
-    ranked(cand, ncand, A.top, A.keys + ((int64_t)row * A.chunks + chunk) * A.top);
+    c = min(c, max(A.top, ncand));
+    ranked(cand, c, A.top, A.keys + ((int64_t)row * A.chunks + chunk) * A.top);
 }
 
 constexpr int MAX_CHUNKS = 256;
