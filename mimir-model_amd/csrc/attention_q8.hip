@@ -19,6 +19,20 @@
 // needs no scaling by block. M moves only when a column's new maximum passes
 // it by 2^7 (weights are taken 2^8 up, so they stay below 2^15): the rescaling
 // of O is rare, and no maximum crosses lanes otherwise.
+//
+// Bound: few rows (few_kernel) by the cache's bytes, read once for the query
+// heads of a kv head; many rows of one sequence (many_kernel) by the matrix
+// cores, 8 d flops a (query, key) pair with the two parts, 1240 to 1264 TFLOP/s
+// in a large f16 product. Measured on MI355X, 32 heads, 8 kv heads, d = 128:
+//   64 sequences of 2048 keys   41 us, 233 MB: 5.7 TB/s (a read kernel 7.05)
+//   1 sequence of 131072 keys   51 us, 269 MB; 5 of them join_kernel
+//   8 sequences of 2048 keys    10.2 us and join_kernel's 3.1: mostly the way
+//                               from the launch to the first weight
+//   2048 rows behind 6100 keys  389 to 414 us, 478 GFLOP: 1.15 to 1.23 PFLOP/s
+// d = 64, one row of 181 keys 5.7 us. The two parts cost the decode rows nothing
+// that shows (their products take 16 us of the 41, under the loads) and a prompt
+// twice its products; with one part the outputs' error would be 2^-11, not
+// float32's.
 #include <algorithm>
 
 #include "cache_q8.hpp"
@@ -248,16 +262,6 @@ __device__ __forceinline__ int wave_min_i32(int v) {
 }
 __device__ __forceinline__ int wave_max_i32(int v) { return -wave_min_i32(-v); }
 
-__device__ __forceinline__ int wave_sum_i32(int v) {
-    v += lane_xor<32>(v);
-    v += lane_xor<16>(v);
-    v += lane_xor<8>(v);
-    v += lane_xor<4>(v);
-    v += lane_xor<2>(v);
-    v += lane_xor<1>(v);
-    return __builtin_amdgcn_readfirstlane(v);
-}
-
 constexpr int MAX_COLS = 128;  // columns of a tile of many_kernel, and so tokens
 
 // The blocks that a workgroup's columns see, as disjoint rising ranges.
@@ -286,8 +290,9 @@ __device__ __forceinline__ Spans spans_of(const Args& A, int tile) {
 // token and 16 heads, at 0.7 ns from the caches. By a whole wave.
 __device__ __forceinline__ bool takes_many(const Args& A, const Spans& p, int cols) {
     const int span = wave_max_i32(max(p.e0, p.e1)) - wave_min_i32(min(p.e0 ? p.s0 : 0x7fffffff, p.e1 ? p.s1 : 0x7fffffff));
-    const int64_t sum = (int64_t)wave_sum_i32(p.e0 - p.s0 + (p.e1 - p.s1)) * ((A.G + COLS - 1) / COLS);
-    return sum > 0 && span >= A.least && sum >= (int64_t)(cols / 16) * span;
+    // (128 spans of 2^25 blocks pass an int; both kernels round the sum alike)
+    const float sum = wave_sum_f32((float)(p.e0 - p.s0) + (float)(p.e1 - p.s1)) * (float)((A.G + COLS - 1) / COLS);
+    return sum > 0.f && span >= A.least && sum >= (float)(cols / 16) * (float)span;
 }
 // By one wave.
 __device__ __forceinline__ void join_ranges(const Spans& p, Ranges& r) {
@@ -460,10 +465,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
 }
 
 // Many rows: a workgroup per (tile of whole tokens, at most 64 NCT columns, kv
-// head, split of the keys), 16 NCT columns a wave. A block's record is widened once for the four
-// waves into LDS, in operand order (two buffers: the next block is written and
-// the one after it in flight while a block is worked on), and an operand read
-// from there serves 2 NCT products.
+// head, split of the keys), 16 NCT columns a wave. A block's record is widened
+// once for the four waves into LDS, in operand order, and an operand read from
+// there serves 2 NCT products. Three buffers, one barrier a block: while a
+// block is worked on, the next one's scores are taken, the one after it is
+// written, and the one after that is in flight.
 template <int DP, int NCT>
 __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
     constexpr int WC = 16 * NCT, PIECES = DP / 64;  // columns a wave; 16-byte pieces of a record a thread

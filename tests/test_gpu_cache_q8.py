@@ -81,7 +81,7 @@ def test_appends(gpu, rt, hk, d, C):
         assert np.array_equal(g[:C], w.astype(np.float32)) and not g[C:C + 2].any() and np.array_equal(g[C + 2], w[5])
 
 
-@pytest.mark.parametrize("T", [1, 2, 31, 33, 200, 700])
+@pytest.mark.parametrize("T", [1, 2, 31, 33, 200, 700, 1500, 2600])
 def test_indices_in_any_order(gpu, rt, T):
     """Shuffled rows, the same index twice and more, rows outside the cache
     (its last, partial block's unused entries too), many rows a block."""
@@ -120,8 +120,8 @@ def test_scales_and_marks(gpu, rt):
 
 
 @pytest.mark.parametrize("H,hk,d,rotary,inter", [(4, 2, 64, 64, 1), (8, 8, 128, 128, 0), (6, 3, 80, 48, 0), (14, 2, 64, 32, 1),
-                                                 (2, 1, 256, 256, 0)])
-@pytest.mark.parametrize("T", [1, 5, 70])
+                                                 (2, 1, 256, 256, 0), (1030, 1, 256, 64, 1), (600, 600, 8, 8, 0)])
+@pytest.mark.parametrize("T", [1, 5, 70, 1100])
 def test_rope_and_store_in_one_launch(gpu, rt, T, H, hk, d, rotary, inter):
     rng = np.random.default_rng(T + d)
     C = 128

@@ -127,6 +127,25 @@ def test_ties_masks_and_orders(gpu, rt, n, top):
     check(run(gpu, rt, x, t, top), x, t, top)
 
 
+@pytest.mark.parametrize("top", [1, 5, 40, 64])
+def test_few_equal_values_far_apart(gpu, rt, top):
+    """Rows of a few values, each a handful of times all over a row: the ones
+    that share the last place are the lowest indices, wherever they lie."""
+    rng = np.random.default_rng(top)
+    n = 20011
+    x = np.full((24, n), -3.0, np.float32)
+    for r in range(24):
+        for value in (2.0, 1.0, 0.0, -1.0):
+            many = int(rng.integers(0, [2, 9, 40, 90][r % 4]))
+            x[r, rng.integers(0, n, many)] = value
+        if r % 3 == 0:
+            x[r, x[r] == -3.0] = -np.inf
+            x[r, rng.integers(0, n)] = 0.5
+    t = rng.integers(0, n, 24)
+    t[::3] = [int(np.flatnonzero(x[r] == 0.5)[0]) for r in range(0, 24, 3)]
+    check(run(gpu, rt, x, t, top), x, t, top)
+
+
 def test_not_finite(gpu, rt):
     """NaN and +inf, and -inf alone, make a row's results NaN, no other row's;
     NaN is never among the alternatives."""
