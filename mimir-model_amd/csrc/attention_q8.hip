@@ -26,9 +26,9 @@
 // in a large f16 product. Measured on MI355X, 32 heads, 8 kv heads, d = 128:
 //   64 sequences of 2048 keys   41 us, 233 MB: 5.7 TB/s (a read kernel 7.05)
 //   1 sequence of 131072 keys   51 us, 269 MB; 5 of them join_kernel
-//   8 sequences of 2048 keys    10.2 us and join_kernel's 3.1: mostly the way
+//   8 sequences of 2048 keys    10.1 us and join_kernel's 3.1: mostly the way
 //                               from the launch to the first weight
-//   2048 rows behind 6100 keys  389 to 414 us, 478 GFLOP: 1.15 to 1.23 PFLOP/s
+//   2048 rows behind 6100 keys  394 us, 478 GFLOP: 1.21 PFLOP/s
 // d = 64, one row of 181 keys 5.7 us. The two parts cost the decode rows nothing
 // that shows (their products take 16 us of the 41, under the loads) and a prompt
 // twice its products; with one part the outputs' error would be 2^-11, not
@@ -172,11 +172,12 @@ struct State {
 // A block's value scale for the exponents: log2 and reciprocal (of a block of
 // zeros the floor's; its weights are left out below).
 struct Scale {
-    float lv, iv;
+    float lv, iv, lv8;
 };
 __device__ __forceinline__ Scale value_scale(const Scales& m) {
     const float vs = m.vs > 0.f ? m.vs : Q8C_FLOOR;
-    return {__builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+    const float lv = __builtin_amdgcn_logf(vs);
+    return {lv, __builtin_amdgcn_rcpf(vs), lv + 8.f};
 }
 // The factor of a block's scores; at least float32's smallest normal number, so
 // that -inf times it is -inf (a NaN stays).
@@ -184,12 +185,18 @@ __device__ __forceinline__ float key_scale(float scale, const Scales& m) {
     const float c = scale * m.ks;
     return c < 1.17549435e-38f ? 1.17549435e-38f : c;
 }
+// (In a chain: v_max3_f32 takes products as they come, v_max_f32 wants each
+// made canonical first, one instruction more.)
 __device__ __forceinline__ float largest(v4f s0, v4f s1) {
-    return fmaxf(fmaxf(fmaxf(s0.x, s0.y), fmaxf(s0.z, s0.w)), fmaxf(fmaxf(s1.x, s1.y), fmaxf(s1.z, s1.w)));
+    const float a = fmaxf(fmaxf(s0.x, s0.y), s0.z), b = fmaxf(fmaxf(a, s0.w), s1.x), c = fmaxf(fmaxf(b, s1.y), s1.z);
+    return fmaxf(c, s1.w);
 }
-// Whether a lane's scores need no more than weights() of them: M is near
-// enough, and no weight so small that the scale in it could matter. (NaN: no.)
-__device__ __forceinline__ bool near_enough(float top, float M) { return top <= M + 7.f && top >= M - 60.f; }
+// Whether a lane's scores need no more than their weights: the largest exponent
+// is at most 15 (M is near enough), and not so small, -52, that the scale in it
+// could matter. (NaN: no.)
+__device__ __forceinline__ bool near_enough(float top, float cs, float base) {
+    return __builtin_fabsf(__builtin_fmaf(top, cs, base) + 18.5f) <= 33.5f;
+}
 
 // What a block may need before its weights, in lanes or as a whole: entries
 // that a column does not see (-inf) or that are not finite (NaN), M moved, and
@@ -404,8 +411,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         const bool all_seen = k0 <= Q8C_BLOCK * blk && k0 + n >= Q8C_BLOCK * (blk + 1);
         const Scale v = value_scale(mb);
         const float cs = key_scale(rs.scale, mb);
-        float base = v.lv - S.M + 8.f;
-        if (!all_seen || mb.bad || !(mb.vs > 0.f) || !__all(near_enough(largest(s[0], s[1]) * cs + v.lv, S.M)))
+        float base = v.lv8 - S.M;
+        if (!all_seen || mb.bad || !(mb.vs > 0.f) || __builtin_amdgcn_ballot_w64(near_enough(largest(s[0], s[1]), cs, base)) != ~0ull)
             base = correct<DP>(s[0], s[1], mb, cs, v, blk, g, k0, n, S);
         Weights W;
         const float sum = weigh_tile(s[0], cs, base, W.hi, W.lo) + weigh_tile(s[1], cs, base, W.hi + 2, W.lo + 2);
@@ -590,10 +597,10 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
 #pragma unroll
         for (int ct = 0; ct < NCT; ct++) {
             cs[ct] = key_scale(scale[ct], m);
-            fine &= near_enough(top[ct] * cs[ct] + v.lv, S[ct].M);
-            base[ct] = v.lv - S[ct].M + 8.f;
+            base[ct] = v.lv8 - S[ct].M;
+            fine &= near_enough(top[ct], cs[ct], base[ct]);
         }
-        if (!(Q8C_BLOCK * here >= from && Q8C_BLOCK * (here + 1) <= to && m.bad == 0 && m.vs > 0.f && __all(fine))) {
+        if (!(Q8C_BLOCK * here >= from && Q8C_BLOCK * (here + 1) <= to && m.bad == 0 && m.vs > 0.f && __builtin_amdgcn_ballot_w64(fine) == ~0ull)) {
 #pragma unroll
             for (int ct = 0; ct < NCT; ct++) {
                 const int2 k = R.kn[WC * w + 16 * ct + col];
@@ -639,7 +646,10 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
             k1 = n1;
         }
 #pragma unroll
-        for (int ct = 0; ct < NCT; ct++) S[ct].l = __builtin_fmaf(sum[ct][0] + sum[ct][1], v.iv, S[ct].l);
+        for (int ct = 0; ct < NCT; ct++) {
+            S[ct].l = __builtin_fmaf(sum[ct][0] + sum[ct][1], v.iv, S[ct].l);
+            asm volatile("" : "+v"(S[ct].l));  // (the sums among the products above)
+        }
 #pragma unroll
         for (int x = 0; x < NS; x++) {
             __builtin_amdgcn_sched_barrier(0);
@@ -651,7 +661,10 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
             put(pb, raw, x);
             if (x == NS - 1)
 #pragma unroll
-                for (int ct = 0; ct < NCT; ct++) top[ct] = largest(sn[ct][0], sn[ct][1]);
+                for (int ct = 0; ct < NCT; ct++) {
+                    top[ct] = largest(sn[ct][0], sn[ct][1]);
+                    asm volatile("" : "+v"(top[ct]));  // (here, not behind the products)
+                }
 #pragma unroll
             for (int ct = 0; ct < NCT; ct++) {
                 S[ct].o[2 * x] = mfma(v0, W[ct].r(), S[ct].o[2 * x]);
