@@ -72,7 +72,6 @@ struct Args {
     int splits;      // of the keys, in the workspace
     int few_splits;  // those that few_kernel cuts its rows into
     int tpt, fan;    // tokens a tile of many_kernel; workgroups of few_kernel that share one
-    int choose;      // both kernels run: takes_many() says whose a tile is
     int least;       // blocks that many_kernel's tiles span at least
 };
 
@@ -326,8 +325,9 @@ template <int DP>
 constexpr int MANY_COLS = DP <= 128 ? MAX_COLS : MAX_COLS / 2;
 
 // Few rows: a workgroup per (token, kv head, split of the keys) and up to 16
-// query heads (beside many_kernel: for every fan-th token of a tile); its NW
-// waves take the token's blocks in turn, straight from
+// query heads (BESIDE many_kernel: for every fan-th token of a tile; in one
+// instance the loop over tokens cost every call its registers and most of half
+// a microsecond before the first load); its NW waves take the token's blocks in turn, straight from
 // memory, each with a state of its own, joined at the end. A wave has its next
 // block's keys in flight while it works on one, and the values during the
 // score product. The query's parts lie in LDS (for the registers).
@@ -340,17 +340,23 @@ struct FewLds {
     };
     float ml[NW][2][COLS];
 };
-template <int DP>
+template <int DP, bool BESIDE>
 __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A) {
     __shared__ FewLds<DP> S_;
     const int tid = threadIdx.x, l = tid & 63, g = l >> 4, col = l & 15, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     // (divisions only where there is something to divide: a dozen of them are
     // most of a microsecond before the first load)
     const int sub = A.G > COLS ? (int)blockIdx.x / A.Hkv : 0, hk = (int)blockIdx.x - sub * A.Hkv, g0 = sub * COLS;
-    const int ncol = min(COLS, A.G - g0), unit = blockIdx.y, split = blockIdx.z, tile = A.fan > 1 ? unit / A.fan : unit;
-    if (A.choose && takes_many(A, spans_of(A, tile), MANY_COLS<DP>)) return;
-    const int last = min(A.T, (tile + 1) * A.tpt);
-    for (int t = tile * A.tpt + (unit - tile * A.fan); t < last; t += A.fan) {
+    const int ncol = min(COLS, A.G - g0), split = blockIdx.z;
+    int t = blockIdx.y, last = t + 1;
+    if constexpr (BESIDE) {
+        const int unit = blockIdx.y, tile = unit / A.fan;
+        if (takes_many(A, spans_of(A, tile), MANY_COLS<DP>)) return;
+        last = min(A.T, (tile + 1) * A.tpt);
+        t = tile * A.tpt + (unit - tile * A.fan);
+        if (t >= last) return;
+    }
+    do {
     const int head0 = t * A.H + hk * A.G + g0;
     const AttRange r = range_of(A, t);
     Eight x[DP / 32];
@@ -468,7 +474,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
             *(f32x4a4*)(A.out + head * A.d + d4) = none ? v4f{0.f, 0.f, 0.f, 0.f} : o * (L > 0.f ? 1.f / L : __builtin_nanf(""));
         }
     }
-    }
+    } while (BESIDE && (t += A.fan) < last);
 }
 
 // Many rows: a workgroup per (tile of whole tokens, at most 64 NCT columns, kv
@@ -491,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
     const int r0 = ti / turn * turn, tile = (ti / turn) & 1 ? r0 + min(turn, tiles - r0) - 1 - (ti - r0) : ti;
     const int t0 = (tiles - 1 - tile) * A.tpt, cols = min(A.tpt, A.T - t0) * A.G;
     const Spans spans = spans_of(A, tiles - 1 - tile);
-    if (A.choose && !takes_many(A, spans, MANY_COLS<DP>)) return;
+    if (!takes_many(A, spans, MANY_COLS<DP>)) return;
     if (w == 0) join_ranges(spans, R);
     float scale[NCT];
     v8h qhi[NCT][DP / 32], qlo[NCT][DP / 32];
@@ -834,8 +840,9 @@ hipError_t launch(Args A, const Cut& c, hipStream_t s) {
     A.tpt = c.tpt;
     A.fan = c.fan;
     A.least = c.least;
-    A.choose = c.many ? 1 : 0;
-    hipLaunchKernelGGL(few_kernel<DP>, dim3((unsigned)(A.Hkv * c.subs), (unsigned)c.units, (unsigned)c.few_splits), dim3(64 * NW), 0, s, A);
+    const dim3 few((unsigned)(A.Hkv * c.subs), (unsigned)c.units, (unsigned)c.few_splits);
+    if (!c.many) hipLaunchKernelGGL((few_kernel<DP, false>), few, dim3(64 * NW), 0, s, A);
+    else hipLaunchKernelGGL((few_kernel<DP, true>), few, dim3(64 * NW), 0, s, A);
     if (c.many)
         hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.splits), dim3(256), 0, s, A);
     const int rows = A.T * A.H, groups = 1024 / DP;
