@@ -60,6 +60,7 @@ __device__ __forceinline__ void alternate() {
 
 constexpr float M_NONE = -3.0e38f;  // a column's M before its first key
 constexpr int COLS = 16;            // (token, head) pairs of a tile
+constexpr float DONE = -1.f;        // in place of a sum: the row is written, join_kernel leaves it
 
 struct Args {
     const float* q;  // [T][H][d]
@@ -72,7 +73,7 @@ struct Args {
     int splits;      // of the keys, in the workspace
     int few_splits;  // those that few_kernel cuts its rows into
     int tpt, fan;    // tokens a tile of many_kernel; workgroups of few_kernel that share one
-    int least;       // blocks that many_kernel's tiles span at least
+    int least;       // blocks that a token sees at least, or many_kernel takes none
 };
 
 // Eight cache bytes as f16: 0x6400 | byte is 1024 + value + 128.
@@ -285,20 +286,28 @@ __device__ __forceinline__ int2 span_of(const Args& A, int t) {
     const AttRange r = att_range(A.kend, A.kstart, t, A.C, A.maxk);
     return r.n > 0 ? make_int2((int)(r.k0 >> 5), (int)((r.k0 + r.n + 31) >> 5)) : make_int2(0, 0);
 }
-__device__ __forceinline__ Spans spans_of(const Args& A, int tile) {
-    const int l = threadIdx.x & 63, t = tile * A.tpt + l, last = min(A.T, (tile + 1) * A.tpt);
+// Those of the tokens from t0 up to a tile's number.
+__device__ __forceinline__ Spans spans_of(const Args& A, int t0) {
+    const int l = threadIdx.x & 63, t = t0 + l, last = min(A.T, t0 + A.tpt);
     const int2 a = t < last ? span_of(A, t) : make_int2(0, 0), b = t + 64 < last ? span_of(A, t + 64) : make_int2(0, 0);
     return {a.x, a.y, b.x, b.y};
 }
 // Whether many_kernel takes a tile: its tokens see the same blocks (a prompt),
 // not each its own (a decode batch). many_kernel reads a block once for the
 // tile, at 6 ns (128 columns; MI355X, all CUs busy), few_kernel once for each
-// token and 16 heads, at 0.7 ns from the caches. By a whole wave.
-__device__ __forceinline__ bool takes_many(const Args& A, const Spans& p, int cols) {
+// token and 16 heads, at 0.7 ns from the caches. A last tile with few tokens
+// goes as the last full number of tokens does, not to few_kernel, whose splits
+// are for all tokens (128 rows of 14 heads behind 30000 keys, 18 rows a tile,
+// two in the last: 176 us, 56 so). many_kernel takes no tile unless a token of it,
+// or the call's last, sees `least` blocks. By a whole wave.
+__device__ __forceinline__ bool takes_many(const Args& A, int t0, int cols) {
+    const Spans p = spans_of(A, max(min(t0, A.T - A.tpt), 0));
     const int span = wave_max_i32(max(p.e0, p.e1)) - wave_min_i32(min(p.e0 ? p.s0 : 0x7fffffff, p.e1 ? p.s1 : 0x7fffffff));
     // (128 spans of 2^25 blocks pass an int; both kernels round the sum alike)
     const float sum = wave_sum_f32((float)(p.e0 - p.s0) + (float)(p.e1 - p.s1)) * (float)((A.G + COLS - 1) / COLS);
-    return sum > 0.f && span >= A.least && sum >= (float)(cols / 16) * (float)span;
+    const int2 end = span_of(A, A.T - 1);  // (a prompt's longest: its tiles go one way)
+    const int most = max(wave_max_i32(max(p.e0 - p.s0, p.e1 - p.s1)), end.y - end.x);
+    return sum > 0.f && most >= A.least && sum >= (float)(cols / 16) * (float)span;
 }
 // By one wave.
 __device__ __forceinline__ void join_ranges(const Spans& p, Ranges& r) {
@@ -326,9 +335,10 @@ constexpr int MANY_COLS = DP <= 128 ? MAX_COLS : MAX_COLS / 2;
 
 // Few rows: a workgroup per (token, kv head, split of the keys) and up to 16
 // query heads (BESIDE many_kernel: for every fan-th token of a tile; in one
-// instance the loop over tokens cost every call its registers and most of half
-// a microsecond before the first load); its NW waves take the token's blocks in turn, straight from
-// memory, each with a state of its own, joined at the end. A wave has its next
+// instance the loop over tokens cost every call its registers and nearly half
+// a microsecond before the first load). Its NW waves take the token's blocks
+// in turn, straight from memory, each with a state of its own, joined at the
+// end. A wave has its next
 // block's keys in flight while it works on one, and the values during the
 // score product. The query's parts lie in LDS (for the registers).
 constexpr int NW = 4;
@@ -351,7 +361,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
     int t = blockIdx.y, last = t + 1;
     if constexpr (BESIDE) {
         const int unit = blockIdx.y, tile = unit / A.fan;
-        if (takes_many(A, spans_of(A, tile), MANY_COLS<DP>)) return;
+        if (takes_many(A, tile * A.tpt, MANY_COLS<DP>)) return;
         last = min(A.T, (tile + 1) * A.tpt);
         t = tile * A.tpt + (unit - tile * A.fan);
         if (t >= last) return;
@@ -461,14 +471,15 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
             o += *(const v4f*)&S_.o[j][c][d4] * (f * f);
         }
         const int64_t head = head0 + c;
-        if (A.splits > 1) {
+        const bool whole = A.splits == 1 || (BESIDE && A.few_splits == 1);
+        float2* ml = (float2*)(A.part + (int64_t)A.splits * rows * DP);
+        if (BESIDE && A.splits > 1 && whole && d4 == 0) ml[head] = make_float2(0.f, DONE);
+        if (!whole) {
             const int64_t at = (int64_t)split * rows + head;
-            if (d4 == 0)
-                ((float2*)(A.part + (int64_t)A.splits * rows * DP))[at] = make_float2(none ? -__builtin_inff() : M, L);
+            if (d4 == 0) ml[at] = make_float2(none ? -__builtin_inff() : M, L);
             if (!none) *(v4f*)(A.part + at * DP + d4) = o;
             if (d4 == 0 && split == 0)  // (splits that few_kernel does not use)
-                for (int y = A.few_splits; y < A.splits; y++)
-                    ((float2*)(A.part + (int64_t)A.splits * rows * DP))[y * rows + head] = make_float2(-__builtin_inff(), 0.f);
+                for (int y = A.few_splits; y < A.splits; y++) ml[y * rows + head] = make_float2(-__builtin_inff(), 0.f);
         } else if (d4 < A.d) {
             // a row that sees no key gives zeros, one whose weights are all zero NaN
             *(f32x4a4*)(A.out + head * A.d + d4) = none ? v4f{0.f, 0.f, 0.f, 0.f} : o * (L > 0.f ? 1.f / L : __builtin_nanf(""));
@@ -496,9 +507,8 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
     const int tiles = gridDim.x / (unsigned)A.Hkv, turn = max(256 / A.Hkv, 1), ti = blockIdx.x / (unsigned)A.Hkv;
     const int r0 = ti / turn * turn, tile = (ti / turn) & 1 ? r0 + min(turn, tiles - r0) - 1 - (ti - r0) : ti;
     const int t0 = (tiles - 1 - tile) * A.tpt, cols = min(A.tpt, A.T - t0) * A.G;
-    const Spans spans = spans_of(A, tiles - 1 - tile);
-    if (!takes_many(A, spans, MANY_COLS<DP>)) return;
-    if (w == 0) join_ranges(spans, R);
+    if (!takes_many(A, t0, MANY_COLS<DP>)) return;
+    if (w == 0) join_ranges(spans_of(A, t0), R);
     float scale[NCT];
     v8h qhi[NCT][DP / 32], qlo[NCT][DP / 32];
     State<DP> S[NCT];
@@ -737,6 +747,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
     if constexpr (WIDE) {
         const int l = tid & 63;
         const float2 x = l < A.splits ? pml[l * rows + row] : make_float2(-__builtin_inff(), 0.f);  // at most 64 splits
+        if (__shfl(x.y, 0) == DONE) return;
         const bool none = x.x == -__builtin_inff();
         M = wave_max_f32(x.x);
         const float wh = none ? 0.f : exp2_hw(0.5f * (x.x - M));
@@ -760,6 +771,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
             v4f v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = s0 + j < A.splits ? pml[(s0 + j) * rows + row] : make_float2(-__builtin_inff(), 0.f);
+            if (s0 == 0 && x[0].y == DONE) return;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int s = min(s0 + j, A.splits - 1);
@@ -808,23 +820,28 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     Cut c{};
     // Prompts of many tokens are many_kernel's, a decode batch of as many
     // sequences few_kernel's: the ranges, on the device, tell them apart, so
-    // both are launched, and each leaves the other's tiles (3 to 4 us). Alone,
-    // few_kernel is ahead below 96 tokens (d = 64 and 128, 8 kv heads, 64
-    // tokens: 22 and 30 us behind 2000 cached ones, many_kernel the same; 128
-    // tokens: 35 and 51 us against 27 and 33) and where the keys are few (512
-    // tokens, nothing cached: 30 and 44 us against 34 and 40; 1024: 79 and 122
-    // against 57 and 73). Below 192 tokens many_kernel is left the tiles that
-    // span 24 blocks and more (128 tokens, nothing cached: 7 and 10 us against
-    // 13 and 17).
-    c.least = T < 192 ? 24 : 0;
-    c.many = T >= 96 && G <= cols && blocks >= c.least && T * Hkv * subs * blocks >= 1 << 16;
+    // both are launched, and each leaves the other's tiles (a decode batch pays some
+    // 10 us of 50 and more, so not for smaller ones). A prompt's rows cost few_kernel their number
+    // times the blocks, many_kernel a start of some 20 us; they meet near 5000
+    // row-blocks of 8 kv heads (64 rows behind 2000 / 8000 keys 19 and 54 us
+    // against 23 and 34 at d = 64, 27 and 89 against 32 and 45 at 128; 128 rows
+    // behind 1000 / 2000 keys 18 and 29 against 24 and 27, 28 and 46 against 33
+    // and 34; 256 rows behind none / 1000 12 and 33 against 18 and 31). The
+    // host knows max_keys, the device what the rows see, so that many blocks are
+    // asked for there too (below 512 rows, which see that many by themselves).
+    const int64_t rows = T * Hkv * subs;
+    c.least = T < 512 ? (int)(40000 / rows) : 0;
+    c.many = T >= 64 && G <= cols && blocks >= c.least && rows * blocks >= 1 << 16;
     c.tpt = c.many ? (int)(cols / G) : 1;
     const int64_t tiles = (T + c.tpt - 1) / c.tpt;
     c.many_wgs = tiles * Hkv;
     c.fan = 1;
     if (c.many) {
-        const int64_t f = (512 + c.many_wgs * subs - 1) / (c.many_wgs * subs);
-        c.fan = (int)(f < c.tpt ? f : c.tpt);
+        // Tokens a workgroup of few_kernel beside many_kernel, equally many: of d =
+        // 64 a CU takes four (256 rows of 2000 keys each 86 us, in twos 100), of d =
+        // 128 two are enough (164 us, in fours 178).
+        const int64_t each = std::max<int64_t>(rows / (d <= 64 ? 1024 : 512), 1);
+        c.fan = (int)((c.tpt + each - 1) / each);
     }
     c.units = tiles * c.fan;
     c.subs = subs;

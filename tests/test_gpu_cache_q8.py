@@ -200,7 +200,7 @@ def check(got, ref, q, kend, kstart=None, maxk=None):
 # kernel beside the other)
 @pytest.mark.parametrize("room", [None, 1 << 18])
 @pytest.mark.parametrize("T,H,hk,d,slots,stride", [
-    (100, 144, 1, 64, 1, 250), (97, 34, 1, 64, 2, 150), (260, 8, 8, 128, 1, 900), (120, 3, 1, 256, 1, 400), (1, 1, 1, 64, 1, 32), (1, 4, 1, 8, 1, 1), (1, 32, 8, 64, 1, 181), (2, 16, 16, 128, 2, 33), (3, 14, 2, 64, 3, 500),
+    (100, 144, 1, 64, 1, 250), (128, 14, 2, 64, 1, 1400), (64, 8, 2, 128, 1, 2500), (109, 14, 2, 128, 3, 260), (97, 34, 1, 64, 2, 150), (260, 8, 8, 128, 1, 900), (120, 3, 1, 256, 1, 400), (1, 1, 1, 64, 1, 32), (1, 4, 1, 8, 1, 1), (1, 32, 8, 64, 1, 181), (2, 16, 16, 128, 2, 33), (3, 14, 2, 64, 3, 500),
     (8, 32, 8, 128, 8, 300), (5, 40, 2, 80, 5, 77), (1, 34, 2, 256, 1, 700), (4, 6, 3, 192, 2, 129), (1, 8, 2, 128, 1, 6000),
     (1, 3, 1, 64, 1, 20001), (64, 4, 2, 64, 16, 70), (70, 14, 2, 64, 7, 90), (200, 32, 8, 128, 1, 200), (133, 8, 8, 64, 1, 300),
     (130, 34, 2, 80, 3, 130), (181, 14, 2, 64, 1, 181), (65, 12, 4, 256, 2, 100), (150, 16, 2, 128, 150, 13), (300, 6, 2, 192, 2, 400)])
