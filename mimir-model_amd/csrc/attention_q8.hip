@@ -34,6 +34,7 @@
 // twice its products; with one part the outputs' error would be 2^-11, not
 // float32's.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_q8.hpp"
 #include "decoder_math.hpp"
@@ -60,7 +61,8 @@ __device__ __forceinline__ void alternate() {
 
 constexpr float M_NONE = -3.0e38f;  // a column's M before its first key
 constexpr int COLS = 16;            // (token, head) pairs of a tile
-constexpr float DONE = -1.f;        // in place of a sum: the row is written, join_kernel leaves it
+// In place of a split's sum: the row is written (split 0); no more splits.
+constexpr float DONE = -1.f, STOP = -2.f;
 
 struct Args {
     const float* q;  // [T][H][d]
@@ -70,9 +72,11 @@ struct Args {
     int64_t C, maxk, nb;
     float* out;      // [T][H][d]
     float* part;     // [splits][T * H][DP] sums, then [splits][T * H] of {M, l}
-    int splits;      // of the keys, in the workspace
-    int few_splits;  // those that few_kernel cuts its rows into
-    int tpt, fan;    // tokens a tile of many_kernel; workgroups of few_kernel that share one
+    int splits;      // of the keys, places in the workspace
+    int few_splits;  // those that few_kernel cuts a token's keys into
+    int many_splits; // and many_kernel a tile's
+    int tpt, fan;    // tokens a tile of many_kernel; groups of workgroups of few_kernel that share one
+    int group, inv;  // tokens whose columns fit a tile of 16; 256 / G, rounded up: c / G = c * inv / 256
     int least;       // blocks that a token sees at least, or many_kernel takes none
 };
 
@@ -349,33 +353,87 @@ struct FewLds {
         float o[NW][COLS][DP + 4];  // rows four banks apart
     };
     float ml[NW][2][COLS];
+    int keys[COLS];  // that a column sees (a group's)
 };
-template <int DP, bool BESIDE>
+template <int DP, bool BESIDE, bool GROUP>
 __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A) {
     __shared__ FewLds<DP> S_;
     const int tid = threadIdx.x, l = tid & 63, g = l >> 4, col = l & 15, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     // (divisions only where there is something to divide: a dozen of them are
     // most of a microsecond before the first load)
-    const int sub = A.G > COLS ? (int)blockIdx.x / A.Hkv : 0, hk = (int)blockIdx.x - sub * A.Hkv, g0 = sub * COLS;
-    const int ncol = min(COLS, A.G - g0), split = blockIdx.z;
-    int t = blockIdx.y, last = t + 1;
+    const int sub = GROUP || A.G > COLS ? (int)blockIdx.x / A.Hkv : 0, hk = (int)blockIdx.x - sub * A.Hkv;
+    const int g0 = GROUP ? 0 : sub * COLS, P = GROUP ? A.group : 1;  // (GROUP: sub is the workgroup's place)
+    int t0 = (int)blockIdx.y * P, last = min(A.T, t0 + P);
     if constexpr (BESIDE) {
         const int unit = blockIdx.y, tile = unit / A.fan;
         if (takes_many(A, tile * A.tpt, MANY_COLS<DP>)) return;
         last = min(A.T, (tile + 1) * A.tpt);
-        t = tile * A.tpt + (unit - tile * A.fan);
-        if (t >= last) return;
+        t0 = tile * A.tpt + (unit - tile * A.fan) * P;
+        if (t0 >= last) return;
     }
     do {
-    const int head0 = t * A.H + hk * A.G + g0;
-    const AttRange r = range_of(A, t);
+    // The workgroup's columns: heads of a token, or of the group's tokens.
+    const int t = t0 + (GROUP ? sub : 0);
+    const AttRange own = range_of(A, min(t, A.T - 1));
+    int head0 = t * A.H + hk * A.G + g0, step = 0, ncol = min(COLS, A.G - g0);
+    int split = blockIdx.z, nsplit = A.few_splits;
+    int k0 = (int)own.k0, n = (int)own.n;  // the keys that the lane's column sees
+    int from = k0, to = k0 + n;            // and those that all columns see
+    int b0 = k0 >> 5, total = n > 0 ? ((k0 + n + 31) >> 5) - b0 : 0;
+    bool packed = false;
+    if constexpr (GROUP) {
+        const int tc = (col * A.inv) >> 8, tn = min(P, last - t0);
+        const AttRange r = att_range(A.kend, A.kstart, t0 + min(tc, tn - 1), A.C, A.maxk);
+        const int rn = (int)r.n;
+        int lo = rn > 0 ? (int)r.k0 : 0x7fffffff, hi = rn > 0 ? (int)r.k0 + rn : 0;
+        int sum = rn > 0 && tc < tn && col == tc * A.G ? rn : 0;
+        auto row16 = [&](auto f) {
+            f(std::integral_constant<int, 1>{});
+            f(std::integral_constant<int, 2>{});
+            f(std::integral_constant<int, 4>{});
+            f(std::integral_constant<int, 8>{});
+        };
+        row16([&](auto m) {
+            lo = min(lo, lane_xor<m.value>(lo));
+            hi = max(hi, lane_xor<m.value>(hi));
+            sum += lane_xor<m.value>(sum);
+        });
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        sum = __builtin_amdgcn_readfirstlane(sum);
+        packed = tn > 1 && hi > lo && (float)sum >= 0.75f * (float)tn * (float)(hi - lo);
+        if (packed) {
+            k0 = (int)r.k0;
+            n = rn;
+            from = k0;
+            to = rn > 0 ? k0 + rn : 0;
+            row16([&](auto m) {
+                from = max(from, lane_xor<m.value>(from));
+                to = min(to, lane_xor<m.value>(to));
+            });
+            from = __builtin_amdgcn_readfirstlane(from);
+            to = __builtin_amdgcn_readfirstlane(to);
+            b0 = lo >> 5;
+            total = ((hi + 31) >> 5) - b0;
+            head0 = t0 * A.H + hk * A.G;
+            step = A.H - A.G;
+            ncol = tn * A.G;
+            nsplit = min(min(A.few_splits * P, A.splits), (total + 7) / 8);
+            split = split * P + sub;
+            if (w == 0 && l < COLS) S_.keys[l] = n;
+        } else if (sub >= tn) {
+            split = nsplit;  // (nothing for this one)
+        }
+    }
+    b0 = __builtin_amdgcn_readfirstlane(b0);
+    total = __builtin_amdgcn_readfirstlane(total);
+    if (split < nsplit) {
+    const int mycol = min(col, ncol - 1);
     Eight x[DP / 32];
-    const float* row = A.q + (int64_t)(head0 + min(col, ncol - 1)) * A.d;
+    const float* row = A.q + (int64_t)(head0 + mycol + (GROUP ? ((mycol * A.inv) >> 8) * step : 0)) * A.d;
 #pragma unroll
     for (int s = 0; s < DP / 32; s++) x[s] = query_step(row, A.d, s, g);
-    const int k0 = (int)r.k0, n = (int)r.n;
-    const int b0 = k0 >> 5, total = n > 0 ? ((k0 + n + 31) >> 5) - b0 : 0;
-    const int per = A.few_splits > 1 ? max((total + A.few_splits - 1) / A.few_splits, NW) : max(total, NW);
+    const int per = nsplit > 1 ? max((total + nsplit - 1) / nsplit, NW) : max(total, NW);
     int b = b0 + split * per + w;
     const int b1 = min(b0 + total, b0 + (split + 1) * per);
     const u32x4* rec = (const u32x4*)A.cache + l;
@@ -392,7 +450,6 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
     };
     if (b < b1) fetch_k(b);
     const RowScale rs = row_scale<DP>(x, A.d);
-    __syncthreads();  // (the last token's sums are read)
 #pragma unroll
     for (int s = 0; s < DP / 32; s++)
         if (s % NW == w) two_parts(x[s], rs, S_.q[0][s][l], S_.q[1][s][l]);
@@ -424,7 +481,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         const int blk = b;
         b += NW;
         if (b < b1) fetch_k(b);
-        const bool all_seen = k0 <= Q8C_BLOCK * blk && k0 + n >= Q8C_BLOCK * (blk + 1);
+        const bool all_seen = from <= Q8C_BLOCK * blk && to >= Q8C_BLOCK * (blk + 1);
         const Scale v = value_scale(mb);
         const float cs = key_scale(rs.scale, mb);
         float base = v.lv8 - S.M;
@@ -456,7 +513,6 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         for (int i = 0; i < DP / 16; i++) *(v4f*)&S_.o[w][col][16 * i + 4 * g] = S.o[i];
     __syncthreads();
     const int64_t rows = (int64_t)A.T * A.H;
-    const bool none = split * per >= total;
     for (int i = tid; i < ncol * (DP / 4); i += 64 * NW) {
         const int c = i / (DP / 4), d4 = (i - c * (DP / 4)) * 4;
         float M = S_.ml[0][0][c];
@@ -470,22 +526,24 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
             L += S_.ml[j][1][c] * f * f;
             o += *(const v4f*)&S_.o[j][c][d4] * (f * f);
         }
-        const int64_t head = head0 + c;
-        const bool whole = A.splits == 1 || (BESIDE && A.few_splits == 1);
+        const int64_t head = head0 + c + (GROUP ? ((c * A.inv) >> 8) * step : 0);
+        const bool none = split * per >= total || (GROUP && packed && S_.keys[c] <= 0);
         float2* ml = (float2*)(A.part + (int64_t)A.splits * rows * DP);
-        if (BESIDE && A.splits > 1 && whole && d4 == 0) ml[head] = make_float2(0.f, DONE);
-        if (!whole) {
+        if (nsplit > 1) {
             const int64_t at = (int64_t)split * rows + head;
             if (d4 == 0) ml[at] = make_float2(none ? -__builtin_inff() : M, L);
             if (!none) *(v4f*)(A.part + at * DP + d4) = o;
-            if (d4 == 0 && split == 0)  // (splits that few_kernel does not use)
-                for (int y = A.few_splits; y < A.splits; y++) ml[y * rows + head] = make_float2(-__builtin_inff(), 0.f);
-        } else if (d4 < A.d) {
+            if (d4 == 0 && split == 0 && A.splits > nsplit) ml[nsplit * rows + head] = make_float2(0.f, STOP);
+        } else {
+            if (d4 == 0 && A.splits > 1) ml[head] = make_float2(0.f, DONE);
             // a row that sees no key gives zeros, one whose weights are all zero NaN
-            *(f32x4a4*)(A.out + head * A.d + d4) = none ? v4f{0.f, 0.f, 0.f, 0.f} : o * (L > 0.f ? 1.f / L : __builtin_nanf(""));
+            if (d4 < A.d)
+                *(f32x4a4*)(A.out + head * A.d + d4) = none ? v4f{0.f, 0.f, 0.f, 0.f} : o * (L > 0.f ? 1.f / L : __builtin_nanf(""));
         }
     }
-    } while (BESIDE && (t += A.fan) < last);
+    }
+    if constexpr (BESIDE) __syncthreads();  // (the last group's sums are read)
+    } while (BESIDE && (t0 += A.fan * P) < last);
 }
 
 // Many rows: a workgroup per (tile of whole tokens, at most 64 NCT columns, kv
@@ -535,7 +593,7 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
     from = wave_max_i32(from);
     to = wave_min_i32(to);
     __syncthreads();
-    const int total = R.total, per = max((total + A.splits - 1) / A.splits, 8);
+    const int total = R.total, per = max((total + A.many_splits - 1) / A.many_splits, 8);
     const int p0 = (int)blockIdx.y * per, p1 = min(total, p0 + per);
     // The block of position p (rising): ranges [.., end) lie `shift` above theirs.
     int i = -1, end = 0, shift = 0;
@@ -715,8 +773,11 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
         const bool none = p0 >= p1 || R.kn[WC * w + 16 * ct + col].y <= 0;
         if (A.splits > 1) {
             const int64_t at = (int64_t)blockIdx.y * rows + head;
-            if (g == 0)
-                ((float2*)(A.part + (int64_t)A.splits * rows * DP))[at] = make_float2(none ? -__builtin_inff() : S[ct].M, L);
+            if (g == 0) {
+                float2* ml = (float2*)(A.part + (int64_t)A.splits * rows * DP);
+                ml[at] = make_float2(none ? -__builtin_inff() : S[ct].M, L);
+                if (blockIdx.y == 0 && A.splits > A.many_splits) ml[A.many_splits * rows + head] = make_float2(0.f, STOP);
+            }
             if (none) continue;
 #pragma unroll
             for (int x = 0; x < DP / 16; x++) *(v4f*)(A.part + at * DP + 16 * x + 4 * g) = S[ct].o[x];
@@ -748,15 +809,17 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
         const int l = tid & 63;
         const float2 x = l < A.splits ? pml[l * rows + row] : make_float2(-__builtin_inff(), 0.f);  // at most 64 splits
         if (__shfl(x.y, 0) == DONE) return;
-        const bool none = x.x == -__builtin_inff();
-        M = wave_max_f32(x.x);
+        const unsigned long long stop = __ballot(x.y == STOP);
+        const int splits = stop ? __builtin_ctzll(stop) : A.splits;
+        const bool none = l >= splits || x.x == -__builtin_inff();
+        M = wave_max_f32(none ? -__builtin_inff() : x.x);
         const float wh = none ? 0.f : exp2_hw(0.5f * (x.x - M));
         L = wave_sum_f32(none ? 0.f : x.y * wh * wh);
 #pragma unroll 8
-        for (int s0 = 0; s0 < A.splits; s0 += GROUPS) {
+        for (int s0 = 0; s0 < splits; s0 += GROUPS) {
             const int s = s0 + u;
             const float f = __shfl(wh, s & 63);  // 0 where a split holds nothing: its sums are not read
-            if (u < GROUPS && s < A.splits && f != 0.f) o += *(const v4f*)(A.part + ((int64_t)s * rows + row) * DP + d4) * (f * f);
+            if (u < GROUPS && s < splits && f != 0.f) o += *(const v4f*)(A.part + ((int64_t)s * rows + row) * DP + d4) * (f * f);
         }
         if (u < GROUPS) *(v4f*)&os[u][d4] = o;
         __syncthreads();
@@ -766,12 +829,18 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
     } else {
         if (u >= GROUPS || row >= rows) return;
         // in batches of eight splits, all loads of one on their way together
-        for (int s0 = 0; s0 < A.splits; s0 += 8) {
+        int splits = A.splits;
+        for (int s0 = 0; s0 < splits; s0 += 8) {
             float2 x[8];
             v4f v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = s0 + j < A.splits ? pml[(s0 + j) * rows + row] : make_float2(-__builtin_inff(), 0.f);
             if (s0 == 0 && x[0].y == DONE) return;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (x[j].y == STOP) splits = min(splits, s0 + j);
+                if (s0 + j >= splits) x[j] = make_float2(-__builtin_inff(), 0.f);
+            }
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int s = min(s0 + j, A.splits - 1);
@@ -801,9 +870,9 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
 // How a call is cut.
 struct Cut {
     bool many;
-    int tpt, fan, least;
+    int tpt, fan, least, group;
     int64_t units, subs, many_wgs;
-    int splits, few_splits;
+    int splits, few_splits, many_splits;
 };
 Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     const int64_t G = H / Hkv, subs = (G + COLS - 1) / COLS, blocks = (maxk + Q8C_BLOCK - 1) / Q8C_BLOCK;
@@ -832,8 +901,16 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     const int64_t rows = T * Hkv * subs;
     c.least = T < 512 ? (int)(40000 / rows) : 0;
     c.many = T >= 64 && G <= cols && blocks >= c.least && rows * blocks >= 1 << 16;
-    c.tpt = c.many ? (int)(cols / G) : 1;
-    const int64_t tiles = (T + c.tpt - 1) / c.tpt;
+    if (c.many) c.tpt = (int)(cols / G);
+    // Rows that split their keys may be of one sequence each, or a short prompt's:
+    // the device packs the latter's tokens into a tile's columns, and their
+    // workgroups share the keys (16 / 32 rows behind 8000 keys, d = 128: 30 and 50 us
+    // become 19 and 24; without splits it gains nothing: 64 rows behind 2000
+    // 27 and 27, behind none 6.4 and 8.7).
+    c.few_splits = splits(T * subs * Hkv);
+    c.group = c.few_splits > 1 && G <= COLS / 2 ? (int)std::min<int64_t>(COLS / G, T) : 1;
+    if (!c.many) c.tpt = c.group;
+    const int64_t tiles = (T + c.tpt - 1) / c.tpt, groups = (c.tpt + c.group - 1) / c.group;
     c.many_wgs = tiles * Hkv;
     c.fan = 1;
     if (c.many) {
@@ -841,12 +918,13 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
         // 64 a CU takes four (256 rows of 2000 keys each 86 us, in twos 100), of d =
         // 128 two are enough (164 us, in fours 178).
         const int64_t each = std::max<int64_t>(rows / (d <= 64 ? 1024 : 512), 1);
-        c.fan = (int)((c.tpt + each - 1) / each);
+        c.fan = (int)((groups + each - 1) / each);
     }
     c.units = tiles * c.fan;
     c.subs = subs;
-    c.few_splits = splits(T * subs * Hkv);
-    c.splits = c.many ? std::max(splits(c.many_wgs), c.few_splits) : c.few_splits;
+    c.many_splits = c.many ? splits(c.many_wgs) : 1;
+    c.splits = c.few_splits > 1 ? std::min(c.few_splits * c.group, 64) : 1;
+    if (c.many_splits > c.splits) c.splits = c.many_splits;
     return c;
 }
 
@@ -854,14 +932,19 @@ template <int DP>
 hipError_t launch(Args A, const Cut& c, hipStream_t s) {
     A.splits = c.splits;
     A.few_splits = c.few_splits;
+    A.many_splits = c.many_splits;
+    A.group = c.group;
+    A.inv = (256 + A.G - 1) / A.G;
     A.tpt = c.tpt;
     A.fan = c.fan;
     A.least = c.least;
-    const dim3 few((unsigned)(A.Hkv * c.subs), (unsigned)c.units, (unsigned)c.few_splits);
-    if (!c.many) hipLaunchKernelGGL((few_kernel<DP, false>), few, dim3(64 * NW), 0, s, A);
-    else hipLaunchKernelGGL((few_kernel<DP, true>), few, dim3(64 * NW), 0, s, A);
+    const dim3 few((unsigned)(A.Hkv * c.subs * c.group), (unsigned)c.units, (unsigned)c.few_splits);
+    if (c.many && c.group > 1) hipLaunchKernelGGL((few_kernel<DP, true, true>), few, dim3(64 * NW), 0, s, A);
+    else if (c.many) hipLaunchKernelGGL((few_kernel<DP, true, false>), few, dim3(64 * NW), 0, s, A);
+    else if (c.group > 1) hipLaunchKernelGGL((few_kernel<DP, false, true>), few, dim3(64 * NW), 0, s, A);
+    else hipLaunchKernelGGL((few_kernel<DP, false, false>), few, dim3(64 * NW), 0, s, A);
     if (c.many)
-        hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.splits), dim3(256), 0, s, A);
+        hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.many_splits), dim3(256), 0, s, A);
     const int rows = A.T * A.H, groups = 1024 / DP;
     if (c.splits > 1 && rows <= 1024)
         hipLaunchKernelGGL((join_kernel<DP, true>), dim3((unsigned)rows), dim3(256), 0, s, A);
