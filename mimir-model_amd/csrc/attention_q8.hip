@@ -338,13 +338,22 @@ template <int DP>
 constexpr int MANY_COLS = DP <= 128 ? MAX_COLS : MAX_COLS / 2;
 
 // Few rows: a workgroup per (token, kv head, split of the keys) and up to 16
-// query heads (BESIDE many_kernel: for every fan-th token of a tile; in one
-// instance the loop over tokens cost every call its registers and nearly half
-// a microsecond before the first load). Its NW waves take the token's blocks
-// in turn, straight from memory, each with a state of its own, joined at the
-// end. A wave has its next
+// query heads. Its NW waves take the token's blocks in turn, straight from
+// memory, each with a state of its own, joined at the end. A wave has its next
 // block's keys in flight while it works on one, and the values during the
-// score product. The query's parts lie in LDS (for the registers).
+// score product (the values a block ahead as well, or both two blocks: 64 x
+// 2048 keys 45 and 49 us against 40, with registers for four and three waves a
+// SIMD where this has four; two are there). The query's parts lie in LDS (for
+// the registers).
+//
+// GROUP (keys that are split, at most 8 query heads a kv head): the tokens whose
+// heads fill the 16 columns, where three quarters of what they see is shared (a
+// short prompt, a draft), are taken together, and the group's workgroups, one a
+// token else, are further splits.
+//
+// BESIDE many_kernel: a workgroup takes every fan-th group of a tile that is not
+// many_kernel's. (In one instance this loop cost every call its registers and
+// nearly half a microsecond before the first load.)
 constexpr int NW = 4;
 template <int DP>
 struct FewLds {
@@ -793,8 +802,8 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
 }
 
 // The splits of a row joined, DP / 4 threads a row and split. WIDE: a workgroup
-// per row, 1024 / DP of its splits at a time (few rows, which many splits may
-// hold); else 1024 / DP rows a workgroup.
+// per row, 1024 / DP of its splits at a time (few rows or more than 8 splits: 32
+// splits of 2048 rows take 2 to 5 us less so); else 1024 / DP rows a workgroup.
 template <int DP, bool WIDE>
 __global__ __launch_bounds__(256) void join_kernel(Args A) {
     constexpr int LANES = DP / 4, GROUPS = 256 / LANES;
@@ -946,7 +955,7 @@ hipError_t launch(Args A, const Cut& c, hipStream_t s) {
     if (c.many)
         hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.many_splits), dim3(256), 0, s, A);
     const int rows = A.T * A.H, groups = 1024 / DP;
-    if (c.splits > 1 && rows <= 1024)
+    if (c.splits > 1 && (rows <= 1024 || c.splits > 8))
         hipLaunchKernelGGL((join_kernel<DP, true>), dim3((unsigned)rows), dim3(256), 0, s, A);
     else if (c.splits > 1)
         hipLaunchKernelGGL((join_kernel<DP, false>), dim3((unsigned)((rows + groups - 1) / groups)), dim3(256), 0, s, A);

@@ -200,7 +200,7 @@ def check(got, ref, q, kend, kstart=None, maxk=None):
 # kernel beside the other)
 @pytest.mark.parametrize("room", [None, 1 << 18])
 @pytest.mark.parametrize("T,H,hk,d,slots,stride", [
-    (100, 144, 1, 64, 1, 250), (128, 14, 2, 64, 1, 1400), (64, 8, 2, 128, 1, 2500), (109, 14, 2, 128, 3, 260), (97, 34, 1, 64, 2, 150), (260, 8, 8, 128, 1, 900), (120, 3, 1, 256, 1, 400), (1, 1, 1, 64, 1, 32), (1, 4, 1, 8, 1, 1), (1, 32, 8, 64, 1, 181), (2, 16, 16, 128, 2, 33), (3, 14, 2, 64, 3, 500),
+    (100, 144, 1, 64, 1, 250), (128, 14, 2, 64, 1, 1400), (20, 8, 2, 128, 1, 900), (7, 3, 1, 64, 1, 1500), (33, 4, 4, 192, 1, 700), (2, 16, 2, 256, 1, 4000), (63, 6, 6, 80, 1, 1300), (64, 8, 2, 128, 1, 2500), (109, 14, 2, 128, 3, 260), (97, 34, 1, 64, 2, 150), (260, 8, 8, 128, 1, 900), (120, 3, 1, 256, 1, 400), (1, 1, 1, 64, 1, 32), (1, 4, 1, 8, 1, 1), (1, 32, 8, 64, 1, 181), (2, 16, 16, 128, 2, 33), (3, 14, 2, 64, 3, 500),
     (8, 32, 8, 128, 8, 300), (5, 40, 2, 80, 5, 77), (1, 34, 2, 256, 1, 700), (4, 6, 3, 192, 2, 129), (1, 8, 2, 128, 1, 6000),
     (1, 3, 1, 64, 1, 20001), (64, 4, 2, 64, 16, 70), (70, 14, 2, 64, 7, 90), (200, 32, 8, 128, 1, 200), (133, 8, 8, 64, 1, 300),
     (130, 34, 2, 80, 3, 130), (181, 14, 2, 64, 1, 181), (65, 12, 4, 256, 2, 100), (150, 16, 2, 128, 150, 13), (300, 6, 2, 192, 2, 400)])
@@ -225,6 +225,25 @@ def test_attention(gpu, rt, T, H, hk, d, slots, stride, room):
         used[a:b + 1] = True
     ref.bad[:] = (~used).reshape(-1, 32) @ (1 << np.arange(32, dtype=np.uint64))
     check(run(gpu, rt, q, ref, end, start if slots > 1 else None, room), ref, q, end, start if slots > 1 else None)
+
+
+@pytest.mark.parametrize("room", [900, 1 << 20])
+@pytest.mark.parametrize("H,hk,d", [(4, 1, 64), (8, 8, 128), (14, 2, 64), (3, 1, 192), (16, 2, 256), (10, 2, 8), (36, 2, 128)])
+def test_few_rows_of_a_sequence(gpu, rt, H, hk, d, room):
+    """Rows that share their keys, as a short prompt's or a draft's: one sequence
+    of 20, several of 1 to 5 rows, rows that see nothing, windows, marks."""
+    rng = np.random.default_rng(H * d)
+    C = 8 * 900
+    ref = random_cache(rng, hk, C, d, spread=0.5)
+    ref.bad[0, 2 * 900 // 32 + 7] = 5
+    for lens in ([20], [1, 5, 3, 4, 2], [2, 2], [7, 1, 1, 1, 1, 1, 1]):
+        start = np.concatenate([np.full(n, 900 * i) for i, n in enumerate(lens)])
+        end = np.concatenate([900 * i + 880 - 37 * i + np.arange(n) for i, n in enumerate(lens)])
+        q = rng.standard_normal((len(end), H, d)).astype(np.float32)
+        check(run(gpu, rt, q, ref, end, start, room), ref, q, end, start, room)
+        end[-1] = start[-1] - 1
+        start[:-1] += rng.integers(0, 40, len(end) - 1)
+        check(run(gpu, rt, q, ref, end, start, room), ref, q, end, start, room)
 
 
 def test_prompts_and_decode_rows_in_one_call(gpu, rt):
