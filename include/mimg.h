@@ -583,8 +583,8 @@ int mimg_kv_load_q8_dev(const void *cache, const int64_t *cache_index, int64_t T
  * one pass), not the reference's float order. A query that sees nothing gets
  * zeros; one that sees an entry marked not finite, or is not finite itself, or
  * whose largest score is not finite, NaN. ws: device scratch of
- * mimg_attention_q8_workspace_bytes (which may be 0, then ws may be NULL),
- * 16-byte aligned. */
+ * mimg_attention_q8_workspace_bytes (which may be 0, then ws may be NULL; fewer
+ * queries may need more: ask for each T), 16-byte aligned. */
 uint64_t mimg_attention_q8_workspace_bytes(int64_t T, int heads, int kv_heads, int d, int64_t max_keys);
 int mimg_attention_q8_dev(const float *q, const void *cache, const int64_t *kend, const int64_t *kstart, int64_t T,
                           int heads, int kv_heads, int d, int64_t context, int64_t max_keys, float *out, void *ws,
