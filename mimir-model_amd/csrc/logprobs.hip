@@ -16,8 +16,8 @@
 // Bound: the logits' bytes, once, for many rows; for few the two launches'
 // chains of reductions. Measured on MI355X: 512 rows of 128256 logits, top 5,
 // 48 us (263 MB: 6.0 TB/s in chunk_kernel's 44 us; a read kernel 7.05), top 64
-// 69 us; one row, top 20, 13 us; 37 rows of 32003 of which a mask leaves 50, top
-// 8, 11.6 us; without alternatives 44, 6.0 and 6.7 us.
+// 65 us; one row, top 20, 11.6 us; 37 rows of 32003 of which a mask leaves 50, top
+// 8, 12.0 us; without alternatives 44, 6.0 and 6.7 us.
 #include "decoder_math.hpp"
 #include "mimg_device.hpp"
 #include "mimg_kernels.hpp"
@@ -152,28 +152,32 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A) {
     const uint32_t tau = tau_s;
     const bool all = tau < 0x007FFFFFu;
     const float tf = all ? -__builtin_inff() : value_of(tau);
-    auto key = [&](int j) {
-        return (uint64_t)order_of(x[j]) << 32 | (uint32_t)~(uint32_t)(i0 + 1024 * (j >> 2) + (j & 3));
-    };
-    uint32_t same = 0;  // the thread's values equal to tau
-    if (mx >= tf) {
-        int mine = 0;
+    // Those above tau, by the wave: counted, then stored (of 64 values mostly none).
+    if (__any(mx > tf)) {
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 4 * VEC; j++) n += __popcll(__ballot(x[j] > tf));
+        int at = 0;
+        if (l == 0) at = atomicAdd(&ncand, n);
+        at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
         for (int j = 0; j < 4 * VEC; j++) {
-            mine += x[j] > tf ? 1 : 0;
-            same |= x[j] == tf && i0 + 1024 * (j >> 2) + (j & 3) < A.n ? 1u << j : 0u;
-        }
-        if (mine) {
-            int at = atomicAdd(&ncand, mine);
-#pragma unroll
-            for (int j = 0; j < 4 * VEC; j++)
-                if (x[j] > tf) cand[at++] = key(j);
+            const unsigned long long has = __ballot(x[j] > tf);
+            if (has == 0) continue;
+            if (x[j] > tf)
+                cand[at + __popcll(has & ((1ull << l) - 1))] =
+                    (uint64_t)order_of(x[j]) << 32 | (uint32_t)~(uint32_t)(i0 + 1024 * (j >> 2) + (j & 3));
+            at += __popcll(has);
         }
     }
     __syncthreads();
     // Then those equal to tau of the lowest indices, 1024 j + 4 thread + b, step
     // by step until there are k (mostly one step: they are one, or a mask's).
     int c = ncand;
+    uint32_t same = 0;
+    if (c < A.top && mx >= tf)
+#pragma unroll
+        for (int j = 0; j < 4 * VEC; j++) same |= x[j] == tf && i0 + 1024 * (j >> 2) + (j & 3) < A.n ? 1u << j : 0u;
     for (int j = 0; j < VEC && c < A.top; j++) {
         const uint32_t four = (same >> (4 * j)) & 15u;
         int n = 0, at = 0;
