@@ -802,8 +802,9 @@ __global__ __launch_bounds__(256, 2) void many_kernel(Args A) {
 }
 
 // The splits of a row joined, DP / 4 threads a row and split. WIDE: a workgroup
-// per row, 1024 / DP of its splits at a time (few rows or more than 8 splits: 32
-// splits of 2048 rows take 2 to 5 us less so); else 1024 / DP rows a workgroup.
+// per row, 1024 / DP of its splits at a time (up to 1024 rows, or 4096 of more than 8
+// splits: 32 splits of 2048 rows take 2 to 5 us less so, 9 of 7168 as much more);
+// else 1024 / DP rows a workgroup.
 template <int DP, bool WIDE>
 __global__ __launch_bounds__(256) void join_kernel(Args A) {
     constexpr int LANES = DP / 4, GROUPS = 256 / LANES;
@@ -886,15 +887,11 @@ struct Cut {
 Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     const int64_t G = H / Hkv, subs = (G + COLS - 1) / COLS, blocks = (maxk + Q8C_BLOCK - 1) / Q8C_BLOCK;
     const int64_t cols = d <= 128 ? MAX_COLS : MAX_COLS / 2;
-    // Splits that give about 512 workgroups, of eight blocks and more (of four or
-    // sixteen: 2048 keys of one sequence 9.6 and 12.2 us against 10.1, of 8 x
-    // 8192 the same), none up to 512 keys (9.4 us against 10.0 with join_kernel).
-    auto splits = [&](int64_t wgs) {
-        int64_t s = (512 + wgs - 1) / wgs;
-        if (s > blocks / 8) s = blocks / 8;
-        if (blocks <= 16) s = 1;
-        return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
-    };
+    // At most 64 splits of eight blocks and more (of four or sixteen: 2048 keys of
+    // one sequence 9.6 and 12.2 us against 10.1, of 8 x 8192 the same), none up to
+    // 512 keys (9.4 us against 10.0 with join_kernel). few_kernel takes as many as
+    // give 512 workgroups.
+    const int64_t most = blocks <= 16 ? 1 : std::min<int64_t>(blocks / 8, 64);
     Cut c{};
     // Prompts of many tokens are many_kernel's, a decode batch of as many
     // sequences few_kernel's: the ranges, on the device, tell them apart, so
@@ -916,7 +913,7 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     // workgroups share the keys (16 / 32 rows behind 8000 keys, d = 128: 30 and 50 us
     // become 19 and 24; without splits it gains nothing: 64 rows behind 2000
     // 27 and 27, behind none 6.4 and 8.7).
-    c.few_splits = splits(T * subs * Hkv);
+    c.few_splits = (int)std::min((511 + T * subs * Hkv) / (T * subs * Hkv), most);
     c.group = c.few_splits > 1 && G <= COLS / 2 ? (int)std::min<int64_t>(COLS / G, T) : 1;
     if (!c.many) c.tpt = c.group;
     const int64_t tiles = (T + c.tpt - 1) / c.tpt, groups = (c.tpt + c.group - 1) / c.group;
@@ -931,7 +928,20 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     }
     c.units = tiles * c.fan;
     c.subs = subs;
-    c.many_splits = c.many ? splits(c.many_wgs) : 1;
+    // many_kernel's splits: the least work of the fullest compute unit, its
+    // workgroups times their blocks, each with a start worth some 16 blocks; one
+    // alone has 0.6 of the rate of two (at d = 256 all of it). 384 rows behind 8000
+    // keys, d = 128, 96 workgroups: 142 us in 6 splits, 113 in 5; 1280 rows, 320:
+    // 410 us whole, 370 in 2, 331 in 4; behind none 64, 65 and 75.
+    c.many_splits = 1;
+    for (int64_t s = 1, best = INT64_MAX; c.many && s <= most; s++) {
+        const int64_t n = (c.many_wgs * s + 255) / 256;
+        const int64_t cost = n * ((blocks + s - 1) / s + 16) * (n == 1 && d <= 192 ? 5 : 3);
+        if (cost < best) {
+            best = cost;
+            c.many_splits = (int)s;
+        }
+    }
     c.splits = c.few_splits > 1 ? std::min(c.few_splits * c.group, 64) : 1;
     if (c.many_splits > c.splits) c.splits = c.many_splits;
     return c;
@@ -955,7 +965,7 @@ hipError_t launch(Args A, const Cut& c, hipStream_t s) {
     if (c.many)
         hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.many_splits), dim3(256), 0, s, A);
     const int rows = A.T * A.H, groups = 1024 / DP;
-    if (c.splits > 1 && (rows <= 1024 || c.splits > 8))
+    if (c.splits > 1 && (rows <= 1024 || (c.splits > 8 && rows <= 4096)))
         hipLaunchKernelGGL((join_kernel<DP, true>), dim3((unsigned)rows), dim3(256), 0, s, A);
     else if (c.splits > 1)
         hipLaunchKernelGGL((join_kernel<DP, false>), dim3((unsigned)((rows + groups - 1) / groups)), dim3(256), 0, s, A);
