@@ -75,6 +75,7 @@ struct Args {
     int splits;      // of the keys, places in the workspace
     int few_splits;  // those that few_kernel cuts a token's keys into
     int many_splits; // and many_kernel a tile's
+    int fours;       // see splits_of()
     int tpt, fan;    // tokens a tile of many_kernel; groups of workgroups of few_kernel that share one
     int group, inv;  // tokens whose columns fit a tile of 16; 256 / G, rounded up: c / G = c * inv / 256
     int least;       // blocks that a token sees at least, or many_kernel takes none
@@ -364,6 +365,16 @@ struct FewLds {
     float ml[NW][2][COLS];
     int keys[COLS];  // that a column sees (a group's)
 };
+// The splits that so many blocks are worth, of n: of eight blocks, with `fours`
+// (few workgroups) of four up to 16 of them; none up to 8 blocks (one sequence,
+// at most 8192 keys: 100 keys 5.9 us against 7.2, 500 in four 7.2 against 8.4,
+// 2000 in 16 7.3 against 8.0; but 24 rows of 16 heads behind 2000 12.7 against
+// 11.0).
+__host__ __device__ __forceinline__ int splits_of(int64_t n, int64_t blocks, bool fours) {
+    const int64_t eight = (blocks + 7) / 8, four = (blocks + 3) / 4;
+    const int64_t s = !fours || eight > 16 ? eight : (four < 16 ? four : 16);
+    return blocks <= 8 ? 1 : (int)(n < s ? n : s);
+}
 template <int DP, bool BESIDE, bool GROUP>
 __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A) {
     __shared__ FewLds<DP> S_;
@@ -385,10 +396,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
     const int t = t0 + (GROUP ? sub : 0);
     const AttRange own = range_of(A, min(t, A.T - 1));
     int head0 = t * A.H + hk * A.G + g0, step = 0, ncol = min(COLS, A.G - g0);
-    int split = blockIdx.z, nsplit = A.few_splits;
+    int split = blockIdx.z;
     int k0 = (int)own.k0, n = (int)own.n;  // the keys that the lane's column sees
     int from = k0, to = k0 + n;            // and those that all columns see
     int b0 = k0 >> 5, total = n > 0 ? ((k0 + n + 31) >> 5) - b0 : 0;
+    int nsplit = splits_of(A.few_splits, total, A.fours);
     bool packed = false;
     if constexpr (GROUP) {
         const int tc = (col * A.inv) >> 8, tn = min(P, last - t0);
@@ -427,7 +439,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
             head0 = t0 * A.H + hk * A.G;
             step = A.H - A.G;
             ncol = tn * A.G;
-            nsplit = min(min(A.few_splits * P, A.splits), (total + 7) / 8);
+            nsplit = splits_of(min(A.few_splits * P, A.splits), total, false);
             split = split * P + sub;
             if (w == 0 && l < COLS) S_.keys[l] = n;
         } else if (sub >= tn) {
@@ -879,7 +891,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
 
 // How a call is cut.
 struct Cut {
-    bool many;
+    bool many, fours;
     int tpt, fan, least, group;
     int64_t units, subs, many_wgs;
     int splits, few_splits, many_splits;
@@ -887,11 +899,8 @@ struct Cut {
 Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     const int64_t G = H / Hkv, subs = (G + COLS - 1) / COLS, blocks = (maxk + Q8C_BLOCK - 1) / Q8C_BLOCK;
     const int64_t cols = d <= 128 ? MAX_COLS : MAX_COLS / 2;
-    // At most 64 splits of eight blocks and more (of four or sixteen: 2048 keys of
-    // one sequence 9.6 and 12.2 us against 10.1, of 8 x 8192 the same), none up to
-    // 512 keys (9.4 us against 10.0 with join_kernel). few_kernel takes as many as
-    // give 512 workgroups.
-    const int64_t most = blocks <= 16 ? 1 : std::min<int64_t>(blocks / 8, 64);
+    // At most 64 splits, none up to 512 keys (9.4 us against 10.0 with join_kernel).
+    // few_kernel takes as many as give 512 workgroups.
     Cut c{};
     // Prompts of many tokens are many_kernel's, a decode batch of as many
     // sequences few_kernel's: the ranges, on the device, tell them apart, so
@@ -913,7 +922,8 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     // workgroups share the keys (16 / 32 rows behind 8000 keys, d = 128: 30 and 50 us
     // become 19 and 24; without splits it gains nothing: 64 rows behind 2000
     // 27 and 27, behind none 6.4 and 8.7).
-    c.few_splits = (int)std::min((511 + T * subs * Hkv) / (T * subs * Hkv), most);
+    c.fours = T * subs * Hkv <= 16;
+    c.few_splits = (int)std::min<int64_t>((511 + T * subs * Hkv) / (T * subs * Hkv), blocks <= 16 ? 1 : splits_of(64, blocks, c.fours));
     c.group = c.few_splits > 1 && G <= COLS / 2 ? (int)std::min<int64_t>(COLS / G, T) : 1;
     if (!c.many) c.tpt = c.group;
     const int64_t tiles = (T + c.tpt - 1) / c.tpt, groups = (c.tpt + c.group - 1) / c.group;
@@ -934,6 +944,7 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     // keys, d = 128, 96 workgroups: 142 us in 6 splits, 113 in 5; 1280 rows, 320:
     // 410 us whole, 370 in 2, 331 in 4; behind none 64, 65 and 75.
     c.many_splits = 1;
+    const int64_t most = blocks <= 16 ? 1 : std::min<int64_t>(blocks / 8, 64);
     for (int64_t s = 1, best = INT64_MAX; c.many && s <= most; s++) {
         const int64_t n = (c.many_wgs * s + 255) / 256;
         const int64_t cost = n * ((blocks + s - 1) / s + 16) * (n == 1 && d <= 192 ? 5 : 3);
@@ -952,6 +963,7 @@ hipError_t launch(Args A, const Cut& c, hipStream_t s) {
     A.splits = c.splits;
     A.few_splits = c.few_splits;
     A.many_splits = c.many_splits;
+    A.fours = c.fours;
     A.group = c.group;
     A.inv = (256 + A.G - 1) / A.G;
     A.tpt = c.tpt;
