@@ -29,7 +29,7 @@
 //   8 sequences of 2048 keys    10.1 us and join_kernel's 3.1: mostly the way
 //                               from the launch to the first weight
 //   2048 rows behind 6100 keys  394 us, 478 GFLOP: 1.21 PFLOP/s
-// d = 64, one row of 181 keys 5.2 us. The two parts cost the decode rows nothing
+// d = 64, one row of 181 keys 5.4 us. The two parts cost the decode rows nothing
 // that shows (their products take 16 us of the 41, under the loads) and a prompt
 // twice its products; with one part the outputs' error would be 2^-11, not
 // float32's.
