@@ -25,10 +25,10 @@
 // cores, 8 d flops a (query, key) pair with the two parts, 1240 to 1264 TFLOP/s
 // in a large f16 product. Measured on MI355X, 32 heads, 8 kv heads, d = 128:
 //   64 sequences of 2048 keys   41 us, 233 MB: 5.7 TB/s (a read kernel 7.05)
-//   1 sequence of 131072 keys   51 us, 269 MB; 5 of them join_kernel
+//   1 sequence of 131072 keys   48 us, 269 MB; 4.6 of them join_kernel
 //   8 sequences of 2048 keys    10.1 us and join_kernel's 3.1: mostly the way
 //                               from the launch to the first weight
-//   2048 rows behind 6100 keys  394 us, 478 GFLOP: 1.21 PFLOP/s
+//   2048 rows behind 6100 keys  385 us, 478 GFLOP: 1.24 PFLOP/s
 // d = 64, one row of 181 keys 5.4 us. The two parts cost the decode rows nothing
 // that shows (their products take 16 us of the 41, under the loads) and a prompt
 // twice its products; with one part the outputs' error would be 2^-11, not
