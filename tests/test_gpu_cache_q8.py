@@ -316,6 +316,34 @@ def test_not_finite(gpu, rt, T):
     assert np.isnan(run(gpu, rt, np.full((T, 4, 128), 1e10, np.float32), big, np.full(T, 40))).all()
 
 
+def test_the_most_rows(gpu, rt):
+    """65535 rows in one call: a store of as many (a prompt's, then one row a
+    block), rope beside it, and attention by either kernel."""
+    T, hk, d = 65535, 1, 8
+    rng = np.random.default_rng(0)
+    for C, index in ((T, np.arange(T)), (32 * T, 32 * np.arange(T) + 5)):
+        dc = DeviceCache(gpu, rt, hk, C, d)
+        q, k, v = values(rng, T, 2, d), values(rng, T, hk, d), values(rng, T, hk, d)
+        dc.store(k, v, index)
+        for x, y in zip((k, v), dc.load(index)):  # half a step, of the block's largest / 127, and two roundings
+            block = index // 32 - index[0] // 32
+            amax = np.zeros(block[-1] + 1)
+            np.maximum.at(amax, block, np.abs(x).max((1, 2)))
+            assert (np.abs(x.astype(np.float64) - y).max((1, 2)) <= amax[block] / 127 * (0.5 + 127 * 2.0 ** -22)).all()
+        one, s = DeviceCache(gpu, rt, hk, C, d), rt.Stream()
+        pos, freq = np.zeros(T, np.int64), np.array([1.0, 0.5])
+        b = [dev(rt, a) for a in (q, k, v, pos, index.astype(np.int64), freq)]
+        gpu.rope_kv_q8_dev(*(x.ptr for x in b), T, 2, hk, d, 4, 1, C, one.buf.ptr, s.handle)  # (an angle of 0)
+        s.sync()
+        assert np.array_equal(one.raw(), dc.raw()) and np.array_equal(b[0].download(np.float32).reshape(q.shape), q)
+    small = random_cache(rng, hk, 300, d)
+    end = rng.integers(-1, 300, T)
+    some = np.concatenate([[0, 1, 32767, 65533, 65534], rng.integers(0, T, 300)])
+    for room in (32, 64, 300, 1 << 20):
+        got = run(gpu, rt, q, small, end, None, room)
+        check(got[some], small, q[some], end[some], None, room)
+
+
 @pytest.mark.parametrize("T,room", [(1, 1 << 16), (8, 3000), (200, 1 << 18)])
 def test_the_same_bits_every_time(gpu, rt, T, room):
     """Nothing depends on the order of workgroups: two calls at once on two

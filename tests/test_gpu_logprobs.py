@@ -71,7 +71,7 @@ def check(got, x, targets, top):
 
 @pytest.mark.parametrize("rows,n,top", [(1, 1, 1), (1, 3, 3), (2, 64, 64), (3, 100, 7), (5, 1023, 64), (2, 1024, 20), (4, 8191, 5),
                                         (1, 8192, 64), (3, 8193, 64), (2, 32003, 8), (1, 128256, 20), (9, 128256, 0), (40, 20000, 33),
-                                        (2, 151936, 64), (1, 1 << 21, 64), (1, 600000, 1), (300, 77, 2)])
+                                        (2, 151936, 64), (1, 1 << 21, 64), (1, 600000, 1), (300, 77, 2), (70000, 5, 5)])
 def test_rows(gpu, rt, rows, n, top):
     rng = np.random.default_rng(n + top)
     x = (rng.standard_normal((rows, n)) * rng.choice([0.1, 2.5, 30.0], (rows, 1))).astype(np.float32)
