@@ -395,6 +395,33 @@ def test_graphs_share_a_workspace(gpu, rt):
             assert np.array_equal(c.result(), w)
 
 
+@pytest.mark.parametrize("T,H,hk", [(1, 4, 1), (6, 8, 2), (40, 4, 1), (100, 8, 4), (130, 14, 2)])
+def test_a_graph_over_growing_keys(gpu, rt, T, H, hk):
+    """One captured call, replayed with the rows' keys changed: more and fewer,
+    one sequence and many, none; what an earlier replay left in the workspace
+    does not matter."""
+    rng = np.random.default_rng(T)
+    C, room = 6000, 1 << 17
+    ref = random_cache(rng, hk, C, 64)
+    q = rng.standard_normal((T, H, 64)).astype(np.float32)
+    c, s = Call(gpu, rt, q, ref, np.zeros(T), np.zeros(T), room), rt.Stream()
+    g = rt.Graph(s, lambda: c.enqueue(s))
+    for n in (5, 5999, 40, 256, 2000, 257, -1, 600, 4100):
+        for spread in (False, True):
+            start = rng.integers(0, C, T) if spread else np.zeros(T, np.int64)
+            end = start + rng.integers(-1, max(n, 1), T) if spread else np.maximum(n - T, -1) + np.arange(T)
+            c.bufs[2].upload(end.astype(np.int64))
+            c.bufs[3].upload(start.astype(np.int64))
+            g.launch(s)
+            s.sync()
+            got = c.result()
+            c.enqueue(s)
+            s.sync()
+            assert np.array_equal(got, c.result(), equal_nan=True)
+            some = rng.integers(0, T, 12)
+            check(got[some], ref, q[some], end[some], start[some], room)
+
+
 def test_offsets_past_32_bits(gpu, rt):
     """The last blocks of a cache whose bytes pass 2^32: stored, read back and
     attended to."""
