@@ -920,15 +920,16 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     Cut c{};
     // Prompts of many tokens are many_kernel's, a decode batch of as many
     // sequences few_kernel's: the ranges, on the device, tell them apart, so
-    // both are launched, and each leaves the other's tiles (a decode batch pays some
-    // 10 us of 50 and more, so not for smaller ones). A prompt's rows cost few_kernel their number
-    // times the blocks, many_kernel a start of some 20 us; they meet near 5000
-    // row-blocks of 8 kv heads (64 rows behind 2000 / 8000 keys 19 and 54 us
-    // against 23 and 34 at d = 64, 27 and 89 against 32 and 45 at 128; 128 rows
-    // behind 1000 / 2000 keys 18 and 29 against 24 and 27, 28 and 46 against 33
-    // and 34; 256 rows behind none / 1000 12 and 33 against 18 and 31). The
-    // host knows max_keys, the device what the rows see, so that many blocks are
-    // asked for there too (below 512 rows, which see that many by themselves).
+    // both are launched, and each leaves the other's tiles (a decode batch pays
+    // some 10 us of 50 and more, so not for smaller ones). A prompt's rows cost
+    // few_kernel their number times the blocks, many_kernel a start of some 20
+    // us; they meet near 5000 row-blocks of 8 kv heads (64 rows behind 2000 /
+    // 8000 keys 19 and 54 us against 23 and 34 at d = 64, 27 and 89 against 32
+    // and 45 at 128; 128 rows behind 1000 / 2000 keys 18 and 29 against 24 and
+    // 27, 28 and 46 against 33 and 34; 256 rows behind none / 1000 12 and 33
+    // against 18 and 31). The host knows max_keys, the device what the rows see,
+    // so that many blocks are asked for there too (below 512 rows, which see that
+    // many by themselves).
     const int64_t rows = T * Hkv * subs;
     c.least = T < 512 ? (int)(40000 / rows) : 0;
     c.many = T >= 64 && G <= cols && blocks >= c.least && rows * blocks >= 1 << 16;
@@ -938,8 +939,8 @@ Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     // workgroups share the keys (16 / 32 rows behind 8000 keys, d = 128: 30 and 50 us
     // become 19 and 24; without splits it gains nothing: 64 rows behind 2000
     // 27 and 27, behind none 6.4 and 8.7).
-    c.fours = T * subs * Hkv <= 16;
-    c.few_splits = (int)std::min<int64_t>((511 + T * subs * Hkv) / (T * subs * Hkv), blocks <= 16 ? 1 : splits_of(64, blocks, c.fours));
+    c.fours = rows <= 16;
+    c.few_splits = (int)std::min<int64_t>((511 + rows) / rows, blocks <= 16 ? 1 : splits_of(64, blocks, c.fours));
     c.group = c.few_splits > 1 && G <= COLS / 2 ? (int)std::min<int64_t>(COLS / G, T) : 1;
     if (!c.many) c.tpt = c.group;
     const int64_t tiles = (T + c.tpt - 1) / c.tpt, groups = (c.tpt + c.group - 1) / c.group;

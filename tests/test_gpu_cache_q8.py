@@ -196,7 +196,7 @@ def check(got, ref, q, kend, kstart=None, maxk=None):
 
 
 # `room`: max_keys, which with T, heads and kv heads decides on the kernels: the
-# cache's length, and far more than it (many splits; from 96 tokens the prompt
+# cache's length, and far more than it (many splits; from 64 tokens the prompt
 # kernel beside the other)
 @pytest.mark.parametrize("room", [None, 1 << 18])
 @pytest.mark.parametrize("T,H,hk,d,slots,stride", [
