@@ -579,8 +579,10 @@ int mimg_kv_load_q8_dev(const void *cache, const int64_t *cache_index, int64_t T
  * kstart[t]..kend[t] (kstart may be NULL for 0) of kv head h / (heads /
  * kv_heads), clipped to the cache and to the first max_keys (1..2^30: no limit
  * of 8192 here); scale 1/sqrt(d); q, out [T, heads, d], out not overlapping q.
- * Float32 accuracy (products of 22-bit parts summed in float32; the softmax in
- * one pass), not the reference's float order. A query that sees nothing gets
+ * Float32 accuracy, not the reference's float order: products of 22-bit parts
+ * summed in float32, the softmax in one pass. A key's weight (its share of the
+ * softmax times its block's value scale) is kept to 2^-22 of itself or 2^-44
+ * of the row's largest, whichever is more, rounded to nearest. A query that sees nothing gets
  * zeros; one that sees an entry marked not finite, or is not finite itself, or
  * whose largest score is not finite, NaN. ws: device scratch of
  * mimg_attention_q8_workspace_bytes (which may be 0, then ws may be NULL; fewer
