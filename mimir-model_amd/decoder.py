@@ -456,13 +456,15 @@ class Decoder:
     def _ensure_logprobs(self, rows, top):
         """Buffers for the log probabilities of `rows` rows with `top`
         alternatives: floats [rows] each of log probability and entropy,
-        [rows, top] log probabilities and ids of the alternatives."""
+        [rows, top] log probabilities and ids of the alternatives. They only
+        grow, each by itself."""
         need, wsb = rows * (2 + 2 * top) * 4, mimg.logprobs_workspace_bytes(rows, self.vocab, top)
         if wsb == 0:
             raise ValueError(f"{top} alternatives of {self.vocab} tokens")
-        if self.lp is None or self.lp.nbytes < need or self.lp_ws.nbytes < wsb:
-            self._drop_graphs()  # captured with the old buffers
-            self.lp, self.lp_ws = hiprt.DeviceBuffer(need), hiprt.DeviceBuffer(wsb)
+        for name, nbytes in (("lp", need), ("lp_ws", wsb)):
+            if getattr(self, name) is None or getattr(self, name).nbytes < nbytes:
+                self._drop_graphs(lambda n, top: top is not None)  # captured with the old buffer
+                setattr(self, name, hiprt.DeviceBuffer(nbytes))
         if self.targets is None:
             self.targets = hiprt.DeviceBuffer(self.R * 4)
 
@@ -522,11 +524,10 @@ class Decoder:
             g = self.graphs[n, top] = hiprt.Graph(self.stream, lambda: self._decode_step(n, top))
         return g
 
-    def _drop_graphs(self):
+    def _drop_graphs(self, which=lambda n, top: True):
         self.stream.sync()
-        for g in self.graphs.values():
-            g.destroy()
-        self.graphs = {}
+        for key in [k for k in self.graphs if which(*k)]:
+            self.graphs.pop(key).destroy()
 
     def _ensure_out(self, cap, n):
         if self.out is None or self.out_cap < cap or self.out.nbytes < cap * n * 4:
