@@ -183,15 +183,21 @@ struct State {
     float M, l;
 };
 
-// A block's value scale for the exponents: log2 and reciprocal (of a block of
+// A block's value scale for the exponents: log2 in whole steps and the rest in
+// [0, 1), so that it costs no bits beside M, however far from one the scale is
+// (as one number 1.6e-6 of an output where scales are near 2^-90 or 2^64, so 4e-7;
+// 2048 rows behind 6100 keys 416 us as one, so 419); reciprocal (of a block of
 // zeros the floor's; its weights are left out below).
 struct Scale {
-    float lv, iv, lv8;
+    float whole8, rest, iv;  // (weights are taken 2^8 up)
+    __device__ __forceinline__ float log2() const { return whole8 - 8.f + rest; }
+    // Of the exponents, with M taken off.
+    __device__ __forceinline__ float offset(float M) const { return (whole8 - M) + rest; }
 };
 __device__ __forceinline__ Scale value_scale(const Scales& m) {
     const float vs = m.vs > 0.f ? m.vs : Q8C_FLOOR;
-    const float lv = __builtin_amdgcn_logf(vs);
-    return {lv, __builtin_amdgcn_rcpf(vs), lv + 8.f};
+    const uint32_t b = __float_as_uint(vs);  // (a normal number)
+    return {(float)((int)(b >> 23) - (127 - 8)), __builtin_amdgcn_logf(__uint_as_float((b & 0x7fffffu) | 0x3f800000u)), __builtin_amdgcn_rcpf(vs)};
 }
 // The factor of a block's scores; at least float32's smallest normal number, so
 // that -inf times it is -inf (a NaN stays).
@@ -225,7 +231,7 @@ __device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Scales& m, floa
         if ((m.bad >> e) & 1) x = __builtin_nanf("");
         if ((unsigned)(Q8C_BLOCK * blk + e - k0) >= (unsigned)n) x = -__builtin_inff();
     }
-    const float mx = largest(s0, s1) * cs + v.lv;
+    const float mx = largest(s0, s1) * cs + v.log2();
     if (__any(mx > S.M + 7.f)) {
         float cm = fmaxf(mx, lane_xor_f32<16>(mx));
         cm = fmaxf(cm, lane_xor_f32<32>(cm));
@@ -239,16 +245,17 @@ __device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Scales& m, floa
     // count in the sum alone, as p: with the scale in them they could pass
     // float32's range.
     const bool zeros = !(m.vs > 0.f), out = zeros || mx < S.M - 60.f;
-    if (!__any(out)) return v.lv - S.M + 8.f;
+    if (!__any(out)) return v.offset(S.M);
     // (p beside w: at most 2^8 * 2^96, where the block's floor set M)
-    const float base = zeros && !(mx < S.M - 60.f) ? v.lv - S.M + 8.f : 8.f - S.M, iv = base == 8.f - S.M ? 1.f : v.iv;
+    const bool with = zeros && !(mx < S.M - 60.f);  // the scale
+    const float base = with ? v.offset(S.M) : 8.f - S.M, iv = with ? v.iv : 1.f;
     if (out) {
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j++) sum += exp2_hw(__builtin_fmaf(j < 4 ? s0[j & 3] : s1[j & 3], cs, base));
         S.l = __builtin_fmaf(sum, iv, S.l);
     }
-    return out ? -__builtin_inff() : v.lv - S.M + 8.f;
+    return out ? -__builtin_inff() : v.offset(S.M);
 }
 
 // The eight weights of a lane in two parts, each rounded to nearest: h =
@@ -524,7 +531,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         const bool all_seen = from <= Q8C_BLOCK * blk && to >= Q8C_BLOCK * (blk + 1);
         const Scale v = value_scale(mb);
         const float cs = key_scale(rs.scale, mb);
-        float base = v.lv8 - S.M;
+        float base = v.offset(S.M);
         if (!all_seen || mb.bad || !(mb.vs > 0.f) || __builtin_amdgcn_ballot_w64(near_enough(largest(s[0], s[1]), cs, base)) != ~0ull)
             base = correct<DP>(s[0], s[1], mb, cs, v, blk, g, k0, n, S);
         Weights W;
@@ -712,7 +719,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void many_kernel(Args A) {
 #pragma unroll
         for (int ct = 0; ct < NCT; ct++) {
             cs[ct] = key_scale(scale[ct], m);
-            base[ct] = v.lv8 - S[ct].M;
+            base[ct] = v.offset(S[ct].M);
             fine &= near_enough(top[ct], cs[ct], base[ct]);
         }
         if (!(Q8C_BLOCK * here >= from && Q8C_BLOCK * (here + 1) <= to && m.bad == 0 && m.vs > 0.f && __builtin_amdgcn_ballot_w64(fine) == ~0ull)) {

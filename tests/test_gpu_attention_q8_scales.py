@@ -1,0 +1,32 @@
+"""Attention over the 8-bit cache with scales far from one: its weights hold the
+value scales, its scores' factor the key scales and the query's exponent."""
+import numpy as np
+import pytest
+
+import q8_ref
+import test_gpu_cache_q8 as cache_tests
+
+pytestmark = pytest.mark.gpu
+rt = cache_tests.rt
+
+
+@pytest.mark.parametrize("T,room", [(1, None), (3, 1 << 18), (128, 1 << 18)])
+@pytest.mark.parametrize("near", [-90, -64, -30, 0, 30, 64, 100])
+def test_value_scales(gpu, rt, T, room, near):
+    """Equal scores, so an output is the mean of the values, of two blocks whose
+    scales are around 2^near. A weight's error: the logarithm of its scale's
+    fraction, 2^-23, the offset, of magnitude 8 to 16, 2^-21, together times
+    ln 2; the exponential, one unit in the last place, 2^-23; two parts, 2^-22. In the
+    sum of weights the scale's reciprocal, 2^-23 twice. Sums and the division: five
+    roundings of 2^-24. (2^-23 + 2^-21) ln 2 + 3 * 2^-23 + 2^-22 + 5 * 2^-24 =
+    1.3e-6 of the sum of p v (no value is negative)."""
+    hk, d, n = 512, 64, 64
+    rng = np.random.default_rng(near + 200)
+    ref = cache_tests.random_cache(rng, hk, n, d)
+    ref.k[:], ref.v = 0, np.abs(ref.v)
+    ref.vs[:] = np.ldexp(1 + rng.random(ref.vs.shape), near + rng.integers(0, 2, ref.vs.shape)).astype(np.float32)
+    q = rng.standard_normal((T, hk, d)).astype(np.float32)
+    got = cache_tests.run(gpu, rt, q, ref, np.full(T, n - 1), None, room)
+    v = ref.values()[1]
+    off = (np.abs(got - v.mean(1)) / v.mean(1)).max()
+    assert off <= 1.3e-6, off
