@@ -36,6 +36,7 @@
 // twice its products; with one part the outputs' error would be 2^-11, not
 // float32's.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "cache_q8.hpp"
@@ -71,6 +72,7 @@ struct Args {
     const uint8_t* cache;
     const int64_t *kend, *kstart;
     int T, H, Hkv, G, d;
+    float factor;    // log2(e) / sqrt(d)
     int64_t C, maxk, nb;
     float* out;      // [T][H][d]
     float* part;     // [splits][T * H][DP] sums, then [splits][T * H] of {M, l}
@@ -138,14 +140,10 @@ __device__ __forceinline__ Eight query_step(const float* row, int d, int s, int 
     }
     return Eight{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
-// A row's exponent e, amax * 2^e in [2^14, 2^15), and the factor of its scores
-// (log2, without the block's key scale; NaN where the row is not finite).
-struct RowScale {
-    int e;
-    float scale;
-};
+// A row in two parts, scaled to a largest value in [2^14, 2^15) (NaN where it is
+// not finite): returns the exponent that takes this back.
 template <int DP>
-__device__ __forceinline__ RowScale row_scale(const Eight* x, int d) {
+__device__ __forceinline__ int row_exponent(const Eight* x, bool& finite) {
     float amax = 0.f;
     int f = 1;
 #pragma unroll
@@ -159,16 +157,13 @@ __device__ __forceinline__ RowScale row_scale(const Eight* x, int d) {
     amax = fmaxf(amax, lane_xor_f32<32>(amax));
     f &= lane_xor<16>(f);
     f &= lane_xor<32>(f);
-    RowScale r;
-    r.e = amax > 0.f && f ? 15 - __builtin_amdgcn_frexp_expf(amax) : 0;
-    const float k = (float)(1.4426950408889634 / sqrt((double)d));
-    r.scale = f ? __builtin_ldexpf(k, -r.e) : __builtin_nanf("");
-    return r;
+    finite = f;
+    return amax > 0.f && f ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
 }
-__device__ __forceinline__ void two_parts(const Eight& x, const RowScale& r, v8h& hi, v8h& lo) {
+__device__ __forceinline__ void two_parts(const Eight& x, int exponent, bool finite, v8h& hi, v8h& lo) {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const float v = r.scale == r.scale ? __builtin_ldexpf(x.x[j], r.e) : 0.f;
+        const float v = finite ? __builtin_ldexpf(x.x[j], -exponent) : __builtin_nanf("");
         const _Float16 h = (_Float16)v;
         hi[j] = h;
         lo[j] = (_Float16)(v - (float)h);
@@ -199,11 +194,11 @@ __device__ __forceinline__ Scale value_scale(const Scales& m) {
     const uint32_t b = __float_as_uint(vs);  // (a normal number)
     return {(float)((int)(b >> 23) - (127 - 8)), __builtin_amdgcn_logf(__uint_as_float((b & 0x7fffffu) | 0x3f800000u)), __builtin_amdgcn_rcpf(vs)};
 }
-// The factor of a block's scores; at least float32's smallest normal number, so
-// that -inf times it is -inf (a NaN stays).
-__device__ __forceinline__ float key_scale(float scale, const Scales& m) {
-    const float c = scale * m.ks;
-    return c < 1.17549435e-38f ? 1.17549435e-38f : c;
+// The factor of a row's scores of a block: the block's, log2(e) / sqrt(d) times
+// its key scale, with the row's exponent (which alone may pass float32's range).
+// At least float32's smallest normal number, so that -inf times it is -inf.
+__device__ __forceinline__ float key_scale(float block, int exponent) {
+    return __builtin_amdgcn_fmed3f(__builtin_ldexpf(block, exponent), 1.17549435e-38f, 3.40282347e38f);
 }
 // (In a chain: v_max3_f32 takes products as they come, v_max_f32 wants each
 // made canonical first, one instruction more.)
@@ -496,10 +491,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         m = scales_of(meta, blk);
     };
     if (b < b1) fetch_k(b);
-    const RowScale rs = row_scale<DP>(x, A.d);
+    bool finite;
+    const int exponent = row_exponent<DP>(x, finite);
 #pragma unroll
     for (int s = 0; s < DP / 32; s++)
-        if (s % NW == w) two_parts(x[s], rs, S_.q[0][s][l], S_.q[1][s][l]);
+        if (s % NW == w) two_parts(x[s], exponent, finite, S_.q[0][s][l], S_.q[1][s][l]);
     __syncthreads();
     State<DP> S;
 #pragma unroll
@@ -530,7 +526,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         if (b < b1) fetch_k(b);
         const bool all_seen = from <= Q8C_BLOCK * blk && to >= Q8C_BLOCK * (blk + 1);
         const Scale v = value_scale(mb);
-        const float cs = key_scale(rs.scale, mb);
+        const float cs = key_scale(A.factor * mb.ks, exponent);
         float base = v.offset(S.M);
         if (!all_seen || mb.bad || !(mb.vs > 0.f) || __builtin_amdgcn_ballot_w64(near_enough(largest(s[0], s[1]), cs, base)) != ~0ull)
             base = correct<DP>(s[0], s[1], mb, cs, v, blk, g, k0, n, S);
@@ -615,7 +611,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void many_kernel(Args A) {
     const int t0 = (tiles - 1 - tile) * A.tpt, cols = min(A.tpt, A.T - t0) * A.G;
     if (!takes_many(A, t0, MANY_COLS<DP>)) return;
     if (w == 0) join_ranges(spans_of(A, t0), R);
-    float scale[NCT];
+    int exponent[NCT];
     v8h qhi[NCT][DP / 32], qlo[NCT][DP / 32];
     State<DP> S[NCT];
     int from = 0, to = 0x7fffffff;  // keys that all of the wave's columns see
@@ -629,10 +625,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void many_kernel(Args A) {
         Eight x[DP / 32];
 #pragma unroll
         for (int s = 0; s < DP / 32; s++) x[s] = query_step(A.q + (int64_t)head * A.d, A.d, s, g);
-        const RowScale rs = row_scale<DP>(x, A.d);
-        scale[ct] = rs.scale;
+        bool finite;
+        exponent[ct] = row_exponent<DP>(x, finite);
 #pragma unroll
-        for (int s = 0; s < DP / 32; s++) two_parts(x[s], rs, qhi[ct][s], qlo[ct][s]);
+        for (int s = 0; s < DP / 32; s++) two_parts(x[s], exponent[ct], finite, qhi[ct][s], qlo[ct][s]);
 #pragma unroll
         for (int i = 0; i < DP / 16; i++) S[ct].o[i] = v4f{0.f, 0.f, 0.f, 0.f};
         S[ct].M = M_NONE;
@@ -714,11 +710,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void many_kernel(Args A) {
         v8h k0 = kb[0][l], k1 = kb[NS][l];
         const Scales m = mh;
         const Scale v = value_scale(m);
+        const float block = A.factor * m.ks;
         float cs[NCT], base[NCT];
         bool fine = true;
 #pragma unroll
         for (int ct = 0; ct < NCT; ct++) {
-            cs[ct] = key_scale(scale[ct], m);
+            cs[ct] = key_scale(block, exponent[ct]);
             base[ct] = v.offset(S[ct].M);
             fine &= near_enough(top[ct], cs[ct], base[ct]);
         }
@@ -1049,6 +1046,7 @@ hipError_t launch_attention_q8(const float* q, const void* cache, const int64_t*
     A.Hkv = Hkv;
     A.G = H / Hkv;
     A.d = d;
+    A.factor = (float)(1.4426950408889634 / std::sqrt((double)d));
     A.C = C;
     A.maxk = maxk;
     A.nb = q8c_blocks(C);

@@ -3,7 +3,7 @@ value scales, its scores' factor the key scales and the query's exponent."""
 import numpy as np
 import pytest
 
-import q8_ref
+import attention_bound
 import test_gpu_cache_q8 as cache_tests
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +30,21 @@ def test_value_scales(gpu, rt, T, room, near):
     v = ref.values()[1]
     off = (np.abs(got - v.mean(1)) / v.mean(1)).max()
     assert off <= 1.3e-6, off
+
+
+@pytest.mark.parametrize("T,room", [(1, None), (3, 1 << 18), (160, 1 << 18)])
+@pytest.mark.parametrize("power", [-130, -126, -118, -100, 90])
+def test_queries_and_key_scales_at_opposite_ends(gpu, rt, T, room, power):
+    """Queries down to subnormal numbers over keys near float32's largest, and the
+    other way round, whose scores are ordinary: within the bound of any others."""
+    rng = np.random.default_rng(power + 200)
+    ref = cache_tests.random_cache(rng, 2, 500, 64, spread=0.3)
+    q = rng.standard_normal((T, 4, 64)).astype(np.float32)
+    q, by = np.ldexp(q, power).astype(np.float32), -power if power > 0 else min(-power, 123)
+    ref.ks[:] = np.ldexp(ref.ks, by)
+    kend = 499 - np.arange(T)[::-1]
+    got = cache_tests.run(gpu, rt, q, ref, kend, None, room)
+    rows = sorted({0, T // 2, T - 1})
+    want, bound = attention_bound.attention(q[rows], ref, kend[rows])
+    off = np.abs(got[rows] - want)
+    assert (off <= bound).all(), (off / bound).max()
