@@ -215,9 +215,10 @@ __device__ __forceinline__ bool near_enough(float top, float cs, float base) {
 
 // What a block may need before its weights, in lanes or as a whole: entries
 // that a column does not see (-inf) or that are not finite (NaN), M moved, and
-// weights left out. Returns the exponents' offset.
+// weights left out. Returns the exponents' offset; may change the scores and
+// their factor.
 template <int DP>
-__device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Scales& m, float cs, Scale v, int blk, int g, int k0, int n,
+__device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Scales& m, float& cs, Scale v, int blk, int g, int k0, int n,
                                          State<DP>& S) {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -226,8 +227,8 @@ __device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Scales& m, floa
         if ((m.bad >> e) & 1) x = __builtin_nanf("");
         if ((unsigned)(Q8C_BLOCK * blk + e - k0) >= (unsigned)n) x = -__builtin_inff();
     }
-    const float mx = largest(s0, s1) * cs + v.log2();
-    if (__any(mx > S.M + 7.f)) {
+    const float lv = v.log2(), mx = largest(s0, s1) * cs + lv;
+    if (__any(mx - S.M > 7.f)) {
         float cm = fmaxf(mx, lane_xor_f32<16>(mx));
         cm = fmaxf(cm, lane_xor_f32<32>(cm));
         const float M = fmaxf(S.M, cm), a = exp2_hw(0.5f * (S.M - M));
@@ -236,21 +237,36 @@ __device__ __forceinline__ float correct(v4f& s0, v4f& s1, const Scales& m, floa
 #pragma unroll
         for (int i = 0; i < DP / 16; i++) S.o[i] *= a * a;
     }
+    const bool zeros = !(m.vs > 0.f), below = mx < S.M - 60.f, out = zeros || below;
+    float base = v.offset(S.M), pbase = 8.f - S.M;
+    // Where M is 2^20 or more its own rounding shows beside the fused product's,
+    // which has none: by 2^28 a column's largest exponent would be far from 8. The
+    // products are rounded as they are in M there, and become the exponents.
+    const bool far = __builtin_fabsf(S.M) >= 0x1p20f;
+    if (__any(far)) {
+        if (far) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                s0[j] = (s0[j] * cs + lv) - S.M + 8.f;
+                s1[j] = (s1[j] * cs + lv) - S.M + 8.f;
+            }
+            cs = 1.f;
+            base = 0.f;
+            pbase = -lv;
+        }
+    }
     // A block of zeros, and lanes whose w are all below 2^-60 of the largest,
     // count in the sum alone, as p: with the scale in them they could pass
-    // float32's range.
-    const bool zeros = !(m.vs > 0.f), out = zeros || mx < S.M - 60.f;
-    if (!__any(out)) return v.offset(S.M);
-    // (p beside w: at most 2^8 * 2^96, where the block's floor set M)
-    const bool with = zeros && !(mx < S.M - 60.f);  // the scale
-    const float base = with ? v.offset(S.M) : 8.f - S.M, iv = with ? v.iv : 1.f;
+    // float32's range (p beside w: at most 2^8 * 2^96, where the block's floor set M).
+    if (!__any(out)) return base;
     if (out) {
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) sum += exp2_hw(__builtin_fmaf(j < 4 ? s0[j & 3] : s1[j & 3], cs, base));
-        S.l = __builtin_fmaf(sum, iv, S.l);
+        for (int j = 0; j < 8; j++) sum += exp2_hw(__builtin_fmaf(j < 4 ? s0[j & 3] : s1[j & 3], cs, below ? pbase : base));
+        S.l = __builtin_fmaf(sum, below ? 1.f : v.iv, S.l);
+        base = -__builtin_inff();
     }
-    return out ? -__builtin_inff() : v.offset(S.M);
+    return base;
 }
 
 // The eight weights of a lane in two parts, each rounded to nearest: h =
@@ -526,7 +542,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 3 : 1) void few_kernel(Args A)
         if (b < b1) fetch_k(b);
         const bool all_seen = from <= Q8C_BLOCK * blk && to >= Q8C_BLOCK * (blk + 1);
         const Scale v = value_scale(mb);
-        const float cs = key_scale(A.factor * mb.ks, exponent);
+        float cs = key_scale(A.factor * mb.ks, exponent);
         float base = v.offset(S.M);
         if (!all_seen || mb.bad || !(mb.vs > 0.f) || __builtin_amdgcn_ballot_w64(near_enough(largest(s[0], s[1]), cs, base)) != ~0ull)
             base = correct<DP>(s[0], s[1], mb, cs, v, blk, g, k0, n, S);

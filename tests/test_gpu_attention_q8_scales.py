@@ -48,3 +48,25 @@ def test_queries_and_key_scales_at_opposite_ends(gpu, rt, T, room, power):
     want, bound = attention_bound.attention(q[rows], ref, kend[rows])
     off = np.abs(got[rows] - want)
     assert (off <= bound).all(), (off / bound).max()
+
+
+@pytest.mark.parametrize("T,n,room", [(1, 300, None), (1, 6000, None), (130, 600, 1 << 18)])
+@pytest.mark.parametrize("power", [12, 20, 23, 26, 27, 28, 30, 40, 60, 100])
+def test_scores_far_past_the_exponential(gpu, rt, T, n, room, power):
+    """Scores up to 2^power (of log2 weights): a row is its best key's value, where
+    float32 tells it from the next (40 and 2^-20 of its size apart). The best
+    weight is 2^8 to 2^15 in two parts, of error 2^-22, the sum takes a reciprocal
+    twice: 2^-20 of the value. The n others weigh at most 2^-40 of it each, with a
+    scale in common: n 2^-40 of the largest value more."""
+    rng = np.random.default_rng(power)
+    ref = cache_tests.random_cache(rng, 1, n, 64)
+    q = rng.standard_normal((T, 4, 64)).astype(np.float32)
+    k, v = (x[0] for x in ref.values())
+    scores = lambda q: q.astype(np.float64) @ k.T * np.log2(np.e) / 8  # noqa: E731
+    q = (q * (2.0 ** power / np.abs(scores(q)).max())).astype(np.float32)
+    z = scores(q)
+    two = np.sort(z, -1)[..., -2:]
+    clear = two[..., 1] - two[..., 0] > 40 + 2.0 ** -20 * two[..., 1]
+    assert clear.any()
+    got, want = cache_tests.run(gpu, rt, q, ref, np.full(T, n - 1), None, room)[clear], v[z.argmax(-1)][clear]
+    assert (np.abs(got - want) <= 2.0 ** -20 * np.abs(want) + n * 2.0 ** -40 * np.abs(v).max()).all()
