@@ -527,8 +527,9 @@ int mimg_attention_dev(const float *q, const void *kcache, const void *vcache, c
                        int64_t max_keys, int f16, float *out, void *ws, uint64_t ws_bytes, void *stream);
 
 /* ---- the 8-bit key-value cache -------------------------------------------
- * A cache of half the bytes of an f16 one: int8 values, with one float32
- * scale for each block of 32 entries and kv head, for keys and for values. One
+ * A cache of half the bytes of an f16 one (d a multiple of 64): int8 values,
+ * with one float32 scale for each block of 32 entries and kv head, for keys and
+ * for values, so an entry's rounding depends on the others of its block too. One
  * buffer of mimg_cache_q8_bytes holds the keys and values of a layer; it must
  * be zeroed before its first use. No reference counterpart (its caches are f32
  * or f16, importer/llama.go:489-503).

@@ -24,16 +24,16 @@
 //
 // Bound: few rows (few_kernel) by the cache's bytes, read once for the query
 // heads of a kv head; many rows of one sequence (many_kernel) by the matrix
-// cores, 8 d flops a (query, key) pair with the two parts, 1240 to 1264 TFLOP/s
+// cores, 8 d flops a (query, key) pair with the two parts, 1240 to 1296 TFLOP/s
 // in a large f16 product. Measured on MI355X, 32 heads, 8 kv heads, d = 128:
 //   64 sequences of 2048 keys   41 us, 233 MB: 5.7 TB/s (a read kernel 7.05)
-//   1 sequence of 131072 keys   48 us, 269 MB; 4.6 of them join_kernel
-//   8 sequences of 2048 keys    10.1 us and join_kernel's 3.1: mostly the way
+//   1 sequence of 131072 keys   49 us, 269 MB; 4.6 of them join_kernel
+//   8 sequences of 2048 keys    10.8 us and join_kernel's 3.1: mostly the way
 //                               from the launch to the first weight
-//   2048 rows behind 6100 keys  385 us, 478 GFLOP: 1.24 PFLOP/s
+//   2048 rows behind 6100 keys  406 to 419 us, 478 GFLOP: 1.14 to 1.18 PFLOP/s
 // d = 64, one row of 181 keys 5.4 us. The two parts cost the decode rows nothing
-// that shows (their products take 16 us of the 41, under the loads) and a prompt
-// twice its products; with one part the outputs' error would be 2^-11, not
+// that shows (the matrix cores are at work 7 us of the 41, under the loads) and a
+// prompt twice its products; with one part the outputs' error would be 2^-11, not
 // float32's.
 #include <algorithm>
 #include <cmath>
@@ -336,12 +336,14 @@ __device__ __forceinline__ Spans spans_of(const Args& A, int t0) {
 }
 // Whether many_kernel takes a tile: its tokens see the same blocks (a prompt),
 // not each its own (a decode batch). many_kernel reads a block once for the
-// tile, at 6 ns (128 columns; MI355X, all CUs busy), few_kernel once for each
-// token and 16 heads, at 0.7 ns from the caches. A last tile with few tokens
-// goes as the last full number of tokens does, not to few_kernel, whose splits
-// are for all tokens (128 rows of 14 heads behind 30000 keys, 18 rows a tile,
-// two in the last: 176 us, 56 so). many_kernel takes no tile unless a token of it,
-// or the call's last, sees `least` blocks. By a whole wave.
+// tile, at 3.6 ns (128 columns of 128 dims, all compute units busy; on smaller
+// grids twice that and more), few_kernel once for each token and 16 heads, at
+// 0.8 ns from the caches: taken where the tokens' blocks are the tile's times its
+// columns / 16. A last tile with few tokens goes as the last full number of tokens
+// does, not to few_kernel, whose splits are for all tokens (130 rows of 32 heads
+// behind 8000 keys, two in the last tile: 67 us, else 140). many_kernel takes no
+// tile unless a token of it, or the call's last, sees `least` blocks. By a whole
+// wave.
 __device__ __forceinline__ bool takes_many(const Args& A, int t0, int cols) {
     const Spans p = spans_of(A, max(min(t0, A.T - A.tpt), 0));
     const int span = wave_max_i32(max(p.e0, p.e1)) - wave_min_i32(min(p.e0 ? p.s0 : 0x7fffffff, p.e1 ? p.s1 : 0x7fffffff));
@@ -403,10 +405,10 @@ struct FewLds {
     int keys[COLS];  // that a column sees (a group's)
 };
 // The splits that so many blocks are worth, of n: of eight blocks, with `fours`
-// (few workgroups) of four up to 16 of them; none up to 8 blocks (one sequence,
-// at most 8192 keys: 100 keys 5.9 us against 7.2, 500 in four 7.2 against 8.4,
-// 2000 in 16 7.3 against 8.0; but 24 rows of 16 heads behind 2000 12.7 against
-// 11.0).
+// (few workgroups) of four up to 16 of them; none up to 8 blocks. In a cache of
+// 8192 keys, d = 64 / 128: 200 keys 7.1 / 8.5 us whole, 7.5 / 8.4 in two; 500 in
+// four 7.5 / 8.4, in two 8.3 / 9.5; 2000 in 16 7.7 / 8.6, in eight 8.3 / 9.5. But 24
+// rows of 16 heads behind 2000 keys in fours 12.5 us, in eights 11.2.
 __host__ __device__ __forceinline__ int splits_of(int64_t n, int64_t blocks, bool fours) {
     const int64_t eight = (blocks + 7) / 8, four = (blocks + 3) / 4;
     const int64_t s = !fours || eight > 16 ? eight : (four < 16 ? four : 16);
@@ -856,9 +858,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void many_kernel(Args A) {
 }
 
 // The splits of a row joined, DP / 4 threads a row and split. WIDE: a workgroup
-// per row, 1024 / DP of its splits at a time (up to 1024 rows, or 4096 of more than 8
-// splits: 32 splits of 2048 rows take 2 to 5 us less so, 9 of 7168 as much more);
-// else 1024 / DP rows a workgroup.
+// per row, 1024 / DP of its splits at a time; else 1024 / DP rows a workgroup.
 template <int DP, bool WIDE>
 __global__ __launch_bounds__(256) void join_kernel(Args A) {
     constexpr int LANES = DP / 4, GROUPS = 256 / LANES;
@@ -954,59 +954,78 @@ struct Cut {
     int64_t units, subs, many_wgs;
     int splits, few_splits, many_splits;
 };
+// The rules' constants, each with both sides as measured (MI355X, 32 heads, 8 kv
+// heads, us, d = 64 / 128 where two are given).
+
+// Up to these blocks of max_keys nothing is split: 8 sequences of 300 / 500 keys of
+// 128 dims 8.0 / 9.0, with splits and join_kernel 10.3 / 10.6.
+constexpr int64_t WHOLE_BLOCKS = 16;
+// few_kernel's workgroups that splits are to give, two for each compute unit.
+constexpr int64_t FEW_WGS = 512;
+// Rows (times kv heads and 16s of query heads) from which few_kernel splits by
+// eights of blocks, not by fours: see splits_of().
+constexpr int64_t FOURS_ROWS = 16;
+// Prompts are many_kernel's, a decode batch of as many sequences few_kernel's:
+// the ranges, on the device, tell them apart, so both are launched, and each
+// leaves the other's tiles. That costs a decode batch 5 to 9 us (64 sequences of 2000
+// keys of 128 dims 40 in a cache of theirs, 48 where max_keys is 4096 and more; 256
+// 82 and 87 / 155 and 164), so it is done from so many tokens and row-blocks
+// (rows as above times blocks of max_keys) on.
+constexpr int64_t MANY_TOKENS = 64, MANY_ROW_BLOCKS = 1 << 16;
+// A prompt's rows cost few_kernel their number times the blocks, many_kernel a
+// start of some 20 us: from as many row-blocks that the rows see on (on the device;
+// the host knows max_keys) it takes them. few_kernel and many_kernel: 64 rows behind
+// 2000 keys 21 and 24 / 31 and 33, behind 4000 34 and 28 / 52 and 34; 128 behind 1000
+// 21 and 25 / 32 and 33, behind 2000 34 and 28 / 52 and 35; 256 behind none 12 and
+// 19 / 19 and 25, behind 1000 37 and 29 / 58 and 38. From 512 tokens on that many are
+// seen in any case.
+constexpr int64_t LEAST_ROW_BLOCKS = 40000, LEAST_TOKENS = 512;
+// Rows a workgroup of few_kernel beside many_kernel takes, by dims up to 64 and more:
+// as many as give so many workgroups. 256 sequences of 2000 keys one by one / by twos
+// / by fours 90, 87 and 102 / 168, 177 and 165.
+constexpr int64_t BESIDE_WGS_64 = 1024, BESIDE_WGS = 512;
+// many_kernel's splits: the least work of the fullest compute unit, its
+// workgroups times their blocks, each with a start worth so many blocks; one
+// alone on a unit has 3 / 5 of the rate of two (past 192 dims all of it). 384 rows
+// behind 8000 keys of 128 dims, 96 workgroups: 147 in 6 splits, 118 in 5, 134 in 4;
+// 1280 rows, 320: 450 whole, 385 in 2, 343 in 3 and 4; behind none 66, 66 and 75 in 3.
+constexpr int64_t START_BLOCKS = 16;
+// Rows up to which join_kernel takes a workgroup a row, and with more than so many
+// splits: 256 rows (8 behind 8000 keys, 64 splits) 16 for the call, the other way
+// 25; 2048 (64 behind 30000) 81 and 88; 4096 (128 behind 8000, 16) 57 and 59; but
+// 8192 (256 behind 8000, 8) 88 and 86.
+constexpr int WIDE_ROWS = 1024, WIDE_SPLITS = 8, WIDE_ROWS_SPLIT = 4096;
+
 Cut cut(int64_t T, int H, int Hkv, int d, int64_t maxk) {
     const int64_t G = H / Hkv, subs = (G + COLS - 1) / COLS, blocks = (maxk + Q8C_BLOCK - 1) / Q8C_BLOCK;
-    const int64_t cols = d <= 128 ? MAX_COLS : MAX_COLS / 2;
-    // At most 64 splits, none up to 512 keys (9.4 us against 10.0 with join_kernel).
-    // few_kernel takes as many as give 512 workgroups.
+    const int64_t cols = d <= 128 ? MAX_COLS : MAX_COLS / 2, rows = T * Hkv * subs;
     Cut c{};
-    // Prompts of many tokens are many_kernel's, a decode batch of as many
-    // sequences few_kernel's: the ranges, on the device, tell them apart, so
-    // both are launched, and each leaves the other's tiles (a decode batch pays
-    // some 10 us of 50 and more, so not for smaller ones). A prompt's rows cost
-    // few_kernel their number times the blocks, many_kernel a start of some 20
-    // us; they meet near 5000 row-blocks of 8 kv heads (64 rows behind 2000 /
-    // 8000 keys 19 and 54 us against 23 and 34 at d = 64, 27 and 89 against 32
-    // and 45 at 128; 128 rows behind 1000 / 2000 keys 18 and 29 against 24 and
-    // 27, 28 and 46 against 33 and 34; 256 rows behind none / 1000 12 and 33
-    // against 18 and 31). The host knows max_keys, the device what the rows see,
-    // so that many blocks are asked for there too (below 512 rows, which see that
-    // many by themselves).
-    const int64_t rows = T * Hkv * subs;
-    c.least = T < 512 ? (int)(40000 / rows) : 0;
-    c.many = T >= 64 && G <= cols && blocks >= c.least && rows * blocks >= 1 << 16;
+    c.least = T < LEAST_TOKENS ? (int)(LEAST_ROW_BLOCKS / rows) : 0;
+    c.many = T >= MANY_TOKENS && G <= cols && blocks >= c.least && rows * blocks >= MANY_ROW_BLOCKS;
     if (c.many) c.tpt = (int)(cols / G);
+    c.fours = rows <= FOURS_ROWS;
+    c.few_splits = (int)std::min<int64_t>((FEW_WGS - 1 + rows) / rows, blocks <= WHOLE_BLOCKS ? 1 : splits_of(64, blocks, c.fours));
     // Rows that split their keys may be of one sequence each, or a short prompt's:
     // the device packs the latter's tokens into a tile's columns, and their
-    // workgroups share the keys (16 / 32 rows behind 8000 keys, d = 128: 30 and 50 us
-    // become 19 and 24; without splits it gains nothing: 64 rows behind 2000
-    // 27 and 27, behind none 6.4 and 8.7).
-    c.fours = rows <= 16;
-    c.few_splits = (int)std::min<int64_t>((511 + rows) / rows, blocks <= 16 ? 1 : splits_of(64, blocks, c.fours));
+    // workgroups share the keys (16 / 32 rows behind 8000 keys, d = 128, 33 and 55 us
+    // apart, 19 and 25 so; without splits it gains nothing: 48 rows behind none 6.5
+    // apart, 8.8 so).
     c.group = c.few_splits > 1 && G <= COLS / 2 ? (int)std::min<int64_t>(COLS / G, T) : 1;
     if (!c.many) c.tpt = c.group;
     const int64_t tiles = (T + c.tpt - 1) / c.tpt, groups = (c.tpt + c.group - 1) / c.group;
     c.many_wgs = tiles * Hkv;
     c.fan = 1;
     if (c.many) {
-        // Tokens a workgroup of few_kernel beside many_kernel, equally many: of d =
-        // 64 a CU takes four (256 rows of 2000 keys each 86 us, in twos 100), of d =
-        // 128 two are enough (164 us, in fours 178).
-        const int64_t each = std::max<int64_t>(rows / (d <= 64 ? 1024 : 512), 1);
+        const int64_t each = std::max<int64_t>(rows / (d <= 64 ? BESIDE_WGS_64 : BESIDE_WGS), 1);
         c.fan = (int)((groups + each - 1) / each);
     }
     c.units = tiles * c.fan;
     c.subs = subs;
-    // many_kernel's splits: the least work of the fullest compute unit, its
-    // workgroups times their blocks, each with a start worth some 16 blocks; one
-    // alone has 0.6 of the rate of two (at d = 256 all of it). 384 rows behind 8000
-    // keys, d = 128, 96 workgroups: 142 us in 6 splits, 113 in 5; 1280 rows, 320:
-    // 410 us whole, 370 in 2, 331 in 4; behind none 64, 65 and 75.
     c.many_splits = 1;
-    const int64_t most = blocks <= 16 ? 1 : std::min<int64_t>(blocks / 8, 64);
+    const int64_t most = blocks <= WHOLE_BLOCKS ? 1 : std::min<int64_t>(blocks / 8, 64);
     for (int64_t s = 1, best = INT64_MAX; c.many && s <= most; s++) {
         const int64_t n = (c.many_wgs * s + 255) / 256;
-        const int64_t cost = n * ((blocks + s - 1) / s + 16) * (n == 1 && d <= 192 ? 5 : 3);
+        const int64_t cost = n * ((blocks + s - 1) / s + START_BLOCKS) * (n == 1 && d <= 192 ? 5 : 3);
         if (cost < best) {
             best = cost;
             c.many_splits = (int)s;
@@ -1036,7 +1055,7 @@ hipError_t launch(Args A, const Cut& c, hipStream_t s) {
     if (c.many)
         hipLaunchKernelGGL((many_kernel<DP, MANY_COLS<DP> / 64>), dim3((unsigned)c.many_wgs, (unsigned)c.many_splits), dim3(256), 0, s, A);
     const int rows = A.T * A.H, groups = 1024 / DP;
-    if (c.splits > 1 && (rows <= 1024 || (c.splits > 8 && rows <= 4096)))
+    if (c.splits > 1 && (rows <= WIDE_ROWS || (c.splits > WIDE_SPLITS && rows <= WIDE_ROWS_SPLIT)))
         hipLaunchKernelGGL((join_kernel<DP, true>), dim3((unsigned)rows), dim3(256), 0, s, A);
     else if (c.splits > 1)
         hipLaunchKernelGGL((join_kernel<DP, false>), dim3((unsigned)((rows + groups - 1) / groups)), dim3(256), 0, s, A);

@@ -14,11 +14,15 @@
 //
 // Bound: 8 d bytes read and 2 d written a row and kv head; at the usual sizes
 // the chain from the index to the rows, the maximum and the bytes. Measured on
-// MI355X, 8 kv heads of 128 dims: 1 row 3.9 us, 64 rows of 64 sequences 5.1, a
-// prompt of 512 rows 7.4, of 2048 10.8 (21 MB: 2.0 TB/s), of 4000 20; there the
-// look through the index is a third (4 x 1000 rows of 64 dims: 15.9 us, of
-// which 4.6). One workgroup for several heads looks once: 16384 rows 97 us become
-// 63, but 2048 10.8 become 13.5 and more, so each head looks for itself.
+// MI355X, 8 kv heads of 128 dims: 1 row 4.2 us, 64 rows of 64 sequences 5.3, a
+// prompt of 512 rows 7.9, of 2048 11 (21 MB: 1.9 TB/s), of 4000 19, 16384 90, 65535
+// 1000: each block's workgroups look through the whole index, a third of the
+// time at 4 x 1000 rows of 64 dims (15.6 us, of which 4.6) and most of it from 16384
+// rows on. One workgroup for several heads looks once: 16384 rows by a third less,
+// but 2048 by a quarter more, so each head looks for itself. With rope (32 query
+// heads): 1 row 4.8 us, 64 rows of 64 sequences 6.4, prompts of 512 / 2048 / 4000 rows
+// 13 / 30 / 50: a 64-bit sine and cosine for each pair of a row, once in each kv
+// head's keys and once in q's.
 #include "cache_q8.hpp"
 #include "mimg_device.hpp"
 #include "decoder_math.hpp"
@@ -207,9 +211,8 @@ __global__ __launch_bounds__(256) void store_q8_kernel(StoreArgs A) {
             if (it >= items) continue;
             float &xa = xs[2 * j], &xb = xs[2 * j + 1];
             if (ROPE && half == 0) {
-                // (unrolled, so that the pairs' sines overlap; a loop of one copy into
-                // LDS is 0.3 us faster where the code is cold, but 7.7 against 5.8 us
-                // for 64 rows of 8 heads of 128 dims and 47 against 38 us for 2048)
+                // (unrolled, so that the pairs' sines overlap: a loop of one copy into LDS
+                // takes a third longer for 64 rows of 8 heads of 128 dims)
                 const int u = (int)(((uint32_t)it * inv_np) >> 20), i = it - u * np;
                 if (pair_of(i, A.rotary, A.interleaved).rot) turn(xa, xb, turn_of(A.pos[list[u].y], A.inv_freq[i]));
             }
@@ -324,13 +327,12 @@ hipError_t launch_store(StoreArgs a, hipStream_t s) {
     // one after another in the grid (then those of the rows behind these), so
     // that a prompt's, which all have such a row or all the one at the same
     // place, are spread over the compute units, and the rest end in their
-    // shadow: 10.8 us for a prompt of 2048 rows of 8 heads of 128 dims, in the
-    // rows' order 18.2. Rows a workgroup: prompts of 512 / 1024 / 2048 / 4000
-    // rows 7.4 / 8.4 / 15.8 / 30.5 us with 2, 7.3 / 8.2 / 10.8 / 19.8 with 8;
-    // decode batches of 128 / 256 / 512 / 1024 / 2048 rows 7.1 / 11.2 / 23 / 42 /
-    // 80 with 2, 15.6 / 17 / 26 / 47 / 79 with 8. 4 prompts of 1000 rows of 64 dims
-    // 18.4 us with 8, 15.9 with 32. 64 decode rows 4.9 us one by one in their
-    // order (as a prompt 6.9), 6.1 (6.5) by twos.
+    // shadow: 10.6 us for a prompt of 2048 rows of 8 heads of 128 dims, in the
+    // rows' order 17.7. Rows a workgroup, 1 / 2 / 8 / 32: prompts of 512 rows 8.0, 7.8,
+    // 7.7, 7.7 us, 1024 11.2, 8.5, 8.4, 8.4, 2048 20, 14, 10.6, 10.5, 4000 38, 27, 19.4,
+    // 19.3; decode batches of 128 rows 7.9, 7.7, 16, 55, 512 25, 23, 26, 76, 2048 87, 80,
+    // 80, 101. 64 decode rows 5.1 us one by one in their order (as a prompt's the
+    // same, a prompt of 65 rows 7.4 and 7.0), by twos 6.4.
     a.each = a.T <= 64 ? 1 : (a.T <= 1024 ? 2 : (a.T <= 2048 ? 8 : 32));
     a.runs = a.T <= 64 ? 1 : (a.T + 31) / 32;
     a.groups = a.T <= 64 ? a.T : a.runs * (32 / a.each);

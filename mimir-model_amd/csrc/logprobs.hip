@@ -15,9 +15,11 @@
 //
 // Bound: the logits' bytes, once, for many rows; for few the two launches'
 // chains of reductions. Measured on MI355X: 512 rows of 128256 logits, top 5,
-// 48 us (263 MB: 6.0 TB/s in chunk_kernel's 44 us; a read kernel 7.05), top 64
-// 65 us; one row, top 20, 11.6 us; 37 rows of 32003 of which a mask leaves 50, top
-// 8, 12.0 us; without alternatives 44, 6.0 and 6.7 us.
+// 47 to 50 us (263 MB: 6.0 TB/s in chunk_kernel's 44 us; a read kernel 7.05), top 20
+// / 33 / 64 53 / 55 / 63 us (k keys of each of 16 chunks written, read and ranked by
+// comparing all pairs, so the square of k); one row, top 20, 11.8 us, top 64 13.8; 37
+// rows of 32003 of which a mask leaves 50, top 8, 12 us; without alternatives 44,
+// 6.2 and 6.7 us.
 #include "decoder_math.hpp"
 #include "mimg_device.hpp"
 #include "mimg_kernels.hpp"

@@ -112,7 +112,8 @@ class Decoder:
     spec's bound for dequant_matmul.v1 but not in the reference's float
     order; 0 keeps the reference's order everywhere. cache_q8: keys and values
     in 8 bits (mimg_kv_store_q8_dev, mimg_attention_q8_dev), half the memory
-    and traffic of cache_f16, contexts past 8192; not the reference's bits.
+    and traffic of cache_f16 at head sizes that are multiples of 64, contexts
+    past 8192; not the reference's bits.
     """
 
     def __init__(self, config, tensors, a8=True, cache_f16=False, max_rows=64, slots=1, procs=16, kquant_block=256,
@@ -490,7 +491,9 @@ class Decoder:
         dict(logprobs [P - 1], entropy [P], top_ids and top_logprobs [P, top]),
         position i of the last three being the choice after tokens[i]. The mean
         of -logprobs is the log of the perplexity. The tokens take the slot's
-        cache from its start."""
+        cache from its start. With an 8-bit cache a token's scores depend a
+        little on the up to 31 behind it in its block that are stored in the
+        same chunk of max_rows: their values are in the block's scale."""
         tokens = np.asarray(tokens, np.int32).ravel()
         P, R = tokens.size, self.R
         if P < 1 or P > self.c.context:
