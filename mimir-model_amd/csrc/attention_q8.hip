@@ -180,7 +180,7 @@ struct State {
 
 // A block's value scale for the exponents: log2 in whole steps and the rest in
 // [0, 1), so that it costs no bits beside M, however far from one the scale is
-// (as one number 1.6e-6 of an output where scales are near 2^-90 or 2^64, so 4e-7;
+// (as one number 1.6e-6 of an output where scales are near 2^-90 or 2^64, so 5e-7;
 // 2048 rows behind 6100 keys 416 us as one, so 419); reciprocal (of a block of
 // zeros the floor's; its weights are left out below).
 struct Scale {
