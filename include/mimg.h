@@ -609,6 +609,68 @@ int mimg_logprobs_dev(const float *logits, int64_t rows, int64_t n, int64_t ld, 
                       float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs, void *ws, uint64_t ws_bytes,
                       void *stream);
 
+/* ---- a mixture of experts ------------------------------------------------
+ * A feed-forward layer whose tokens each go through `top` of `experts`
+ * experts (1..512; top 1..32, at most experts), a pair p = t * top + j being
+ * token t's choice j. No reference counterpart (its importer builds dense
+ * layers only, importer/llama.go:505-534); a GGUF file holds the experts'
+ * matrices of a layer one behind the other, [experts, N, K], which is one
+ * registered weight of experts * N rows.
+ *
+ * A plan puts the pairs in order by expert: int32 first[experts + 1] (the place
+ * of each expert's first pair in the order; the last one: how many pairs have
+ * an expert); from entry round_up(experts + 1, 64) on the order (pairs by
+ * expert, an expert's in rising order, pairs without one behind all); from
+ * round_up(pairs, 64) entries behind that each pair's expert, -1 without one. */
+
+/* Bytes of a plan; 0 for shapes that have none (T 0..2^20, T * top at most
+ * 2^24). 4-byte aligned. */
+uint64_t mimg_experts_plan_bytes(int64_t T, int top, int experts);
+
+/* The plan of given choices ids [T, top], for a router of the caller's own. A
+ * pair whose id is outside 0..experts-1 (a padded token, an expert that is
+ * elsewhere) has no expert. */
+int mimg_experts_plan_dev(const int32_t *ids, int64_t T, int top, int experts, void *plan, uint64_t plan_bytes, void *stream);
+
+/* The router: logits = x [T, k] . router [experts, k]^T, summed in float64 (a
+ * choice is a step function of them); ids [T, top] the largest in falling
+ * order, equal ones by the lowest index, NaN behind all others; weights [T,
+ * top] = exp(logit - m) / sum exp(logit - m), m the largest, the sum over the
+ * chosen (normalize != 0) or over all experts; NaN where that formula gives it.
+ * plan (may be NULL): the plan of ids. k a multiple of 4, x and router 16-byte
+ * aligned. ws: mimg_experts_route_workspace_bytes, 256-byte aligned. */
+uint64_t mimg_experts_route_workspace_bytes(int64_t T, int experts);
+int mimg_experts_route_dev(const float *x, const float *router, int64_t T, int64_t k, int experts, int top, int normalize,
+                           int32_t *ids, float *weights, void *plan, uint64_t plan_bytes, void *ws, uint64_t ws_bytes,
+                           void *stream);
+
+/* h[p] = swiglu(x_t . gate_e^T, x_t . up_e^T) for each pair p of the plan with an
+ * expert e, t its token; the rows of other pairs are left as they were. gate
+ * and up: weights of experts * n rows of one dtype and K; x [T, K] and h
+ * [T * top, n] 16-byte aligned, not overlapping. x is quantized into ws as the
+ * dtype's 8-bit products do (blocks of 256 for Q4_K and Q6_K, of 32 for Q8_0);
+ * a product is, bit for bit, what mimg_linear_a8_dev gives with block 256 and
+ * the expert's matrix alone, for Q8_0 what
+ * mimg_matmul_a8_quantized_q8_0_tiled_dev gives (also where K is no multiple of
+ * 256), refused rows always in the order of at most eight rows; swiglu is
+ * mimg_swiglu_dev's formula for a whole piece (its vector one). The plan must
+ * be of the same T, top and experts. ws:
+ * mimg_experts_swiglu_workspace_bytes, 256-byte aligned. Returns
+ * MIMG_NOT_HANDLED (nothing launched) for weights of different dtypes or of
+ * one without such a product. */
+uint64_t mimg_experts_swiglu_workspace_bytes(int64_t T, int top, int64_t n, int64_t k);
+int mimg_experts_swiglu_a8_dev(uint64_t gate, uint64_t up, int experts, const float *x, int64_t T, int top, const void *plan,
+                               uint64_t plan_bytes, float *h, void *ws, uint64_t ws_bytes, void *stream);
+
+/* y[t] = sum_j weights[t, j] * (h[t * top + j] . down_e^T) over the pairs of
+ * token t that have an expert e, in the order of the choices, one fma each
+ * (zeros for a token without any). down: a weight of experts * n rows; h
+ * [T * top, K], weights [T, top], y [T, n]; products, plan, alignment and
+ * refusals as above; y must not overlap h or weights. */
+uint64_t mimg_experts_combine_workspace_bytes(int64_t T, int top, int64_t n, int64_t k);
+int mimg_experts_combine_a8_dev(uint64_t down, int experts, const float *h, const float *weights, int64_t T, int top,
+                                const void *plan, uint64_t plan_bytes, float *y, void *ws, uint64_t ws_bytes, void *stream);
+
 /* One step of the greedy loop on the device (reference cmd/mim-run/main.go
  * generate, 184-257), for n sequences: ids[i] = chosen[i], out[count*n+i] =
  * chosen[i] while count < cap (out holds cap*n ids), pos[i] += 1,

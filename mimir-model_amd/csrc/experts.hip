@@ -1,0 +1,586 @@
+// The products of a mixture of experts: block-quantized weights of many
+// experts [experts][N][K] x 8-bit activations, each (token, choice) pair with
+// its expert's matrix, in the order of a plan (experts.hpp).
+//
+// Numerics. Per (weight row, activation row) and block the exact int32 sums of
+// the other 8-bit products, then one float chain in block order:
+//   Q4_K  S = sum_k sc_s(k) q_k y_k, M = sum_s m_s xs_s,
+//         tot = fma(f32(S), d*dx, tot), off = fma(f32(M), dmin*dx, off)
+//   Q6_K  S = sum_k sc_s(k) (q_k - 32) y_k, tot = fma(f32(S), d*dx, tot)
+//   Q8_0  (blocks of 32) S = sum_k q_k y_k, tot = fma(f32(S), d*dx, tot)
+// so a pair's row is bit for bit what its expert's matrix alone gives with
+// dequant_matmul_a8.v2 (block 256), and for Q8_0 what the tiled product with
+// blocks of 32 gives, whatever else the call holds.
+//
+// Layout. A workgroup of four waves takes BM = 32 or 64 pairs of one expert
+// against 128 weight rows (32 a wave), or with swiglu against 64 rows of gate
+// and the same 64 of up. The integer products are v_mfma_i32_32x32x32_i8: the
+// activations are the row operand, the weights the column operand (lane l holds
+// weight row l % 32), so a lane needs one block scale. A wave's raw blocks lie
+// in an LDS slot of its own (read into registers, then overwritten by the
+// next block's copies), the pairs' int8 rows (16-byte chunks XOR-swizzled by
+// row) and scales in two shared stages; all of it by global_load_lds, one
+// barrier a block. sc*q of Q4_K is split in two int8 planes, sc = 8 sh + sl, its
+// mins are one v_mfma_f32_32x32x16_f16 over xs = 64 hi + lo (every operand and
+// partial sum an integer that f16 and f32 hold exactly), as in gemm_q4k.hip;
+// sc*(q - 32) of Q6_K is 256 hi + lo.
+//
+// Which workgroup has which tile is decided on the device: the grid is as
+// large as any choice of that many pairs could need, a wave adds up the
+// experts' tiles from the plan, and what is past the last tile ends. The tiles
+// are in order by expert, row tile, pairs, dealt to the XCDs in eight runs, so
+// that the tiles that share weights meet in one L2.
+//
+// Rows of x the quantizer refused and weight rows with a non-finite block
+// scale take the float32 path (f32path.hpp) at the end.
+#include "decoder_math.hpp"
+#include "experts.hpp"
+#include "f32path.hpp"
+#include "mimg_device.hpp"
+#include "mimg_kernels.hpp"
+
+namespace mimg {
+namespace xp {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
+struct Mat {
+    const uint8_t* W;     // [experts * N] rows
+    const uint8_t* wref;  // [experts * N]
+};
+
+struct Args {
+    Mat mat[2];           // the matrix, or gate and up
+    float* y;             // [pairs][N]
+    const int32_t* plan;
+    int64_t rb, K;
+    int64_t wbytes;       // bytes of a matrix of all experts
+    int N, nb, experts, pairs;  // nb: blocks (of 256; of 32 for Q8_0) of a row
+    int rowdiv;           // a pair's activation row is pair / rowdiv
+    ActPtrs act;
+    const float* x;       // f32 activations (fallback)
+};
+
+template <uint32_t DT, int MT_>
+struct Cfg {
+    static constexpr int MT = MT_, T = 256, BM = 32 * MT;
+    static constexpr bool K32 = DT == DT_Q8_0;
+    // A row's group of 256 weights: the 16-byte chunks of its slot. Q6_K and
+    // Q8_0 groups are 2-byte aligned: copied from the 16-byte boundary below
+    // them, the chunks that cover them and one more where that spreads the
+    // rows' dwords over the banks (60 and 76 dwords a row).
+    static constexpr int GROUP = DT == DT_Q4_K ? Q4K_BYTES : DT == DT_Q6_K ? Q6K_BYTES : 8 * Q80_BYTES;
+    static constexpr int WCH = DT == DT_Q4_K ? 9 : DT == DT_Q6_K ? 15 : 19;
+    static constexpr int WSLOT = 16 * WCH;
+    static constexpr int WDMA = (32 * WCH + 63) / 64;
+    static constexpr int WWAVE = WDMA * 1024;  // incl. slack for the last copy
+    static constexpr int WBYTES = 4 * WWAVE;
+    static constexpr int ADMA = BM * 16 / T;
+    static constexpr int ABYTES = BM * 256;
+    static constexpr int XBYTES = DT == DT_Q4_K ? 1024 : 0;        // 16 bytes of sums a row
+    static constexpr int DBYTES = K32 ? BM * 32 : 256;             // 8 scales a row, or one
+    static constexpr int BUF = ABYTES + XBYTES + DBYTES;
+    static constexpr int SMEM = WBYTES + 2 * BUF;
+    static_assert(ADMA * T == BM * 16 && BM <= 64 && 2 * 64 * BM * 4 <= SMEM && SMEM <= 80 * 1024, "tile shape");
+};
+
+__device__ __forceinline__ void wait_vmcnt0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+// A workgroup's tile: expert e, its pairs' first place in the order, how many
+// of them the tile has, and the tile of weight rows.
+struct Tile {
+    int e, f0, m, nt;
+};
+
+template <int PER>
+__device__ __forceinline__ bool find_tile_of(const Args& A, int ntn, int BM, Tile& r) {
+    const int lane = threadIdx.x & 63;
+    int f[PER], cnt[PER], upto[PER], total = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int e = 64 * i + lane, c = min(e, A.experts - 1);
+        const int a = A.plan[c], b = A.plan[c + 1];
+        f[i] = min(max(a, 0), A.pairs);
+        cnt[i] = e < A.experts ? min(max(b, f[i]), A.pairs) - f[i] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        int s = (cnt[i] + BM - 1) / BM;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(s, d);
+            s += lane >= d ? o : 0;
+        }
+        upto[i] = total + s;
+        total = __builtin_amdgcn_readlane(upto[i], 63);
+    }
+    const int64_t all = (int64_t)total * ntn, per = (all + 7) / 8;
+    const int64_t wg = blockIdx.x, idx = (wg & 7) * per + (wg >> 3);
+    if ((wg >> 3) >= per || idx >= all) return false;
+    const int u = (int)(idx / ntn);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const uint64_t past = __ballot(upto[i] > u);
+        if (past == 0) continue;
+        const int l = __ffsll((unsigned long long)past) - 1;
+        const int n = __builtin_amdgcn_readlane(cnt[i], l), tiles = (n + BM - 1) / BM;
+        const int first = __builtin_amdgcn_readlane(upto[i], l) - tiles;
+        const int in = (int)(idx - (int64_t)first * ntn), mc = in % tiles;
+        r.e = 64 * i + l;
+        r.nt = in / tiles;
+        r.f0 = __builtin_amdgcn_readlane(f[i], l) + mc * BM;
+        r.m = min(n - mc * BM, BM);
+        return true;
+    }
+    return false;
+}
+__device__ __forceinline__ bool find_tile(const Args& A, int ntn, int BM, Tile& r) {
+    if (A.experts <= 64) return find_tile_of<1>(A, ntn, BM, r);
+    if (A.experts <= 128) return find_tile_of<2>(A, ntn, BM, r);
+    return find_tile_of<8>(A, ntn, BM, r);
+}
+
+// The copies of a thread: group 0's sources; group b adds a constant step.
+template <uint32_t DT, class C>
+struct Copies {
+    const uint8_t *w[C::WDMA], *a[C::ADMA], *s;
+    const uint8_t* wlast;  // the last 16 bytes that a copy may read (Q8_0)
+    const uint8_t* d8[C::K32 ? C::DBYTES / 1024 : 1];
+    uint32_t wave;
+    __device__ __forceinline__ void init(const Args& A, const Mat& M, int64_t row0, int n0, const int* rows) {
+        const int t = threadIdx.x, l = t & 63;
+        wave = __builtin_amdgcn_readfirstlane(t >> 6);
+#pragma unroll
+        for (int i = 0; i < C::WDMA; i++) {
+            const int c = min(64 * i + l, 32 * C::WCH - 1), r = c / C::WCH, j = c - C::WCH * r;
+            const uint8_t* p = M.W + (row0 + min(n0 + r, A.N - 1)) * A.rb;
+            w[i] = DT == DT_Q4_K ? p + 16 * j : p;
+        }
+        wlast = (const uint8_t*)__builtin_align_down(M.W + A.wbytes + WEIGHT_PAD - 16, 16);
+#pragma unroll
+        for (int i = 0; i < C::ADMA; i++) {
+            const int c = C::T * i + t, r = c >> 4, k = c & 15;
+            a[i] = (const uint8_t*)A.act.q + (int64_t)rows[r] * A.K + 16 * (k ^ (r & 15));
+        }
+        const int64_t row = (int64_t)rows[min(l, C::BM - 1)] * (A.K / 32);
+        s = wave == 0 && DT == DT_Q4_K ? (const uint8_t*)(A.act.xs + row) : (const uint8_t*)(A.act.d32 + row);
+        if constexpr (C::K32) {
+#pragma unroll
+            for (int i = 0; i < C::DBYTES / 1024; i++) {
+                const int c = C::T * i + t;
+                d8[i] = (const uint8_t*)(A.act.d32 + (int64_t)rows[c >> 3] * (A.K / 32) + (c & 7));
+            }
+        }
+    }
+    __device__ __forceinline__ void weights(int b, uint32_t lds) const {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < C::WDMA; i++) {
+            const uint8_t* p = w[i] + (int64_t)b * C::GROUP;
+            if constexpr (DT != DT_Q4_K) {
+                const int c = min(64 * i + l, 32 * C::WCH - 1), j = c % C::WCH;
+                p = (const uint8_t*)__builtin_align_down(p, 16) + 16 * j;
+                p = p < wlast ? p : wlast;
+            }
+            lds_copy16(p, lds + C::WWAVE * wave + 1024 * i);
+        }
+    }
+    __device__ __forceinline__ void activations(int b, uint32_t lds) const {
+#pragma unroll
+        for (int i = 0; i < C::ADMA; i++) lds_copy16(a[i] + 256 * (int64_t)b, lds + 1024 * wave + 16 * C::T * i);
+        if constexpr (C::K32) {
+#pragma unroll
+            for (int i = 0; i < C::DBYTES / 1024; i++)
+                lds_copy4(d8[i] + 32 * (int64_t)b, lds + C::ABYTES + 256 * wave + 4 * C::T * i);
+        } else {
+            if (DT == DT_Q4_K && wave == 0) lds_copy16(s + 16 * (int64_t)b, lds + C::ABYTES);
+            if (wave == 1) lds_copy4(s + 32 * (int64_t)b, lds + C::ABYTES + C::XBYTES);
+        }
+    }
+};
+
+// 16 bytes at an LDS address that is 2-byte aligned: five aligned dwords and
+// a byte realignment.
+__device__ __forceinline__ u32x4 lds_read16_a2(const uint8_t* p) {
+    const uint32_t sh = (uint32_t)((uintptr_t)p & 3);
+    const uint32_t* w = (const uint32_t*)__builtin_align_down(p, 4);
+    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = w[4];
+    return u32x4{__builtin_amdgcn_alignbyte(w1, w0, sh), __builtin_amdgcn_alignbyte(w2, w1, sh),
+                 __builtin_amdgcn_alignbyte(w3, w2, sh), __builtin_amdgcn_alignbyte(w4, w3, sh)};
+}
+__device__ __forceinline__ uint32_t lds_read2_a2(const uint8_t* p) {
+    const uint32_t w = *(const uint32_t*)__builtin_align_down(p, 4);
+    return ((uintptr_t)p & 2) ? w >> 16 : w & 0xFFFFu;
+}
+
+// A lane's part of its weight row's group: the raw bytes in registers, from
+// which the operands of a k step of 32 are built (lanes g = 0 and 1 of a row
+// hold its elements 16 g .. 16 g + 15).
+template <uint32_t DT>
+struct Group;
+
+template <>
+struct Group<DT_Q4_K> {
+    u32x4 q[4];
+    Q4KScales s;
+    float d, dmin;
+    __device__ __forceinline__ void read(const uint8_t* wr, int g) {
+        const u32x4 h = *(const u32x4*)wr;
+        d = f16_to_f32(h.x & 0xFFFFu);
+        dmin = f16_to_f32(h.x >> 16);
+        s = q4k_scales(h.y, h.z, h.w);
+#pragma unroll
+        for (int c = 0; c < 4; c++) q[c] = *(const u32x4*)(wr + 16 + 32 * c + 16 * g);
+    }
+    __device__ __forceinline__ void planes(int ks, int, v4i& H, v4i& L) const {
+        const uint32_t sc = byte_of(s.sc, ks);
+        const short sh = (short)(sc >> 3), sl = (short)(sc & 7);
+        const s16x2 shp = {sh, sh}, slp = {sl, sl};
+        const u32x4 qd = q[ks >> 1];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const s16x2 nib = as_s16x2((qd[k] >> (4 * (ks & 1))) & 0x0F0F0F0Fu);
+            H[k] = (int)as_u32(nib * shp);
+            L[k] = (int)as_u32(nib * slp);
+        }
+    }
+    // The mins as the column operand of the f16 product: 64 m_s (g = 0), m_s (g = 1).
+    __device__ __forceinline__ v8h mins(int g) const {
+        const uint32_t mw[2] = {(uint32_t)s.m, (uint32_t)(s.m >> 32)};
+        const h2 mul = g ? h2{(_Float16)1.0f, (_Float16)1.0f} : h2{(_Float16)64.0f, (_Float16)64.0f};
+        const h2 c1024 = {(_Float16)1024.0f, (_Float16)1024.0f};
+        v8h r;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t u = __builtin_amdgcn_perm(0u, mw[j >> 1], (j & 1) ? 0x0C030C02u : 0x0C010C00u);
+            const h2 f = (__builtin_bit_cast(h2, u | 0x64006400u) - c1024) * mul;
+            r[2 * j] = f.x;
+            r[2 * j + 1] = f.y;
+        }
+        return r;
+    }
+};
+
+template <>
+struct Group<DT_Q6_K> {
+    u32x4 ql[4], qh[2], sc;
+    float d;
+    __device__ __forceinline__ void read(const uint8_t* wr, int g) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) ql[i] = lds_read16_a2(wr + 64 * (i >> 1) + 32 * (i & 1) + 16 * g);
+#pragma unroll
+        for (int h = 0; h < 2; h++) qh[h] = lds_read16_a2(wr + 128 + 32 * h + 16 * g);
+        sc = lds_read16_a2(wr + 192);
+        d = f16_to_f32(lds_read2_a2(wr + 208));
+    }
+    __device__ __forceinline__ void planes(int ks, int g, v4i& H, v4i& L) const {
+        const int h = ks >> 2, p = ks & 3;
+        const u32x4 lo = ql[2 * h + (p & 1)], hi = qh[h];
+        // scale 8 h + 2 p + g, and w + 128 = scale q - 32 scale + 128 in 16 bits
+        const uint32_t sw = sc[2 * h + (p >> 1)] >> (16 * (p & 1));
+        const int s = (int)(int8_t)(uint8_t)(g ? sw >> 8 : sw);
+        const short cu = (short)(128 - 32 * s);
+        const s16x2 s2 = {(short)s, (short)s}, c2 = {cu, cu};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t q6 = (((p >> 1) ? (lo[k] >> 4) : lo[k]) & 0x0F0F0F0Fu) | (((hi[k] >> (2 * p)) & 0x03030303u) << 4);
+            const uint32_t ue = as_u32(as_s16x2(__builtin_amdgcn_perm(0u, q6, 0x0C020C00u)) * s2 + c2);
+            const uint32_t uo = as_u32(as_s16x2(__builtin_amdgcn_perm(0u, q6, 0x0C030C01u)) * s2 + c2);
+            H[k] = (int)__builtin_amdgcn_perm(uo, ue, 0x07030501u);
+            L[k] = (int)(__builtin_amdgcn_perm(uo, ue, 0x06020400u) ^ 0x80808080u);
+        }
+    }
+};
+
+template <>
+struct Group<DT_Q8_0> {
+    const uint8_t* p;
+    __device__ __forceinline__ void read(const uint8_t* wr, int) { p = wr; }
+    __device__ __forceinline__ v4i block(int ks, int g, float& d) const {
+        d = f16_to_f32(lds_read2_a2(p + Q80_BYTES * ks));
+        return __builtin_bit_cast(v4i, lds_read16_a2(p + Q80_BYTES * ks + 2 + 16 * g));
+    }
+};
+
+template <uint32_t DT, class C, bool SW>
+__global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
+    constexpr int MT = C::MT, BM = C::BM, BN = SW ? 64 : 128;
+    __shared__ __align__(16) uint8_t smem[C::SMEM];  // weights, then two activation stages
+    __shared__ int rows[BM], outs[BM], flags[1];
+    const int t = threadIdx.x, l = t & 63, wave = t >> 6;
+    const int a = l & 31, g = l >> 5;
+    Tile tile;
+    if (!find_tile(A, (A.N + BN - 1) / BN, BM, tile)) return;
+    if (t < BM) {
+        // (past the tile's pairs: the last one again, whose results are not written)
+        const PlanLayout pl = plan_layout(A.pairs, A.experts);
+        const int pair = min(max(A.plan[pl.order + tile.f0 + min(t, tile.m - 1)], 0), A.pairs - 1);
+        outs[t] = pair;
+        rows[t] = pair / A.rowdiv;
+    }
+    if (t == 0) flags[0] = 0;
+    __syncthreads();
+    const int n0 = tile.nt * BN, wn0 = n0 + 32 * (SW ? wave & 1 : wave);  // this wave's first weight row
+    const int64_t row0 = (int64_t)tile.e * A.N;
+    const Mat M = SW && wave >= 2 ? A.mat[1] : A.mat[0];
+
+    Copies<DT, C> cp;
+    cp.init(A, M, row0, wn0, rows);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
+    cp.weights(0, lds0);
+    cp.activations(0, lds0 + C::WBYTES);
+    {
+        int f = 0;
+        if (l < 32) f |= wn0 + l < A.N && M.wref[row0 + wn0 + l] != 0;
+        if (t < tile.m) f |= A.act.ok[rows[t]] == 0;
+        if (f) flags[0] = 1;
+    }
+    float tot[MT][16], off[DT == DT_Q4_K ? MT : 1][16];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            tot[i][r] = 0.f;
+            if (DT == DT_Q4_K) off[i][r] = 0.f;
+        }
+    const int asw = (a & 15) ^ g;  // chunk 2 ks + g of row a: slot 2 ks ^ asw
+    // the lane's group in its slot (Q6_K, Q8_0: from the boundary below it)
+    const uint32_t wmis = DT == DT_Q4_K ? 0 : (uint32_t)(uintptr_t)(M.W + (row0 + min(wn0 + a, A.N - 1)) * A.rb);
+    const int ng = C::K32 ? (A.nb + 7) / 8 : A.nb;
+    for (int b = 0; b < ng; b++) {
+        wait_vmcnt0();
+        lds_barrier();  // group b's copies have landed, group b - 1's activations are read
+        const uint8_t* buf = smem + C::WBYTES + (b & 1) * C::BUF;
+        const uint8_t* al = buf + a * 256;
+        const uint8_t* ws = smem + C::WWAVE * cp.wave + a * C::WSLOT;
+        if constexpr (DT != DT_Q4_K) ws += (wmis + (uint32_t)b * C::GROUP) & 15u;
+        Group<DT> grp;
+        grp.read(ws, g);
+        v16i acc[2][MT];
+        if constexpr (!C::K32) {
+            if (b + 1 < ng) {
+                cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
+                wait_lgkm0();  // the wave's weight slot is read
+                cp.weights(b + 1, lds0);
+            }
+            v4i av[MT];
+#pragma unroll
+            for (int i = 0; i < MT; i++) av[i] = *(const v4i*)(al + i * 8192 + 16 * asw);
+            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++) {
+                v4i pH, pL, nx[MT];
+                grp.planes(ks, g, pH, pL);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+                    if (ks < 7) nx[i] = *(const v4i*)(al + i * 8192 + 16 * ((2 * ks + 2) ^ asw));
+                const v16i z = {};
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    acc[0][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], pH, ks ? acc[0][i] : z, 0, 0, 0);
+                    acc[1][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], pL, ks ? acc[1][i] : z, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < MT; i++) av[i] = nx[i];
+            }
+            // The float step at raised priority: the waves of a SIMD drift
+            // apart, one's MFMAs under the other's vector instructions.
+            __builtin_amdgcn_s_setprio(1);
+            const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
+            v8h bm;
+            if constexpr (DT == DT_Q4_K) bm = grp.mins(g);
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                if constexpr (DT == DT_Q4_K) {
+                    // d*dx and dmin*dx of the tile as outer products (lanes
+                    // g = 0 hold d, g = 1 dmin)
+                    typedef float v32f __attribute__((ext_vector_type(32)));
+                    const v32f z = {};
+                    const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * i + a], g ? grp.dmin : grp.d, z, 0, 0, 0);
+                    const u32x4 xw = *(const u32x4*)(buf + C::ABYTES + 16 * (32 * i + a));
+                    const short sh = g ? 0 : 6;
+                    const s16x2 sh2 = {sh, sh};
+                    const uint32_t msk = g ? 0x003F003Fu : 0xFFFFFFFFu;
+                    const h2 cf = g ? h2{(_Float16)1024.0f, (_Float16)1024.0f} : h2{(_Float16)1088.0f, (_Float16)1088.0f};
+                    const s16x2 cadd = g ? s16x2{0x6400, 0x6400} : s16x2{0x6440, 0x6440};
+                    v8h v;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t u = as_u32(as_s16x2(xw[j]) >> sh2) & msk;
+                        const h2 f = __builtin_bit_cast(h2, as_u32(as_s16x2(u) + cadd)) - cf;
+                        v[2 * j] = f.x;
+                        v[2 * j + 1] = f.y;
+                    }
+                    v16f Mm = {};
+                    Mm = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bm, Mm, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int S = (acc[0][i][r] << 3) + acc[1][i][r];
+                        tot[i][r] = __builtin_fmaf((float)S, dd[r], tot[i][r]);
+                        off[i][r] = __builtin_fmaf(Mm[r], dd[16 + r], off[i][r]);
+                    }
+                } else if constexpr (DT == DT_Q6_K) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float4 dx = *(const float4*)(dl + 32 * i + 8 * j + 4 * g);
+                        const float dv[4] = {dx.x, dx.y, dx.z, dx.w};
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int S = (acc[0][i][4 * j + r] << 8) + acc[1][i][4 * j + r];
+                            tot[i][4 * j + r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][4 * j + r]);
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            const float* dl = (const float*)(buf + C::ABYTES);
+            if (b + 1 < ng) cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
+            const int nk = min(8, A.nb - 8 * b);
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++) {
+                if (ks < nk) {
+                    float d;
+                    const v4i w = grp.block(ks, g, d);
+                    const v16i z = {};
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        const v4i av = *(const v4i*)(al + i * 8192 + 16 * ((2 * ks) ^ asw));
+                        acc[0][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, w, z, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const float dx = dl[8 * (32 * i + 8 * (r >> 2) + 4 * g + (r & 3)) + ks];
+                            tot[i][r] = __builtin_fmaf((float)acc[0][i][r], d * dx, tot[i][r]);
+                        }
+                }
+            }
+            if (b + 1 < ng) {
+                wait_lgkm0();  // the wave's weight slot is read
+                cp.weights(b + 1, lds0);
+            }
+        }
+    }
+
+    // Result i of a lane: weight row wn0 + a, pair 8 (i / 4) + 4 g + i % 4.
+    const int n = wn0 + a;
+    const int refused = flags[0];
+    auto result = [&](int i, int r) { return DT == DT_Q4_K ? tot[i][r] - off[DT == DT_Q4_K ? i : 0][r] : tot[i][r]; };
+    if constexpr (SW) {
+        // gate and up meet in LDS: ex[matrix][pair][row of the tile]
+        float* ex = (float*)smem;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                ex[((wave >> 1) * BM + 32 * i + 8 * (r >> 2) + 4 * g + (r & 3)) * 64 + 32 * (wave & 1) + a] = result(i, r);
+        __syncthreads();
+        if (refused) {
+            for (int p = t >> 3; p < 2 * BM * 64; p += C::T / 8) {
+                const int c = p & 63, m = (p >> 6) % BM, k = p / (64 * BM);
+                const Mat& Mk = A.mat[k];
+                if (n0 + c >= A.N || m >= tile.m) continue;
+                const int64_t w = row0 + n0 + c;
+                if (Mk.wref[w] == 0 && A.act.ok[rows[m]] != 0) continue;
+                const float v = f32dot_g8<DT>(Mk.W + w * A.rb, A.x + (int64_t)rows[m] * A.K, A.K, true);
+                if ((t & 7) == 0) ex[p] = v;
+            }
+            __syncthreads();
+        }
+        for (int p = t; p < 64 * tile.m; p += C::T) {
+            const int c = p & 63, m = p >> 6;
+            if (n0 + c < A.N) A.y[(int64_t)outs[m] * A.N + n0 + c] = silu_mul_vec(ex[p], ex[BM * 64 + p]);
+        }
+    } else {
+        if (n < A.N && !(refused && M.wref[row0 + n] != 0)) {
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int m = 32 * i + 8 * (r >> 2) + 4 * g + (r & 3);
+                    if (m >= tile.m || (refused && A.act.ok[rows[m]] == 0)) continue;
+                    A.y[(int64_t)outs[m] * A.N + n] = result(i, r);
+                }
+        }
+        if (!refused) return;
+        for (int p = t >> 3; p < BN * tile.m; p += C::T / 8) {
+            const int c = p % BN, m = p / BN;
+            const int64_t w = row0 + n0 + c;
+            if (n0 + c >= A.N || (M.wref[w] == 0 && A.act.ok[rows[m]] != 0)) continue;
+            const float v = f32dot_g8<DT>(M.W + w * A.rb, A.x + (int64_t)rows[m] * A.K, A.K, true);
+            if ((t & 7) == 0) A.y[(int64_t)outs[m] * A.N + n0 + c] = v;
+        }
+    }
+}
+
+// The most tiles of BM pairs that any choice of that many could need: whole
+// ones, and one partly filled for each expert.
+static int64_t max_tiles(const Args& A, int BM) {
+    const int64_t some = A.pairs < A.experts ? A.pairs : A.experts;
+    return (A.pairs + some * (BM - 1)) / BM;
+}
+
+template <uint32_t DT, int MT, bool SW>
+static hipError_t launch(const Args& A, hipStream_t stream) {
+    using C = Cfg<DT, MT>;
+    const int BN = SW ? 64 : 128;
+    const int64_t wgs = (max_tiles(A, C::BM) * ((A.N + BN - 1) / BN) + 7) / 8 * 8;
+    if (wgs > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((tile_kernel<DT, C, SW>), dim3((unsigned)wgs), dim3(C::T), 0, stream, A);
+    return hipGetLastError();
+}
+
+template <uint32_t DT, bool SW>
+static hipError_t launch_dt(const Args& A, hipStream_t stream) {
+    // (64 pairs a workgroup where the experts have as many on average)
+    return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, 2, SW>(A, stream) : launch<DT, 1, SW>(A, stream);
+}
+
+}  // namespace xp
+
+bool experts_ok(const DevWeight& w) {
+    const bool k256 = w.dt == DT_Q4_K || w.dt == DT_Q6_K;
+    return (k256 || w.dt == DT_Q8_0) && w.k % (k256 ? 256 : 32) == 0 && (uintptr_t)w.data % (w.dt == DT_Q4_K ? 16 : 2) == 0 &&
+           w.n <= (1ll << 31) - 1;
+}
+
+hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int64_t T, int top,
+                          bool per_pair, const int32_t* plan, float* y, hipStream_t stream) {
+    const DevWeight& w = *ws[0];
+    xp::Args A;
+    for (int i = 0; i < 2; i++) {
+        const DevWeight& m = *ws[i < nmat ? i : 0];
+        A.mat[i].W = m.data;
+        A.mat[i].wref = m.wref;
+    }
+    A.y = y;
+    A.plan = plan;
+    A.rb = w.row_bytes;
+    A.K = w.k;
+    A.wbytes = w.n * w.row_bytes;
+    A.N = (int)(w.n / experts);
+    A.nb = (int)(w.k / (w.dt == DT_Q8_0 ? 32 : 256));
+    A.experts = experts;
+    A.pairs = (int)(T * top);
+    A.rowdiv = per_pair ? 1 : top;
+    A.act = a;
+    A.x = x;
+    if (nmat == 2) {
+        if (w.dt == DT_Q4_K) return xp::launch_dt<DT_Q4_K, true>(A, stream);
+        if (w.dt == DT_Q6_K) return xp::launch_dt<DT_Q6_K, true>(A, stream);
+        return xp::launch_dt<DT_Q8_0, true>(A, stream);
+    }
+    if (w.dt == DT_Q4_K) return xp::launch_dt<DT_Q4_K, false>(A, stream);
+    if (w.dt == DT_Q6_K) return xp::launch_dt<DT_Q6_K, false>(A, stream);
+    return xp::launch_dt<DT_Q8_0, false>(A, stream);
+}
+
+}  // namespace mimg

@@ -17,6 +17,7 @@
 
 #include "../../include/mimg.h"
 #include "cache_q8.hpp"
+#include "experts.hpp"
 #include "mimg_device.hpp"
 #include "mimg_kernels.hpp"
 
@@ -1647,6 +1648,151 @@ int mimg_logprobs_dev(const float* logits, int64_t rows, int64_t n, int64_t ld, 
     if (int rc = ensure_device()) return rc;
     HIP_TRY(launch_logprobs(logits, rows, n, ld, targets, top, logprob, entropy, top_ids, top_logprobs, ws,
                             (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+// ---- a mixture of experts -------------------------------------------------------
+
+static bool experts_shape(int64_t T, int top, int experts) {
+    return T >= 0 && T <= (1 << 20) && experts >= 1 && experts <= EXPERTS_MAX && top >= 1 && top <= EXPERTS_MAX_TOP &&
+           top <= experts && T * top <= (1 << 24);
+}
+
+static int check_experts(const char* what, int64_t T, int top, int experts) {
+    if (!experts_shape(T, top, experts))
+        return fail(MIMG_ERR_ARG, "%s: T %lld, top %d of %d experts (T <= 2^20, T * top <= 2^24, experts <= %d, top <= %d and experts)",
+                    what, (long long)T, top, experts, EXPERTS_MAX, EXPERTS_MAX_TOP);
+    return MIMG_OK;
+}
+
+static bool overlaps(const void* a, uint64_t na, const void* b, uint64_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
+uint64_t mimg_experts_plan_bytes(int64_t T, int top, int experts) {
+    return experts_shape(T, top, experts) ? (uint64_t)plan_layout(T * top, experts).total * 4 : 0;
+}
+
+static int check_plan(const char* what, const void* plan, uint64_t plan_bytes, int64_t T, int top, int experts) {
+    if (!plan || !aligned(plan, 4)) return fail(MIMG_ERR_ARG, "%s: the plan must be 4-byte aligned", what);
+    const uint64_t need = mimg_experts_plan_bytes(T, top, experts);
+    if (plan_bytes < need)
+        return fail(MIMG_ERR_WORKSPACE, "%s: plan %llu < %llu bytes", what, (unsigned long long)plan_bytes, (unsigned long long)need);
+    return MIMG_OK;
+}
+
+int mimg_experts_plan_dev(const int32_t* ids, int64_t T, int top, int experts, void* plan, uint64_t plan_bytes, void* stream) {
+    int rc;
+    if ((rc = check_experts("experts_plan", T, top, experts))) return rc;
+    if ((rc = check_plan("experts_plan", plan, plan_bytes, T, top, experts))) return rc;
+    if (T > 0 && !ids) return fail(MIMG_ERR_ARG, "null pointer");
+    if (overlaps(ids, (uint64_t)T * top * 4, plan, mimg_experts_plan_bytes(T, top, experts)))
+        return fail(MIMG_ERR_ARG, "experts_plan: the plan overlaps ids");
+    if ((rc = ensure_device())) return rc;
+    HIP_TRY(launch_experts_plan(ids, T, top, experts, (int32_t*)plan, (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+uint64_t mimg_experts_route_workspace_bytes(int64_t T, int experts) {
+    return T > 0 && experts_shape(T, 1, experts) ? (uint64_t)T * experts * 8 : 0;
+}
+
+int mimg_experts_route_dev(const float* x, const float* router, int64_t T, int64_t k, int experts, int top, int normalize,
+                           int32_t* ids, float* weights, void* plan, uint64_t plan_bytes, void* ws, uint64_t ws_bytes,
+                           void* stream) {
+    int rc;
+    if ((rc = check_experts("experts_route", T, top, experts))) return rc;
+    if (k <= 0 || k % 4 || k > (1ll << 24)) return fail(MIMG_ERR_ARG, "experts_route: K = %lld (a multiple of 4, at most 2^24)", (long long)k);
+    if (plan && (rc = check_plan("experts_route", plan, plan_bytes, T, top, experts))) return rc;
+    if (T > 0) {
+        if (!x || !router || !ids || !weights || !ws) return fail(MIMG_ERR_ARG, "null pointer");
+        if (!aligned(x, 16) || !aligned(router, 16) || !aligned(ws, 256))
+            return fail(MIMG_ERR_ARG, "experts_route: x and router must be 16-byte and ws 256-byte aligned");
+        const uint64_t need = mimg_experts_route_workspace_bytes(T, experts);
+        if (ws_bytes < need)
+            return fail(MIMG_ERR_WORKSPACE, "experts_route workspace %llu < %llu bytes", (unsigned long long)ws_bytes,
+                        (unsigned long long)need);
+    }
+    if ((rc = ensure_device())) return rc;
+    if (T == 0) {
+        if (plan) HIP_TRY(launch_experts_plan(ids, 0, top, experts, (int32_t*)plan, (hipStream_t)stream));
+        return MIMG_OK;
+    }
+    HIP_TRY(launch_experts_route(x, router, T, k, experts, top, normalize != 0, ids, weights, (int32_t*)plan, (double*)ws,
+                                 (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+// The quantized rows, then (combine) each pair's product.
+uint64_t mimg_experts_swiglu_workspace_bytes(int64_t T, int top, int64_t n, int64_t k) {
+    if (!experts_shape(T, top, EXPERTS_MAX) || n <= 0 || k <= 0 || T == 0) return 0;
+    return act_layout(T, k).total;
+}
+uint64_t mimg_experts_combine_workspace_bytes(int64_t T, int top, int64_t n, int64_t k) {
+    if (!experts_shape(T, top, EXPERTS_MAX) || n <= 0 || k <= 0 || T == 0) return 0;
+    return act_layout(T * top, k).total + (uint64_t)T * top * n * 4;
+}
+
+// What both products check; their rows and K, and the rows of an expert.
+static int check_experts_product(const char* what, const Weight* w, const Weight* other, int64_t T, int top, int experts,
+                                 const void* in, const void* out, const void* plan, uint64_t plan_bytes, const void* ws,
+                                 int64_t* n, int64_t* k) {
+    const DevWeight& d = w->dw;
+    if (d.n % experts) return fail(MIMG_ERR_ARG, "%s: %lld rows are not those of %d experts", what, (long long)d.n, experts);
+    if (other && (other->dw.n != d.n || other->dw.k != d.k)) return fail(MIMG_ERR_ARG, "%s: gate and up must have one shape", what);
+    if ((other && other->dw.dt != d.dt) || !experts_ok(d) || (other && !experts_ok(other->dw)))
+        return fail(MIMG_NOT_HANDLED, "%s: no product for %s%s%s weights of K = %lld", what, dt_name(d.dt), other ? " and " : "",
+                    other ? dt_name(other->dw.dt) : "", (long long)d.k);
+    *n = d.n / experts;
+    *k = d.k;
+    if (T == 0) return MIMG_OK;
+    if (!in || !out || !ws) return fail(MIMG_ERR_ARG, "null pointer");
+    if (!aligned(in, 16) || !aligned(out, 16) || !aligned(ws, 256))
+        return fail(MIMG_ERR_ARG, "%s: inputs and outputs must be 16-byte and ws 256-byte aligned", what);
+    return check_plan(what, plan, plan_bytes, T, top, experts);
+}
+
+int mimg_experts_swiglu_a8_dev(uint64_t gate, uint64_t up, int experts, const float* x, int64_t T, int top, const void* plan,
+                               uint64_t plan_bytes, float* h, void* ws, uint64_t ws_bytes, void* stream) {
+    int rc;
+    Held g, u;
+    if ((rc = check_experts("experts_swiglu", T, top, experts)) || (rc = ensure_device()) || (rc = g.acquire(gate)) || (rc = u.acquire(up))) return rc;
+    int64_t n, k;
+    if ((rc = check_experts_product("experts_swiglu", g.get(), u.get(), T, top, experts, x, h, plan, plan_bytes, ws, &n, &k)) || T == 0)
+        return rc;
+    if (overlaps(x, (uint64_t)T * k * 4, h, (uint64_t)T * top * n * 4)) return fail(MIMG_ERR_ARG, "experts_swiglu: h overlaps x");
+    const ActLayout l = act_layout(T, k);
+    if (ws_bytes < l.total)
+        return fail(MIMG_ERR_WORKSPACE, "experts_swiglu workspace %llu < %llu bytes", (unsigned long long)ws_bytes, (unsigned long long)l.total);
+    const ActPtrs a = act_ptrs(ws, l);
+    const DevWeight* dws[2] = {&g->dw, &u->dw};
+    HIP_TRY(launch_quantize_act(x, T, k, g->dw.dt == DT_Q8_0 ? 32 : 256, a, (hipStream_t)stream));
+    HIP_TRY(launch_experts(dws, 2, experts, a, x, T, top, false, (const int32_t*)plan, h, (hipStream_t)stream));
+    return MIMG_OK;
+}
+
+int mimg_experts_combine_a8_dev(uint64_t down, int experts, const float* h, const float* weights, int64_t T, int top,
+                                const void* plan, uint64_t plan_bytes, float* y, void* ws, uint64_t ws_bytes, void* stream) {
+    int rc;
+    Held w;
+    if ((rc = check_experts("experts_combine", T, top, experts)) || (rc = ensure_device()) || (rc = w.acquire(down))) return rc;
+    int64_t n, k;
+    if ((rc = check_experts_product("experts_combine", w.get(), nullptr, T, top, experts, h, y, plan, plan_bytes, ws, &n, &k)) || T == 0)
+        return rc;
+    if (!weights) return fail(MIMG_ERR_ARG, "null pointer");
+    const int64_t P = T * top;
+    if (overlaps(h, (uint64_t)P * k * 4, y, (uint64_t)T * n * 4) || overlaps(weights, (uint64_t)P * 4, y, (uint64_t)T * n * 4))
+        return fail(MIMG_ERR_ARG, "experts_combine: y overlaps h or weights");
+    const ActLayout l = act_layout(P, k);
+    const uint64_t need = l.total + (uint64_t)P * n * 4;
+    if (ws_bytes < need)
+        return fail(MIMG_ERR_WORKSPACE, "experts_combine workspace %llu < %llu bytes", (unsigned long long)ws_bytes, (unsigned long long)need);
+    const ActPtrs a = act_ptrs(ws, l);
+    float* part = (float*)((uint8_t*)ws + l.total);
+    const DevWeight* dws[1] = {&w->dw};
+    HIP_TRY(launch_quantize_act(h, P, k, w->dw.dt == DT_Q8_0 ? 32 : 256, a, (hipStream_t)stream));
+    HIP_TRY(launch_experts(dws, 1, experts, a, h, T, top, true, (const int32_t*)plan, part, (hipStream_t)stream));
+    HIP_TRY(launch_experts_sum(part, weights, (const int32_t*)plan + plan_layout(P, experts).expert, T, top, n, y, (hipStream_t)stream));
     return MIMG_OK;
 }
 

@@ -91,6 +91,14 @@ SIGNATURES = {
     "mimg_attention_q8_dev": (_I, [_P, _P, _P, _P, _I64, _I, _I, _I, _I64, _I64, _P, _P, _U64, _P]),
     "mimg_logprobs_workspace_bytes": (_U64, [_I64, _I64, _I]),
     "mimg_logprobs_dev": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _P, _P, _P, _P, _U64, _P]),
+    "mimg_experts_plan_bytes": (_U64, [_I64, _I, _I]),
+    "mimg_experts_plan_dev": (_I, [_P, _I64, _I, _I, _P, _U64, _P]),
+    "mimg_experts_route_workspace_bytes": (_U64, [_I64, _I]),
+    "mimg_experts_route_dev": (_I, [_P, _P, _I64, _I64, _I, _I, _I, _P, _P, _P, _U64, _P, _U64, _P]),
+    "mimg_experts_swiglu_workspace_bytes": (_U64, [_I64, _I, _I64, _I64]),
+    "mimg_experts_swiglu_a8_dev": (_I, [_U64, _U64, _I, _P, _I64, _I, _P, _U64, _P, _P, _U64, _P]),
+    "mimg_experts_combine_workspace_bytes": (_U64, [_I64, _I, _I64, _I64]),
+    "mimg_experts_combine_a8_dev": (_I, [_U64, _I, _P, _P, _I64, _I, _P, _U64, _P, _P, _U64, _P]),
     "mimg_greedy_advance_dev": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _P]),
     "mimg_swiglu_dev": (_I, [_P, _P, _P, _I64, _I, _P]),
     "mimg_argmax_dev": (_I, [_P, _I64, _I64, _P, _P]),
@@ -637,6 +645,60 @@ def logprobs_dev(x_ptr, rows, n, ld, targets_ptr, top, logprob_ptr, entropy_ptr,
     None are not written."""
     rc = load().mimg_logprobs_dev(x_ptr, rows, n, ld, targets_ptr, top, logprob_ptr, entropy_ptr, top_ids_ptr,
                                   top_logprobs_ptr, ws_ptr, ws_bytes, stream)
+    if rc:
+        _check(rc)
+
+
+# ---- a mixture of experts (pointers and streams as Python ints) ------------
+
+def experts_plan_bytes(T, top, experts):
+    return int(load().mimg_experts_plan_bytes(T, top, experts))
+
+
+def experts_plan_dev(ids_ptr, T, top, experts, plan_ptr, plan_bytes, stream):
+    """The pairs of the choices ids [T, top] in order by expert
+    (mimg_experts_plan_dev)."""
+    rc = load().mimg_experts_plan_dev(ids_ptr, T, top, experts, plan_ptr, plan_bytes, stream)
+    if rc:
+        _check(rc)
+
+
+def experts_route_workspace_bytes(T, experts):
+    return int(load().mimg_experts_route_workspace_bytes(T, experts))
+
+
+def experts_route_dev(x_ptr, router_ptr, T, k, experts, top, normalize, ids_ptr, weights_ptr, plan_ptr, plan_bytes, ws_ptr,
+                      ws_bytes, stream):
+    """The `top` experts of each token with their weights, and the plan of
+    them (mimg_experts_route_dev; plan_ptr None: no plan)."""
+    rc = load().mimg_experts_route_dev(x_ptr, router_ptr, T, k, experts, top, int(normalize), ids_ptr, weights_ptr, plan_ptr,
+                                       plan_bytes, ws_ptr, ws_bytes, stream)
+    if rc:
+        _check(rc)
+
+
+def experts_swiglu_workspace_bytes(T, top, n, k):
+    return int(load().mimg_experts_swiglu_workspace_bytes(T, top, n, k))
+
+
+def experts_swiglu_a8_dev(gate, up, experts, x_ptr, T, top, plan_ptr, plan_bytes, h_ptr, ws_ptr, ws_bytes, stream):
+    """h [T * top, n] = swiglu of the gate and up products of each pair's
+    expert (mimg_experts_swiglu_a8_dev)."""
+    rc = load().mimg_experts_swiglu_a8_dev(gate.handle, up.handle, experts, x_ptr, T, top, plan_ptr, plan_bytes, h_ptr, ws_ptr,
+                                           ws_bytes, stream)
+    if rc:
+        _check(rc)
+
+
+def experts_combine_workspace_bytes(T, top, n, k):
+    return int(load().mimg_experts_combine_workspace_bytes(T, top, n, k))
+
+
+def experts_combine_a8_dev(down, experts, h_ptr, weights_ptr, T, top, plan_ptr, plan_bytes, y_ptr, ws_ptr, ws_bytes, stream):
+    """y [T, n] = the weighted sum of the down products of each token's
+    experts (mimg_experts_combine_a8_dev)."""
+    rc = load().mimg_experts_combine_a8_dev(down.handle, experts, h_ptr, weights_ptr, T, top, plan_ptr, plan_bytes, y_ptr, ws_ptr,
+                                            ws_bytes, stream)
     if rc:
         _check(rc)
 
