@@ -30,7 +30,7 @@ class Config:
     """The model shape (reference importer/llama.go LlamaConfig)."""
 
     def __init__(self, arch="llama", layers=1, embed=256, ffn=256, heads=4, kv_heads=None, rope_dims=None,
-                 rope_theta=10000.0, norm_eps=1e-5, context=64, **_):
+                 rope_theta=10000.0, norm_eps=1e-5, context=64, experts=0, experts_used=0, **_):
         self.arch, self.layers, self.embed, self.ffn = arch, int(layers), int(embed), int(ffn)
         self.heads = int(heads)
         self.kv_heads = int(kv_heads or heads)
@@ -42,6 +42,11 @@ class Config:
         self.interleaved = arch != "qwen2"
         if self.embed % self.heads or self.heads % self.kv_heads or self.rope_dims % 2:
             raise ValueError(f"inconsistent shape: embed {embed}, heads {heads}, kv heads {kv_heads}, rope {rope_dims}")
+        # feed-forward layers of `experts` experts of which a token takes
+        # experts_used (0: dense ones)
+        self.experts, self.experts_used = int(experts), int(experts_used)
+        if self.experts and not 0 < self.experts_used <= min(self.experts, 32) or not 0 <= self.experts <= 512:
+            raise ValueError(f"{experts_used} of {experts} experts")
 
 
 MAX_CONTEXT = 1 << 20
@@ -83,6 +88,10 @@ def config_from_metadata(md, context=0):
     eps = md.get(f"{arch}.attention.layer_norm_rms_epsilon")
     if not isinstance(eps, float) or eps <= 0:
         raise ValueError(f"metadata {arch}.attention.layer_norm_rms_epsilon is missing or invalid")
+    if md.get(f"{arch}.expert_count", 0):  # (0: a dense model that says so)
+        if arch != "llama":
+            raise ValueError(f"experts in an architecture {arch!r}: only \"llama\" graphs have them")
+        c["experts"], c["experts_used"] = req("expert_count"), req("expert_used_count")
     # the importer stores f32 metadata widened to f64; the graph's rms_norm
     # attribute keeps it, and rms_norm.v1 rounds it to f32
     c["norm_eps"] = eps
@@ -103,7 +112,7 @@ class Decoder:
 
     tensors: {GGUF tensor name: (dtype, shape, data)}, where data is the
     block bytes (np.uint8) of a quantized matrix, an np.float32 array for a
-    norm scale or bias, or an already registered mimg.Weight. procs is the
+    norm scale, a bias or a router, or an already registered mimg.Weight. procs is the
     GOMAXPROCS of the reference run to reproduce (its swiglu results depend
     on it). kquant_block is the activation block of the Q4_K/Q6_K products
     with 8-bit activations (256: dequant_matmul_a8.v2, 32: .v1).
@@ -114,6 +123,14 @@ class Decoder:
     in 8 bits (mimg_kv_store_q8_dev, mimg_attention_q8_dev), half the memory
     and traffic of cache_f16 at head sizes that are multiples of 64, contexts
     past 8192; not the reference's bits.
+
+    With config.experts the feed-forward layers are mixtures of experts, as
+    GGUF files of this architecture hold them: ffn_gate_inp.weight f32
+    [experts, embed], ffn_gate_exps, ffn_up_exps (one dtype) and ffn_down_exps
+    [experts, n, k], their dtypes Q4_K, Q6_K or Q8_0 (mimg_experts_route_dev,
+    mimg_experts_swiglu_a8_dev, mimg_experts_combine_a8_dev; weights
+    normalized over the chosen experts). 8-bit activations only, of blocks of
+    256 for the K-quants.
     """
 
     def __init__(self, config, tensors, a8=True, cache_f16=False, max_rows=64, slots=1, procs=16, kquant_block=256,
@@ -137,15 +154,20 @@ class Decoder:
         mimg.init()
         self.stream = hiprt.Stream()
         self.w, self.vec = {}, {}
+        if c.experts and not (self.a8 and kquant_block == 256):
+            raise ValueError("experts take 8-bit activations, of blocks of 256 for Q4_K and Q6_K")
         for name, (dt, shape, data) in tensors.items():
             if isinstance(data, mimg.Weight):
                 self.w[name] = data
             elif dt == F32:
-                if len(shape) != 1:
+                if len(shape) != 1 and not (c.experts and name.endswith(".ffn_gate_inp.weight")):
                     raise mimg.NotHandled(1, f"{name}: f32 matrices are not handled")
                 self.vec[name] = hiprt.DeviceBuffer.from_array(np.ascontiguousarray(data, np.float32))
             else:
-                self.w[name] = mimg.Weight(data, dt, int(shape[0]), int(shape[1]))
+                # (an expert tensor's rows: all experts' one behind the other)
+                self.w[name] = mimg.Weight(data, dt, int(np.prod(shape[:-1])), int(shape[-1]))
+        if c.experts:
+            self._check_experts(tensors)
         if c.context > (MAX_CONTEXT if self.q8 else 8192):
             raise ValueError(f"context {c.context}: attention handles at most {MAX_CONTEXT if self.q8 else 8192} "
                              "positions per sequence")
@@ -183,7 +205,14 @@ class Decoder:
         self.qkv_rows_fused = bool(fuse_rope) and not self.q8
         self.q, self.o = B(R * H * D * 4), B(R * H * D * 4)
         self.k, self.v = B(R * Hkv * D * 4), B(R * Hkv * D * 4)
-        self.g, self.u, self.sw = B(R * F * 4), B(R * F * 4), B(R * F * 4)
+        if c.experts:
+            K, n = c.experts_used, c.experts
+            self.eids, self.ew, self.eh = B(R * K * 4), B(R * K * 4), B(R * K * F * 4)
+            self.plan = B(mimg.experts_plan_bytes(R, K, n))
+            self.exp_ws = B(max(mimg.experts_route_workspace_bytes(R, n), mimg.experts_swiglu_workspace_bytes(R, K, F, E),
+                                mimg.experts_combine_workspace_bytes(R, K, E, F)))
+        else:
+            self.g, self.u, self.sw = B(R * F * 4), B(R * F * 4), B(R * F * 4)
         self.logits = B(R * self.vocab * 4)
         self.ids, self.pos = B(R * 4), B(R * 8)
         self.cidx, self.kstart = B(R * 8), B(R * 8)
@@ -199,6 +228,21 @@ class Decoder:
             self.att_ws_bytes = mimg.attention_workspace_bytes(R, H, c.context)
         self.att_ws = B(self.att_ws_bytes)
         self.graphs = {}
+
+    def _check_experts(self, tensors):
+        """The expert tensors' shapes, before a product relies on them."""
+        c = self.c
+        n, E, F = c.experts, c.embed, c.ffn
+        for l in range(c.layers):
+            p = f"blk.{l}."
+            if p + "ffn_gate_inp.weight" not in self.vec or list(tensors[p + "ffn_gate_inp.weight"][1]) != [n, E]:
+                raise ValueError(f"{p}ffn_gate_inp.weight: f32 [{n}, {E}] is wanted")
+            for name, rows, k in (("ffn_gate_exps", n * F, E), ("ffn_up_exps", n * F, E), ("ffn_down_exps", n * E, F)):
+                w = self.w.get(p + name + ".weight")
+                if w is None or (w.n, w.k) != (rows, k):
+                    raise ValueError(f"{p}{name}.weight: quantized [{n}, {rows // n}, {k}] is wanted")
+            if self.w[p + "ffn_gate_exps.weight"].dt != self.w[p + "ffn_up_exps.weight"].dt:
+                raise ValueError(f"{p}: gate and up experts of two dtypes")
 
     # ---- the graph's ops ---------------------------------------------------
 
@@ -321,6 +365,21 @@ class Decoder:
                                            self.ws.ptr, self.ws_bytes, s)
         return True
 
+    def _experts(self, l, T):
+        """A feed-forward layer of experts: x += the attention output, h =
+        rms_norm(x) * scale; the router and its plan; gate, up and swiglu of
+        the chosen experts; their weighted down products."""
+        c, s = self.c, self.stream.handle
+        p = f"blk.{l}."
+        n, top, pb, wsb = c.experts, c.experts_used, self.plan.nbytes, self.exp_ws.nbytes
+        mimg.rms_norm_dev(self.x.ptr, self.ao.ptr, self.vec[p + "ffn_norm.weight"].ptr, c.norm_eps, T, c.embed, self.h.ptr, s)
+        mimg.experts_route_dev(self.h.ptr, self.vec[p + "ffn_gate_inp.weight"].ptr, T, c.embed, n, top, True, self.eids.ptr,
+                               self.ew.ptr, self.plan.ptr, pb, self.exp_ws.ptr, wsb, s)
+        mimg.experts_swiglu_a8_dev(self.w[p + "ffn_gate_exps.weight"], self.w[p + "ffn_up_exps.weight"], n, self.h.ptr, T, top,
+                                   self.plan.ptr, pb, self.eh.ptr, self.exp_ws.ptr, wsb, s)
+        mimg.experts_combine_a8_dev(self.w[p + "ffn_down_exps.weight"], n, self.eh.ptr, self.ew.ptr, T, top, self.plan.ptr, pb,
+                                    self.ao.ptr, self.exp_ws.ptr, wsb, s)
+
     def _norm_qkv_rope(self, l, resid, qkv, qkv_b, pos, cidx):
         """At one row with 8-bit activations: the attention norm, the q/k/v
         products, rope and the cache scatter in one launch (x + resid lands in
@@ -390,6 +449,10 @@ class Decoder:
                 self._rope_store(l, T, pos, cidx)
             self._attend(l, T, cidx, kstart)
             self._linears([p + "attn_output.weight"], self.o.ptr, T, [self.ao.ptr])
+            if c.experts:
+                self._experts(l, T)
+                resid = self.ao.ptr
+                continue
             down = self.w[p + "ffn_down.weight"]
             if T <= 8 and self._ffn_rows(l, T):
                 pass

@@ -3,7 +3,9 @@ benchmarks: a Llama-3.2-1B shape (16 layers, d 2048, FFN 8192, 32/8 heads,
 vocab 128256, theta 500000) and a Llama-3-8B shape (32 layers, d 4096,
 FFN 14336, 32/8 heads, vocab 128256). Weights are N(0, 0.02^2) drawn on the
 GPU and encoded as Q4_K_M: Q4_K for the embedding, q, k, o, gate and up,
-Q6_K for v, down and the output head. Norm scales are ones.
+Q6_K for v, down and the output head. Norm scales are ones. With `experts`
+and `experts_used` in the shape its feed-forward layers are mixtures of that
+many experts of the FFN size.
 
 The matrices are drawn, encoded and registered one at a time, so building
 needs device memory for the weights plus one f32 copy of the largest
@@ -28,20 +30,27 @@ def matrices(cfg):
     for l in range(cfg["layers"]):
         p = f"blk.{l}."
         out += [(p + "attn_q.weight", mimg.Q4_K, H * D, E), (p + "attn_k.weight", mimg.Q4_K, Hkv * D, E),
-                (p + "attn_v.weight", mimg.Q6_K, Hkv * D, E), (p + "attn_output.weight", mimg.Q4_K, E, H * D),
-                (p + "ffn_gate.weight", mimg.Q4_K, F, E), (p + "ffn_up.weight", mimg.Q4_K, F, E),
-                (p + "ffn_down.weight", mimg.Q6_K, E, F)]
+                (p + "attn_v.weight", mimg.Q6_K, Hkv * D, E), (p + "attn_output.weight", mimg.Q4_K, E, H * D)]
+        # (with experts: all of a layer one behind the other)
+        n, s = (cfg["experts"], "_exps") if cfg.get("experts") else (1, "")
+        out += [(f"{p}ffn_gate{s}.weight", mimg.Q4_K, n * F, E), (f"{p}ffn_up{s}.weight", mimg.Q4_K, n * F, E),
+                (f"{p}ffn_down{s}.weight", mimg.Q6_K, n * E, F)]
     out.append(("output.weight", mimg.Q6_K, V, E))
     return out
 
 
 def weight_bytes(cfg, per_token=False):
     """Bytes of the matrices (per_token: those a decode step reads, i.e. all
-    but the embedding table, of which it reads one row)."""
+    but the embedding table, of which it reads one row, and the experts that
+    it does not choose)."""
     total = 0
     for name, dt, n, k in matrices(cfg):
         rb = mimg.row_bytes(dt, k)
-        total += rb if (per_token and name == "token_embd.weight") else n * rb
+        if per_token and name == "token_embd.weight":
+            n = 1
+        elif per_token and "_exps." in name:
+            n = n // cfg["experts"] * cfg["experts_used"]
+        total += n * rb
     return total
 
 
@@ -67,6 +76,9 @@ def build(cfg, seed=0, std=0.02, log=None):
     for l in range(cfg["layers"]):
         tensors[f"blk.{l}.attn_norm.weight"] = (mimg.F32, [cfg["embed"]], ones)
         tensors[f"blk.{l}.ffn_norm.weight"] = (mimg.F32, [cfg["embed"]], ones)
+        if cfg.get("experts"):
+            r = np.random.default_rng(seed * 1000003 + l).standard_normal((cfg["experts"], cfg["embed"]), np.float32)
+            tensors[f"blk.{l}.ffn_gate_inp.weight"] = (mimg.F32, [cfg["experts"], cfg["embed"]], r * np.float32(std))
     tensors["output_norm.weight"] = (mimg.F32, [cfg["embed"]], ones)
     if log:
         log(f"  built {cfg['layers']}-layer model: {weight_bytes(cfg) / 1e9:.2f} GB of weights")

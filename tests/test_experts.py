@@ -106,3 +106,22 @@ def test_the_bound_does_not_keep_a_lost_part(oracle, lost):
     else:
         b[:, 1, 4:8] &= 0xF8
     assert (np.abs(ref.product(x, b, 66, 40, 1024)[0] - y) > bound).mean() > 0.9
+
+
+def test_config_of_a_file_with_experts():
+    import decoder
+
+    md = {"general.architecture": "llama", "llama.block_count": 2, "llama.embedding_length": 256, "llama.feed_forward_length": 512,
+          "llama.attention.head_count": 4, "llama.context_length": 64, "llama.attention.layer_norm_rms_epsilon": 1e-5}
+    assert "experts" not in decoder.config_from_metadata(md)
+    assert "experts" not in decoder.config_from_metadata(dict(md, **{"llama.expert_count": 0}))
+    c = decoder.config_from_metadata(dict(md, **{"llama.expert_count": 8, "llama.expert_used_count": 2}))
+    assert (c["experts"], c["experts_used"]) == (8, 2) and decoder.Config(**c).experts_used == 2
+    with pytest.raises(ValueError, match="expert_used_count"):
+        decoder.config_from_metadata(dict(md, **{"llama.expert_count": 8}))
+    with pytest.raises(ValueError, match="experts"):
+        decoder.config_from_metadata({k.replace("llama", "qwen2"): "qwen2" if v == "llama" else v
+                                      for k, v in dict(md, **{"llama.expert_count": 8, "llama.expert_used_count": 2}).items()})
+    for n, used in ((4, 5), (4, 0), (64, 33), (513, 2), (-1, 1)):
+        with pytest.raises(ValueError, match="experts"):
+            decoder.Config(experts=n, experts_used=used)
