@@ -45,6 +45,7 @@ namespace xp {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v32f __attribute__((ext_vector_type(32)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
@@ -88,7 +89,11 @@ struct Cfg {
     static_assert(ADMA * T == BM * 16 && BM <= 64 && 2 * 64 * BM * 4 <= SMEM && SMEM <= 80 * 1024, "tile shape");
 };
 
-__device__ __forceinline__ void wait_vmcnt0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+// s_waitcnt with vmcnt <= N (N < 64), the other counters unconstrained.
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+}
 __device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
 // A workgroup's tile: expert e, its pairs' first place in the order, how many
@@ -96,6 +101,18 @@ __device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xC07F
 struct Tile {
     int e, f0, m, nt;
 };
+
+// Inclusive sums over the wave: within rows of 16 lanes (shifts by 1, 2, 4, 8),
+// then each row's last lane into the rows behind it.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
 
 template <int PER>
 __device__ __forceinline__ bool find_tile_of(const Args& A, int ntn, int BM, Tile& r) {
@@ -111,11 +128,7 @@ __device__ __forceinline__ bool find_tile_of(const Args& A, int ntn, int BM, Til
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         int s = (cnt[i] + BM - 1) / BM;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(s, d);
-            s += lane >= d ? o : 0;
-        }
+        s = wave_scan(s);
         upto[i] = total + s;
         total = __builtin_amdgcn_readlane(upto[i], 63);
     }
@@ -148,20 +161,31 @@ __device__ __forceinline__ bool find_tile(const Args& A, int ntn, int BM, Tile& 
 // The copies of a thread: group 0's sources; group b adds a constant step.
 template <uint32_t DT, class C>
 struct Copies {
-    const uint8_t *w[C::WDMA], *a[C::ADMA], *s;
-    const uint8_t* wlast;  // the last 16 bytes that a copy may read (Q8_0)
+    // Weights: offsets from a base that the wave shares, 16-byte aligned.
+    const uint8_t* wbase;
+    uint32_t w[C::WDMA];
+    int64_t wroom;  // bytes from the base to the last 16 that a copy may read
+    const uint8_t *a[C::ADMA], *s;
     const uint8_t* d8[C::K32 ? C::DBYTES / 1024 : 1];
     uint32_t wave;
-    __device__ __forceinline__ void init(const Args& A, const Mat& M, int64_t row0, int n0, const int* rows) {
+    __device__ __forceinline__ void init_weights(const Args& A, const Mat& M, int64_t row0, int n0) {
         const int t = threadIdx.x, l = t & 63;
         wave = __builtin_amdgcn_readfirstlane(t >> 6);
+        const uint8_t* p = M.W + (row0 + min(n0, A.N - 1)) * A.rb;  // (a wave past the last row: that row)
+        wbase = (const uint8_t*)__builtin_align_down(p, 16);
+        const uint32_t mis = (uint32_t)(p - wbase);
+        wroom = M.W + A.wbytes + WEIGHT_PAD - 16 - wbase;
 #pragma unroll
         for (int i = 0; i < C::WDMA; i++) {
             const int c = min(64 * i + l, 32 * C::WCH - 1), r = c / C::WCH, j = c - C::WCH * r;
-            const uint8_t* p = M.W + (row0 + min(n0 + r, A.N - 1)) * A.rb;
-            w[i] = DT == DT_Q4_K ? p + 16 * j : p;
+            const uint32_t o = mis + (uint32_t)max(min(r, A.N - 1 - n0), 0) * (uint32_t)A.rb;
+            // (Q6_K: the block's place, rounded down for each block; its chunk
+            // is added then)
+            w[i] = DT == DT_Q6_K ? o : (o & ~15u) + 16 * j;
         }
-        wlast = (const uint8_t*)__builtin_align_down(M.W + A.wbytes + WEIGHT_PAD - 16, 16);
+    }
+    __device__ __forceinline__ void init_rows(const Args& A, const int* rows) {
+        const int t = threadIdx.x, l = t & 63;
 #pragma unroll
         for (int i = 0; i < C::ADMA; i++) {
             const int c = C::T * i + t, r = c >> 4, k = c & 15;
@@ -179,15 +203,18 @@ struct Copies {
     }
     __device__ __forceinline__ void weights(int b, uint32_t lds) const {
         const int l = threadIdx.x & 63;
+        const uint8_t* base = wbase + (DT == DT_Q6_K ? 0 : (int64_t)b * C::GROUP);
+        const int64_t room = wroom - (base - wbase);
+        // A slot has more chunks than its group (Q6_K, Q8_0): those of the
+        // last rows may not lie in the buffer, nor those of a last group of
+        // fewer blocks.
+        const uint32_t last = (uint32_t)min(room, (int64_t)0xFFFFFFF0) & ~15u;
 #pragma unroll
         for (int i = 0; i < C::WDMA; i++) {
-            const uint8_t* p = w[i] + (int64_t)b * C::GROUP;
-            if constexpr (DT != DT_Q4_K) {
-                const int c = min(64 * i + l, 32 * C::WCH - 1), j = c % C::WCH;
-                p = (const uint8_t*)__builtin_align_down(p, 16) + 16 * j;
-                p = p < wlast ? p : wlast;
-            }
-            lds_copy16(p, lds + C::WWAVE * wave + 1024 * i);
+            uint32_t o = w[i];
+            if constexpr (DT == DT_Q6_K) o = ((o + (uint32_t)b * C::GROUP) & ~15u) + 16 * (min(64 * i + l, 32 * C::WCH - 1) % C::WCH);
+            if constexpr (DT != DT_Q4_K) o = min(o, last);
+            lds_copy16_at(base, o, lds + C::WWAVE * wave + 1024 * i);
         }
     }
     __device__ __forceinline__ void activations(int b, uint32_t lds) const {
@@ -299,11 +326,25 @@ struct Group<DT_Q6_K> {
 
 template <>
 struct Group<DT_Q8_0> {
-    const uint8_t* p;
-    __device__ __forceinline__ void read(const uint8_t* wr, int) { p = wr; }
-    __device__ __forceinline__ v4i block(int ks, int g, float& d) const {
-        d = f16_to_f32(lds_read2_a2(p + Q80_BYTES * ks));
-        return __builtin_bit_cast(v4i, lds_read16_a2(p + Q80_BYTES * ks + 2 + 16 * g));
+    // A block's 16 bytes of the lane as the five aligned dwords that hold them.
+    u32x4 w[8];
+    uint32_t w4[8], sh;  // the first block's misalignment; the next one's is the other
+    float d[8];
+    __device__ __forceinline__ void read(const uint8_t* wr, int g) {
+        sh = ((uint32_t)(uintptr_t)wr + 2) & 2;
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++) {
+            const uint8_t* p = wr + Q80_BYTES * ks;
+            const uint32_t* q = (const uint32_t*)__builtin_align_down(p + 2 + 16 * g, 4);
+            w[ks] = u32x4{q[0], q[1], q[2], q[3]};
+            w4[ks] = q[4];
+            d[ks] = f16_to_f32(lds_read2_a2(p));
+        }
+    }
+    __device__ __forceinline__ v4i block(int ks) const {
+        const uint32_t s = ks & 1 ? 2 - sh : sh;
+        return v4i{(int)__builtin_amdgcn_alignbyte(w[ks].y, w[ks].x, s), (int)__builtin_amdgcn_alignbyte(w[ks].z, w[ks].y, s),
+                   (int)__builtin_amdgcn_alignbyte(w[ks].w, w[ks].z, s), (int)__builtin_amdgcn_alignbyte(w4[ks], w[ks].w, s)};
     }
 };
 
@@ -311,28 +352,35 @@ template <uint32_t DT, class C, bool SW>
 __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
     constexpr int MT = C::MT, BM = C::BM, BN = SW ? 64 : 128;
     __shared__ __align__(16) uint8_t smem[C::SMEM];  // weights, then two activation stages
-    __shared__ int rows[BM], outs[BM], flags[1];
+    __shared__ int rows[BM], outs[64], flags[1];
     const int t = threadIdx.x, l = t & 63, wave = t >> 6;
     const int a = l & 31, g = l >> 5;
     Tile tile;
     if (!find_tile(A, (A.N + BN - 1) / BN, BM, tile)) return;
+    const int n0 = tile.nt * BN, wn0 = n0 + 32 * (SW ? wave & 1 : wave);  // this wave's first weight row
+    const int64_t row0 = (int64_t)tile.e * A.N;
+    // (by value through a scalar: the copies take their base from it)
+    const bool second = SW && __builtin_amdgcn_readfirstlane(wave) >= 2;
+    const Mat M = {second ? A.mat[1].W : A.mat[0].W, second ? A.mat[1].wref : A.mat[0].wref};
+
+    Copies<DT, C> cp;
+    cp.init_weights(A, M, row0, __builtin_amdgcn_readfirstlane(wn0));
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
+    // The tile's pairs, behind them the weights (which need the tile alone):
+    // the first ones have landed when at most the weights' copies are left.
+    // (Past the tile's pairs the last one again, whose results are not written.)
+    if (cp.wave == 0) lds_copy4(A.plan + plan_layout(A.pairs, A.experts).order + tile.f0 + min(l, tile.m - 1), outs);
+    cp.weights(0, lds0);
+    if (cp.wave == 0) wait_vmcnt<C::WDMA>();
+    if (t == 0) flags[0] = 0;
+    lds_barrier();
     if (t < BM) {
-        // (past the tile's pairs: the last one again, whose results are not written)
-        const PlanLayout pl = plan_layout(A.pairs, A.experts);
-        const int pair = min(max(A.plan[pl.order + tile.f0 + min(t, tile.m - 1)], 0), A.pairs - 1);
+        const int pair = min(max(outs[t], 0), A.pairs - 1);
         outs[t] = pair;
         rows[t] = pair / A.rowdiv;
     }
-    if (t == 0) flags[0] = 0;
-    __syncthreads();
-    const int n0 = tile.nt * BN, wn0 = n0 + 32 * (SW ? wave & 1 : wave);  // this wave's first weight row
-    const int64_t row0 = (int64_t)tile.e * A.N;
-    const Mat M = SW && wave >= 2 ? A.mat[1] : A.mat[0];
-
-    Copies<DT, C> cp;
-    cp.init(A, M, row0, wn0, rows);
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
-    cp.weights(0, lds0);
+    lds_barrier();
+    cp.init_rows(A, rows);
     cp.activations(0, lds0 + C::WBYTES);
     {
         int f = 0;
@@ -353,7 +401,7 @@ __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
     const uint32_t wmis = DT == DT_Q4_K ? 0 : (uint32_t)(uintptr_t)(M.W + (row0 + min(wn0 + a, A.N - 1)) * A.rb);
     const int ng = C::K32 ? (A.nb + 7) / 8 : A.nb;
     for (int b = 0; b < ng; b++) {
-        wait_vmcnt0();
+        wait_vmcnt<0>();
         lds_barrier();  // group b's copies have landed, group b - 1's activations are read
         const uint8_t* buf = smem + C::WBYTES + (b & 1) * C::BUF;
         const uint8_t* al = buf + a * 256;
@@ -361,13 +409,13 @@ __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
         if constexpr (DT != DT_Q4_K) ws += (wmis + (uint32_t)b * C::GROUP) & 15u;
         Group<DT> grp;
         grp.read(ws, g);
+        if (b + 1 < ng) {
+            cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
+            wait_lgkm0();  // the wave's weight slot is read
+            cp.weights(b + 1, lds0);
+        }
         v16i acc[2][MT];
         if constexpr (!C::K32) {
-            if (b + 1 < ng) {
-                cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
-                wait_lgkm0();  // the wave's weight slot is read
-                cp.weights(b + 1, lds0);
-            }
             v4i av[MT];
 #pragma unroll
             for (int i = 0; i < MT; i++) av[i] = *(const v4i*)(al + i * 8192 + 16 * asw);
@@ -399,7 +447,6 @@ __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
                 if constexpr (DT == DT_Q4_K) {
                     // d*dx and dmin*dx of the tile as outer products (lanes
                     // g = 0 hold d, g = 1 dmin)
-                    typedef float v32f __attribute__((ext_vector_type(32)));
                     const v32f z = {};
                     const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * i + a], g ? grp.dmin : grp.d, z, 0, 0, 0);
                     const u32x4 xw = *(const u32x4*)(buf + C::ABYTES + 16 * (32 * i + a));
@@ -439,32 +486,30 @@ __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
+            // d*dx of two blocks (lanes g = 0 the even one's, g = 1 the odd
+            // one's) as one outer product.
             const float* dl = (const float*)(buf + C::ABYTES);
-            if (b + 1 < ng) cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
             const int nk = min(8, A.nb - 8 * b);
 #pragma unroll
-            for (int ks = 0; ks < 8; ks++) {
+            for (int ks = 0; ks < 8; ks += 2) {
                 if (ks < nk) {
-                    float d;
-                    const v4i w = grp.block(ks, g, d);
+                    const v4i w0 = grp.block(ks), w1 = grp.block(ks + 1);
+                    const float dw = g ? grp.d[ks + 1] : grp.d[ks];
                     const v16i z = {};
+                    const v32f zf = {};
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
-                        const v4i av = *(const v4i*)(al + i * 8192 + 16 * ((2 * ks) ^ asw));
-                        acc[0][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, w, z, 0, 0, 0);
-                    }
+                        acc[0][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const v4i*)(al + i * 8192 + 16 * ((2 * ks) ^ asw)), w0, z, 0, 0, 0);
+                        acc[1][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const v4i*)(al + i * 8192 + 16 * ((2 * ks + 2) ^ asw)), w1, z, 0, 0, 0);
+                        const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[8 * (32 * i + a) + ks + g], dw, zf, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < MT; i++)
+                        for (int r = 0; r < 16; r++) tot[i][r] = __builtin_fmaf((float)acc[0][i][r], dd[r], tot[i][r]);
+                        if (ks + 1 < nk) {
 #pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const float dx = dl[8 * (32 * i + 8 * (r >> 2) + 4 * g + (r & 3)) + ks];
-                            tot[i][r] = __builtin_fmaf((float)acc[0][i][r], d * dx, tot[i][r]);
+                            for (int r = 0; r < 16; r++) tot[i][r] = __builtin_fmaf((float)acc[1][i][r], dd[16 + r], tot[i][r]);
                         }
+                    }
                 }
-            }
-            if (b + 1 < ng) {
-                wait_lgkm0();  // the wave's weight slot is read
-                cp.weights(b + 1, lds0);
             }
         }
     }
@@ -546,6 +591,15 @@ static hipError_t launch_dt(const Args& A, hipStream_t stream) {
 
 }  // namespace xp
 
+// Few pairs each run their expert's matrix by themselves (gemv_kquant.hip), an
+// expert that two of them share twice. Measured on MI355X, us a call with
+// quantizing and sum, alone / in tiles: 4096 x 14336, 8 experts, gate and up
+// (Q4_K) of 2 / 4 / 8 / 16 pairs 29 / 49 / 88 / 160 against 39 / 66 / 98 /
+// 110, down (Q6_K) of 4 / 8 / 16 pairs 46 / 72 / 125 against 111 / 112 / 114;
+// 2048 x 1024, 64 experts, gate and up of 8 / 16 / 32 pairs 11.2 / 16.1 / 26.5
+// against 15.6 / 18.2 / 23.5, down 12.4 / 14.2 / 18.7 against 15.5 / 16.5 / 19.4.
+static bool few_pairs(int pairs, int experts) { return pairs <= 8 || (pairs <= 16 && experts >= 2 * pairs); }
+
 bool experts_ok(const DevWeight& w) {
     const bool k256 = w.dt == DT_Q4_K || w.dt == DT_Q6_K;
     return (k256 || w.dt == DT_Q8_0) && w.k % (k256 ? 256 : 32) == 0 && (uintptr_t)w.data % (w.dt == DT_Q4_K ? 16 : 2) == 0 &&
@@ -555,6 +609,9 @@ bool experts_ok(const DevWeight& w) {
 hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int64_t T, int top,
                           bool per_pair, const int32_t* plan, float* y, hipStream_t stream) {
     const DevWeight& w = *ws[0];
+    const int pairs = (int)(T * top);
+    if (few_pairs(pairs, experts) && gemv_experts_ok(w, experts, nmat == 2))
+        return launch_gemv_experts(ws, nmat, experts, a, x, pairs, per_pair ? 1 : top, plan + plan_layout(pairs, experts).expert, y, stream);
     xp::Args A;
     for (int i = 0; i < 2; i++) {
         const DevWeight& m = *ws[i < nmat ? i : 0];
@@ -569,7 +626,7 @@ hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, con
     A.N = (int)(w.n / experts);
     A.nb = (int)(w.k / (w.dt == DT_Q8_0 ? 32 : 256));
     A.experts = experts;
-    A.pairs = (int)(T * top);
+    A.pairs = pairs;
     A.rowdiv = per_pair ? 1 : top;
     A.act = a;
     A.x = x;

@@ -23,57 +23,102 @@ namespace xr {
 
 typedef double v4d __attribute__((ext_vector_type(4)));
 
-// 16 tokens x 16 experts a workgroup; its waves take every WAVES-th run of 16
-// k, four MFMAs each: lane l holds row l % 16 and, of a run, the elements
-// 4 (l / 16) .. + 3, so that a load is a float4 and MFMA i takes the i-th of
-// each lane. The number of waves is the same for every call, so a logit's sum
-// has one order.
+// A workgroup takes 16 MT tokens x 16 MT experts and every Z-th part of K; its
+// waves take every WAVES-th run of 16 k of that part, four MFMAs each and tile:
+// lane l holds row l % 16 and, of a run, the elements 4 (l / 16) .. + 3, so that
+// a load is a float4 and MFMA i takes the i-th of each lane. The waves' sums
+// meet in LDS, those of the Z parts in the next kernel.
 constexpr int WAVES = 8;
 
+template <int MT>
 __global__ __launch_bounds__(64 * WAVES) void logits_kernel(const float* __restrict__ x, const float* __restrict__ r,
                                                             int64_t T, int64_t K, int E, double* __restrict__ out) {
-    __shared__ double part[WAVES][256];
+    constexpr int N = 16 * MT, U = 4 / MT;  // runs whose loads are in flight together
+    __shared__ double part[WAVES][N * N];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = lane & 15, g = lane >> 4;
-    const int64_t t0 = (int64_t)blockIdx.x * 16;
-    const int e0 = (int)blockIdx.y * 16;
-    const float* xr = x + min(t0 + a, T - 1) * K;
-    const float* rr = r + (int64_t)min(e0 + a, E - 1) * K;
-    v4d acc = {0.0, 0.0, 0.0, 0.0};
-    const int64_t runs = (K + 15) / 16;
-    constexpr int U = 4;  // runs whose loads are in flight together
-    for (int64_t c0 = wave; c0 < runs; c0 += U * WAVES) {
-        float4 xv[U], rv[U];
+    const int64_t t0 = (int64_t)blockIdx.x * N;
+    const int e0 = (int)blockIdx.y * N, Z = (int)gridDim.z, z = (int)blockIdx.z;
+    const float *xr[MT], *rr[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        xr[i] = x + min(t0 + 16 * i + a, T - 1) * K;
+        rr[i] = r + (int64_t)min(e0 + 16 * i + a, E - 1) * K;
+    }
+    v4d acc[MT][MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[i][j] = v4d{0.0, 0.0, 0.0, 0.0};
+    const int64_t all = (K + 15) / 16, part_runs = (all + Z - 1) / Z, runs = min(all, (z + 1) * part_runs);
+    float4 xv[2][U][MT], rv[2][U][MT];
+    auto load = [&](int64_t c0, int s) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int64_t k = min(16 * (c0 + (int64_t)u * WAVES) + 4 * g, K - 4);
-            xv[u] = *(const float4*)(xr + k);
-            rv[u] = *(const float4*)(rr + k);
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                xv[s][u][i] = *(const float4*)(xr[i] + k);
+                rv[s][u][i] = *(const float4*)(rr[i] + k);
+            }
         }
+    };
+    // (whole runs past the end are left out, what is past it inside the last
+    // run counts as zeros)
+    auto multiply = [&](int64_t c0, int s) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            // (past the row's end: zeros, which add nothing but to a sum of a
-            // zero; whole runs past it are left out)
             const int64_t c = c0 + (int64_t)u * WAVES;
             if (c >= runs) break;
             const bool in = 16 * c + 4 * g < K;
-            const float xe[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w}, re[4] = {rv[u].x, rv[u].y, rv[u].z, rv[u].w};
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(in ? (double)xe[i] : 0.0, in ? (double)re[i] : 0.0, acc, 0, 0, 0);
+            for (int q = 0; q < 4; q++) {
+                double xd[MT], rd[MT];
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    const float xe[4] = {xv[s][u][i].x, xv[s][u][i].y, xv[s][u][i].z, xv[s][u][i].w};
+                    const float re[4] = {rv[s][u][i].x, rv[s][u][i].y, rv[s][u][i].z, rv[s][u][i].w};
+                    xd[i] = in ? (double)xe[q] : 0.0;
+                    rd[i] = in ? (double)re[q] : 0.0;
+                }
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int j = 0; j < MT; j++) acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(xd[i], rd[j], acc[i][j], 0, 0, 0);
+            }
+        }
+    };
+    constexpr int64_t STEP = U * WAVES;
+    int64_t c0 = z * part_runs + wave;
+    if constexpr (MT == 1) {  // (a wave has few runs)
+        for (; c0 < runs; c0 += STEP) {
+            load(c0, 0);
+            multiply(c0, 0);
+        }
+    } else {  // the next runs' loads in flight under this one's products: 52 -> 46 us
+        load(c0, 0);
+        for (; c0 < runs; c0 += 2 * STEP) {
+            load(c0 + STEP, 1);
+            multiply(c0, 0);
+            load(c0 + 2 * STEP, 0);
+            multiply(c0 + STEP, 1);
         }
     }
-    // result lane l, register i: token 4 i + l / 16, expert l % 16
+    // result lane l, register q of a tile: token 4 q + l / 16, expert l % 16
 #pragma unroll
-    for (int i = 0; i < 4; i++) part[wave][(4 * i + g) * 16 + a] = acc[i];
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) part[wave][(16 * i + 4 * q + g) * N + 16 * j + a] = acc[i][j][q];
     __syncthreads();
-    const int o = threadIdx.x;
-    if (o >= 256) return;
-    double s = 0.0;
+    for (int o = threadIdx.x; o < N * N; o += 64 * WAVES) {
+        double s = 0.0;
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) s += part[w][o];
-    const int64_t t = t0 + o / 16;
-    const int e = e0 + o % 16;
-    if (t < T && e < E) out[t * E + e] = s;
+        for (int w = 0; w < WAVES; w++) s += part[w][o];
+        const int64_t t = t0 + o / N;
+        const int e = e0 + o % N;
+        if (t < T && e < E) out[((int64_t)z * T + t) * E + e] = s;
+    }
 }
 
 // A double as an integer of the same order; NaN below all numbers, `taken`
@@ -84,13 +129,19 @@ __device__ __forceinline__ int64_t order_key(double v) {
     const int64_t b = __double_as_longlong(v + 0.0);
     return b < 0 ? b ^ INT64_MAX : b;
 }
+template <int M>
+__device__ __forceinline__ int64_t max_xor_i64(int64_t v) {
+    const int lo = lane_xor<M>((int)(v & 0xFFFFFFFFll)), hi = lane_xor<M>((int)(v >> 32));
+    const int64_t o = ((int64_t)hi << 32) | (int64_t)(uint32_t)lo;
+    return o > v ? o : v;
+}
 __device__ __forceinline__ int64_t wave_max_i64(int64_t v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        const int64_t o = __shfl_xor((long long)v, m);
-        v = o > v ? o : v;
-    }
-    return v;
+    v = max_xor_i64<32>(v);
+    v = max_xor_i64<16>(v);
+    v = max_xor_i64<8>(v);
+    v = max_xor_i64<4>(v);
+    v = max_xor_i64<2>(v);
+    return max_xor_i64<1>(v);
 }
 __device__ __forceinline__ int wave_min_i32(int v) {
     v = min(v, __shfl_xor(v, 32));
@@ -102,16 +153,19 @@ __device__ __forceinline__ int wave_min_i32(int v) {
 }
 
 // One token's choices by one wave: lane l holds the logits of the experts l,
-// l + 64, ...
+// l + 64, ..., each the sum of Z parts `stride` apart. Lane j < top returns
+// choice j.
 template <int PER>
-__device__ __forceinline__ void select(const double* logits, int E, int top, int normalize, int32_t* ids, float* weights) {
+__device__ __forceinline__ int select(const double* logits, int Z, int64_t stride, int E, int top, int normalize, int32_t* ids,
+                                      float* weights) {
     const int lane = threadIdx.x & 63;
     double v[PER];
     int64_t key[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const int e = lane + 64 * i;
-        v[i] = e < E ? logits[e] : 0.0;
+        v[i] = 0.0;
+        for (int z = 0; z < Z; z++) v[i] += e < E ? logits[z * stride + e] : 0.0;
         key[i] = e < E ? order_key(v[i]) : KEY_TAKEN;
     }
     double m = 0.0, mine = 0.0;  // the largest; the value of choice `lane`
@@ -145,18 +199,48 @@ __device__ __forceinline__ void select(const double* logits, int E, int top, int
         ids[lane] = id;
         weights[lane] = (float)(exp(mine - m) / sum);
     }
+    return id;
 }
-__device__ __forceinline__ void select_any(const double* logits, int E, int top, int normalize, int32_t* ids, float* weights) {
-    if (E <= 64) select<1>(logits, E, top, normalize, ids, weights);
-    else if (E <= 128) select<2>(logits, E, top, normalize, ids, weights);
-    else if (E <= 256) select<4>(logits, E, top, normalize, ids, weights);
-    else select<8>(logits, E, top, normalize, ids, weights);
+__device__ __forceinline__ int select_any(const double* logits, int Z, int64_t stride, int E, int top, int normalize, int32_t* ids,
+                                          float* weights) {
+    if (E <= 64) return select<1>(logits, Z, stride, E, top, normalize, ids, weights);
+    if (E <= 128) return select<2>(logits, Z, stride, E, top, normalize, ids, weights);
+    if (E <= 256) return select<4>(logits, Z, stride, E, top, normalize, ids, weights);
+    return select<8>(logits, Z, stride, E, top, normalize, ids, weights);
 }
 
-__global__ __launch_bounds__(256) void select_kernel(const double* __restrict__ logits, int64_t T, int E, int top,
+__global__ __launch_bounds__(256) void select_kernel(const double* __restrict__ logits, int Z, int64_t T, int E, int top,
                                                      int normalize, int32_t* __restrict__ ids, float* __restrict__ weights) {
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t < T) select_any(logits + t * E, E, top, normalize, ids + t * top, weights + t * top);
+    if (t < T) select_any(logits + t * E, Z, T * E, E, top, normalize, ids + t * top, weights + t * top);
+}
+
+// Few tokens: their choices and the plan of them by one workgroup.
+constexpr int SMALL_T = 32, SMALL_PAIRS = 512;
+
+__global__ __launch_bounds__(1024) void select_plan_kernel(const double* __restrict__ logits, int Z, int T, int E, int top,
+                                                           int normalize, int32_t* __restrict__ ids, float* __restrict__ weights,
+                                                           int32_t* __restrict__ plan) {
+    __shared__ int chosen[SMALL_PAIRS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, P = T * top;
+    for (int t = wave; t < T; t += 16) {
+        const int id = select_any(logits + (int64_t)t * E, Z, (int64_t)T * E, E, top, normalize, ids + t * top, weights + t * top);
+        if (lane < top) chosen[t * top + lane] = id;
+    }
+    __syncthreads();
+    const PlanLayout l = plan_layout(P, E);
+    for (int p = threadIdx.x; p < P; p += 1024) plan[l.expert + p] = chosen[p];
+    for (int e = wave; e <= E; e += 16) {
+        int at = 0;
+        for (int p = lane; p - lane < P; p += 64) at += __popcll(__ballot(p < P && chosen[min(p, P - 1)] < e));
+        if (lane == 0) plan[e] = at;
+        for (int p = lane; p - lane < P; p += 64) {
+            const bool mine = p < P && chosen[min(p, P - 1)] == e;
+            const uint64_t b = __ballot(mine);
+            if (mine) plan[l.order + at + __popcll(b & ((1ull << lane) - 1))] = p;
+            at += __popcll(b);
+        }
+    }
 }
 
 // The plan: workgroup e of E + 1 counts the pairs of the experts below e, which
@@ -168,35 +252,55 @@ constexpr int PLAN_T = 1024;
 
 __device__ __forceinline__ int expert_of(int id, int E) { return id >= 0 && id < E ? id : E; }
 
+// HOLD: the ids of a wave's run stay in registers between the two passes
+// (P <= HOLD * PLAN_T), 0: they are read again.
+template <int HOLD>
 __global__ __launch_bounds__(PLAN_T) void plan_kernel(const int32_t* __restrict__ ids, int P, int E, int32_t* __restrict__ plan) {
     constexpr int W = PLAN_T / 64;
     __shared__ int below[W], equal[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = (int)blockIdx.x;
     const PlanLayout l = plan_layout(P, E);
-    const int run = (P + PLAN_T - 1) / PLAN_T * 64;  // pairs of a wave, whole 64s
-    const int p0 = min(wave * run, P), p1 = min(p0 + run, P);
+    const int n = (P + PLAN_T - 1) / PLAN_T;  // 64s of pairs of a wave
+    const int p0 = min(wave * n * 64, P), p1 = min(p0 + n * 64, P);
+    auto load = [&](int i) { return p0 + 64 * i + lane < p1 ? expert_of(ids[p0 + 64 * i + lane], E) : INT32_MAX; };
+    int held[HOLD ? HOLD : 1];
+    if constexpr (HOLD > 0) {
+#pragma unroll
+        for (int i = 0; i < HOLD; i++) held[i] = i < n ? load(i) : INT32_MAX;
+    }
     int nb = 0, ne = 0;
-    for (int p = p0; p < p1; p += 64) {
-        const int id = p + lane < p1 ? expert_of(ids[p + lane], E) : INT32_MAX;
+    auto count = [&](int id) {
         nb += __popcll(__ballot(id < e));
         ne += __popcll(__ballot(id == e));
+    };
+    if constexpr (HOLD > 0) {
+#pragma unroll
+        for (int i = 0; i < HOLD; i++) count(held[i]);
+    } else {
+        for (int i = 0; i < n; i++) count(load(i));
     }
     if (lane == 0) below[wave] = nb, equal[wave] = ne;
     __syncthreads();
     int at = 0;
+#pragma unroll
     for (int w = 0; w < W; w++) at += below[w];
     if (threadIdx.x == 0) plan[e] = at;  // e = E: the pairs that have one
     for (int w = 0; w < wave; w++) at += equal[w];
     if (ne == 0) return;
     int32_t *order = plan + l.order, *expert = plan + l.expert;
-    for (int p = p0; p < p1; p += 64) {
-        const int id = p + lane < p1 ? expert_of(ids[p + lane], E) : INT32_MAX;
+    auto place = [&](int i, int id) {
         const uint64_t b = __ballot(id == e);
         if (id == e) {
-            order[at + __popcll(b & ((1ull << lane) - 1))] = p + lane;
-            expert[p + lane] = e < E ? e : -1;
+            order[at + __popcll(b & ((1ull << lane) - 1))] = p0 + 64 * i + lane;
+            expert[p0 + 64 * i + lane] = e < E ? e : -1;
         }
         at += __popcll(b);
+    };
+    if constexpr (HOLD > 0) {
+#pragma unroll
+        for (int i = 0; i < HOLD; i++) place(i, held[i]);
+    } else {
+        for (int i = 0; i < n; i++) place(i, load(i));
     }
 }
 
@@ -232,15 +336,45 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
 }  // namespace xr
 
 hipError_t launch_experts_plan(const int32_t* ids, int64_t T, int top, int experts, int32_t* plan, hipStream_t s) {
-    hipLaunchKernelGGL(xr::plan_kernel, dim3((unsigned)(experts + 1)), dim3(xr::PLAN_T), 0, s, ids, (int)(T * top), experts, plan);
+    const int P = (int)(T * top);
+    const dim3 grid((unsigned)(experts + 1)), block(xr::PLAN_T);
+    if (P <= 4 * xr::PLAN_T) hipLaunchKernelGGL(xr::plan_kernel<4>, grid, block, 0, s, ids, P, experts, plan);
+    else if (P <= 16 * xr::PLAN_T) hipLaunchKernelGGL(xr::plan_kernel<16>, grid, block, 0, s, ids, P, experts, plan);
+    else hipLaunchKernelGGL(xr::plan_kernel<0>, grid, block, 0, s, ids, P, experts, plan);
     return hipGetLastError();
+}
+
+namespace xr {
+// 32 x 32 tiles, which read x and r half as often from the L2, where they
+// give at least 128 workgroups; 16 x 16 below. Parts of K so that there are about as many
+// workgroups as compute units.
+struct Shape {
+    int n, parts;
+};
+static Shape route_shape(int64_t T, int experts) {
+    const int64_t t32 = (T + 31) / 32 * ((experts + 31) / 32), t16 = (T + 15) / 16 * ((experts + 15) / 16);
+    Shape r{t32 >= 128 ? 32 : 16, 1};
+    for (const int64_t tiles = r.n == 32 ? t32 : t16; r.parts < 16 && tiles * r.parts * 2 <= 256;) r.parts *= 2;
+    return r;
+}
+}  // namespace xr
+
+uint64_t experts_route_ws_bytes(int64_t T, int experts) {
+    return (uint64_t)T * experts * 8 * xr::route_shape(T, experts).parts;
 }
 
 hipError_t launch_experts_route(const float* x, const float* router, int64_t T, int64_t K, int experts, int top, int normalize,
                                 int32_t* ids, float* weights, int32_t* plan, double* logits, hipStream_t s) {
-    hipLaunchKernelGGL(xr::logits_kernel, dim3((unsigned)((T + 15) / 16), (unsigned)((experts + 15) / 16)),
-                       dim3(64 * xr::WAVES), 0, s, x, router, T, K, experts, logits);
-    hipLaunchKernelGGL(xr::select_kernel, dim3((unsigned)((T + 3) / 4)), dim3(256), 0, s, logits, T, experts, top, normalize,
+    const xr::Shape r = xr::route_shape(T, experts);
+    const dim3 grid((unsigned)((T + r.n - 1) / r.n), (unsigned)((experts + r.n - 1) / r.n), (unsigned)r.parts), block(64 * xr::WAVES);
+    if (r.n == 32) hipLaunchKernelGGL(xr::logits_kernel<2>, grid, block, 0, s, x, router, T, K, experts, logits);
+    else hipLaunchKernelGGL(xr::logits_kernel<1>, grid, block, 0, s, x, router, T, K, experts, logits);
+    if (plan && T <= xr::SMALL_T && T * top <= xr::SMALL_PAIRS) {
+        hipLaunchKernelGGL(xr::select_plan_kernel, dim3(1), dim3(1024), 0, s, logits, r.parts, (int)T, experts, top, normalize, ids,
+                           weights, plan);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(xr::select_kernel, dim3((unsigned)((T + 3) / 4)), dim3(256), 0, s, logits, r.parts, T, experts, top, normalize,
                        ids, weights);
     if (plan) return launch_experts_plan(ids, T, top, experts, plan, s);
     return hipGetLastError();

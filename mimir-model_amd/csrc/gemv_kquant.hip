@@ -463,6 +463,88 @@ hipError_t launch_gemv_a8k(const DevWeight* const* ws, int nmat, const ActPtrs& 
     return hipErrorInvalidValue;
 }
 
+// The products of a mixture of experts where a call has few (token, choice)
+// pairs: workgroup (tile, p) runs its tile of pair p's expert's matrix (SW: of
+// gate and up) against the pair's activation row, so every output is bit for
+// bit the matrix's own product. A has the matrices of all experts and the rows
+// of the call; the swiglu of a pair is one piece (its vector formula: the
+// total a multiple of eight).
+template <uint32_t DT, int R, bool SW>
+__global__ __launch_bounds__(256) void gemv_experts_kernel(GemvArgs A, const int32_t* __restrict__ expert, int rowdiv) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int p = (int)blockIdx.y, e = expert[p];
+    if (e < 0) return;
+    const int64_t w0 = (int64_t)e * A.N, row = p / rowdiv;
+#pragma unroll
+    for (int i = 0; i < (SW ? 2 : 1); i++) {
+        A.mat[i].W += w0 * A.rb;
+        A.mat[i].wref += w0;
+    }
+    A.W = A.mat[0].W;
+    A.wref = A.mat[0].wref;
+    A.q += row * A.K;
+    A.d32 += row * (A.K / 32);
+    A.s16 += row * (A.K / (DT == DT_Q4_K ? 32 : 16));
+    A.ok += row;
+    A.x += row * A.K;
+    if (SW) A.sw += (int64_t)p * A.N;
+    else A.y += (int64_t)p * A.N;
+    pairs_tile<DT, 1, R, SW>(A, (int)blockIdx.x, smem);
+}
+
+template <uint32_t DT, int R, bool SW>
+static hipError_t launch_experts_r(const GemvArgs& A, const int32_t* expert, int pairs, int rowdiv, hipStream_t stream) {
+    constexpr int RT = SW ? R / 2 : R;
+    const size_t lds = (size_t)R * A.nb * 16 + (size_t)R * 8;
+    hipLaunchKernelGGL((gemv_experts_kernel<DT, R, SW>), dim3((unsigned)((A.N + RT - 1) / RT), (unsigned)pairs), dim3(256), lds,
+                       stream, A, expert, rowdiv);
+    return hipGetLastError();
+}
+
+template <uint32_t DT>
+static hipError_t launch_experts_dt(const GemvArgs& A, bool sw, const int32_t* expert, int pairs, int rowdiv, hipStream_t stream) {
+    if (sw) return launch_experts_r<DT, 2 * PAIRS_U, true>(A, expert, pairs, rowdiv, stream);
+    switch (pairs_rows((int)std::min<int64_t>((int64_t)A.N * pairs, INT_MAX), A.nb, 1)) {
+    case 32:
+    case 16: return launch_experts_r<DT, 16, false>(A, expert, pairs, rowdiv, stream);
+    case 8: return launch_experts_r<DT, 8, false>(A, expert, pairs, rowdiv, stream);
+    case 4: return launch_experts_r<DT, 4, false>(A, expert, pairs, rowdiv, stream);
+    case 2: return launch_experts_r<DT, 2, false>(A, expert, pairs, rowdiv, stream);
+    default: return launch_experts_r<DT, 1, false>(A, expert, pairs, rowdiv, stream);
+    }
+}
+
+bool gemv_experts_ok(const DevWeight& w, int experts, bool sw) {
+    const int64_t N = w.n / experts;
+    return (w.dt == DT_Q4_K || w.dt == DT_Q6_K) && w.k % 256 == 0 && w.k <= 65536 && N <= (1 << 30) && (!sw || N % PAIRS_U == 0);
+}
+
+hipError_t launch_gemv_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int pairs,
+                               int rowdiv, const int32_t* expert, float* y, hipStream_t stream) {
+    const DevWeight& w = *ws[0];
+    GemvArgs A{};
+    A.rb = w.row_bytes;
+    A.N = (int)(w.n / experts);
+    A.nb = (int)(w.k / 256);
+    A.K = w.k;
+    A.q = a.q;
+    A.d32 = a.d32;
+    A.s16 = w.dt == DT_Q4_K ? a.xs : a.ys16;
+    A.ok = a.ok;
+    A.x = x;
+    A.y = A.sw = y;
+    A.fused = 1;
+    A.nmat = nmat;
+    A.sw_total = A.sw_chunk = (A.N + 7) / 8 * 8;
+    for (int i = 0; i < nmat; i++) {
+        A.mat[i].W = ws[i]->data;
+        A.mat[i].wref = ws[i]->wref;
+        A.mat[i].N = A.N;
+    }
+    if (w.dt == DT_Q4_K) return launch_experts_dt<DT_Q4_K>(A, nmat == 2, expert, pairs, rowdiv, stream);
+    return launch_experts_dt<DT_Q6_K>(A, nmat == 2, expert, pairs, rowdiv, stream);
+}
+
 // Independent one-row products in one launch (mimg_linear_a8_set_dev): the
 // segments are matrices with activation rows of their own (a decoder
 // layer's linear set with an input per matrix), Q4_K and Q6_K mixed, K per

@@ -1694,7 +1694,7 @@ int mimg_experts_plan_dev(const int32_t* ids, int64_t T, int top, int experts, v
 }
 
 uint64_t mimg_experts_route_workspace_bytes(int64_t T, int experts) {
-    return T > 0 && experts_shape(T, 1, experts) ? (uint64_t)T * experts * 8 : 0;
+    return T > 0 && experts_shape(T, 1, experts) ? experts_route_ws_bytes(T, experts) : 0;
 }
 
 int mimg_experts_route_dev(const float* x, const float* router, int64_t T, int64_t k, int experts, int top, int normalize,

@@ -143,6 +143,11 @@ __device__ __forceinline__ void lds_copy16(const void* g, uint32_t lds) {
 __device__ __forceinline__ void lds_copy4(const void* g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
 }
+// The same from an address that the wave shares (a scalar) plus each lane's own
+// 32-bit offset.
+__device__ __forceinline__ void lds_copy16_at(const void* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
 __device__ __forceinline__ void lds_copy16(const void* g, const void* lds) { lds_copy16(g, lds_addr(lds)); }
 __device__ __forceinline__ void lds_copy4(const void* g, const void* lds) { lds_copy4(g, lds_addr(lds)); }
 

@@ -240,7 +240,8 @@ uint64_t logprobs_ws_bytes(int64_t rows, int64_t n, int top);
 hipError_t launch_logprobs(const float* x, int64_t rows, int64_t n, int64_t ld, const int32_t* targets, int top,
                            float* logprob, float* entropy, int32_t* top_ids, float* top_lp, void* ws, hipStream_t s);
 // A mixture of experts (experts_route.hip, experts.hip; the plan: experts.hpp).
-// logits: T * experts doubles of workspace; plan may be null.
+// logits: workspace of experts_route_ws_bytes; plan may be null.
+uint64_t experts_route_ws_bytes(int64_t T, int experts);
 hipError_t launch_experts_route(const float* x, const float* router, int64_t T, int64_t K, int experts, int top, int normalize,
                                 int32_t* ids, float* weights, int32_t* plan, double* logits, hipStream_t s);
 hipError_t launch_experts_plan(const int32_t* ids, int64_t T, int top, int experts, int32_t* plan, hipStream_t s);
@@ -250,6 +251,10 @@ hipError_t launch_experts_plan(const int32_t* ids, int64_t T, int top, int exper
 bool experts_ok(const DevWeight& w);
 hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int64_t T, int top,
                           bool per_pair, const int32_t* plan, float* y, hipStream_t s);
+// The same for few pairs, each its own row (gemv_kquant.hip).
+bool gemv_experts_ok(const DevWeight& w, int experts, bool sw);
+hipError_t launch_gemv_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int pairs,
+                               int rowdiv, const int32_t* expert, float* y, hipStream_t s);
 hipError_t launch_experts_sum(const float* part, const float* weights, const int32_t* expert, int64_t T, int top, int64_t N,
                               float* y, hipStream_t s);
 hipError_t launch_greedy_advance(const int32_t* chosen, int32_t* ids, int64_t* pos, int64_t* cidx, int32_t* out,
