@@ -63,6 +63,7 @@ struct Args {
     int N, nb, experts, pairs;  // nb: blocks (of 256; of 32 for Q8_0) of a row
     int rowdiv;           // a pair's activation row is pair / rowdiv
     ActPtrs act;
+    const uint8_t* parts; // Q4_K: the sums of 32 as f16 parts, 32 bytes a block
     const float* x;       // f32 activations (fallback)
 };
 
@@ -78,15 +79,16 @@ struct Cfg {
     static constexpr int WCH = DT == DT_Q4_K ? 9 : DT == DT_Q6_K ? 15 : 19;
     static constexpr int WSLOT = 16 * WCH;
     static constexpr int WDMA = (32 * WCH + 63) / 64;
-    static constexpr int WWAVE = WDMA * 1024;  // incl. slack for the last copy
+    static constexpr int WWAVE = 32 * WSLOT;
     static constexpr int WBYTES = 4 * WWAVE;
     static constexpr int ADMA = BM * 16 / T;
     static constexpr int ABYTES = BM * 256;
-    static constexpr int XBYTES = DT == DT_Q4_K ? 1024 : 0;        // 16 bytes of sums a row
-    static constexpr int DBYTES = K32 ? BM * 32 : 256;             // 8 scales a row, or one
+    static constexpr int XBYTES = DT == DT_Q4_K ? 32 * BM : 0;     // a row's sums in f16 parts
+    static constexpr int DBYTES = K32 ? BM * 32 : (BM + 63) / 64 * 256;  // 8 scales a row, or one
     static constexpr int BUF = ABYTES + XBYTES + DBYTES;
     static constexpr int SMEM = WBYTES + 2 * BUF;
-    static_assert(ADMA * T == BM * 16 && BM <= 64 && 2 * 64 * BM * 4 <= SMEM && SMEM <= 80 * 1024, "tile shape");
+    static_assert(ADMA * T == BM * 16 && BM <= (DT == DT_Q4_K ? 64 : 128) && 2 * 64 * BM * 4 <= SMEM, "tile shape");
+    static_assert(2 * SMEM + 16 * BM <= 160 * 1024, "two workgroups a compute unit");
 };
 
 // s_waitcnt with vmcnt <= N (N < 64), the other counters unconstrained.
@@ -191,8 +193,12 @@ struct Copies {
             const int c = C::T * i + t, r = c >> 4, k = c & 15;
             a[i] = (const uint8_t*)A.act.q + (int64_t)rows[r] * A.K + 16 * (k ^ (r & 15));
         }
-        const int64_t row = (int64_t)rows[min(l, C::BM - 1)] * (A.K / 32);
-        s = wave == 0 && DT == DT_Q4_K ? (const uint8_t*)(A.act.xs + row) : (const uint8_t*)(A.act.d32 + row);
+        // (waves 0 and 1: scales of 64 rows each; 2 and 3: Q4_K's sums of 32)
+        if (DT == DT_Q4_K && wave >= 2) {
+            s = A.parts + (int64_t)rows[min(32 * (int)(wave - 2) + (l >> 1), C::BM - 1)] * (A.K / 8) + 16 * (l & 1);
+        } else {
+            s = (const uint8_t*)(A.act.d32 + (int64_t)rows[min(wave == 1 ? 64 + l : l, C::BM - 1)] * (A.K / 32));
+        }
         if constexpr (C::K32) {
 #pragma unroll
             for (int i = 0; i < C::DBYTES / 1024; i++) {
@@ -214,7 +220,7 @@ struct Copies {
             uint32_t o = w[i];
             if constexpr (DT == DT_Q6_K) o = ((o + (uint32_t)b * C::GROUP) & ~15u) + 16 * (min(64 * i + l, 32 * C::WCH - 1) % C::WCH);
             if constexpr (DT != DT_Q4_K) o = min(o, last);
-            lds_copy16_at(base, o, lds + C::WWAVE * wave + 1024 * i);
+            if (64 * i + 64 <= 32 * C::WCH || l < 32 * C::WCH - 64 * i) lds_copy16_at(base, o, lds + C::WWAVE * wave + 1024 * i);
         }
     }
     __device__ __forceinline__ void activations(int b, uint32_t lds) const {
@@ -225,8 +231,8 @@ struct Copies {
             for (int i = 0; i < C::DBYTES / 1024; i++)
                 lds_copy4(d8[i] + 32 * (int64_t)b, lds + C::ABYTES + 256 * wave + 4 * C::T * i);
         } else {
-            if (DT == DT_Q4_K && wave == 0) lds_copy16(s + 16 * (int64_t)b, lds + C::ABYTES);
-            if (wave == 1) lds_copy4(s + 32 * (int64_t)b, lds + C::ABYTES + C::XBYTES);
+            if (DT == DT_Q4_K && wave >= 2 && 32 * (wave - 2) < C::BM) lds_copy16(s + 32 * (int64_t)b, lds + C::ABYTES + 1024 * (wave - 2));
+            if (64 * wave < C::BM) lds_copy4(s + 32 * (int64_t)b, lds + C::ABYTES + C::XBYTES + 256 * wave);
         }
     }
 };
@@ -352,7 +358,7 @@ template <uint32_t DT, class C, bool SW>
 __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
     constexpr int MT = C::MT, BM = C::BM, BN = SW ? 64 : 128;
     __shared__ __align__(16) uint8_t smem[C::SMEM];  // weights, then two activation stages
-    __shared__ int rows[BM], outs[64], flags[1];
+    __shared__ int rows[BM], outs[(BM + 63) / 64 * 64], flags[1];
     const int t = threadIdx.x, l = t & 63, wave = t >> 6;
     const int a = l & 31, g = l >> 5;
     Tile tile;
@@ -369,9 +375,9 @@ __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
     // The tile's pairs, behind them the weights (which need the tile alone):
     // the first ones have landed when at most the weights' copies are left.
     // (Past the tile's pairs the last one again, whose results are not written.)
-    if (cp.wave == 0) lds_copy4(A.plan + plan_layout(A.pairs, A.experts).order + tile.f0 + min(l, tile.m - 1), outs);
+    if (64 * cp.wave < BM) lds_copy4(A.plan + plan_layout(A.pairs, A.experts).order + tile.f0 + min(t, tile.m - 1), outs + 64 * cp.wave);
     cp.weights(0, lds0);
-    if (cp.wave == 0) wait_vmcnt<C::WDMA>();
+    if (64 * cp.wave < BM) wait_vmcnt<C::WDMA>();
     if (t == 0) flags[0] = 0;
     lds_barrier();
     if (t < BM) {
@@ -449,20 +455,8 @@ __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
                     // g = 0 hold d, g = 1 dmin)
                     const v32f z = {};
                     const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * i + a], g ? grp.dmin : grp.d, z, 0, 0, 0);
-                    const u32x4 xw = *(const u32x4*)(buf + C::ABYTES + 16 * (32 * i + a));
-                    const short sh = g ? 0 : 6;
-                    const s16x2 sh2 = {sh, sh};
-                    const uint32_t msk = g ? 0x003F003Fu : 0xFFFFFFFFu;
-                    const h2 cf = g ? h2{(_Float16)1024.0f, (_Float16)1024.0f} : h2{(_Float16)1088.0f, (_Float16)1088.0f};
-                    const s16x2 cadd = g ? s16x2{0x6400, 0x6400} : s16x2{0x6440, 0x6440};
-                    v8h v;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t u = as_u32(as_s16x2(xw[j]) >> sh2) & msk;
-                        const h2 f = __builtin_bit_cast(h2, as_u32(as_s16x2(u) + cadd)) - cf;
-                        v[2 * j] = f.x;
-                        v[2 * j + 1] = f.y;
-                    }
+                    // 64 hi + lo against 64 m and m
+                    const v8h v = *(const v8h*)(buf + C::ABYTES + 32 * (32 * i + a) + 16 * g);
                     v16f Mm = {};
                     Mm = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bm, Mm, 0, 0, 0);
 #pragma unroll
@@ -585,8 +579,8 @@ static hipError_t launch(const Args& A, hipStream_t stream) {
 
 template <uint32_t DT, bool SW>
 static hipError_t launch_dt(const Args& A, hipStream_t stream) {
-    // (64 pairs a workgroup where the experts have as many on average)
-    return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, 2, SW>(A, stream) : launch<DT, 1, SW>(A, stream);
+    // (64 pairs a workgroup, Q6_K 96, where the experts have as many on average)
+    return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, DT == DT_Q6_K ? 3 : 2, SW>(A, stream) : launch<DT, 1, SW>(A, stream);
 }
 
 }  // namespace xp
@@ -606,13 +600,20 @@ bool experts_ok(const DevWeight& w) {
            w.n <= (1ll << 31) - 1;
 }
 
-hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int64_t T, int top,
-                          bool per_pair, const int32_t* plan, float* y, hipStream_t stream) {
+hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, void* parts, const float* x,
+                          int64_t T, int top, bool per_pair, const int32_t* plan, float* y, hipStream_t stream) {
     const DevWeight& w = *ws[0];
     const int pairs = (int)(T * top);
-    if (few_pairs(pairs, experts) && gemv_experts_ok(w, experts, nmat == 2))
+    const int64_t rows = per_pair ? pairs : T;
+    if (few_pairs(pairs, experts) && gemv_experts_ok(w, experts, nmat == 2)) {
+        const hipError_t e = launch_quantize_act(x, rows, w.k, 256, a, stream);
+        if (e != hipSuccess) return e;
         return launch_gemv_experts(ws, nmat, experts, a, x, pairs, per_pair ? 1 : top, plan + plan_layout(pairs, experts).expert, y, stream);
+    }
+    const hipError_t e = launch_experts_quantize(w.dt, x, rows, w.k, a, parts, stream);
+    if (e != hipSuccess) return e;
     xp::Args A;
+    A.parts = (const uint8_t*)parts;
     for (int i = 0; i < 2; i++) {
         const DevWeight& m = *ws[i < nmat ? i : 0];
         A.mat[i].W = m.data;

@@ -1723,14 +1723,28 @@ int mimg_experts_route_dev(const float* x, const float* router, int64_t T, int64
     return MIMG_OK;
 }
 
-// The quantized rows, then (combine) each pair's product.
+// The quantized rows, their sums as the tiles' f16 operand (the int16 sums'
+// place and more), and for combine each pair's product.
+struct ExpertsLayout {
+    ActLayout act;
+    uint64_t parts, product, total;
+};
+static ExpertsLayout experts_layout(int64_t rows, int64_t k, int64_t products) {
+    ExpertsLayout l;
+    l.act = act_layout(rows, k);
+    l.parts = l.act.total;
+    l.product = (l.parts + (uint64_t)rows * (k / 8) + 255) / 256 * 256;
+    l.total = l.product + (uint64_t)products * 4;
+    return l;
+}
+
 uint64_t mimg_experts_swiglu_workspace_bytes(int64_t T, int top, int64_t n, int64_t k) {
     if (!experts_shape(T, top, EXPERTS_MAX) || n <= 0 || k <= 0 || T == 0) return 0;
-    return act_layout(T, k).total;
+    return experts_layout(T, k, 0).total;
 }
 uint64_t mimg_experts_combine_workspace_bytes(int64_t T, int top, int64_t n, int64_t k) {
     if (!experts_shape(T, top, EXPERTS_MAX) || n <= 0 || k <= 0 || T == 0) return 0;
-    return act_layout(T * top, k).total + (uint64_t)T * top * n * 4;
+    return experts_layout(T * top, k, T * top * n).total;
 }
 
 // What both products check; their rows and K, and the rows of an expert.
@@ -1761,13 +1775,11 @@ int mimg_experts_swiglu_a8_dev(uint64_t gate, uint64_t up, int experts, const fl
     if ((rc = check_experts_product("experts_swiglu", g.get(), u.get(), T, top, experts, x, h, plan, plan_bytes, ws, &n, &k)) || T == 0)
         return rc;
     if (overlaps(x, (uint64_t)T * k * 4, h, (uint64_t)T * top * n * 4)) return fail(MIMG_ERR_ARG, "experts_swiglu: h overlaps x");
-    const ActLayout l = act_layout(T, k);
+    const ExpertsLayout l = experts_layout(T, k, 0);
     if (ws_bytes < l.total)
         return fail(MIMG_ERR_WORKSPACE, "experts_swiglu workspace %llu < %llu bytes", (unsigned long long)ws_bytes, (unsigned long long)l.total);
-    const ActPtrs a = act_ptrs(ws, l);
     const DevWeight* dws[2] = {&g->dw, &u->dw};
-    HIP_TRY(launch_quantize_act(x, T, k, g->dw.dt == DT_Q8_0 ? 32 : 256, a, (hipStream_t)stream));
-    HIP_TRY(launch_experts(dws, 2, experts, a, x, T, top, false, (const int32_t*)plan, h, (hipStream_t)stream));
+    HIP_TRY(launch_experts(dws, 2, experts, act_ptrs(ws, l.act), (uint8_t*)ws + l.parts, x, T, top, false, (const int32_t*)plan, h, (hipStream_t)stream));
     return MIMG_OK;
 }
 
@@ -1783,15 +1795,12 @@ int mimg_experts_combine_a8_dev(uint64_t down, int experts, const float* h, cons
     const int64_t P = T * top;
     if (overlaps(h, (uint64_t)P * k * 4, y, (uint64_t)T * n * 4) || overlaps(weights, (uint64_t)P * 4, y, (uint64_t)T * n * 4))
         return fail(MIMG_ERR_ARG, "experts_combine: y overlaps h or weights");
-    const ActLayout l = act_layout(P, k);
-    const uint64_t need = l.total + (uint64_t)P * n * 4;
-    if (ws_bytes < need)
-        return fail(MIMG_ERR_WORKSPACE, "experts_combine workspace %llu < %llu bytes", (unsigned long long)ws_bytes, (unsigned long long)need);
-    const ActPtrs a = act_ptrs(ws, l);
-    float* part = (float*)((uint8_t*)ws + l.total);
+    const ExpertsLayout l = experts_layout(P, k, P * n);
+    if (ws_bytes < l.total)
+        return fail(MIMG_ERR_WORKSPACE, "experts_combine workspace %llu < %llu bytes", (unsigned long long)ws_bytes, (unsigned long long)l.total);
+    float* part = (float*)((uint8_t*)ws + l.product);
     const DevWeight* dws[1] = {&w->dw};
-    HIP_TRY(launch_quantize_act(h, P, k, w->dw.dt == DT_Q8_0 ? 32 : 256, a, (hipStream_t)stream));
-    HIP_TRY(launch_experts(dws, 1, experts, a, h, T, top, true, (const int32_t*)plan, part, (hipStream_t)stream));
+    HIP_TRY(launch_experts(dws, 1, experts, act_ptrs(ws, l.act), (uint8_t*)ws + l.parts, h, T, top, true, (const int32_t*)plan, part, (hipStream_t)stream));
     HIP_TRY(launch_experts_sum(part, weights, (const int32_t*)plan + plan_layout(P, experts).expert, T, top, n, y, (hipStream_t)stream));
     return MIMG_OK;
 }

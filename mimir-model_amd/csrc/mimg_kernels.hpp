@@ -247,10 +247,14 @@ hipError_t launch_experts_route(const float* x, const float* router, int64_t T, 
 hipError_t launch_experts_plan(const int32_t* ids, int64_t T, int top, int experts, int32_t* plan, hipStream_t s);
 // Each pair's product with its expert's rows of ws[0] (weights of experts * N
 // rows), or swiglu of its products with ws[0] and ws[1]: y [T * top, N], pairs
-// without an expert left out. a holds T quantized rows, or T * top (per_pair).
+// without an expert left out. x [T, K], or [T * top, K] (per_pair), is quantized
+// into a; parts: rows * K / 8 bytes.
 bool experts_ok(const DevWeight& w);
-hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int64_t T, int top,
-                          bool per_pair, const int32_t* plan, float* y, hipStream_t s);
+hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, void* parts, const float* x,
+                          int64_t T, int top, bool per_pair, const int32_t* plan, float* y, hipStream_t s);
+// The rows as the tiles read them (experts_route.hip).
+hipError_t launch_experts_quantize(uint32_t dt, const float* x, int64_t rows, int64_t K, const ActPtrs& a, void* parts,
+                                   hipStream_t s);
 // The same for few pairs, each its own row (gemv_kquant.hip).
 bool gemv_experts_ok(const DevWeight& w, int experts, bool sw);
 hipError_t launch_gemv_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int pairs,

@@ -15,9 +15,14 @@ namespace mimg {
 // first element e0; all 64 lanes of the wave call it) and returns whether a
 // lane's elements refuse the row (NaN or |x| > 2^60). The chunk's outputs
 // depend on its own elements only.
-template <int BLOCK>
+//
+// OUT: QA_ALL every array of `a`; QA_TILE what the expert tiles read: q, the
+// block's scale once (blocks of 32: each), and QA_TILE_MINS also the sums of
+// 32 as two f16 parts, xs = 64 hi + lo, 8 hi and 8 lo a block of 256 in `parts`.
+enum { QA_ALL = 0, QA_TILE = 1, QA_TILE_MINS = 2 };
+template <int BLOCK, int OUT = QA_ALL>
 __device__ __forceinline__ bool qa_chunk(const float4 v, int64_t row, int64_t e0, int64_t K, const ActPtrs& a,
-                                         int lane) {
+                                         int lane, _Float16* parts = nullptr) {
     const int64_t R32 = K / 32;
     // blocks of 32: K is a multiple of 32, so each group of eight lanes is
     // wholly inside or outside the row (the DPP steps stay in-group)
@@ -57,6 +62,10 @@ __device__ __forceinline__ bool qa_chunk(const float4 v, int64_t row, int64_t e0
     uint32_t packed = (uint32_t)(qv[0] & 0xFF) | ((uint32_t)(qv[1] & 0xFF) << 8) |
                       ((uint32_t)(qv[2] & 0xFF) << 16) | ((uint32_t)(qv[3] & 0xFF) << 24);
     *(uint32_t*)(a.q + row * K + e0) = packed;
+    if constexpr (OUT == QA_TILE) {
+        if ((lane & (BLOCK / 4 - 1)) == 0) a.d32[row * R32 + e0 / 32] = amax / 127.0f;
+        return bbad;
+    }
     int s4 = qv[0] + qv[1] + qv[2] + qv[3];
     // run of 16 = 4 lanes, run of 32 = 8 lanes
     int s16 = s4 + __builtin_amdgcn_mov_dpp(s4, DPP_QUAD_1032, 0xF, 0xF, false);
@@ -64,6 +73,15 @@ __device__ __forceinline__ bool qa_chunk(const float4 v, int64_t row, int64_t e0
     int s32 = s16 + __builtin_amdgcn_mov_dpp(s16, DPP_HALF_MIRROR, 0xF, 0xF, false);
     const float d = amax / 127.0f;
     const int64_t run = e0 / 32;
+    if constexpr (OUT == QA_TILE_MINS) {
+        if (lane == 0) a.d32[row * R32 + run] = d;
+        if ((lane & 7) == 0) {
+            _Float16* p = parts + row * (K / 16) + e0 / 256 * 16 + lane / 8;
+            p[0] = (_Float16)(short)(s32 >> 6);
+            p[8] = (_Float16)(short)(s32 & 63);
+        }
+        return bbad;
+    }
     if ((lane & 3) == 0) a.ys16[row * (K / 16) + e0 / 16] = (int16_t)s16;
     if ((lane & 7) == 0) {
         a.xs[row * R32 + run] = (int16_t)s32;
