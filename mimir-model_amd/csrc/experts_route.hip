@@ -31,7 +31,8 @@ typedef double v4d __attribute__((ext_vector_type(4)));
 // meet in LDS, those of the Z parts in the next kernel.
 constexpr int WAVES = 8;
 
-template <int MT>
+// WHOLE: K is a multiple of 16 (no lane past a row's end in the last run).
+template <int MT, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES) void logits_kernel(const float* __restrict__ x, const float* __restrict__ r,
                                                             int64_t T, int64_t K, int E, double* __restrict__ out) {
     constexpr int N = 16 * MT, U = 4 / MT;  // runs whose loads are in flight together
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(64 * WAVES) void logits_kernel(const float* __restr
         for (int u = 0; u < U; u++) {
             const int64_t c = c0 + (int64_t)u * WAVES;
             if (c >= runs) break;
-            const bool in = 16 * c + 4 * g < K;
+            const bool in = WHOLE || 16 * c + 4 * g < K;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 double xd[MT], rd[MT];
@@ -216,19 +217,10 @@ __global__ __launch_bounds__(256) void select_kernel(const double* __restrict__ 
     if (t < T) select_any(logits + t * E, Z, T * E, E, top, normalize, ids + t * top, weights + t * top);
 }
 
-// Few tokens: their choices and the plan of them by one workgroup.
-constexpr int SMALL_T = 32, SMALL_PAIRS = 512;
-
-__global__ __launch_bounds__(1024) void select_plan_kernel(const double* __restrict__ logits, int Z, int T, int E, int top,
-                                                           int normalize, int32_t* __restrict__ ids, float* __restrict__ weights,
-                                                           int32_t* __restrict__ plan) {
-    __shared__ int chosen[SMALL_PAIRS];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, P = T * top;
-    for (int t = wave; t < T; t += 16) {
-        const int id = select_any(logits + (int64_t)t * E, Z, (int64_t)T * E, E, top, normalize, ids + t * top, weights + t * top);
-        if (lane < top) chosen[t * top + lane] = id;
-    }
-    __syncthreads();
+// The plan of the choices in LDS (P <= SMALL_PAIRS), by a workgroup of 16 waves.
+constexpr int SMALL_PAIRS = 512;
+__device__ __forceinline__ void plan_small(const int* chosen, int P, int E, int32_t* __restrict__ plan) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const PlanLayout l = plan_layout(P, E);
     for (int p = threadIdx.x; p < P; p += 1024) plan[l.expert + p] = chosen[p];
     for (int e = wave; e <= E; e += 16) {
@@ -242,6 +234,81 @@ __global__ __launch_bounds__(1024) void select_plan_kernel(const double* __restr
             at += __popcll(b);
         }
     }
+}
+
+// One to four tokens and a small router: logits, choices and plan in one launch
+// of one workgroup, a wave a part of an expert's row at a time, all tokens
+// against it. One compute unit reads and multiplies slower than many, so only
+// up to 2^15 products (us in a graph, one launch / two: K = 4096, 8 experts, 1
+// token 8.6 / 9.4 and called one by one 10.7 / 14.0, 2 tokens 10.0 / 10.3, 4
+// tokens 13 / 10.3; 1 token, 16 experts 11.2 / 10.5; K = 2048, 64 experts 19 / 12.8).
+constexpr int ONE_T = 4, ONE_PARTS = 512;
+constexpr int64_t ONE_PRODUCTS = 1 << 15;
+
+__global__ __launch_bounds__(1024) void route_one_kernel(const float* __restrict__ x, const float* __restrict__ r, int T, int64_t K,
+                                                         int E, int parts, int top, int normalize, int32_t* __restrict__ ids,
+                                                         float* __restrict__ weights, int32_t* __restrict__ plan) {
+    __shared__ double sums[ONE_T * ONE_PARTS];  // [part][token][expert]
+    __shared__ int chosen[ONE_T * EXPERTS_MAX_TOP];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, P = T * top;
+    const int64_t run = ((K + parts - 1) / parts + 3) / 4 * 4;
+    for (int j = wave; j < E * parts; j += 16) {
+        const int e = j / parts, p = j - e * parts;
+        const int64_t k0 = p * run, k1 = min(k0 + run, K);
+        const float* rr = r + (int64_t)e * K;
+        double acc[ONE_T] = {0.0, 0.0, 0.0, 0.0};
+        constexpr int U = 4;  // float4 of a lane in flight together, and of each token
+        for (int64_t k = k0 + 4 * lane; k - 4 * lane < k1; k += 256 * U) {
+            float4 rv[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) rv[u] = *(const float4*)(rr + min(k + 256 * u, K - 4));
+#pragma unroll
+            for (int t = 0; t < ONE_T; t++) {
+                if (t >= T) break;
+                float4 xv[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) xv[u] = *(const float4*)(x + t * K + min(k + 256 * u, K - 4));
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (k + 256 * u >= k1) continue;
+                    acc[t] = __builtin_fma((double)rv[u].x, (double)xv[u].x, acc[t]);
+                    acc[t] = __builtin_fma((double)rv[u].y, (double)xv[u].y, acc[t]);
+                    acc[t] = __builtin_fma((double)rv[u].z, (double)xv[u].z, acc[t]);
+                    acc[t] = __builtin_fma((double)rv[u].w, (double)xv[u].w, acc[t]);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < ONE_T; t++) {
+            if (t >= T) break;
+            const double s = wave_sum_f64(acc[t]);
+            if (lane == 0) sums[(p * T + t) * E + e] = s;
+        }
+    }
+    __syncthreads();
+    for (int t = wave; t < T; t += 16) {
+        const int id = select_any(sums + t * E, parts, (int64_t)T * E, E, top, normalize, ids + t * top, weights + t * top);
+        if (lane < top) chosen[t * top + lane] = id;
+    }
+    if (plan == nullptr) return;
+    __syncthreads();
+    plan_small(chosen, P, E, plan);
+}
+
+// Few tokens: their choices and the plan of them by one workgroup.
+constexpr int SMALL_T = 32;
+
+__global__ __launch_bounds__(1024) void select_plan_kernel(const double* __restrict__ logits, int Z, int T, int E, int top,
+                                                           int normalize, int32_t* __restrict__ ids, float* __restrict__ weights,
+                                                           int32_t* __restrict__ plan) {
+    __shared__ int chosen[SMALL_PAIRS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, P = T * top;
+    for (int t = wave; t < T; t += 16) {
+        const int id = select_any(logits + (int64_t)t * E, Z, (int64_t)T * E, E, top, normalize, ids + t * top, weights + t * top);
+        if (lane < top) chosen[t * top + lane] = id;
+    }
+    __syncthreads();
+    plan_small(chosen, P, E, plan);
 }
 
 // The plan: workgroup e of E + 1 counts the pairs of the experts below e, which
@@ -392,10 +459,19 @@ uint64_t experts_route_ws_bytes(int64_t T, int experts) {
 
 hipError_t launch_experts_route(const float* x, const float* router, int64_t T, int64_t K, int experts, int top, int normalize,
                                 int32_t* ids, float* weights, int32_t* plan, double* logits, hipStream_t s) {
+    if (T <= xr::ONE_T && T * experts * K <= xr::ONE_PRODUCTS && T * top <= xr::SMALL_PAIRS) {
+        // parts of K that keep 16 waves at work
+        int parts = 1;
+        while (experts * parts < 16 && K / parts >= 512) parts *= 2;
+        hipLaunchKernelGGL(xr::route_one_kernel, dim3(1), dim3(1024), 0, s, x, router, (int)T, K, experts, parts, top, normalize, ids,
+                           weights, plan);
+        return hipGetLastError();
+    }
     const xr::Shape r = xr::route_shape(T, experts);
     const dim3 grid((unsigned)((T + r.n - 1) / r.n), (unsigned)((experts + r.n - 1) / r.n), (unsigned)r.parts), block(64 * xr::WAVES);
-    if (r.n == 32) hipLaunchKernelGGL(xr::logits_kernel<2>, grid, block, 0, s, x, router, T, K, experts, logits);
-    else hipLaunchKernelGGL(xr::logits_kernel<1>, grid, block, 0, s, x, router, T, K, experts, logits);
+    if (r.n == 16) hipLaunchKernelGGL((xr::logits_kernel<1, false>), grid, block, 0, s, x, router, T, K, experts, logits);
+    else if (K % 16) hipLaunchKernelGGL((xr::logits_kernel<2, false>), grid, block, 0, s, x, router, T, K, experts, logits);
+    else hipLaunchKernelGGL((xr::logits_kernel<2, true>), grid, block, 0, s, x, router, T, K, experts, logits);
     if (plan && T <= xr::SMALL_T && T * top <= xr::SMALL_PAIRS) {
         hipLaunchKernelGGL(xr::select_plan_kernel, dim3(1), dim3(1024), 0, s, logits, r.parts, (int)T, experts, top, normalize, ids,
                            weights, plan);

@@ -112,7 +112,8 @@ def check_route(got, x, router, top, normalize):
 @pytest.mark.parametrize("T,k,experts,top", [(1, 4096, 8, 2), (1, 4, 1, 1), (1, 20, 3, 3), (3, 2048, 64, 8), (16, 516, 60, 4),
                                              (17, 1000, 17, 1), (181, 2048, 60, 4), (37, 256, 512, 32), (50, 64, 200, 7),
                                              (33, 4100, 128, 8), (300, 132, 65, 5), (700, 260, 200, 6),
-                                             (32, 512, 40, 16), (1030, 68, 130, 3)])
+                                             (32, 512, 40, 16), (1030, 68, 130, 3),
+                                             (4, 256, 32, 32), (3, 1364, 8, 2), (2, 12, 512, 5), (1, 2052, 15, 4)])
 def test_route(gpu, rt, T, k, experts, top, normalize):
     r = np.random.default_rng(T + 10 * k + experts)
     x, router = r.standard_normal((T, k), np.float32), (r.standard_normal((experts, k)) / np.sqrt(k) * 1.5).astype(np.float32)
