@@ -67,16 +67,20 @@ struct Args {
     const float* x;       // f32 activations (fallback)
 };
 
-template <uint32_t DT, int MT_>
+// AL (Q8_0): rows, and with them groups, start 16-byte aligned.
+template <uint32_t DT, int MT_, bool AL_ = false>
 struct Cfg {
+    static constexpr bool AL = AL_;
     static constexpr int MT = MT_, T = 256, BM = 32 * MT;
     static constexpr bool K32 = DT == DT_Q8_0;
     // A row's group of 256 weights: the 16-byte chunks of its slot. Q6_K and
     // Q8_0 groups are 2-byte aligned: copied from the 16-byte boundary below
     // them, the chunks that cover them and one more where that spreads the
-    // rows' dwords over the banks (60 and 76 dwords a row).
+    // rows' dwords over the banks (60 and 76 dwords a row); aligned Q8_0 groups
+    // are 17 whole chunks (68 dwords).
     static constexpr int GROUP = DT == DT_Q4_K ? Q4K_BYTES : DT == DT_Q6_K ? Q6K_BYTES : 8 * Q80_BYTES;
-    static constexpr int WCH = DT == DT_Q4_K ? 9 : DT == DT_Q6_K ? 15 : 19;
+    static constexpr int WCH = DT == DT_Q4_K ? 9 : DT == DT_Q6_K ? 15 : AL ? 17 : 19;
+    static constexpr int OCC = AL && MT == 1 ? 3 : 2;  // workgroups a compute unit holds
     static constexpr int WSLOT = 16 * WCH;
     static constexpr int WDMA = (32 * WCH + 63) / 64;
     static constexpr int WWAVE = 32 * WSLOT;
@@ -88,7 +92,7 @@ struct Cfg {
     static constexpr int BUF = ABYTES + XBYTES + DBYTES;
     static constexpr int SMEM = WBYTES + 2 * BUF;
     static_assert(ADMA * T == BM * 16 && BM <= (DT == DT_Q4_K ? 64 : 128) && 2 * 64 * BM * 4 <= SMEM, "tile shape");
-    static_assert(2 * SMEM + 16 * BM <= 160 * 1024, "two workgroups a compute unit");
+    static_assert(OCC * (SMEM + 8 * BM + 256) <= 160 * 1024, "workgroups a compute unit");
 };
 
 // s_waitcnt with vmcnt <= N (N < 64), the other counters unconstrained.
@@ -254,7 +258,7 @@ __device__ __forceinline__ uint32_t lds_read2_a2(const uint8_t* p) {
 // A lane's part of its weight row's group: the raw bytes in registers, from
 // which the operands of a k step of 32 are built (lanes g = 0 and 1 of a row
 // hold its elements 16 g .. 16 g + 15).
-template <uint32_t DT>
+template <uint32_t DT, bool AL = false>
 struct Group;
 
 template <>
@@ -330,24 +334,26 @@ struct Group<DT_Q6_K> {
     }
 };
 
-template <>
-struct Group<DT_Q8_0> {
-    // A block's 16 bytes of the lane as the five aligned dwords that hold them.
+template <bool AL>
+struct Group<DT_Q8_0, AL> {
+    // A block's 16 bytes of the lane as the five aligned dwords that hold them
+    // (four where they are aligned).
     u32x4 w[8];
     uint32_t w4[8], sh;  // the first block's misalignment; the next one's is the other
     float d[8];
     __device__ __forceinline__ void read(const uint8_t* wr, int g) {
-        sh = ((uint32_t)(uintptr_t)wr + 2) & 2;
+        sh = AL ? 2 : ((uint32_t)(uintptr_t)wr + 2) & 2;
 #pragma unroll
         for (int ks = 0; ks < 8; ks++) {
             const uint8_t* p = wr + Q80_BYTES * ks;
-            const uint32_t* q = (const uint32_t*)__builtin_align_down(p + 2 + 16 * g, 4);
+            const uint32_t* q = (const uint32_t*)(AL ? p + (ks & 1 ? 2 : 0) + 16 * g : __builtin_align_down(p + 2 + 16 * g, 4));
             w[ks] = u32x4{q[0], q[1], q[2], q[3]};
-            w4[ks] = q[4];
-            d[ks] = f16_to_f32(lds_read2_a2(p));
+            w4[ks] = AL && (ks & 1) ? 0 : q[4];
+            d[ks] = f16_to_f32(AL ? (ks & 1 ? *(const uint32_t*)(p - 2) >> 16 : *(const uint32_t*)p & 0xFFFFu) : lds_read2_a2(p));
         }
     }
     __device__ __forceinline__ v4i block(int ks) const {
+        if (AL && (ks & 1)) return __builtin_bit_cast(v4i, w[ks]);
         const uint32_t s = ks & 1 ? 2 - sh : sh;
         return v4i{(int)__builtin_amdgcn_alignbyte(w[ks].y, w[ks].x, s), (int)__builtin_amdgcn_alignbyte(w[ks].z, w[ks].y, s),
                    (int)__builtin_amdgcn_alignbyte(w[ks].w, w[ks].z, s), (int)__builtin_amdgcn_alignbyte(w4[ks], w[ks].w, s)};
@@ -355,7 +361,7 @@ struct Group<DT_Q8_0> {
 };
 
 template <uint32_t DT, class C, bool SW>
-__global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
+__global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
     constexpr int MT = C::MT, BM = C::BM, BN = SW ? 64 : 128;
     __shared__ __align__(16) uint8_t smem[C::SMEM];  // weights, then two activation stages
     __shared__ int rows[BM], outs[(BM + 63) / 64 * 64], flags[1];
@@ -412,8 +418,8 @@ __global__ __launch_bounds__(C::T, 2) void tile_kernel(Args A) {
         const uint8_t* buf = smem + C::WBYTES + (b & 1) * C::BUF;
         const uint8_t* al = buf + a * 256;
         const uint8_t* ws = smem + C::WWAVE * cp.wave + a * C::WSLOT;
-        if constexpr (DT != DT_Q4_K) ws += (wmis + (uint32_t)b * C::GROUP) & 15u;
-        Group<DT> grp;
+        if constexpr (DT != DT_Q4_K && !C::AL) ws += (wmis + (uint32_t)b * C::GROUP) & 15u;
+        Group<DT, C::AL> grp;
         grp.read(ws, g);
         if (b + 1 < ng) {
             cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
@@ -567,9 +573,9 @@ static int64_t max_tiles(const Args& A, int BM) {
     return (A.pairs + some * (BM - 1)) / BM;
 }
 
-template <uint32_t DT, int MT, bool SW>
+template <uint32_t DT, int MT, bool SW, bool AL = false>
 static hipError_t launch(const Args& A, hipStream_t stream) {
-    using C = Cfg<DT, MT>;
+    using C = Cfg<DT, MT, AL>;
     const int BN = SW ? 64 : 128;
     const int64_t wgs = (max_tiles(A, C::BM) * ((A.N + BN - 1) / BN) + 7) / 8 * 8;
     if (wgs > 0x7fffffff) return hipErrorInvalidValue;
@@ -580,6 +586,9 @@ static hipError_t launch(const Args& A, hipStream_t stream) {
 template <uint32_t DT, bool SW>
 static hipError_t launch_dt(const Args& A, hipStream_t stream) {
     // (64 pairs a workgroup, Q6_K 96, where the experts have as many on average)
+    if constexpr (DT == DT_Q8_0)
+        if (A.rb % 16 == 0 && (uintptr_t)A.mat[0].W % 16 == 0 && (uintptr_t)A.mat[1].W % 16 == 0)
+            return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, 2, SW, true>(A, stream) : launch<DT, 1, SW, true>(A, stream);
     return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, DT == DT_Q6_K ? 3 : 2, SW>(A, stream) : launch<DT, 1, SW>(A, stream);
 }
 
