@@ -82,8 +82,14 @@ struct Cfg {
     static constexpr int WCH = DT == DT_Q4_K ? 9 : DT == DT_Q6_K ? 15 : AL ? 17 : 19;
     static constexpr int OCC = AL && MT == 1 ? 3 : 2;  // workgroups a compute unit holds
     static constexpr int WSLOT = 16 * WCH;
-    static constexpr int WDMA = (32 * WCH + 63) / 64;
-    static constexpr int WWAVE = 32 * WSLOT;
+    // Q4_K: a row's bytes in whole lines of 128, two of them in the slot: a
+    // block (144 bytes, from a multiple of 16 on) lies in two lines, and when it
+    // is in registers at least one of them is free for the next. Block by
+    // block every line that two blocks share would be fetched twice. The
+    // chunks of a line are XOR-swizzled by row.
+    static constexpr bool LINES = DT == DT_Q4_K;
+    static constexpr int WDMA = LINES ? 4 : (32 * WCH + 63) / 64;  // copies of a group, or of a line
+    static constexpr int WWAVE = LINES ? 2 * 4096 : 32 * WSLOT;
     static constexpr int WBYTES = 4 * WWAVE;
     static constexpr int ADMA = BM * 16 / T;
     static constexpr int ABYTES = BM * 256;
@@ -183,7 +189,8 @@ struct Copies {
         wroom = M.W + A.wbytes + WEIGHT_PAD - 16 - wbase;
 #pragma unroll
         for (int i = 0; i < C::WDMA; i++) {
-            const int c = min(64 * i + l, 32 * C::WCH - 1), r = c / C::WCH, j = c - C::WCH * r;
+            const int c = min(64 * i + l, 32 * C::WCH - 1);
+            const int r = C::LINES ? 8 * i + (l >> 3) : c / C::WCH, j = C::LINES ? (l & 7) ^ ((r >> 1) & 7) : c - C::WCH * r;
             const uint32_t o = mis + (uint32_t)max(min(r, A.N - 1 - n0), 0) * (uint32_t)A.rb;
             // (Q6_K: the block's place, rounded down for each block; its chunk
             // is added then)
@@ -211,7 +218,20 @@ struct Copies {
             }
         }
     }
+    // (LINES: line b instead of group b, the last one's end perhaps behind
+    // the row, at most 112 bytes behind the buffer's last)
+    __device__ __forceinline__ void line(int b, uint32_t lds) const {
+#pragma unroll
+        for (int i = 0; i < C::WDMA; i++)
+            lds_copy16_at(wbase + 128 * (int64_t)b, w[i], lds + C::WWAVE * wave + 4096 * (b & 1) + 1024 * i);
+    }
+    // The last line that block b needs.
+    static __device__ __forceinline__ int lines_to(int b) { return (9 * b + 8) >> 3; }
     __device__ __forceinline__ void weights(int b, uint32_t lds) const {
+        if constexpr (C::LINES) {
+            for (int i = b > 0 ? lines_to(b - 1) + 1 : 0; i <= lines_to(b); i++) line(i, lds);
+            return;
+        }
         const int l = threadIdx.x & 63;
         const uint8_t* base = wbase + (DT == DT_Q6_K ? 0 : (int64_t)b * C::GROUP);
         const int64_t room = wroom - (base - wbase);
@@ -266,13 +286,19 @@ struct Group<DT_Q4_K> {
     u32x4 q[4];
     Q4KScales s;
     float d, dmin;
-    __device__ __forceinline__ void read(const uint8_t* wr, int g) {
-        const u32x4 h = *(const u32x4*)wr;
+    // From the lines' slot: row is the lane's row in it with its swizzle.
+    // Chunk c of the row (16 bytes) is at row ^ place(c).
+    static __device__ __forceinline__ uint32_t place(int c) { return (uint32_t)(((c & 8) << 9) | ((c & 7) << 4)); }
+    __device__ __forceinline__ void read(const uint8_t* slot, uint32_t row, int b, int g) {
+        const u32x4 h = *(const u32x4*)(slot + (row ^ place(9 * b)));
         d = f16_to_f32(h.x & 0xFFFFu);
         dmin = f16_to_f32(h.x >> 16);
         s = q4k_scales(h.y, h.z, h.w);
 #pragma unroll
-        for (int c = 0; c < 4; c++) q[c] = *(const u32x4*)(wr + 16 + 32 * c + 16 * g);
+        for (int c = 0; c < 4; c++) {
+            const uint32_t p0 = place(9 * b + 1 + 2 * c), p1 = place(9 * b + 2 + 2 * c);
+            q[c] = *(const u32x4*)(slot + (row ^ (g ? p1 : p0)));
+        }
     }
     __device__ __forceinline__ void planes(int ks, int, v4i& H, v4i& L) const {
         const uint32_t sc = byte_of(s.sc, ks);
@@ -417,10 +443,12 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
         lds_barrier();  // group b's copies have landed, group b - 1's activations are read
         const uint8_t* buf = smem + C::WBYTES + (b & 1) * C::BUF;
         const uint8_t* al = buf + a * 256;
-        const uint8_t* ws = smem + C::WWAVE * cp.wave + a * C::WSLOT;
-        if constexpr (DT != DT_Q4_K && !C::AL) ws += (wmis + (uint32_t)b * C::GROUP) & 15u;
         Group<DT, C::AL> grp;
-        grp.read(ws, g);
+        if constexpr (C::LINES) {
+            grp.read(smem + C::WWAVE * cp.wave, (uint32_t)(128 * a + 16 * ((a >> 1) & 7)), b, g);
+        } else {
+            grp.read(smem + C::WWAVE * cp.wave + a * C::WSLOT + (C::AL ? 0 : (wmis + (uint32_t)b * C::GROUP) & 15u), g);
+        }
         if (b + 1 < ng) {
             cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
             wait_lgkm0();  // the wave's weight slot is read
@@ -431,7 +459,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
             v4i av[MT];
 #pragma unroll
             for (int i = 0; i < MT; i++) av[i] = *(const v4i*)(al + i * 8192 + 16 * asw);
-            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int ks = 0; ks < 8; ks++) {
                 v4i pH, pL, nx[MT];
@@ -448,9 +476,10 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
 #pragma unroll
                 for (int i = 0; i < MT; i++) av[i] = nx[i];
             }
-            // The float step at raised priority: the waves of a SIMD drift
-            // apart, one's MFMAs under the other's vector instructions.
-            __builtin_amdgcn_s_setprio(1);
+            // The products at raised priority, the float step in what they
+            // leave of the vector unit (2048 tokens 2 % faster than the other
+            // way round, and that faster than neither).
+            __builtin_amdgcn_s_setprio(0);
             const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
             v8h bm;
             if constexpr (DT == DT_Q4_K) bm = grp.mins(g);

@@ -246,6 +246,10 @@ SHAPES = [  # dt, experts, n, k, T, top, choices
     (Q8_0, 8, 128, 512, 1, 2, "even"), (Q8_0, 8, 97, 32, 1, 1, "even"), (Q8_0, 4, 70, 736, 5, 2, "even"),
     (Q8_0, 3, 35, 1312, 40, 2, "padded"), (Q8_0, 60, 64, 96, 33, 4, "even"), (Q8_0, 5, 129, 544, 200, 3, "one"),
     (Q8_0, 2, 256, 512, 300, 2, "again"), (Q8_0, 6, 64, 224, 9, 2, "none"),
+    # long rows (whole turns of the slots), tiles of 32 and of 64 and 96 pairs
+    (Q4_K, 3, 64, 2560, 30, 2, "even"), (Q4_K, 2, 40, 4352, 70, 1, "padded"), (Q4_K, 1, 66, 4864, 80, 1, "even"),
+    (Q6_K, 3, 64, 2560, 30, 2, "even"), (Q6_K, 1, 130, 2304, 100, 1, "even"), (Q6_K, 2, 33, 4352, 190, 2, "one"),
+    (Q8_0, 3, 64, 2560, 30, 2, "even"), (Q8_0, 1, 66, 2336, 80, 1, "even"), (Q8_0, 2, 65, 2304, 190, 2, "padded"),
 ]
 
 
