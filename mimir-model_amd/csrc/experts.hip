@@ -623,14 +623,19 @@ static hipError_t launch_dt(const Args& A, hipStream_t stream) {
 
 }  // namespace xp
 
-// Few pairs each run their expert's matrix by themselves (gemv_kquant.hip), an
+// Few pairs each run their expert's matrices by themselves (gemv_kquant.hip), an
 // expert that two of them share twice. Measured on MI355X, us a call with
-// quantizing and sum, alone / in tiles: 4096 x 14336, 8 experts, gate and up
-// (Q4_K) of 2 / 4 / 8 / 16 pairs 29 / 49 / 88 / 160 against 39 / 66 / 98 /
-// 110, down (Q6_K) of 4 / 8 / 16 pairs 46 / 72 / 125 against 111 / 112 / 114;
-// 2048 x 1024, 64 experts, gate and up of 8 / 16 / 32 pairs 11.2 / 16.1 / 26.5
-// against 15.6 / 18.2 / 23.5, down 12.4 / 14.2 / 18.7 against 15.5 / 16.5 / 19.4.
-static bool few_pairs(int pairs, int experts) { return pairs <= 8 || (pairs <= 16 && experts >= 2 * pairs); }
+// quantizing and sum, alone / in tiles: gate and up (Q4_K), 4096 x 14336, 8
+// experts, 2 / 4 / 8 / 16 pairs 29 / 49 / 88 / 160 against 39 / 66 / 98 / 105;
+// 2048 x 1024, 64 experts, 8 / 16 / 32 pairs 11.2 / 16.1 / 26.5 against 15.6 /
+// 18.2 / 23.5.
+static bool few_pairs_swiglu(int pairs, int experts) { return pairs <= 8 || (pairs <= 16 && experts >= 2 * pairs); }
+// down with the sum in its launch, alone / in tiles: 4096 x 14336, 8 experts, 2
+// / 4 / 8 / 16 pairs Q6_K 28 / 45 / 74 / 130 against 111 / 111 / 112 / 113, 12 /
+// 16 pairs Q4_K 66 / 82 against 73 / 74; 2048 x 1024 Q4_K, 64 experts, 8 / 16 /
+// 32 / 64 pairs 8.7 / 10.0 / 13.0 / 19.3 against 15.5 / 16.5 / 19.6 / 24.9; 2048 x
+// 1536 Q6_K, 60 experts, 32 / 48 pairs 27.1 / 35.4 against 29.8 / 35.1.
+static bool few_pairs_combine(int pairs, int experts) { return pairs <= 8 || (pairs <= 64 && experts >= pairs); }
 
 bool experts_ok(const DevWeight& w) {
     const bool k256 = w.dt == DT_Q4_K || w.dt == DT_Q6_K;
@@ -638,16 +643,11 @@ bool experts_ok(const DevWeight& w) {
            w.n <= (1ll << 31) - 1;
 }
 
-hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, void* parts, const float* x,
-                          int64_t T, int top, bool per_pair, const int32_t* plan, float* y, hipStream_t stream) {
+// The tiles' products of ws[0], or swiglu of those of ws[0] and ws[1].
+static hipError_t launch_tiles(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, void* parts, const float* x,
+                               int64_t T, int top, bool per_pair, const int32_t* plan, float* y, hipStream_t stream) {
     const DevWeight& w = *ws[0];
-    const int pairs = (int)(T * top);
-    const int64_t rows = per_pair ? pairs : T;
-    if (few_pairs(pairs, experts) && gemv_experts_ok(w, experts, nmat == 2)) {
-        const hipError_t e = launch_quantize_act(x, rows, w.k, 256, a, stream);
-        if (e != hipSuccess) return e;
-        return launch_gemv_experts(ws, nmat, experts, a, x, pairs, per_pair ? 1 : top, plan + plan_layout(pairs, experts).expert, y, stream);
-    }
+    const int64_t rows = per_pair ? T * top : T;
     const hipError_t e = launch_experts_quantize(w.dt, x, rows, w.k, a, parts, stream);
     if (e != hipSuccess) return e;
     xp::Args A;
@@ -665,7 +665,7 @@ hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, con
     A.N = (int)(w.n / experts);
     A.nb = (int)(w.k / (w.dt == DT_Q8_0 ? 32 : 256));
     A.experts = experts;
-    A.pairs = pairs;
+    A.pairs = (int)(T * top);
     A.rowdiv = per_pair ? 1 : top;
     A.act = a;
     A.x = x;
@@ -677,6 +677,32 @@ hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, con
     if (w.dt == DT_Q4_K) return xp::launch_dt<DT_Q4_K, false>(A, stream);
     if (w.dt == DT_Q6_K) return xp::launch_dt<DT_Q6_K, false>(A, stream);
     return xp::launch_dt<DT_Q8_0, false>(A, stream);
+}
+
+hipError_t launch_experts_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, void* parts,
+                                 const float* x, int64_t T, int top, const int32_t* plan, float* h, hipStream_t stream) {
+    const int pairs = (int)(T * top);
+    if (few_pairs_swiglu(pairs, experts) && gemv_experts_swiglu_ok(gate, experts)) {
+        const hipError_t e = launch_quantize_act(x, T, gate.k, 256, a, stream);
+        if (e != hipSuccess) return e;
+        return launch_gemv_experts_swiglu(gate, up, experts, a, x, T, top, plan + plan_layout(pairs, experts).expert, h, stream);
+    }
+    const DevWeight* ws[2] = {&gate, &up};
+    return launch_tiles(ws, 2, experts, a, parts, x, T, top, false, plan, h, stream);
+}
+
+hipError_t launch_experts_combine(const DevWeight& w, int experts, const ActPtrs& a, void* parts, const float* h,
+                                  const float* weights, int64_t T, int top, const int32_t* plan, float* product, float* y,
+                                  hipStream_t stream) {
+    const int pairs = (int)(T * top);
+    const int32_t* expert = plan + plan_layout(pairs, experts).expert;
+    if (few_pairs_combine(pairs, experts) && gemv_experts_sum_ok(w, experts, top)) {
+        const hipError_t e = launch_quantize_act(h, pairs, w.k, 256, a, stream);
+        return e != hipSuccess ? e : launch_gemv_experts_sum(w, experts, a, h, weights, T, top, expert, y, stream);
+    }
+    const DevWeight* ws[1] = {&w};
+    const hipError_t e = launch_tiles(ws, 1, experts, a, parts, h, T, top, true, plan, product, stream);
+    return e != hipSuccess ? e : launch_experts_sum(product, weights, expert, T, top, w.n / experts, y, stream);
 }
 
 }  // namespace mimg

@@ -1778,8 +1778,8 @@ int mimg_experts_swiglu_a8_dev(uint64_t gate, uint64_t up, int experts, const fl
     const ExpertsLayout l = experts_layout(T, k, 0);
     if (ws_bytes < l.total)
         return fail(MIMG_ERR_WORKSPACE, "experts_swiglu workspace %llu < %llu bytes", (unsigned long long)ws_bytes, (unsigned long long)l.total);
-    const DevWeight* dws[2] = {&g->dw, &u->dw};
-    HIP_TRY(launch_experts(dws, 2, experts, act_ptrs(ws, l.act), (uint8_t*)ws + l.parts, x, T, top, false, (const int32_t*)plan, h, (hipStream_t)stream));
+    HIP_TRY(launch_experts_swiglu(g->dw, u->dw, experts, act_ptrs(ws, l.act), (uint8_t*)ws + l.parts, x, T, top, (const int32_t*)plan,
+                                  h, (hipStream_t)stream));
     return MIMG_OK;
 }
 
@@ -1798,10 +1798,8 @@ int mimg_experts_combine_a8_dev(uint64_t down, int experts, const float* h, cons
     const ExpertsLayout l = experts_layout(P, k, P * n);
     if (ws_bytes < l.total)
         return fail(MIMG_ERR_WORKSPACE, "experts_combine workspace %llu < %llu bytes", (unsigned long long)ws_bytes, (unsigned long long)l.total);
-    float* part = (float*)((uint8_t*)ws + l.product);
-    const DevWeight* dws[1] = {&w->dw};
-    HIP_TRY(launch_experts(dws, 1, experts, act_ptrs(ws, l.act), (uint8_t*)ws + l.parts, h, T, top, true, (const int32_t*)plan, part, (hipStream_t)stream));
-    HIP_TRY(launch_experts_sum(part, weights, (const int32_t*)plan + plan_layout(P, experts).expert, T, top, n, y, (hipStream_t)stream));
+    HIP_TRY(launch_experts_combine(w->dw, experts, act_ptrs(ws, l.act), (uint8_t*)ws + l.parts, h, weights, T, top,
+                                   (const int32_t*)plan, (float*)((uint8_t*)ws + l.product), y, (hipStream_t)stream));
     return MIMG_OK;
 }
 

@@ -245,20 +245,28 @@ uint64_t experts_route_ws_bytes(int64_t T, int experts);
 hipError_t launch_experts_route(const float* x, const float* router, int64_t T, int64_t K, int experts, int top, int normalize,
                                 int32_t* ids, float* weights, int32_t* plan, double* logits, hipStream_t s);
 hipError_t launch_experts_plan(const int32_t* ids, int64_t T, int top, int experts, int32_t* plan, hipStream_t s);
-// Each pair's product with its expert's rows of ws[0] (weights of experts * N
-// rows), or swiglu of its products with ws[0] and ws[1]: y [T * top, N], pairs
-// without an expert left out. x [T, K], or [T * top, K] (per_pair), is quantized
-// into a; parts: rows * K / 8 bytes.
 bool experts_ok(const DevWeight& w);
-hipError_t launch_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, void* parts, const float* x,
-                          int64_t T, int top, bool per_pair, const int32_t* plan, float* y, hipStream_t s);
+// The weighted sum of each token's products (mimg_experts_combine_a8_dev): product
+// [T * top, N] is scratch.
+hipError_t launch_experts_combine(const DevWeight& w, int experts, const ActPtrs& a, void* parts, const float* h,
+                                  const float* weights, int64_t T, int top, const int32_t* plan, float* product, float* y,
+                                  hipStream_t s);
+// swiglu of each pair's products with its expert's rows of gate and up (weights
+// of experts * N rows): h [T * top, N], pairs without an expert left out. x [T, K]
+// is quantized into a; parts: rows * K / 8 bytes.
+hipError_t launch_experts_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, void* parts,
+                                 const float* x, int64_t T, int top, const int32_t* plan, float* h, hipStream_t s);
 // The rows as the tiles read them (experts_route.hip).
 hipError_t launch_experts_quantize(uint32_t dt, const float* x, int64_t rows, int64_t K, const ActPtrs& a, void* parts,
                                    hipStream_t s);
-// The same for few pairs, each its own row (gemv_kquant.hip).
-bool gemv_experts_ok(const DevWeight& w, int experts, bool sw);
-hipError_t launch_gemv_experts(const DevWeight* const* ws, int nmat, int experts, const ActPtrs& a, const float* x, int pairs,
-                               int rowdiv, const int32_t* expert, float* y, hipStream_t s);
+// The same for few pairs, each with a row of workgroups of its own (gemv_kquant.hip).
+bool gemv_experts_swiglu_ok(const DevWeight& w, int experts);
+hipError_t launch_gemv_experts_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, const float* x,
+                                      int64_t T, int top, const int32_t* expert, float* h, hipStream_t s);
+// The products of the pairs with the weighted sum in the same launch.
+bool gemv_experts_sum_ok(const DevWeight& w, int experts, int top);
+hipError_t launch_gemv_experts_sum(const DevWeight& w, int experts, const ActPtrs& a, const float* x, const float* weights,
+                                   int64_t T, int top, const int32_t* expert, float* y, hipStream_t s);
 hipError_t launch_experts_sum(const float* part, const float* weights, const int32_t* expert, int64_t T, int top, int64_t N,
                               float* y, hipStream_t s);
 hipError_t launch_greedy_advance(const int32_t* chosen, int32_t* ids, int64_t* pos, int64_t* cidx, int32_t* out,
