@@ -628,13 +628,18 @@ static hipError_t launch_dt(const Args& A, hipStream_t stream) {
 // quantizing and sum, alone / in tiles: gate and up (Q4_K), 4096 x 14336, 8
 // experts, 2 / 4 / 8 / 16 pairs 29 / 49 / 88 / 160 against 39 / 66 / 98 / 105;
 // 2048 x 1024, 64 experts, 8 / 16 / 32 pairs 11.2 / 16.1 / 26.5 against 15.6 /
-// 18.2 / 23.5.
-static bool few_pairs_swiglu(int pairs, int experts) { return pairs <= 8 || (pairs <= 16 && experts >= 2 * pairs); }
+// 18.2 / 23.5; Q8_0 (experts_q8.hip) 4096 x 7168, 8 experts, 8 pairs 89 against
+// 82, 2048 x 1408, 60 experts, 8 / 16 / 32 pairs 17.1 / 26.5 / 42 against 22.9 /
+// 31.5 / 37.7.
+static bool few_pairs_swiglu(uint32_t dt, int pairs, int experts) {
+    return pairs <= (dt == DT_Q8_0 ? 4 : 8) || (pairs <= 16 && experts >= 2 * pairs);
+}
 // down with the sum in its launch, alone / in tiles: 4096 x 14336, 8 experts, 2
 // / 4 / 8 / 16 pairs Q6_K 28 / 45 / 74 / 130 against 111 / 111 / 112 / 113, 12 /
 // 16 pairs Q4_K 66 / 82 against 73 / 74; 2048 x 1024 Q4_K, 64 experts, 8 / 16 /
 // 32 / 64 pairs 8.7 / 10.0 / 13.0 / 19.3 against 15.5 / 16.5 / 19.6 / 24.9; 2048 x
-// 1536 Q6_K, 60 experts, 32 / 48 pairs 27.1 / 35.4 against 29.8 / 35.1.
+// 1536 Q6_K, 60 experts, 32 / 48 pairs 27.1 / 35.4 against 29.8 / 35.1; Q8_0 2048 x
+// 1408, 60 experts, 16 / 32 / 64 pairs 18.1 / 28.5 / 44.2 against 26.2 / 33.8 / 47.8.
 static bool few_pairs_combine(int pairs, int experts) { return pairs <= 8 || (pairs <= 64 && experts >= pairs); }
 
 bool experts_ok(const DevWeight& w) {
@@ -682,10 +687,15 @@ static hipError_t launch_tiles(const DevWeight* const* ws, int nmat, int experts
 hipError_t launch_experts_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, void* parts,
                                  const float* x, int64_t T, int top, const int32_t* plan, float* h, hipStream_t stream) {
     const int pairs = (int)(T * top);
-    if (few_pairs_swiglu(pairs, experts) && gemv_experts_swiglu_ok(gate, experts)) {
+    if (few_pairs_swiglu(gate.dt, pairs, experts) && gemv_experts_swiglu_ok(gate, experts)) {
         const hipError_t e = launch_quantize_act(x, T, gate.k, 256, a, stream);
         if (e != hipSuccess) return e;
         return launch_gemv_experts_swiglu(gate, up, experts, a, x, T, top, plan + plan_layout(pairs, experts).expert, h, stream);
+    }
+    if (few_pairs_swiglu(gate.dt, pairs, experts) && gemv_experts_q8_ok(gate, 2)) {
+        const hipError_t e = launch_quantize_act(x, T, gate.k, 32, a, stream);
+        if (e != hipSuccess) return e;
+        return launch_gemv_experts_q8_swiglu(gate, up, experts, a, x, T, top, plan + plan_layout(pairs, experts).expert, h, stream);
     }
     const DevWeight* ws[2] = {&gate, &up};
     return launch_tiles(ws, 2, experts, a, parts, x, T, top, false, plan, h, stream);
@@ -699,6 +709,10 @@ hipError_t launch_experts_combine(const DevWeight& w, int experts, const ActPtrs
     if (few_pairs_combine(pairs, experts) && gemv_experts_sum_ok(w, experts, top)) {
         const hipError_t e = launch_quantize_act(h, pairs, w.k, 256, a, stream);
         return e != hipSuccess ? e : launch_gemv_experts_sum(w, experts, a, h, weights, T, top, expert, y, stream);
+    }
+    if (few_pairs_combine(pairs, experts) && gemv_experts_q8_ok(w, top)) {
+        const hipError_t e = launch_quantize_act(h, pairs, w.k, 32, a, stream);
+        return e != hipSuccess ? e : launch_gemv_experts_q8_sum(w, experts, a, h, weights, T, top, expert, y, stream);
     }
     const DevWeight* ws[1] = {&w};
     const hipError_t e = launch_tiles(ws, 1, experts, a, parts, h, T, top, true, plan, product, stream);

@@ -267,6 +267,12 @@ hipError_t launch_gemv_experts_swiglu(const DevWeight& gate, const DevWeight& up
 bool gemv_experts_sum_ok(const DevWeight& w, int experts, int top);
 hipError_t launch_gemv_experts_sum(const DevWeight& w, int experts, const ActPtrs& a, const float* x, const float* weights,
                                    int64_t T, int top, const int32_t* expert, float* y, hipStream_t s);
+// Both for Q8_0 (experts_q8.hip); sets: 2 (gate and up), or top.
+bool gemv_experts_q8_ok(const DevWeight& w, int sets);
+hipError_t launch_gemv_experts_q8_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, const float* x,
+                                         int64_t T, int top, const int32_t* expert, float* h, hipStream_t s);
+hipError_t launch_gemv_experts_q8_sum(const DevWeight& w, int experts, const ActPtrs& a, const float* x, const float* weights,
+                                      int64_t T, int top, const int32_t* expert, float* y, hipStream_t s);
 hipError_t launch_experts_sum(const float* part, const float* weights, const int32_t* expert, int64_t T, int top, int64_t N,
                               float* y, hipStream_t s);
 hipError_t launch_greedy_advance(const int32_t* chosen, int32_t* ids, int64_t* pos, int64_t* cidx, int32_t* out,
