@@ -67,7 +67,8 @@ struct Args {
     const float* x;       // f32 activations (fallback)
 };
 
-// AL (Q8_0): rows, and with them groups, start 16-byte aligned.
+// AL (Q8_0): rows, and with them groups, start 4-byte aligned (K a multiple of
+// 64), as the copies need it.
 template <uint32_t DT, int MT_, bool AL_ = false>
 struct Cfg {
     static constexpr bool AL = AL_;
@@ -184,7 +185,7 @@ struct Copies {
         const int t = threadIdx.x, l = t & 63;
         wave = __builtin_amdgcn_readfirstlane(t >> 6);
         const uint8_t* p = M.W + (row0 + min(n0, A.N - 1)) * A.rb;  // (a wave past the last row: that row)
-        wbase = (const uint8_t*)__builtin_align_down(p, 16);
+        wbase = C::AL ? p : (const uint8_t*)__builtin_align_down(p, 16);
         const uint32_t mis = (uint32_t)(p - wbase);
         wroom = M.W + A.wbytes + WEIGHT_PAD - 16 - wbase;
 #pragma unroll
@@ -194,7 +195,7 @@ struct Copies {
             const uint32_t o = mis + (uint32_t)max(min(r, A.N - 1 - n0), 0) * (uint32_t)A.rb;
             // (Q6_K: the block's place, rounded down for each block; its chunk
             // is added then)
-            w[i] = DT == DT_Q6_K ? o : (o & ~15u) + 16 * j;
+            w[i] = DT == DT_Q6_K ? o : (C::AL ? o : o & ~15u) + 16 * j;
         }
     }
     __device__ __forceinline__ void init_rows(const Args& A, const int* rows) {
@@ -616,7 +617,7 @@ template <uint32_t DT, bool SW>
 static hipError_t launch_dt(const Args& A, hipStream_t stream) {
     // (64 pairs a workgroup, Q6_K 96, where the experts have as many on average)
     if constexpr (DT == DT_Q8_0)
-        if (A.rb % 16 == 0 && (uintptr_t)A.mat[0].W % 16 == 0 && (uintptr_t)A.mat[1].W % 16 == 0)
+        if (A.rb % 4 == 0 && (uintptr_t)A.mat[0].W % 4 == 0 && (uintptr_t)A.mat[1].W % 4 == 0)
             return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, 2, SW, true>(A, stream) : launch<DT, 1, SW, true>(A, stream);
     return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, DT == DT_Q6_K ? 3 : 2, SW>(A, stream) : launch<DT, 1, SW>(A, stream);
 }
@@ -645,7 +646,7 @@ static bool few_pairs_combine(int pairs, int experts) { return pairs <= 8 || (pa
 bool experts_ok(const DevWeight& w) {
     const bool k256 = w.dt == DT_Q4_K || w.dt == DT_Q6_K;
     return (k256 || w.dt == DT_Q8_0) && w.k % (k256 ? 256 : 32) == 0 && (uintptr_t)w.data % (w.dt == DT_Q4_K ? 16 : 2) == 0 &&
-           w.n <= (1ll << 31) - 1;
+           w.n <= (1ll << 31) - 1 && w.row_bytes < (1 << 26);
 }
 
 // The tiles' products of ws[0], or swiglu of those of ws[0] and ws[1].

@@ -26,4 +26,11 @@ __host__ __device__ __forceinline__ PlanLayout plan_layout(int64_t pairs, int ex
     return l;
 }
 
+// A pair's expert as the plan has it, held to the call's own experts: a plan of
+// another call gives wrong results, and no access elsewhere.
+__device__ __forceinline__ int plan_expert(const int32_t* expert, int64_t pair, int experts) {
+    const int e = expert[pair];
+    return e < experts ? e : -1;
+}
+
 }  // namespace mimg

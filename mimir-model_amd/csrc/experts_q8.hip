@@ -30,7 +30,7 @@ constexpr int ROWS = 4;  // of a set
 struct Args {
     const uint8_t *W[2], *wref[2];  // the matrices of all experts (two: gate and up)
     int64_t rb, K;
-    int N, nb, top;                 // nb: blocks of a row
+    int N, nb, top, experts;        // nb: blocks of a row
     const int8_t* q;
     const float* d32;
     const int32_t* ok;
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void gemv_kernel(Args A) {
     uint2* table = (uint2*)smem;                                // [R][nb]: S, d*dx
     int* refused = (int*)(smem + (size_t)R * A.nb * 8);         // [R]
     float* yr = (float*)(refused + R);                          // [R]
-    if (t < sets) chosen[t] = A.expert[SW ? p0 : p0 + t];
+    if (t < sets) chosen[t] = plan_expert(A.expert, SW ? p0 : p0 + t, A.experts);
     __syncthreads();
     if (SW && chosen[0] < 0) return;
     auto matrix_row = [&](int s, int r) {  // row r of set s, in the matrices of all experts
@@ -135,6 +135,7 @@ static Args args(const DevWeight& w, int experts, const ActPtrs& a, const float*
     A.N = (int)(w.n / experts);
     A.nb = (int)(w.k / 32);
     A.top = top;
+    A.experts = experts;
     A.q = a.q;
     A.d32 = a.d32;
     A.ok = a.ok;

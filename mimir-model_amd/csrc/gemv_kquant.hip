@@ -470,9 +470,10 @@ hipError_t launch_gemv_a8k(const DevWeight* const* ws, int nmat, const ActPtrs& 
 // has the matrices of all experts and the rows of the call; a pair's swiglu is
 // one piece (its vector formula: the total a multiple of eight).
 template <uint32_t DT>
-__global__ __launch_bounds__(256) void gemv_experts_swiglu_kernel(GemvArgs A, const int32_t* __restrict__ expert, int top) {
+__global__ __launch_bounds__(256) void gemv_experts_swiglu_kernel(GemvArgs A, const int32_t* __restrict__ expert, int top,
+                                                                  int experts) {
     extern __shared__ __align__(16) uint8_t smem[];
-    const int p = (int)blockIdx.y, e = expert[p];
+    const int p = (int)blockIdx.y, e = plan_expert(expert, p, experts);
     if (e < 0) return;
     const int64_t w0 = (int64_t)e * A.N, row = p / top;
 #pragma unroll
@@ -500,7 +501,7 @@ __global__ __launch_bounds__(256) void gemv_experts_swiglu_kernel(GemvArgs A, co
 // 2048 x 1024 Q4_K 12.4 -> 8.7.
 template <uint32_t DT>
 __global__ __launch_bounds__(256) void gemv_experts_sum_kernel(GemvArgs A, const int32_t* __restrict__ expert,
-                                                               const float* __restrict__ weights, int top) {
+                                                               const float* __restrict__ weights, int top, int experts) {
     constexpr int U = PAIRS_U;
     extern __shared__ __align__(16) uint8_t smem[];
     const int g = threadIdx.x >> 3, l = threadIdx.x & 7, t = threadIdx.x;
@@ -514,7 +515,7 @@ __global__ __launch_bounds__(256) void gemv_experts_sum_kernel(GemvArgs A, const
     __shared__ int chosen[EXPERTS_MAX_TOP];
     // (pairs without an expert run the first one's matrix, and are left out of the sum)
     const int fr = min(t, R - 1), fj = fr / U, frow = min(row0 + fr % U, A.N - 1);
-    const int fe = expert[p0 + fj], okm = A.ok[p0 + fj];
+    const int fe = plan_expert(expert, p0 + fj, experts), okm = A.ok[p0 + fj];
     if (t < R && t % U == 0) chosen[fj] = fe;
     __syncthreads();
     const int wr = A.wref[(int64_t)max(fe, 0) * A.N + frow];
@@ -614,8 +615,8 @@ hipError_t launch_gemv_experts_swiglu(const DevWeight& gate, const DevWeight& up
     constexpr int R = 2 * PAIRS_U;
     const size_t lds = (size_t)R * A.nb * 16 + (size_t)R * 8;
     const dim3 grid((unsigned)(A.N / PAIRS_U), (unsigned)(T * top)), block(256);
-    if (gate.dt == DT_Q4_K) hipLaunchKernelGGL(gemv_experts_swiglu_kernel<DT_Q4_K>, grid, block, lds, stream, A, expert, top);
-    else hipLaunchKernelGGL(gemv_experts_swiglu_kernel<DT_Q6_K>, grid, block, lds, stream, A, expert, top);
+    if (gate.dt == DT_Q4_K) hipLaunchKernelGGL(gemv_experts_swiglu_kernel<DT_Q4_K>, grid, block, lds, stream, A, expert, top, experts);
+    else hipLaunchKernelGGL(gemv_experts_swiglu_kernel<DT_Q6_K>, grid, block, lds, stream, A, expert, top, experts);
     return hipGetLastError();
 }
 
@@ -630,8 +631,10 @@ hipError_t launch_gemv_experts_sum(const DevWeight& w, int experts, const ActPtr
     const int R = PAIRS_U * top;
     const size_t lds = (size_t)R * A.nb * 16 + (size_t)R * 8;
     const dim3 grid((unsigned)((A.N + PAIRS_U - 1) / PAIRS_U), (unsigned)T), block(256);
-    if (w.dt == DT_Q4_K) hipLaunchKernelGGL(gemv_experts_sum_kernel<DT_Q4_K>, grid, block, lds, stream, A, expert, weights, top);
-    else hipLaunchKernelGGL(gemv_experts_sum_kernel<DT_Q6_K>, grid, block, lds, stream, A, expert, weights, top);
+    if (w.dt == DT_Q4_K) hipLaunchKernelGGL(gemv_experts_sum_kernel<DT_Q4_K>, grid, block, lds, stream, A, expert, weights, top,
+                                                experts);
+    else hipLaunchKernelGGL(gemv_experts_sum_kernel<DT_Q6_K>, grid, block, lds, stream, A, expert, weights, top,
+                                                experts);
     return hipGetLastError();
 }
 

@@ -246,6 +246,12 @@ SHAPES = [  # dt, experts, n, k, T, top, choices
     (Q8_0, 8, 128, 512, 1, 2, "even"), (Q8_0, 8, 97, 32, 1, 1, "even"), (Q8_0, 4, 70, 736, 5, 2, "even"),
     (Q8_0, 3, 35, 1312, 40, 2, "padded"), (Q8_0, 60, 64, 96, 33, 4, "even"), (Q8_0, 5, 129, 544, 200, 3, "one"),
     (Q8_0, 2, 256, 512, 300, 2, "again"), (Q8_0, 6, 64, 224, 9, 2, "none"),
+    # few pairs, some without an expert or with one twice; too many choices or
+    # blocks for one workgroup's table
+    (Q4_K, 8, 64, 512, 3, 2, "padded"), (Q4_K, 8, 63, 1024, 4, 2, "again"), (Q4_K, 64, 20, 256, 2, 8, "none"),
+    (Q4_K, 64, 8, 8192, 2, 32, "even"), (Q6_K, 8, 64, 512, 3, 2, "padded"), (Q6_K, 8, 63, 1024, 4, 2, "again"),
+    (Q6_K, 40, 33, 768, 5, 8, "padded"), (Q8_0, 8, 64, 512, 3, 2, "padded"), (Q8_0, 8, 63, 1056, 2, 2, "again"),
+    (Q8_0, 64, 20, 96, 2, 8, "none"), (Q8_0, 16, 9, 8192, 1, 8, "even"), (Q8_0, 40, 33, 800, 5, 8, "padded"),
     # long rows (whole turns of the slots), tiles of 32 and of 64 and 96 pairs
     (Q4_K, 3, 64, 2560, 30, 2, "even"), (Q4_K, 2, 40, 4352, 70, 1, "padded"), (Q4_K, 1, 66, 4864, 80, 1, "even"),
     (Q6_K, 3, 64, 2560, 30, 2, "even"), (Q6_K, 1, 130, 2304, 100, 1, "even"), (Q6_K, 2, 33, 4352, 190, 2, "one"),
@@ -350,6 +356,25 @@ def test_a_pair_does_not_depend_on_the_others(gpu, rt, oracle):
     many = run_swiglu(gpu, rt, gate, up, x, ids).reshape(300, 2, 64)
     for t in (0, 7, 299):
         np.testing.assert_array_equal(bits(run_swiglu(gpu, rt, gate, up, x[t:t + 1], ids[t:t + 1])), bits(many[t]))
+
+
+def test_two_streams_with_workspaces_of_their_own(gpu, rt, oracle):
+    """Calls under way at the same time on two streams, equal bits each time."""
+    gate, up = (Layer(gpu, oracle, Q4_K, 6, 128, 1024, seed) for seed in (50, 51))
+    B, streams, runs = rt.DeviceBuffer, [rt.Stream(), rt.Stream()], []
+    for i, s in enumerate(streams):
+        T = (90, 3)[i]
+        x, ids = acts_for(52 + i, T, 1024), choices(54 + i, T, 2, 6)
+        want = run_swiglu(gpu, rt, gate, up, x, ids)
+        plan, dx, h = B.from_array(ref.packed_plan(ids, 6)), B.from_array(x), B(T * 2 * 128 * 4)
+        wsb = gpu.experts_swiglu_workspace_bytes(T, 2, 128, 1024)
+        runs.append((T, plan, dx, h, B(wsb), wsb, s, want))
+    for _ in range(5):
+        for T, plan, dx, h, ws, wsb, s, _w in runs:
+            gpu.experts_swiglu_a8_dev(gate.w, up.w, 6, dx.ptr, T, 2, plan.ptr, plan.nbytes, h.ptr, ws.ptr, wsb, s.handle)
+    for T, plan, dx, h, ws, wsb, s, want in runs:
+        s.sync()
+        np.testing.assert_array_equal(bits(h.download(np.float32).reshape(T * 2, 128)), bits(want))
 
 
 def test_a_layer_captured_and_replayed(gpu, rt, oracle):
