@@ -12,24 +12,32 @@
 // dequant_matmul_a8.v2 (block 256), and for Q8_0 what the tiled product with
 // blocks of 32 gives, whatever else the call holds.
 //
-// Layout. A workgroup of four waves takes BM = 32 or 64 pairs of one expert
-// against 128 weight rows (32 a wave), or with swiglu against 64 rows of gate
-// and the same 64 of up. The integer products are v_mfma_i32_32x32x32_i8: the
-// activations are the row operand, the weights the column operand (lane l holds
-// weight row l % 32), so a lane needs one block scale. A wave's raw blocks lie
-// in an LDS slot of its own (read into registers, then overwritten by the
-// next block's copies), the pairs' int8 rows (16-byte chunks XOR-swizzled by
-// row) and scales in two shared stages; all of it by global_load_lds, one
-// barrier a block. sc*q of Q4_K is split in two int8 planes, sc = 8 sh + sl, its
-// mins are one v_mfma_f32_32x32x16_f16 over xs = 64 hi + lo (every operand and
-// partial sum an integer that f16 and f32 hold exactly), as in gemm_q4k.hip;
-// sc*(q - 32) of Q6_K is 256 hi + lo.
+// Layout. A workgroup of four waves takes BM = 32, 64 or (Q6_K) 96 pairs of one
+// expert against 128 weight rows (32 a wave), or with swiglu against 64 rows of
+// gate and the same 64 of up. The integer products are v_mfma_i32_32x32x32_i8:
+// the activations are the row operand, the weights the column operand (lane l
+// holds weight row l % 32), so a lane needs one block scale. A wave's raw blocks
+// lie in an LDS slot of its own (read into registers, then overwritten by the
+// next block's copies; Q4_K by whole lines of 128 bytes, two a row), the pairs'
+// int8 rows (16-byte chunks XOR-swizzled by row) and scales in two shared stages;
+// all of it by global_load_lds, one barrier a block. sc*q of Q4_K is split in
+// two int8 planes, sc = 8 sh + sl, its mins are one v_mfma_f32_32x32x16_f16 over
+// xs = 64 hi + lo (every operand and partial sum an integer that f16 and f32 hold
+// exactly), as in gemm_q4k.hip; sc*(q - 32) of Q6_K is 256 hi + lo.
 //
 // Which workgroup has which tile is decided on the device: the grid is as
 // large as any choice of that many pairs could need, a wave adds up the
 // experts' tiles from the plan, and what is past the last tile ends. The tiles
-// are in order by expert, row tile, pairs, dealt to the XCDs in eight runs, so
+// are in order by expert, weight rows, pairs, dealt to the XCDs in eight runs, so
 // that the tiles that share weights meet in one L2.
+//
+// Bounds. Few pairs an expert: the weights' way into LDS. 64 tokens, two of 8
+// experts, 4096 x 14336 Q4_K gate and up 118 us: 537 MB at 4.6 TB/s, where the
+// copies alone take 108 to 117 us and the instructions alone 100; 181 tokens, four of
+// 60, 2048 x 1408 Q8_0 81 us: 373 MB at 4.6 TB/s. Many: vector instructions beside
+// the matrix cores. 2048 tokens, two of 8: gate and up 1250 us, 0.77 POP/s of
+// products and 1.54 of the planes' (the matrix cores at work 46 % of the cycles,
+// vector instructions 65 %), down 4096 x 14336 Q6_K 705 us, 0.68 and 1.37 POP/s.
 //
 // Rows of x the quantizer refused and weight rows with a non-finite block
 // scale take the float32 path (f32path.hpp) at the end.
@@ -608,7 +616,7 @@ static hipError_t launch(const Args& A, hipStream_t stream) {
     using C = Cfg<DT, MT, AL>;
     const int BN = SW ? 64 : 128;
     const int64_t wgs = (max_tiles(A, C::BM) * ((A.N + BN - 1) / BN) + 7) / 8 * 8;
-    if (wgs > 0x7fffffff) return hipErrorInvalidValue;
+    if (wgs * C::T >= (1ll << 32)) return hipErrorInvalidValue;  // (275 GB of results)
     hipLaunchKernelGGL((tile_kernel<DT, C, SW>), dim3((unsigned)wgs), dim3(C::T), 0, stream, A);
     return hipGetLastError();
 }

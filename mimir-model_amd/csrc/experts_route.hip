@@ -11,8 +11,10 @@
 // to float32 a token whose experts are nearly alike would go to another one
 // whenever the order of the sum changes (with the batch, say). Products of two
 // float32 are exact in float64 and their sum is kept there, on
-// v_mfma_f64_16x16x4: 2 T E K operations, where reading x and r takes about
-// as long (2048 tokens, 128 experts, K = 4096).
+// v_mfma_f64_16x16x4: 2 T E K operations, which bound it for many tokens (2048
+// of 128 experts, K = 4096: 30 us at the rate a float64 product reaches, x and r
+// are read in 5; the logits take 42, choices 6 and plan 9). Few tokens are
+// bound by launches (181 of 60 experts, K = 2048: 5 + 5 + 3 us).
 #include "decoder_math.hpp"
 #include "experts.hpp"
 #include "mimg_device.hpp"
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(PLAN_T) void plan_kernel(const int32_t* __restrict_
 // The quantizer of the tiles' activations: a row by one workgroup, CPW chunks
 // of 256 a wave with their loads in flight together, only what the tiles read
 // (q, scales, Q4_K's sums in the form of its f16 operand, ok): 4096 rows of
-// 14336 take 55 us against 84 with every array of the other products.
+// 14336 take 74 us (4.0 TB/s) against 84 with every array of the other products.
 template <int BLOCK, int OUT, int CPW>
 __global__ __launch_bounds__(1024) void quantize_kernel(const float* __restrict__ x, int64_t K, ActPtrs a, _Float16* parts) {
     const int64_t row = blockIdx.x, nch = (K + 255) / 256;
@@ -487,7 +489,8 @@ namespace xr {
 template <int BLOCK, int OUT>
 static void launch_quantize(const float* x, int64_t rows, int64_t K, const ActPtrs& a, _Float16* parts, hipStream_t s) {
     const int64_t chunks = (K + 255) / 256;
-    const int waves = (int)(chunks < 16 ? chunks : 16);
+    int waves = (int)(chunks < 16 ? chunks : 16);
+    while (waves > 1 && rows * 64 * waves >= (1ll << 32)) waves /= 2;  // (a launch has less than 2^32 threads)
     const int64_t cpw = (chunks + waves - 1) / waves;
     const dim3 grid((unsigned)rows), block(64 * waves);
     if (cpw == 1) hipLaunchKernelGGL((quantize_kernel<BLOCK, OUT, 1>), grid, block, 0, s, x, K, a, parts);

@@ -442,3 +442,29 @@ def test_product_refusals(gpu, rt, oracle):
     assert swiglu(u=wide) == -1
     assert swiglu(u=six) == 1 and swiglu(g=b32) == 1  # not handled: two dtypes
     assert L.mimg_experts_swiglu_a8_dev(gate.w.handle, 1 << 40, 4, x.ptr, 6, 2, plan.ptr, nb, h.ptr, ws.ptr, 1 << 20, None) == -4
+
+
+def test_most_pairs(gpu, rt, oracle):
+    """2^24 pairs of 1024 values (a launch of as many workgroups, 64 GiB): the
+    same 2^18 over and over, each result as the one of these alone."""
+    T, top, k, some = 1 << 20, 16, 1024, 1 << 14
+    down = Layer(gpu, oracle, Q4_K, 16, 4, k, 50)
+    ids = np.tile(choices(51, 64, top, 16), (some // 64, 1))
+    weights = np.random.default_rng(52).random((some, top), np.float32)
+    h = np.random.default_rng(53).standard_normal((some * top, k), np.float32)
+    want = run_combine(gpu, rt, down, h, weights, ids)
+    s, nb, wsb = rt.Stream(), gpu.experts_plan_bytes(T, top, 16), gpu.experts_combine_workspace_bytes(T, top, 4, k)
+    dh, dw, di = rt.DeviceBuffer(T * top * k * 4), rt.DeviceBuffer(T * top * 4), rt.DeviceBuffer(T * top * 4)
+    for b, a in ((dh, h), (dw, weights), (di, ids)):
+        b.upload(a)
+        at = a.nbytes
+        while at < b.nbytes:
+            rt.copy_async(b.ptr + at, b.ptr, at, s)
+            at *= 2
+    s.sync()
+    plan, ws, y = rt.DeviceBuffer(nb), rt.DeviceBuffer(wsb), rt.DeviceBuffer(T * 16)
+    gpu.experts_plan_dev(di.ptr, T, top, 16, plan.ptr, nb, s.handle)
+    gpu.experts_combine_a8_dev(down.w, 16, dh.ptr, dw.ptr, T, top, plan.ptr, nb, y.ptr, ws.ptr, wsb, s.handle)
+    s.sync()
+    got = y.download(np.float32).reshape(T // some, some, 4)
+    assert (bits(got) == bits(want)[None]).all()
