@@ -638,7 +638,8 @@ int mimg_experts_plan_dev(const int32_t *ids, int64_t T, int top, int experts, v
  * top] = exp(logit - m) / sum exp(logit - m), m the largest, the sum over the
  * chosen (normalize != 0) or over all experts; NaN where that formula gives it.
  * plan (may be NULL): the plan of ids. k a multiple of 4, x and router 16-byte
- * aligned. ws: mimg_experts_route_workspace_bytes, 256-byte aligned. */
+ * aligned. ws: mimg_experts_route_workspace_bytes, 256-byte aligned (as those
+ * below, that of the most tokens is enough for fewer). */
 uint64_t mimg_experts_route_workspace_bytes(int64_t T, int experts);
 int mimg_experts_route_dev(const float *x, const float *router, int64_t T, int64_t k, int experts, int top, int normalize,
                            int32_t *ids, float *weights, void *plan, uint64_t plan_bytes, void *ws, uint64_t ws_bytes,

@@ -13,8 +13,8 @@
 // float32 are exact in float64 and their sum is kept there, on
 // v_mfma_f64_16x16x4: 2 T E K operations, which bound it for many tokens (2048
 // of 128 experts, K = 4096: 30 us at the rate a float64 product reaches, x and r
-// are read in 5; the logits take 42, choices 6 and plan 9). Few tokens are
-// bound by launches (181 of 60 experts, K = 2048: 5 + 5 + 3 us).
+// are read in 5; the logits take 39, choices 5 and plan 9). Few tokens are
+// bound by launches (181 of 60 experts, K = 2048: 5.2, 3.5 and 2.8 us).
 #include "decoder_math.hpp"
 #include "experts.hpp"
 #include "mimg_device.hpp"
@@ -133,30 +133,20 @@ __device__ __forceinline__ int64_t order_key(double v) {
     const int64_t b = __double_as_longlong(v + 0.0);
     return b < 0 ? b ^ INT64_MAX : b;
 }
-template <int M>
-__device__ __forceinline__ int64_t max_xor_i64(int64_t v) {
-    const int lo = lane_xor<M>((int)(v & 0xFFFFFFFFll)), hi = lane_xor<M>((int)(v >> 32));
-    const int64_t o = ((int64_t)hi << 32) | (int64_t)(uint32_t)lo;
-    return o > v ? o : v;
-}
-__device__ __forceinline__ int64_t wave_max_i64(int64_t v) {
-    v = max_xor_i64<32>(v);
-    v = max_xor_i64<16>(v);
-    v = max_xor_i64<8>(v);
-    v = max_xor_i64<4>(v);
-    v = max_xor_i64<2>(v);
-    return max_xor_i64<1>(v);
-}
-__device__ __forceinline__ int wave_min_i32(int v) {
-    v = min(v, __shfl_xor(v, 32));
-    v = min(v, lane_xor<16>(v));
-    v = min(v, lane_xor<8>(v));
-    v = min(v, lane_xor<4>(v));
-    v = min(v, lane_xor<2>(v));
-    return min(v, lane_xor<1>(v));
+// The wave's largest value, in every lane: within rows of 16 lanes (shifts by 1,
+// 2, 4, 8), each row's last lane into the rows behind it, the last lane to all.
+__device__ __forceinline__ int wave_max_last(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xF, 0xF, false));  // row_shr:1
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
-// One token's choices by one wave: lane l holds the logits of the experts l,
+// One token's choices by one wave (a choice by ballots and maxima of 32 bits: eight
+// of 64 experts 2.9 us less than by maxima of 64 bits through all lanes): lane l holds the logits of the experts l,
 // l + 64, ..., each the sum of Z parts `stride` apart. Lane j < top returns
 // choice j.
 template <int PER>
@@ -166,29 +156,57 @@ __device__ __forceinline__ int select(const double* logits, int Z, int64_t strid
     double v[PER];
     int64_t key[PER];
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = lane + 64 * i;
-        v[i] = 0.0;
-        for (int z = 0; z < Z; z++) v[i] += e < E ? logits[z * stride + e] : 0.0;
-        key[i] = e < E ? order_key(v[i]) : KEY_TAKEN;
+    for (int i = 0; i < PER; i++) v[i] = 0.0;
+    constexpr int ZU = PER <= 2 ? 8 : 2;  // parts whose loads are in flight together
+    for (int z = 0; z < Z; z += ZU) {
+        double p[ZU][PER];
+#pragma unroll
+        for (int u = 0; u < ZU; u++)
+#pragma unroll
+            for (int i = 0; i < PER; i++) p[u][i] = logits[min(z + u, Z - 1) * stride + min(lane + 64 * i, E - 1)];
+#pragma unroll
+        for (int u = 0; u < ZU; u++)
+#pragma unroll
+            for (int i = 0; i < PER; i++) v[i] += z + u < Z ? p[u][i] : 0.0;
     }
+#pragma unroll
+    for (int i = 0; i < PER; i++) key[i] = lane + 64 * i < E ? order_key(v[i]) : KEY_TAKEN;
     double m = 0.0, mine = 0.0;  // the largest; the value of choice `lane`
     int id = 0;
     for (int j = 0; j < top; j++) {
         int64_t b = key[0];
         int at = 0;
+        double bv = v[0];
 #pragma unroll
         for (int i = 1; i < PER; i++)
-            if (key[i] > b) b = key[i], at = i;
-        const int64_t best = wave_max_i64(b);
-        const int e = wave_min_i32(b == best ? lane + 64 * at : INT32_MAX);
-        double mv = 0.0;
+            if (key[i] > b) b = key[i], at = i, bv = v[i];
+        // the keys' upper halves, and their lower ones where lanes share it (as
+        // signed numbers of the same order)
+        const int hi = (int)(b >> 32), lo = (int)((uint32_t)b ^ 0x80000000u), best = wave_max_last(hi);
+        uint64_t in = __ballot(hi == best);
+        if (in & (in - 1)) {
+            const int bl = wave_max_last(hi == best ? lo : INT32_MIN);
+            in = __ballot(hi == best && lo == bl);
+        }
+        // of equal ones the lowest index
+        uint64_t first = in;
+        int slot = 0;
+        if constexpr (PER > 1) {
+#pragma unroll
+            for (int i = PER - 1; i >= 0; i--) {
+                const uint64_t here = __ballot(at == i) & in;
+                if (here) first = here, slot = i;
+            }
+        }
+        const int l = __ffsll((unsigned long long)first) - 1;
 #pragma unroll
         for (int i = 0; i < PER; i++)
-            if (lane + 64 * i == e) key[i] = KEY_TAKEN, mv = v[i];
-        const double bv = __shfl(mv, e & 63);
+            if (lane == l && slot == i) key[i] = KEY_TAKEN;
+        const int64_t bits = __double_as_longlong(bv);
+        const int bh = __builtin_amdgcn_readlane((int)(bits >> 32), l), bl = __builtin_amdgcn_readlane((int)bits, l);
+        bv = __longlong_as_double((int64_t)((uint64_t)(uint32_t)bh << 32 | (uint32_t)bl));
         if (j == 0) m = bv;
-        if (lane == j) mine = bv, id = e;
+        if (lane == j) mine = bv, id = 64 * slot + l;
     }
     double sum = 0.0;
     if (normalize) {
@@ -221,29 +239,41 @@ __global__ __launch_bounds__(256) void select_kernel(const double* __restrict__ 
 
 // The plan of the choices in LDS (P <= SMALL_PAIRS), by a workgroup of 16 waves.
 constexpr int SMALL_PAIRS = 512;
-__device__ __forceinline__ void plan_small(const int* chosen, int P, int E, int32_t* __restrict__ plan) {
+template <int N>  // P <= 64 N
+__device__ __forceinline__ void plan_held(const int* chosen, int P, int E, int32_t* __restrict__ plan) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const PlanLayout l = plan_layout(P, E);
     for (int p = threadIdx.x; p < P; p += 1024) plan[l.expert + p] = chosen[p];
+    int id[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) id[i] = 64 * i + lane < P ? chosen[64 * i + lane] : INT32_MAX;
     for (int e = wave; e <= E; e += 16) {
         int at = 0;
-        for (int p = lane; p - lane < P; p += 64) at += __popcll(__ballot(p < P && chosen[min(p, P - 1)] < e));
+#pragma unroll
+        for (int i = 0; i < N; i++) at += 64 * i < P ? __popcll(__ballot(id[i] < e)) : 0;
         if (lane == 0) plan[e] = at;
-        for (int p = lane; p - lane < P; p += 64) {
-            const bool mine = p < P && chosen[min(p, P - 1)] == e;
-            const uint64_t b = __ballot(mine);
-            if (mine) plan[l.order + at + __popcll(b & ((1ull << lane) - 1))] = p;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (64 * i >= P) break;
+            const uint64_t b = __ballot(id[i] == e);
+            if (id[i] == e) plan[l.order + at + __popcll(b & ((1ull << lane) - 1))] = 64 * i + lane;
             at += __popcll(b);
         }
     }
+}
+
+__device__ __forceinline__ void plan_small(const int* chosen, int P, int E, int32_t* __restrict__ plan) {
+    if (P <= 64) return plan_held<1>(chosen, P, E, plan);
+    plan_held<SMALL_PAIRS / 64>(chosen, P, E, plan);
 }
 
 // One to four tokens and a small router: logits, choices and plan in one launch
 // of one workgroup, a wave a part of an expert's row at a time, all tokens
 // against it. One compute unit reads and multiplies slower than many, so only
 // up to 2^15 products (us in a graph, one launch / two: K = 4096, 8 experts, 1
-// token 8.6 / 9.4 and called one by one 10.7 / 14.0, 2 tokens 10.0 / 10.3, 4
-// tokens 13 / 10.3; 1 token, 16 experts 11.2 / 10.5; K = 2048, 64 experts 19 / 12.8).
+// token 5.9 / 6.6, called one by one 3 less, 2 tokens 7.4 / 6.9, 4 tokens 9.7 / 6.9;
+// 1 token, 16 experts 8.1 / 6.7; K = 1024, 32 experts 6.8 / 6.5; K = 2048, 64 experts
+// 14.5 / 7.4).
 constexpr int ONE_T = 4, ONE_PARTS = 512;
 constexpr int64_t ONE_PRODUCTS = 1 << 15;
 
@@ -297,8 +327,11 @@ __global__ __launch_bounds__(1024) void route_one_kernel(const float* __restrict
     plan_small(chosen, P, E, plan);
 }
 
-// Few tokens: their choices and the plan of them by one workgroup.
-constexpr int SMALL_T = 32;
+// Few tokens and a small router: choices and plan by one workgroup, a wave a token
+// (us in a graph, so / in a launch each: K = 4096, 8 experts, 8 tokens 7.3 / 9.0, 16
+// tokens 8.5 / 9.2, with two tokens a wave 32 tokens 11.4 / 9.4; 64 experts, 8 tokens
+// 8.9 / 9.8, 16 tokens 11.6 / 10.1; K = 2048, 128 experts, 8 tokens 12.2 / 10.8).
+constexpr int SMALL_T = 16, SMALL_LOGITS = 512;
 
 __global__ __launch_bounds__(1024) void select_plan_kernel(const double* __restrict__ logits, int Z, int T, int E, int top,
                                                            int normalize, int32_t* __restrict__ ids, float* __restrict__ weights,
@@ -355,15 +388,16 @@ __global__ __launch_bounds__(PLAN_T) void plan_kernel(const int32_t* __restrict_
 #pragma unroll
     for (int w = 0; w < W; w++) at += below[w];
     if (threadIdx.x == 0) plan[e] = at;  // e = E: the pairs that have one
+    for (int p = e * PLAN_T + (int)threadIdx.x; p < P; p += (E + 1) * PLAN_T) {  // pairs' experts: a share of them all
+        const int id = expert_of(ids[p], E);
+        plan[l.expert + p] = id < E ? id : -1;
+    }
     for (int w = 0; w < wave; w++) at += equal[w];
     if (ne == 0) return;
-    int32_t *order = plan + l.order, *expert = plan + l.expert;
+    int32_t* order = plan + l.order;
     auto place = [&](int i, int id) {
         const uint64_t b = __ballot(id == e);
-        if (id == e) {
-            order[at + __popcll(b & ((1ull << lane) - 1))] = p0 + 64 * i + lane;
-            expert[p0 + 64 * i + lane] = e < E ? e : -1;
-        }
+        if (id == e) order[at + __popcll(b & ((1ull << lane) - 1))] = p0 + 64 * i + lane;
         at += __popcll(b);
     };
     if constexpr (HOLD > 0) {
@@ -442,21 +476,27 @@ hipError_t launch_experts_plan(const int32_t* ids, int64_t T, int top, int exper
 
 namespace xr {
 // 32 x 32 tiles, which read x and r half as often from the L2, where they
-// give at least 128 workgroups; 16 x 16 below. Parts of K so that there are about as many
-// workgroups as compute units.
+// give at least 128 workgroups; 16 x 16 below. Parts of K so that a compute unit
+// has one workgroup, of the small tiles one or two (us in a graph with one / two:
+// K = 4096, 8 experts, 2048 tokens 23.6 / 19.2, 1024 13.9 / 13.0, 512 11.1 / 11.2;
+// K = 2048, 128 experts, 181 tokens 15.2 / 14.6; of the large ones 60 experts, 2048
+// tokens 24.2 / 26.0).
 struct Shape {
     int n, parts;
 };
 static Shape route_shape(int64_t T, int experts) {
     const int64_t t32 = (T + 31) / 32 * ((experts + 31) / 32), t16 = (T + 15) / 16 * ((experts + 15) / 16);
     Shape r{t32 >= 128 ? 32 : 16, 1};
-    for (const int64_t tiles = r.n == 32 ? t32 : t16; r.parts < 16 && tiles * r.parts * 2 <= 256;) r.parts *= 2;
+    for (const int64_t tiles = r.n == 32 ? t32 : t16; r.parts < 16 && tiles * r.parts * 2 <= (r.n == 32 ? 256 : 512);) r.parts *= 2;
     return r;
 }
 }  // namespace xr
 
+// More tokens never need less: parts beyond one are of at most 512 small or 256
+// large tiles, 2^18 sums.
 uint64_t experts_route_ws_bytes(int64_t T, int experts) {
-    return (uint64_t)T * experts * 8 * xr::route_shape(T, experts).parts;
+    const int64_t n = T * experts, parted = 16 * n < (1 << 18) ? 16 * n : 1 << 18;
+    return 8 * (uint64_t)(n > parted ? n : parted);
 }
 
 hipError_t launch_experts_route(const float* x, const float* router, int64_t T, int64_t K, int experts, int top, int normalize,
@@ -474,7 +514,7 @@ hipError_t launch_experts_route(const float* x, const float* router, int64_t T, 
     if (r.n == 16) hipLaunchKernelGGL((xr::logits_kernel<1, false>), grid, block, 0, s, x, router, T, K, experts, logits);
     else if (K % 16) hipLaunchKernelGGL((xr::logits_kernel<2, false>), grid, block, 0, s, x, router, T, K, experts, logits);
     else hipLaunchKernelGGL((xr::logits_kernel<2, true>), grid, block, 0, s, x, router, T, K, experts, logits);
-    if (plan && T <= xr::SMALL_T && T * top <= xr::SMALL_PAIRS) {
+    if (plan && T <= xr::SMALL_T && T * experts <= xr::SMALL_LOGITS && T * top <= xr::SMALL_PAIRS) {
         hipLaunchKernelGGL(xr::select_plan_kernel, dim3(1), dim3(1024), 0, s, logits, r.parts, (int)T, experts, top, normalize, ids,
                            weights, plan);
         return hipGetLastError();

@@ -32,6 +32,15 @@ def test_plan_bytes(lib):
         assert f(*bad) == 0, bad
 
 
+def test_workspace_bytes_of_more_tokens_are_enough_for_fewer(lib):
+    for f in (lambda t: lib.mimg_experts_route_workspace_bytes(t, 8), lambda t: lib.mimg_experts_route_workspace_bytes(t, 60),
+              lambda t: lib.mimg_experts_route_workspace_bytes(t, 512), lambda t: lib.mimg_experts_plan_bytes(t, 2, 8),
+              lambda t: lib.mimg_experts_swiglu_workspace_bytes(t, 2, 100, 512),
+              lambda t: lib.mimg_experts_combine_workspace_bytes(t, 2, 100, 512)):
+        n = [f(t) for t in range(1, 5000)]
+        assert n == sorted(n)
+
+
 def test_workspace_bytes(lib):
     a8 = lib.mimg_a8_workspace_bytes
     assert lib.mimg_experts_route_workspace_bytes(7, 60) >= 7 * 60 * 8

@@ -129,6 +129,30 @@ def test_route_equal_logits_go_by_the_index(gpu, rt):
     check_route(run_route(gpu, rt, x, router, 12, True), x, router, 12, True)
 
 
+# a token a wave of one workgroup, a plan of more than 64 pairs there; parts of K
+# that do not fill the loads of eight; the lower halves of equal upper ones
+@pytest.mark.parametrize("T,k,experts,top", [(16, 2300, 32, 20), (16, 4096, 32, 4), (8, 3000, 64, 32), (5, 4096, 100, 9), (17, 2048, 30, 6),
+                                             (600, 1040, 8, 2), (64, 1024, 300, 3)])
+def test_route_in_parts(gpu, rt, T, k, experts, top):
+    r = np.random.default_rng(T + k)
+    x, router = r.standard_normal((T, k), np.float32), (r.standard_normal((experts, k)) / np.sqrt(k)).astype(np.float32)
+    check_route(run_route(gpu, rt, x, router, top, True), x, router, top, True)
+
+
+@pytest.mark.parametrize("T,experts", [(2, 70), (40, 70), (40, 200), (40, 500)])
+def test_route_equal_and_close_logits(gpu, rt, T, experts):
+    """Logits 1 + 2^-40 i, exact sums of two products: equal upper halves in
+    many lanes and slots; every third one equal to the one before it."""
+    x = np.zeros((T, 4), np.float32)
+    x[:, 0], x[:, 1] = 1, 2.0 ** -40
+    x[1] *= -1
+    router = np.zeros((experts, 4), np.float32)
+    router[:, 0] = 1
+    router[:, 1] = np.random.default_rng(experts).permutation(experts)
+    router[2::3, 1] = router[1::3, 1][:len(router[2::3])]
+    check_route(run_route(gpu, rt, x, router, 20, True), x, router, 20, True)
+
+
 @pytest.mark.parametrize("experts", [9, 100])
 def test_route_of_values_that_are_not_finite(gpu, rt, experts):
     r = np.random.default_rng(6)
