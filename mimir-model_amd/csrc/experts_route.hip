@@ -13,7 +13,7 @@
 // float32 are exact in float64 and their sum is kept there, on
 // v_mfma_f64_16x16x4: 2 T E K operations, which bound it for many tokens (2048
 // of 128 experts, K = 4096: 30 us at the rate a float64 product reaches, x and r
-// are read in 5; the logits take 39, choices 5 and plan 9). Few tokens are
+// are read in 5; the logits take 39 to 42, choices 5 and plan 5). Few tokens are
 // bound by launches (181 of 60 experts, K = 2048: 5.2, 3.5 and 2.8 us).
 #include "decoder_math.hpp"
 #include "experts.hpp"
@@ -356,31 +356,31 @@ constexpr int PLAN_T = 1024;
 __device__ __forceinline__ int expert_of(int id, int E) { return id >= 0 && id < E ? id : E; }
 
 // HOLD: the ids of a wave's run stay in registers between the two passes
-// (P <= HOLD * PLAN_T), 0: they are read again.
+// (P <= HOLD * PLAN_T), 0: they are read again, eight in flight together. (Read
+// one by one 16384 pairs of 128 experts took 8.9 us, so 4.8.)
 template <int HOLD>
 __global__ __launch_bounds__(PLAN_T) void plan_kernel(const int32_t* __restrict__ ids, int P, int E, int32_t* __restrict__ plan) {
-    constexpr int W = PLAN_T / 64;
+    constexpr int W = PLAN_T / 64, U = HOLD ? HOLD : 8;
     __shared__ int below[W], equal[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = (int)blockIdx.x;
     const PlanLayout l = plan_layout(P, E);
     const int n = (P + PLAN_T - 1) / PLAN_T;  // 64s of pairs of a wave
     const int p0 = min(wave * n * 64, P), p1 = min(p0 + n * 64, P);
-    auto load = [&](int i) { return p0 + 64 * i + lane < p1 ? expert_of(ids[p0 + 64 * i + lane], E) : INT32_MAX; };
-    int held[HOLD ? HOLD : 1];
-    if constexpr (HOLD > 0) {
+    int id[U] = {};
+    auto load = [&](int i0) {
 #pragma unroll
-        for (int i = 0; i < HOLD; i++) held[i] = i < n ? load(i) : INT32_MAX;
-    }
-    int nb = 0, ne = 0;
-    auto count = [&](int id) {
-        nb += __popcll(__ballot(id < e));
-        ne += __popcll(__ballot(id == e));
+        for (int u = 0; u < U; u++) id[u] = ids[min(p0 + 64 * (i0 + u) + lane, P - 1)];
+#pragma unroll
+        for (int u = 0; u < U; u++) id[u] = p0 + 64 * (i0 + u) + lane < p1 ? expert_of(id[u], E) : INT32_MAX;
     };
-    if constexpr (HOLD > 0) {
+    int nb = 0, ne = 0;
+    for (int i = 0; i < n; i += U) {
+        load(i);
 #pragma unroll
-        for (int i = 0; i < HOLD; i++) count(held[i]);
-    } else {
-        for (int i = 0; i < n; i++) count(load(i));
+        for (int u = 0; u < U; u++) {
+            nb += __popcll(__ballot(id[u] < e));
+            ne += __popcll(__ballot(id[u] == e));
+        }
     }
     if (lane == 0) below[wave] = nb, equal[wave] = ne;
     __syncthreads();
@@ -389,22 +389,19 @@ __global__ __launch_bounds__(PLAN_T) void plan_kernel(const int32_t* __restrict_
     for (int w = 0; w < W; w++) at += below[w];
     if (threadIdx.x == 0) plan[e] = at;  // e = E: the pairs that have one
     for (int p = e * PLAN_T + (int)threadIdx.x; p < P; p += (E + 1) * PLAN_T) {  // pairs' experts: a share of them all
-        const int id = expert_of(ids[p], E);
-        plan[l.expert + p] = id < E ? id : -1;
+        const int x = expert_of(ids[p], E);
+        plan[l.expert + p] = x < E ? x : -1;
     }
     for (int w = 0; w < wave; w++) at += equal[w];
     if (ne == 0) return;
-    int32_t* order = plan + l.order;
-    auto place = [&](int i, int id) {
-        const uint64_t b = __ballot(id == e);
-        if (id == e) order[at + __popcll(b & ((1ull << lane) - 1))] = p0 + 64 * i + lane;
-        at += __popcll(b);
-    };
-    if constexpr (HOLD > 0) {
+    for (int i = 0; i < n; i += U) {
+        if constexpr (HOLD == 0) load(i);
 #pragma unroll
-        for (int i = 0; i < HOLD; i++) place(i, held[i]);
-    } else {
-        for (int i = 0; i < n; i++) place(i, load(i));
+        for (int u = 0; u < U; u++) {
+            const uint64_t b = __ballot(id[u] == e);
+            if (id[u] == e) plan[l.order + at + __popcll(b & ((1ull << lane) - 1))] = p0 + 64 * (i + u) + lane;
+            at += __popcll(b);
+        }
     }
 }
 
