@@ -441,6 +441,47 @@ def test_a_layer_captured_and_replayed(gpu, rt, oracle):
     g.destroy()
 
 
+class View:
+    """Bytes of a weights section from `offset` on, as a layer."""
+
+    def __init__(self, section, offset, dt, experts, n, k, nbytes):
+        self.dt, self.experts, self.n, self.k = dt, experts, n, k
+        self.w = section.view(offset, nbytes, dt, experts * n, k)
+
+
+@pytest.mark.parametrize("dt,offset", [(Q4_K, 16), (Q4_K, 208), (Q6_K, 2), (Q6_K, 62), (Q8_0, 2), (Q8_0, 4), (Q8_0, 94)])
+@pytest.mark.parametrize("T", [2, 40, 300])
+def test_weights_at_the_alignment_of_their_blocks(gpu, rt, oracle, dt, offset, T):
+    """Bit for bit what the same bytes at an aligned place give."""
+    layer = Layer(gpu, oracle, dt, 4, 72, 512, 60)
+    section = gpu.WeightsSection(np.concatenate([np.full(offset, 0xFF, np.uint8), layer.raw.reshape(-1)]))
+    view = View(section, offset, dt, 4, 72, 512, layer.raw.size)
+    x, ids = acts_for(61, T, 512), choices(62, T, 2, 4)
+    want, got = (run_swiglu(gpu, rt, w, w, x, ids) for w in (layer, view))
+    np.testing.assert_array_equal(bits(got), bits(want))
+    h, weights = acts_for(63, T * 2, 512), np.random.default_rng(64).random((T, 2), np.float32)
+    want, got = (run_combine(gpu, rt, w, h, weights, ids) for w in (layer, view))
+    np.testing.assert_array_equal(bits(got), bits(want))
+
+
+@pytest.mark.parametrize("dt,n", [(Q4_K, 4096), (Q6_K, 2816), (Q8_0, 2176)])
+def test_experts_of_more_than_4_gib(gpu, rt, oracle, dt, n):
+    """The same eight experts 64 times, those behind 4 GiB chosen."""
+    small = Layer(gpu, oracle, dt, 8, n, 4096, 65)
+    section = gpu.WeightsSection(np.tile(small.raw.reshape(-1), 64))
+    big = View(section, 0, dt, 512, n, 4096, small.raw.size * 64)
+    assert small.raw.size * 60 > 1 << 32
+    for T in (2, 40, 600):
+        x, ids = acts_for(66, T, 4096), np.random.default_rng(67).integers(480, 512, (T, 2)).astype(np.int32)
+        want = run_swiglu(gpu, rt, small, small, x, ids % 8)
+        np.testing.assert_array_equal(bits(run_swiglu(gpu, rt, big, big, x, ids)), bits(want))
+        h, weights = acts_for(68, T * 2, 4096), np.random.default_rng(69).random((T, 2), np.float32)
+        want = run_combine(gpu, rt, small, h, weights, ids % 8)
+        np.testing.assert_array_equal(bits(run_combine(gpu, rt, big, h, weights, ids)), bits(want))
+    big.w = None
+    section.free()
+
+
 def test_product_refusals(gpu, rt, oracle):
     """What the host turns away: nothing is launched."""
     L = gpu.load()
