@@ -533,3 +533,21 @@ def test_most_pairs(gpu, rt, oracle):
     s.sync()
     got = y.download(np.float32).reshape(T // some, some, 4)
     assert (bits(got) == bits(want)[None]).all()
+
+
+@pytest.mark.parametrize("dt", [Q4_K, Q6_K, Q8_0])
+@pytest.mark.parametrize("T", [2, 40, 300])
+def test_products_of_scales_below_the_normal_ones(gpu, rt, oracle, dt, T):
+    """x of 2^-118 and less: products of two scales that are subnormal float32;
+    bit for bit what a token alone gives, for the K-quants what the oracle
+    gives."""
+    down = Layer(gpu, oracle, dt, 2, 64, 512, 70)
+    h, ids = acts_for(71, T, 512), choices(72, T, 1, 2)
+    h *= np.float32(2.0) ** -(118 + 3 * (np.arange(T)[:, None] % 7)).astype(np.float32)
+    one = np.ones((T, 1), np.float32)
+    got = run_combine(gpu, rt, down, h, one, ids)
+    assert (got != 0).any()
+    if dt != Q8_0:
+        np.testing.assert_array_equal(bits(got), bits(expert_products(oracle, down, h, ids, True)[0]))
+    alone = [run_combine(gpu, rt, down, h[t:t + 1], one[:1], ids[t:t + 1]) for t in range(0, T, 7)]
+    np.testing.assert_array_equal(bits(got[::7]), bits(np.concatenate(alone)))
