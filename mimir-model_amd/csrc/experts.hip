@@ -37,7 +37,7 @@
 // 60, 2048 x 1408 Q8_0 81 us: 373 MB at 4.6 TB/s. Many: vector instructions beside
 // the matrix cores. 2048 tokens, two of 8: gate and up 1250 us, 0.77 POP/s of
 // products and 1.54 of the planes' (the matrix cores at work 45 % of the cycles,
-// vector instructions 66 %), down 4096 x 14336 Q6_K 705 us, 0.68 and 1.37 POP/s.
+// vector instructions 66 %), down 4096 x 14336 Q6_K 675 us, 0.71 and 1.42 POP/s.
 //
 // Rows of x the quantizer refused and weight rows with a non-finite block
 // scale take the float32 path (f32path.hpp) at the end.
@@ -201,9 +201,8 @@ struct Copies {
             const int c = min(64 * i + l, 32 * C::WCH - 1);
             const int r = C::LINES ? 8 * i + (l >> 3) : c / C::WCH, j = C::LINES ? (l & 7) ^ ((r >> 1) & 7) : c - C::WCH * r;
             const uint32_t o = mis + (uint32_t)max(min(r, A.N - 1 - n0), 0) * (uint32_t)A.rb;
-            // (Q6_K: the block's place, rounded down for each block; its chunk
-            // is added then)
-            w[i] = DT == DT_Q6_K ? o : (C::AL ? o : o & ~15u) + 16 * j;
+            // (Q6_K: rounded down for each block)
+            w[i] = (C::AL || DT == DT_Q6_K ? o : o & ~15u) + 16 * j;
         }
     }
     __device__ __forceinline__ void init_rows(const Args& A, const int* rows) {
@@ -251,7 +250,7 @@ struct Copies {
 #pragma unroll
         for (int i = 0; i < C::WDMA; i++) {
             uint32_t o = w[i];
-            if constexpr (DT == DT_Q6_K) o = ((o + (uint32_t)b * C::GROUP) & ~15u) + 16 * (min(64 * i + l, 32 * C::WCH - 1) % C::WCH);
+            if constexpr (DT == DT_Q6_K) o = (o + (uint32_t)b * C::GROUP) & ~15u;
             if constexpr (DT != DT_Q4_K) o = min(o, last);
             if (64 * i + 64 <= 32 * C::WCH || l < 32 * C::WCH - 64 * i) lds_copy16_at(base, o, lds + C::WWAVE * wave + 1024 * i);
         }
@@ -492,6 +491,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
             const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
             v8h bm;
             if constexpr (DT == DT_Q4_K) bm = grp.mins(g);
+            v32f dd6;
 #pragma unroll
             for (int i = 0; i < MT; i++) {
                 if constexpr (DT == DT_Q4_K) {
@@ -510,15 +510,16 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
                         off[i][r] = __builtin_fmaf(Mm[r], dd[16 + r], off[i][r]);
                     }
                 } else if constexpr (DT == DT_Q6_K) {
+                    // d*dx of two tiles of pairs as one outer product (lanes
+                    // g = 0 hold the even one's dx; 2048 tokens 793 -> 772 us)
+                    if (i % 2 == 0) {
+                        const v32f z = {};
+                        dd6 = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * min(i + g, MT - 1) + a], grp.d, z, 0, 0, 0);
+                    }
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float4 dx = *(const float4*)(dl + 32 * i + 8 * j + 4 * g);
-                        const float dv[4] = {dx.x, dx.y, dx.z, dx.w};
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int S = (acc[0][i][4 * j + r] << 8) + acc[1][i][4 * j + r];
-                            tot[i][4 * j + r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][4 * j + r]);
-                        }
+                    for (int r = 0; r < 16; r++) {
+                        const int S = (acc[0][i][r] << 8) + acc[1][i][r];
+                        tot[i][r] = __builtin_fmaf((float)S, dd6[16 * (i % 2) + r], tot[i][r]);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
