@@ -41,6 +41,8 @@
 //
 // Rows of x the quantizer refused and weight rows with a non-finite block
 // scale take the float32 path (f32path.hpp) at the end.
+#include <type_traits>
+
 #include "decoder_math.hpp"
 #include "experts.hpp"
 #include "f32path.hpp"
@@ -446,112 +448,121 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
     // the lane's group in its slot (Q6_K, Q8_0: from the boundary below it)
     const uint32_t wmis = DT == DT_Q4_K ? 0 : (uint32_t)(uintptr_t)(M.W + (row0 + min(wn0 + a, A.N - 1)) * A.rb);
     const int ng = C::K32 ? (A.nb + 7) / 8 : A.nb;
-    for (int b = 0; b < ng; b++) {
-        wait_vmcnt<0>();
-        lds_barrier();  // group b's copies have landed, group b - 1's activations are read
-        const uint8_t* buf = smem + C::WBYTES + (b & 1) * C::BUF;
-        const uint8_t* al = buf + a * 256;
-        Group<DT, C::AL> grp;
-        if constexpr (C::LINES) {
-            grp.read(smem + C::WWAVE * cp.wave, (uint32_t)(128 * a + 16 * ((a >> 1) & 7)), b, g);
-        } else {
-            grp.read(smem + C::WWAVE * cp.wave + a * C::WSLOT + (C::AL ? 0 : (wmis + (uint32_t)b * C::GROUP) & 15u), g);
-        }
-        if (b + 1 < ng) {
-            cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
-            wait_lgkm0();  // the wave's weight slot is read
-            cp.weights(b + 1, lds0);
-        }
-        v16i acc[2][MT];
-        if constexpr (!C::K32) {
-            v4i av[MT];
-#pragma unroll
-            for (int i = 0; i < MT; i++) av[i] = *(const v4i*)(al + i * 8192 + 16 * asw);
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int ks = 0; ks < 8; ks++) {
-                v4i pH, pL, nx[MT];
-                grp.planes(ks, g, pH, pL);
-#pragma unroll
-                for (int i = 0; i < MT; i++)
-                    if (ks < 7) nx[i] = *(const v4i*)(al + i * 8192 + 16 * ((2 * ks + 2) ^ asw));
-                const v16i z = {};
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    acc[0][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], pH, ks ? acc[0][i] : z, 0, 0, 0);
-                    acc[1][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], pL, ks ? acc[1][i] : z, 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < MT; i++) av[i] = nx[i];
+    // The row's groups, for the first 32 L pairs: of tiles of 64 an expert's last
+    // one is often half empty (512 tokens, gate and up of eight of 64 experts 2048 x
+    // 1024 84.6 -> 81.5 us, of two of 8 4096 x 14336 402 -> 393, 2048 tokens 1280 ->
+    // 1273; tiles of 96 have no registers left for a second form, 772 -> 796).
+    auto groups = [&](auto live) __attribute__((always_inline)) {
+        constexpr int L = decltype(live)::value;
+        for (int b = 0; b < ng; b++) {
+            wait_vmcnt<0>();
+            lds_barrier();  // group b's copies have landed, group b - 1's activations are read
+            const uint8_t* buf = smem + C::WBYTES + (b & 1) * C::BUF;
+            const uint8_t* al = buf + a * 256;
+            Group<DT, C::AL> grp;
+            if constexpr (C::LINES) {
+                grp.read(smem + C::WWAVE * cp.wave, (uint32_t)(128 * a + 16 * ((a >> 1) & 7)), b, g);
+            } else {
+                grp.read(smem + C::WWAVE * cp.wave + a * C::WSLOT + (C::AL ? 0 : (wmis + (uint32_t)b * C::GROUP) & 15u), g);
             }
-            // The products at raised priority, the float step in what they
-            // leave of the vector unit (2048 tokens 2 % faster than the other
-            // way round, and that faster than neither).
-            __builtin_amdgcn_s_setprio(0);
-            const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
-            v8h bm;
-            if constexpr (DT == DT_Q4_K) bm = grp.mins(g);
-            v32f dd6;
-#pragma unroll
-            for (int i = 0; i < MT; i++) {
-                if constexpr (DT == DT_Q4_K) {
-                    // d*dx and dmin*dx of the tile as outer products (lanes
-                    // g = 0 hold d, g = 1 dmin)
-                    const v32f z = {};
-                    const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * i + a], g ? grp.dmin : grp.d, z, 0, 0, 0);
-                    // 64 hi + lo against 64 m and m
-                    const v8h v = *(const v8h*)(buf + C::ABYTES + 32 * (32 * i + a) + 16 * g);
-                    v16f Mm = {};
-                    Mm = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bm, Mm, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int S = (acc[0][i][r] << 3) + acc[1][i][r];
-                        tot[i][r] = __builtin_fmaf((float)S, dd[r], tot[i][r]);
-                        off[i][r] = __builtin_fmaf(Mm[r], dd[16 + r], off[i][r]);
-                    }
-                } else if constexpr (DT == DT_Q6_K) {
-                    // d*dx of two tiles of pairs as one outer product (lanes
-                    // g = 0 hold the even one's dx; 2048 tokens 793 -> 772 us)
-                    if (i % 2 == 0) {
-                        const v32f z = {};
-                        dd6 = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * min(i + g, MT - 1) + a], grp.d, z, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int S = (acc[0][i][r] << 8) + acc[1][i][r];
-                        tot[i][r] = __builtin_fmaf((float)S, dd6[16 * (i % 2) + r], tot[i][r]);
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            if (b + 1 < ng) {
+                cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
+                wait_lgkm0();  // the wave's weight slot is read
+                cp.weights(b + 1, lds0);
             }
-        } else {
-            // d*dx of two blocks (lanes g = 0 the even one's, g = 1 the odd
-            // one's) as one outer product.
-            const float* dl = (const float*)(buf + C::ABYTES);
-            const int nk = min(8, A.nb - 8 * b);
+            v16i acc[2][L];
+            if constexpr (!C::K32) {
+                v4i av[L];
 #pragma unroll
-            for (int ks = 0; ks < 8; ks += 2) {
-                if (ks < nk) {
-                    const v4i w0 = grp.block(ks), w1 = grp.block(ks + 1);
-                    const float dw = g ? grp.d[ks + 1] : grp.d[ks];
+                for (int i = 0; i < L; i++) av[i] = *(const v4i*)(al + i * 8192 + 16 * asw);
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int ks = 0; ks < 8; ks++) {
+                    v4i pH, pL, nx[L];
+                    grp.planes(ks, g, pH, pL);
+#pragma unroll
+                    for (int i = 0; i < L; i++)
+                        if (ks < 7) nx[i] = *(const v4i*)(al + i * 8192 + 16 * ((2 * ks + 2) ^ asw));
                     const v16i z = {};
-                    const v32f zf = {};
 #pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        acc[0][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const v4i*)(al + i * 8192 + 16 * ((2 * ks) ^ asw)), w0, z, 0, 0, 0);
-                        acc[1][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const v4i*)(al + i * 8192 + 16 * ((2 * ks + 2) ^ asw)), w1, z, 0, 0, 0);
-                        const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[8 * (32 * i + a) + ks + g], dw, zf, 0, 0, 0);
+                    for (int i = 0; i < L; i++) {
+                        acc[0][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], pH, ks ? acc[0][i] : z, 0, 0, 0);
+                        acc[1][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], pL, ks ? acc[1][i] : z, 0, 0, 0);
+                    }
 #pragma unroll
-                        for (int r = 0; r < 16; r++) tot[i][r] = __builtin_fmaf((float)acc[0][i][r], dd[r], tot[i][r]);
-                        if (ks + 1 < nk) {
+                    for (int i = 0; i < L; i++) av[i] = nx[i];
+                }
+                // The products at raised priority, the float step in what they
+                // leave of the vector unit (2048 tokens 2 % faster than the other
+                // way round, and that faster than neither).
+                __builtin_amdgcn_s_setprio(0);
+                const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
+                v8h bm;
+                if constexpr (DT == DT_Q4_K) bm = grp.mins(g);
+                v32f dd6;
 #pragma unroll
-                            for (int r = 0; r < 16; r++) tot[i][r] = __builtin_fmaf((float)acc[1][i][r], dd[16 + r], tot[i][r]);
+                for (int i = 0; i < L; i++) {
+                    if constexpr (DT == DT_Q4_K) {
+                        // d*dx and dmin*dx of the tile as outer products (lanes
+                        // g = 0 hold d, g = 1 dmin)
+                        const v32f z = {};
+                        const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * i + a], g ? grp.dmin : grp.d, z, 0, 0, 0);
+                        // 64 hi + lo against 64 m and m
+                        const v8h v = *(const v8h*)(buf + C::ABYTES + 32 * (32 * i + a) + 16 * g);
+                        v16f Mm = {};
+                        Mm = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bm, Mm, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const int S = (acc[0][i][r] << 3) + acc[1][i][r];
+                            tot[i][r] = __builtin_fmaf((float)S, dd[r], tot[i][r]);
+                            off[i][r] = __builtin_fmaf(Mm[r], dd[16 + r], off[i][r]);
+                        }
+                    } else if constexpr (DT == DT_Q6_K) {
+                        // d*dx of two tiles of pairs as one outer product (lanes
+                        // g = 0 hold the even one's dx; 2048 tokens 793 -> 772 us)
+                        if (i % 2 == 0) {
+                            const v32f z = {};
+                            dd6 = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * min(i + g, L - 1) + a], grp.d, z, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const int S = (acc[0][i][r] << 8) + acc[1][i][r];
+                            tot[i][r] = __builtin_fmaf((float)S, dd6[16 * (i % 2) + r], tot[i][r]);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+                // d*dx of two blocks (lanes g = 0 the even one's, g = 1 the odd
+                // one's) as one outer product.
+                const float* dl = (const float*)(buf + C::ABYTES);
+                const int nk = min(8, A.nb - 8 * b);
+#pragma unroll
+                for (int ks = 0; ks < 8; ks += 2) {
+                    if (ks < nk) {
+                        const v4i w0 = grp.block(ks), w1 = grp.block(ks + 1);
+                        const float dw = g ? grp.d[ks + 1] : grp.d[ks];
+                        const v16i z = {};
+                        const v32f zf = {};
+#pragma unroll
+                        for (int i = 0; i < L; i++) {
+                            acc[0][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const v4i*)(al + i * 8192 + 16 * ((2 * ks) ^ asw)), w0, z, 0, 0, 0);
+                            acc[1][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const v4i*)(al + i * 8192 + 16 * ((2 * ks + 2) ^ asw)), w1, z, 0, 0, 0);
+                            const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[8 * (32 * i + a) + ks + g], dw, zf, 0, 0, 0);
+#pragma unroll
+                            for (int r = 0; r < 16; r++) tot[i][r] = __builtin_fmaf((float)acc[0][i][r], dd[r], tot[i][r]);
+                            if (ks + 1 < nk) {
+#pragma unroll
+                                for (int r = 0; r < 16; r++) tot[i][r] = __builtin_fmaf((float)acc[1][i][r], dd[16 + r], tot[i][r]);
+                            }
                         }
                     }
                 }
             }
         }
-    }
+    };
+    if (MT == 2 && tile.m <= 32) groups(std::integral_constant<int, 1>());
+    else groups(std::integral_constant<int, MT>());
 
     // Result i of a lane: weight row wn0 + a, pair 8 (i / 4) + 4 g + i % 4.
     const int n = wn0 + a;
@@ -624,11 +635,21 @@ static hipError_t launch(const Args& A, hipStream_t stream) {
 
 template <uint32_t DT, bool SW>
 static hipError_t launch_dt(const Args& A, hipStream_t stream) {
-    // (64 pairs a workgroup, Q6_K 96, where the experts have as many on average)
+    // 64 pairs a workgroup where the experts have as many on average, of Q6_K
+    // where they have 48, and 96 from that on (us a call in tiles of 32 / 64 / 96:
+    // down 2048 x 1024, 64 experts, 32 pairs each 57.8 / 60.6 / -, 48 70.7 / 69.6 /
+    // -, 64 - / 79.1 / 84.1, 128 - / 123.4 / 124.9, 256 - / 212 / 200; 4096 x 14336,
+    // 8 experts, 48 206 / 192 / -, 64 - / 207 / 219, 128 - / 341 / 267. Q4_K gate
+    // and up 2048 x 1024, 48 71 / 75, 56 78 / 79; 4096 x 14336, 48 211 / 206.)
+    const int64_t E = A.experts;
+    if constexpr (DT == DT_Q6_K) {
+        if (A.pairs >= 96 * E) return launch<DT, 3, SW>(A, stream);
+        return A.pairs >= 48 * E ? launch<DT, 2, SW>(A, stream) : launch<DT, 1, SW>(A, stream);
+    }
     if constexpr (DT == DT_Q8_0)
         if (A.rb % 4 == 0 && (uintptr_t)A.mat[0].W % 4 == 0 && (uintptr_t)A.mat[1].W % 4 == 0)
-            return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, 2, SW, true>(A, stream) : launch<DT, 1, SW, true>(A, stream);
-    return A.pairs >= 64 * (int64_t)A.experts ? launch<DT, DT == DT_Q6_K ? 3 : 2, SW>(A, stream) : launch<DT, 1, SW>(A, stream);
+            return A.pairs >= 64 * E ? launch<DT, 2, SW, true>(A, stream) : launch<DT, 1, SW, true>(A, stream);
+    return A.pairs >= 64 * E ? launch<DT, 2, SW>(A, stream) : launch<DT, 1, SW>(A, stream);
 }
 
 }  // namespace xp

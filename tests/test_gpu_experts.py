@@ -305,6 +305,16 @@ def test_combine(gpu, rt, oracle, dt, experts, n, k, T, top, what):
     check_combine(run_combine(gpu, rt, down, h, weights, ids), oracle, down, h, weights, ids)
 
 
+# tiles of 64 pairs of which the last one has all, more than half, few
+TILES = [(dt, 2, 97, 768, T, 1, what) for dt in (Q4_K, Q6_K, Q8_0) for T, what in ((128, "even"), (180, "one"), (150, "even"), (130, "one"))]
+
+
+@pytest.mark.parametrize("dt,experts,n,k,T,top,what", TILES)
+def test_last_tiles(gpu, rt, oracle, dt, experts, n, k, T, top, what):
+    test_swiglu(gpu, rt, oracle, dt, experts, n, k, T, top, what)
+    test_combine(gpu, rt, oracle, dt, experts, n, k, T, top, what)
+
+
 @pytest.mark.parametrize("dt", [Q4_K, Q6_K])
 @pytest.mark.parametrize("T", [1, 3, 50, 200])
 def test_products_equal_the_oracle_bit_for_bit(gpu, rt, oracle, dt, T):
