@@ -448,12 +448,16 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
     // the lane's group in its slot (Q6_K, Q8_0: from the boundary below it)
     const uint32_t wmis = DT == DT_Q4_K ? 0 : (uint32_t)(uintptr_t)(M.W + (row0 + min(wn0 + a, A.N - 1)) * A.rb);
     const int ng = C::K32 ? (A.nb + 7) / 8 : A.nb;
-    // The row's groups, for the first 32 L pairs: of tiles of 64 an expert's last
+    // The row's groups, for the first 32 L pairs and R results of a lane (the
+    // pairs below 2 R of 32). Half the float step where a tile of 32 has at most 16
+    // pairs: 64 tokens, eight of 64 experts, gate and up 2048 x 1024 44.0 -> 42.6 us,
+    // 8 tokens 29.4 -> 29.0, 37 tokens, four of 60, down Q8_0 50.5 -> 49.3; a quarter
+    // for 8 gives nothing more. Half of all: of tiles of 64 an expert's last
     // one is often half empty (512 tokens, gate and up of eight of 64 experts 2048 x
     // 1024 84.6 -> 81.5 us, of two of 8 4096 x 14336 402 -> 393, 2048 tokens 1280 ->
     // 1273; tiles of 96 have no registers left for a second form, 772 -> 796).
-    auto groups = [&](auto live) __attribute__((always_inline)) {
-        constexpr int L = decltype(live)::value;
+    auto groups = [&](auto live, auto results) __attribute__((always_inline)) {
+        constexpr int L = decltype(live)::value, R = decltype(results)::value;
         for (int b = 0; b < ng; b++) {
             wait_vmcnt<0>();
             lds_barrier();  // group b's copies have landed, group b - 1's activations are read
@@ -512,7 +516,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
                         v16f Mm = {};
                         Mm = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bm, Mm, 0, 0, 0);
 #pragma unroll
-                        for (int r = 0; r < 16; r++) {
+                        for (int r = 0; r < R; r++) {
                             const int S = (acc[0][i][r] << 3) + acc[1][i][r];
                             tot[i][r] = __builtin_fmaf((float)S, dd[r], tot[i][r]);
                             off[i][r] = __builtin_fmaf(Mm[r], dd[16 + r], off[i][r]);
@@ -525,7 +529,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
                             dd6 = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[32 * min(i + g, L - 1) + a], grp.d, z, 0, 0, 0);
                         }
 #pragma unroll
-                        for (int r = 0; r < 16; r++) {
+                        for (int r = 0; r < R; r++) {
                             const int S = (acc[0][i][r] << 8) + acc[1][i][r];
                             tot[i][r] = __builtin_fmaf((float)S, dd6[16 * (i % 2) + r], tot[i][r]);
                         }
@@ -550,10 +554,10 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
                             acc[1][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const v4i*)(al + i * 8192 + 16 * ((2 * ks + 2) ^ asw)), w1, z, 0, 0, 0);
                             const v32f dd = __builtin_amdgcn_mfma_f32_32x32x1f32(dl[8 * (32 * i + a) + ks + g], dw, zf, 0, 0, 0);
 #pragma unroll
-                            for (int r = 0; r < 16; r++) tot[i][r] = __builtin_fmaf((float)acc[0][i][r], dd[r], tot[i][r]);
+                            for (int r = 0; r < R; r++) tot[i][r] = __builtin_fmaf((float)acc[0][i][r], dd[r], tot[i][r]);
                             if (ks + 1 < nk) {
 #pragma unroll
-                                for (int r = 0; r < 16; r++) tot[i][r] = __builtin_fmaf((float)acc[1][i][r], dd[16 + r], tot[i][r]);
+                                for (int r = 0; r < R; r++) tot[i][r] = __builtin_fmaf((float)acc[1][i][r], dd[16 + r], tot[i][r]);
                             }
                         }
                     }
@@ -561,8 +565,9 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
             }
         }
     };
-    if (MT == 2 && tile.m <= 32) groups(std::integral_constant<int, 1>());
-    else groups(std::integral_constant<int, MT>());
+    if (MT == 2 && tile.m <= 32) groups(std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
+    else if (MT == 1 && tile.m <= 16) groups(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
+    else groups(std::integral_constant<int, MT>(), std::integral_constant<int, 16>());
 
     // Result i of a lane: weight row wn0 + a, pair 8 (i / 4) + 4 g + i % 4.
     const int n = wn0 + a;
