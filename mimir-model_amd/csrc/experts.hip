@@ -36,8 +36,8 @@
 // copies alone take 108 to 117 us and the instructions alone 100; 181 tokens, four of
 // 60, 2048 x 1408 Q8_0 81 us: 373 MB at 4.6 TB/s. Many: vector instructions beside
 // the matrix cores. 2048 tokens, two of 8: gate and up 1250 us, 0.77 POP/s of
-// products and 1.54 of the planes' (the matrix cores at work 45 % of the cycles,
-// vector instructions 66 %), down 4096 x 14336 Q6_K 675 us, 0.71 and 1.42 POP/s.
+// products and 1.54 of the planes' (the matrix cores at work 42 % of the cycles,
+// vector instructions 65 %), down 4096 x 14336 Q6_K 675 us, 0.71 and 1.42 POP/s.
 //
 // Rows of x the quantizer refused and weight rows with a non-finite block
 // scale take the float32 path (f32path.hpp) at the end.
