@@ -667,8 +667,13 @@ static hipError_t launch_dt(const Args& A, hipStream_t stream) {
 // 18.2 / 23.5; Q8_0 (experts_q8.hip) 4096 x 7168, 8 experts, 8 pairs 89 against
 // 82, 2048 x 1408, 60 experts, 8 / 16 / 32 pairs 17.1 / 26.5 / 42 against 22.9 /
 // 31.5 / 37.7.
-static bool few_pairs_swiglu(uint32_t dt, int pairs, int experts) {
-    return pairs <= (dt == DT_Q8_0 ? 4 : 8) || (pairs <= 16 && experts >= 2 * pairs);
+// Of many more experts (Q4_K): 2048 x 768, 128 experts, 24 / 32 / 64 pairs 17.8 /
+// 22.1 / 34.5 against 19.7 / 21.0 / 28.2; 4096 x 1536, 128 experts, 32 pairs 42
+// against 49 (Q6_K 69 against 81), 256 experts, 48 / 64 pairs 63 / 81 against 76 / 91;
+// Q8_0 2048 x 1408, 160 experts, 24 pairs 36.7 against 33.9.
+static bool few_pairs_swiglu(const DevWeight& w, int pairs, int experts) {
+    if (pairs <= (w.dt == DT_Q8_0 ? 4 : 8) || (pairs <= 16 && experts >= 2 * pairs)) return true;
+    return w.dt != DT_Q8_0 && experts >= 4 * pairs && pairs <= (w.k >= 4096 ? 48 : 24);
 }
 // down with the sum in its launch, alone / in tiles: 4096 x 14336, 8 experts, 2
 // / 4 / 8 / 16 pairs Q6_K 28 / 45 / 74 / 130 against 111 / 111 / 112 / 113, 12 /
@@ -676,7 +681,13 @@ static bool few_pairs_swiglu(uint32_t dt, int pairs, int experts) {
 // 32 / 64 pairs 8.7 / 10.0 / 13.0 / 19.3 against 15.5 / 16.5 / 19.6 / 24.9; 2048 x
 // 1536 Q6_K, 60 experts, 32 / 48 pairs 27.1 / 35.4 against 29.8 / 35.1; Q8_0 2048 x
 // 1408, 60 experts, 16 / 32 / 64 pairs 18.1 / 28.5 / 44.2 against 26.2 / 33.8 / 47.8.
-static bool few_pairs_combine(int pairs, int experts) { return pairs <= 8 || (pairs <= 64 && experts >= pairs); }
+// 128 experts, 72 / 96 / 128 pairs: 768 -> 2048 Q4_K 20.7 / 24.6 / 28.8 against 28.8 /
+// 31.6 / 34.2, Q6_K 30.8 / 37.2 / 44.7 against 35.0 / 38.2 / 41.5, Q8_0 31.8 / 37.4 /
+// 45.5 against 33.9 / 36.8 / 41.6; 1536 -> 4096 Q4_K 52 / 66 / 84 against 60 / 69 / 79,
+// Q6_K 86 / - / 142 against 83 / - / 113.
+static bool few_pairs_combine(uint32_t dt, int pairs, int experts) {
+    return pairs <= 8 || (pairs <= (dt == DT_Q4_K ? 128 : 64) && experts >= pairs);
+}
 
 bool experts_ok(const DevWeight& w) {
     const bool k256 = w.dt == DT_Q4_K || w.dt == DT_Q6_K;
@@ -723,12 +734,12 @@ static hipError_t launch_tiles(const DevWeight* const* ws, int nmat, int experts
 hipError_t launch_experts_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, void* parts,
                                  const float* x, int64_t T, int top, const int32_t* plan, float* h, hipStream_t stream) {
     const int pairs = (int)(T * top);
-    if (few_pairs_swiglu(gate.dt, pairs, experts) && gemv_experts_swiglu_ok(gate, experts)) {
+    if (few_pairs_swiglu(gate, pairs, experts) && gemv_experts_swiglu_ok(gate, experts)) {
         const hipError_t e = launch_quantize_act(x, T, gate.k, 256, a, stream);
         if (e != hipSuccess) return e;
         return launch_gemv_experts_swiglu(gate, up, experts, a, x, T, top, plan + plan_layout(pairs, experts).expert, h, stream);
     }
-    if (few_pairs_swiglu(gate.dt, pairs, experts) && gemv_experts_q8_ok(gate, 2)) {
+    if (few_pairs_swiglu(gate, pairs, experts) && gemv_experts_q8_ok(gate, 2)) {
         const hipError_t e = launch_quantize_act(x, T, gate.k, 32, a, stream);
         if (e != hipSuccess) return e;
         return launch_gemv_experts_q8_swiglu(gate, up, experts, a, x, T, top, plan + plan_layout(pairs, experts).expert, h, stream);
@@ -742,11 +753,11 @@ hipError_t launch_experts_combine(const DevWeight& w, int experts, const ActPtrs
                                   hipStream_t stream) {
     const int pairs = (int)(T * top);
     const int32_t* expert = plan + plan_layout(pairs, experts).expert;
-    if (few_pairs_combine(pairs, experts) && gemv_experts_sum_ok(w, experts, top)) {
+    if (few_pairs_combine(w.dt, pairs, experts) && gemv_experts_sum_ok(w, experts, top)) {
         const hipError_t e = launch_quantize_act(h, pairs, w.k, 256, a, stream);
         return e != hipSuccess ? e : launch_gemv_experts_sum(w, experts, a, h, weights, T, top, expert, y, stream);
     }
-    if (few_pairs_combine(pairs, experts) && gemv_experts_q8_ok(w, top)) {
+    if (few_pairs_combine(w.dt, pairs, experts) && gemv_experts_q8_ok(w, top)) {
         const hipError_t e = launch_quantize_act(h, pairs, w.k, 32, a, stream);
         return e != hipSuccess ? e : launch_gemv_experts_q8_sum(w, experts, a, h, weights, T, top, expert, y, stream);
     }

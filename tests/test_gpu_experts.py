@@ -315,6 +315,18 @@ def test_last_tiles(gpu, rt, oracle, dt, experts, n, k, T, top, what):
     test_combine(gpu, rt, oracle, dt, experts, n, k, T, top, what)
 
 
+# pairs each by itself where there are many more experts, and just above
+MANY = [(dt, experts, n, k, T, 8, what) for dt in (Q4_K, Q6_K) for experts, n, k, T, what in (
+    (128, 24, 512, 3, "even"), (200, 16, 4096, 6, "padded"), (200, 16, 4096, 7, "even"), (128, 12, 256, 12, "again"),
+    (130, 12, 512, 16, "padded"), (130, 12, 256, 17, "even"))]
+
+
+@pytest.mark.parametrize("dt,experts,n,k,T,top,what", MANY)
+def test_pairs_of_many_experts(gpu, rt, oracle, dt, experts, n, k, T, top, what):
+    test_swiglu(gpu, rt, oracle, dt, experts, n, k, T, top, what)
+    test_combine(gpu, rt, oracle, dt, experts, n, k, T, top, what)
+
+
 @pytest.mark.parametrize("dt", [Q4_K, Q6_K])
 @pytest.mark.parametrize("T", [1, 3, 50, 200])
 def test_products_equal_the_oracle_bit_for_bit(gpu, rt, oracle, dt, T):
