@@ -54,6 +54,7 @@ namespace xp {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef float v32f __attribute__((ext_vector_type(32)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -79,8 +80,9 @@ struct Args {
 
 // AL (Q8_0): rows, and with them groups, start 4-byte aligned (K a multiple of
 // 64), as the copies need it.
-template <uint32_t DT, int MT_, bool AL_ = false>
+template <uint32_t DT, int MT_, bool AL_ = false, int RW_ = 32>
 struct Cfg {
+    static constexpr int RW = RW_;  // weight rows of a wave
     static constexpr bool AL = AL_;
     static constexpr int MT = MT_, T = 256, BM = 32 * MT;
     static constexpr bool K32 = DT == DT_Q8_0;
@@ -99,8 +101,8 @@ struct Cfg {
     // block every line that two blocks share would be fetched twice. The
     // chunks of a line are XOR-swizzled by row.
     static constexpr bool LINES = DT == DT_Q4_K;
-    static constexpr int WDMA = LINES ? 4 : (32 * WCH + 63) / 64;  // copies of a group, or of a line
-    static constexpr int WWAVE = LINES ? 2 * 4096 : 32 * WSLOT;
+    static constexpr int WDMA = LINES ? RW / 8 : (RW * WCH + 63) / 64;  // copies of a group, or of a line
+    static constexpr int WWAVE = RW * (LINES ? 256 : WSLOT);
     static constexpr int WBYTES = 4 * WWAVE;
     static constexpr int ADMA = BM * 16 / T;
     static constexpr int ABYTES = BM * 256;
@@ -200,7 +202,7 @@ struct Copies {
         wroom = M.W + A.wbytes + WEIGHT_PAD - 16 - wbase;
 #pragma unroll
         for (int i = 0; i < C::WDMA; i++) {
-            const int c = min(64 * i + l, 32 * C::WCH - 1);
+            const int c = min(64 * i + l, C::RW * C::WCH - 1);
             const int r = C::LINES ? 8 * i + (l >> 3) : c / C::WCH, j = C::LINES ? (l & 7) ^ ((r >> 1) & 7) : c - C::WCH * r;
             const uint32_t o = mis + (uint32_t)max(min(r, A.N - 1 - n0), 0) * (uint32_t)A.rb;
             // (Q6_K: rounded down for each block)
@@ -233,7 +235,7 @@ struct Copies {
     __device__ __forceinline__ void line(int b, uint32_t lds) const {
 #pragma unroll
         for (int i = 0; i < C::WDMA; i++)
-            lds_copy16_at(wbase + 128 * (int64_t)b, w[i], lds + C::WWAVE * wave + 4096 * (b & 1) + 1024 * i);
+            lds_copy16_at(wbase + 128 * (int64_t)b, w[i], lds + C::WWAVE * wave + C::RW * 128 * (b & 1) + 1024 * i);
     }
     // The last line that block b needs.
     static __device__ __forceinline__ int lines_to(int b) { return (9 * b + 8) >> 3; }
@@ -254,7 +256,7 @@ struct Copies {
             uint32_t o = w[i];
             if constexpr (DT == DT_Q6_K) o = (o + (uint32_t)b * C::GROUP) & ~15u;
             if constexpr (DT != DT_Q4_K) o = min(o, last);
-            if (64 * i + 64 <= 32 * C::WCH || l < 32 * C::WCH - 64 * i) lds_copy16_at(base, o, lds + C::WWAVE * wave + 1024 * i);
+            if (64 * i + 64 <= C::RW * C::WCH || l < C::RW * C::WCH - 64 * i) lds_copy16_at(base, o, lds + C::WWAVE * wave + 1024 * i);
         }
     }
     __device__ __forceinline__ void activations(int b, uint32_t lds) const {
@@ -621,6 +623,193 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
     }
 }
 
+// The same products with 16 weight rows a wave, on v_mfma_i32_16x16x64_i8, and 32
+// pairs: half the unpacking a wave and twice the waves, where tiles of 32 rows a
+// wave leave SIMDs without one. Lane l holds weight row a = l % 16 and of a k step
+// of 64 the elements 16 g .. 16 g + 15, g = l / 16; of a 16 x 16 result the pairs
+// 4 g .. 4 g + 3.
+template <uint32_t DT>
+struct ThinGroup;
+
+template <>
+struct ThinGroup<DT_Q4_K> {
+    u32x4 q[4];
+    uint64_t sc, m;  // sc: from the lane's sub-block of a pair on
+    float d, dmin;
+    static __device__ __forceinline__ uint32_t place(int c) { return (uint32_t)(((c & 8) << 8) | ((c & 7) << 4)); }
+    __device__ __forceinline__ void read(const uint8_t* slot, uint32_t row, int b, int g) {
+        const u32x4 h = *(const u32x4*)(slot + (row ^ place(9 * b)));
+        d = f16_to_f32(h.x & 0xFFFFu);
+        dmin = f16_to_f32(h.x >> 16);
+        const Q4KScales s = q4k_scales(h.y, h.z, h.w);
+        sc = s.sc >> (8 * (g >> 1));
+        m = s.m;
+        const int sh = 4 * (g >> 1);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint32_t p0 = place(9 * b + 1 + 2 * c), p1 = place(9 * b + 2 + 2 * c);
+            const u32x4 v = *(const u32x4*)(slot + (row ^ ((g & 1) ? p1 : p0)));
+            q[c] = u32x4{v.x >> sh & 0x0F0F0F0Fu, v.y >> sh & 0x0F0F0F0Fu, v.z >> sh & 0x0F0F0F0Fu, v.w >> sh & 0x0F0F0F0Fu};
+        }
+    }
+    __device__ __forceinline__ void planes(int ks, int, v4i& H, v4i& L) const {
+        const uint32_t s = byte_of(sc, 2 * ks);
+        const short sh = (short)(s >> 3), sl = (short)(s & 7);
+        const s16x2 shp = {sh, sh}, slp = {sl, sl};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            H[k] = (int)as_u32(as_s16x2(q[ks][k]) * shp);
+            L[k] = (int)as_u32(as_s16x2(q[ks][k]) * slp);
+        }
+    }
+};
+
+template <>
+struct ThinGroup<DT_Q6_K> {
+    u32x4 ql[2], qh[2], sc;
+    float d;
+    __device__ __forceinline__ void read(const uint8_t* wr, int g) {
+        const int sh = 2 * (g >> 1);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            ql[h] = lds_read16_a2(wr + 64 * h + 16 * g);
+            const u32x4 v = lds_read16_a2(wr + 128 + 32 * h + 16 * (g & 1));
+            qh[h] = u32x4{v.x >> sh, v.y >> sh, v.z >> sh, v.w >> sh};
+        }
+        sc = lds_read16_a2(wr + 192);
+        d = f16_to_f32(lds_read2_a2(wr + 208));
+    }
+    // (as Group's, quarter 2 (ks % 2) + g / 2 of half ks / 2, scale 4 ks + g)
+    __device__ __forceinline__ void planes(int ks, int g, v4i& H, v4i& L) const {
+        const u32x4 lo = ql[ks >> 1], hi = qh[ks >> 1];
+        const int s = (int)(int8_t)(uint8_t)(sc[ks] >> (8 * g));
+        const short cu = (short)(128 - 32 * s);
+        const s16x2 s2 = {(short)s, (short)s}, c2 = {cu, cu};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t q6 = ((lo[k] >> (4 * (ks & 1))) & 0x0F0F0F0Fu) | (((hi[k] >> (4 * (ks & 1))) & 0x03030303u) << 4);
+            const uint32_t ue = as_u32(as_s16x2(__builtin_amdgcn_perm(0u, q6, 0x0C020C00u)) * s2 + c2);
+            const uint32_t uo = as_u32(as_s16x2(__builtin_amdgcn_perm(0u, q6, 0x0C030C01u)) * s2 + c2);
+            H[k] = (int)__builtin_amdgcn_perm(uo, ue, 0x07030501u);
+            L[k] = (int)(__builtin_amdgcn_perm(uo, ue, 0x06020400u) ^ 0x80808080u);
+        }
+    }
+};
+
+template <uint32_t DT>
+__global__ __launch_bounds__(256, 4) void thin_kernel(Args A) {
+    using C = Cfg<DT, 1, false, 16>;
+    constexpr int BM = 32, BN = 64;
+    __shared__ __align__(16) uint8_t smem[C::SMEM];
+    __shared__ int rows[BM], outs[64], flags[1];
+    const int t = threadIdx.x, l = t & 63, wave = t >> 6;
+    const int a = l & 15, g = l >> 4;
+    Tile tile;
+    if (!find_tile(A, (A.N + BN - 1) / BN, BM, tile)) return;
+    const int n0 = tile.nt * BN, wn0 = n0 + 16 * wave;
+    const int64_t row0 = (int64_t)tile.e * A.N;
+    const Mat M = A.mat[0];
+    Copies<DT, C> cp;
+    cp.init_weights(A, M, row0, __builtin_amdgcn_readfirstlane(wn0));
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
+    if (cp.wave == 0) lds_copy4(A.plan + plan_layout(A.pairs, A.experts).order + tile.f0 + min(t, tile.m - 1), outs);
+    cp.weights(0, lds0);
+    if (cp.wave == 0) wait_vmcnt<C::WDMA>();
+    if (t == 0) flags[0] = 0;
+    lds_barrier();
+    if (t < BM) {
+        const int pair = min(max(outs[t], 0), A.pairs - 1);
+        outs[t] = pair;
+        rows[t] = pair / A.rowdiv;
+    }
+    lds_barrier();
+    cp.init_rows(A, rows);
+    cp.activations(0, lds0 + C::WBYTES);
+    {
+        int f = 0;
+        if (l < 16) f |= wn0 + l < A.N && M.wref[row0 + wn0 + l] != 0;
+        if (t < tile.m) f |= A.act.ok[rows[t]] == 0;
+        if (f) flags[0] = 1;
+    }
+    float tot[2][4] = {}, off[2][4] = {};
+    const uint32_t wmis = DT == DT_Q4_K ? 0 : (uint32_t)(uintptr_t)(M.W + (row0 + min(wn0 + a, A.N - 1)) * A.rb);
+    for (int b = 0; b < A.nb; b++) {
+        wait_vmcnt<0>();
+        lds_barrier();
+        const uint8_t* buf = smem + C::WBYTES + (b & 1) * C::BUF;
+        ThinGroup<DT> grp;
+        if constexpr (C::LINES) grp.read(smem + C::WWAVE * cp.wave, (uint32_t)(128 * a + 16 * ((a >> 1) & 7)), b, g);
+        else grp.read(smem + C::WWAVE * cp.wave + a * C::WSLOT + ((wmis + (uint32_t)b * C::GROUP) & 15u), g);
+        if (b + 1 < A.nb) {
+            cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
+            wait_lgkm0();
+            cp.weights(b + 1, lds0);
+        }
+        v4i acc[2][2];
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            v4i pH, pL;
+            grp.planes(ks, g, pH, pL);
+            const v4i z = {};
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const v4i av = *(const v4i*)(buf + (16 * i + a) * 256 + 16 * ((4 * ks + g) ^ a));
+                acc[0][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pH, ks ? acc[0][i] : z, 0, 0, 0);
+                acc[1][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pL, ks ? acc[1][i] : z, 0, 0, 0);
+            }
+        }
+        const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float4 dx = *(const float4*)(dl + 16 * i + 4 * g);
+            const float dv[4] = {dx.x, dx.y, dx.z, dx.w};
+            if constexpr (DT == DT_Q4_K) {
+                // (k 16 .. 31 of the mins' product are zeros: lanes g = 2, 3)
+                v8h bm = {};
+                if (g < 2) {
+                    Group<DT_Q4_K> full;
+                    full.s.m = grp.m;
+                    bm = full.mins(g);
+                }
+                const v8h v = *(const v8h*)(buf + C::ABYTES + 32 * (16 * i + a) + 16 * (g & 1));
+                v4f Mm = {};
+                Mm = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, bm, Mm, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int S = (acc[0][i][r] << 3) + acc[1][i][r];
+                    tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
+                    off[i][r] = __builtin_fmaf(Mm[r], grp.dmin * dv[r], off[i][r]);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int S = (acc[0][i][r] << 8) + acc[1][i][r];
+                    tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
+                }
+            }
+        }
+    }
+    const int n = wn0 + a, refused = flags[0];
+    if (n < A.N && !(refused && M.wref[row0 + n] != 0)) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int m = 16 * i + 4 * g + r;
+                if (m >= tile.m || (refused && A.act.ok[rows[m]] == 0)) continue;
+                A.y[(int64_t)outs[m] * A.N + n] = DT == DT_Q4_K ? tot[i][r] - off[i][r] : tot[i][r];
+            }
+    }
+    if (!refused) return;
+    for (int p = t >> 3; p < BN * tile.m; p += C::T / 8) {
+        const int c = p % BN, m = p / BN;
+        const int64_t w = row0 + n0 + c;
+        if (n0 + c >= A.N || (M.wref[w] == 0 && A.act.ok[rows[m]] != 0)) continue;
+        const float v = f32dot_g8<DT>(M.W + w * A.rb, A.x + (int64_t)rows[m] * A.K, A.K, true);
+        if ((t & 7) == 0) A.y[(int64_t)outs[m] * A.N + n0 + c] = v;
+    }
+}
+
 // The most tiles of BM pairs that any choice of that many could need: whole
 // ones, and one partly filled for each expert.
 static int64_t max_tiles(const Args& A, int BM) {
@@ -638,8 +827,29 @@ static hipError_t launch(const Args& A, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <uint32_t DT>
+static hipError_t launch_thin(const Args& A, hipStream_t stream) {
+    const int64_t wgs = (max_tiles(A, 32) * ((A.N + 63) / 64) + 7) / 8 * 8;
+    if (wgs * 256 >= (1ll << 32)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(thin_kernel<DT>, dim3((unsigned)wgs), dim3(256), 0, stream, A);
+    return hipGetLastError();
+}
+// Where they are taken, us of tiles of 32 / of 16 rows a wave (down, 8 experts,
+// two a token): Q6_K 8192 -> 2048, 8 tokens 67.3 / 46.7, 64 69.3 / 50.6, 14336 -> 4096,
+// 8 tokens 113 / 109, 128 tokens 175 / 152, 160 tokens (672 tiles of 32) 180 / 185; 16
+// experts, 8192 -> 4096, 64 tokens (616) 115 / 123; short rows, 64 experts, 1024 -> 2048
+// 44.2 / 41.8, 60 experts, 1536 51.5 / 48.3. Q4_K 8192 -> 2048, 64 tokens 46.1 / 41.7,
+// 14336 -> 4096, 8 tokens 72.6 / 75.6. Weights of two groups in LDS: 1 to 3 % slower.
+static bool thin(uint32_t dt, const Args& A) {
+    if (A.pairs >= 48 * (int64_t)A.experts) return false;
+    const int64_t wgs = max_tiles(A, 32) * ((A.N + 127) / 128);
+    return dt == DT_Q6_K ? wgs <= 512 || A.nb <= 8 : dt == DT_Q4_K && wgs <= 192;
+}
+
 template <uint32_t DT, bool SW>
 static hipError_t launch_dt(const Args& A, hipStream_t stream) {
+    if constexpr (!SW && DT != DT_Q8_0)
+        if (thin(DT, A)) return launch_thin<DT>(A, stream);
     // 64 pairs a workgroup where the experts have as many on average, of Q6_K
     // where they have 48, and 96 from that on (us a call in tiles of 32 / 64 / 96:
     // down 2048 x 1024, 64 experts, 32 pairs each 57.8 / 60.6 / -, 48 70.7 / 69.6 /

@@ -315,6 +315,16 @@ def test_last_tiles(gpu, rt, oracle, dt, experts, n, k, T, top, what):
     test_combine(gpu, rt, oracle, dt, experts, n, k, T, top, what)
 
 
+# tiles of 32 and of 16 weight rows a wave where the other ones of these sizes run
+GRIDS = [(Q4_K, 60, 530, 512, 33, 4, "padded"), (Q4_K, 9, 200, 1280, 60, 2, "even"), (Q4_K, 3, 65, 4864, 40, 1, "even"),
+         (Q6_K, 20, 1730, 2304, 150, 4, "padded"), (Q6_K, 60, 70, 2048, 90, 4, "even"), (Q6_K, 3, 79, 4864, 40, 1, "even")]
+
+
+@pytest.mark.parametrize("dt,experts,n,k,T,top,what", GRIDS)
+def test_rows_of_a_wave(gpu, rt, oracle, dt, experts, n, k, T, top, what):
+    test_combine(gpu, rt, oracle, dt, experts, n, k, T, top, what)
+
+
 # pairs each by itself where there are many more experts, and just above
 MANY = [(dt, experts, n, k, T, 8, what) for dt in (Q4_K, Q6_K) for experts, n, k, T, what in (
     (128, 24, 512, 3, "even"), (200, 16, 4096, 6, "padded"), (200, 16, 4096, 7, "even"), (128, 12, 256, 12, "again"),
@@ -461,6 +471,36 @@ def test_a_layer_captured_and_replayed(gpu, rt, oracle):
         s.sync()
         np.testing.assert_array_equal(bits(got), bits(eager.download(np.float32).reshape(T, k)))
     g.destroy()
+
+
+@pytest.mark.parametrize("dt,T,experts,n,k", [(dt, T, 3, 70, 512) for dt in (Q4_K, Q6_K, Q8_0) for T in (2, 70, 220)] +
+                         [(Q4_K, 100, 60, 520, 512), (Q6_K, 100, 60, 1154, 2304)])
+def test_refused_rows_of_the_sum(gpu, rt, oracle, dt, T, experts, n, k):
+    """The same for down, one choice of weight one."""
+    nb, off = {Q4_K: (144, 0), Q6_K: (210, 208), Q8_0: (34, 0)}[dt]
+
+    def edit(raw):
+        b = raw.reshape(experts, n, -1, nb)
+        b[1, 7, 0, off:off + 2] = [0, 0x7C]
+        b[2, n - 1, -1, off:off + 2] = [1, 0x7E]
+
+    down = Layer(gpu, oracle, dt, experts, n, k, 75, edit)
+    h, ids = acts_for(76, T, k), choices(77, T, 1, experts)
+    ids[:4, 0] = [0, 1, 2, 1][:T]
+    h[1, 9] = np.nan
+    h[0, k - 12] = 2.0 ** 61
+    got = run_combine(gpu, rt, down, h, np.ones((T, 1), np.float32), ids)
+    with np.errstate(all="ignore"):
+        for t in [*range(min(T, 6)), *range(6, T, 9)]:
+            e = ids[t, 0]
+            want = oracle.linear_a8(h[t:t + 1], down.raw[e], dt, n, k, block=32 if dt == Q8_0 else 256)[0]
+            np.testing.assert_array_equal(np.isnan(got[t]), np.isnan(want))
+            fine = ~np.isnan(want)
+            if dt == Q8_0:  # (its tiles' order)
+                fine &= np.isfinite(want)
+                assert (np.abs(got[t] - want)[fine] <= 8 * k * ref.EPS * np.abs(want[fine]).max(initial=0)).all()
+            else:
+                np.testing.assert_array_equal(bits(got[t][fine]), bits(want[fine]))
 
 
 class View:
