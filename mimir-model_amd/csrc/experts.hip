@@ -696,9 +696,36 @@ struct ThinGroup<DT_Q6_K> {
     }
 };
 
-template <uint32_t DT>
+// (AL: see Cfg) Blocks of 32 on v_mfma_i32_16x16x32_i8: of each block the lane
+// holds the elements 8 g .. 8 g + 7.
+template <bool AL>
+struct ThinGroupQ8 {
+    uint32_t w[8][3], sh;  // a block's 8 bytes in the dwords that hold them
+    float d[2];            // scales of the blocks 4 i + g
+    __device__ __forceinline__ void read(const uint8_t* wr, int g) {
+        sh = AL ? 2 : ((uint32_t)(uintptr_t)wr + 2) & 2;
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++) {
+            const uint8_t* p = wr + Q80_BYTES * ks + 2 + 8 * g;
+            const uint32_t* q = (const uint32_t*)(AL ? p - (ks & 1 ? 0 : 2) : __builtin_align_down(p, 4));
+            w[ks][0] = q[0];
+            w[ks][1] = q[1];
+            w[ks][2] = AL && (ks & 1) ? 0 : q[2];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) d[i] = f16_to_f32(lds_read2_a2(wr + Q80_BYTES * (4 * i + g)));
+    }
+    __device__ __forceinline__ long block(int ks) const {
+        const uint32_t s = ks & 1 ? 2 - sh : sh;
+        const uint32_t lo = AL && (ks & 1) ? w[ks][0] : __builtin_amdgcn_alignbyte(w[ks][1], w[ks][0], s);
+        const uint32_t hi = AL && (ks & 1) ? w[ks][1] : __builtin_amdgcn_alignbyte(w[ks][2], w[ks][1], s);
+        return (long)((uint64_t)hi << 32 | lo);
+    }
+};
+
+template <uint32_t DT, bool AL = false>
 __global__ __launch_bounds__(256, 4) void thin_kernel(Args A) {
-    using C = Cfg<DT, 1, false, 16>;
+    using C = Cfg<DT, 1, AL, 16>;
     constexpr int BM = 32, BN = 64;
     __shared__ __align__(16) uint8_t smem[C::SMEM];
     __shared__ int rows[BM], outs[64], flags[1];
@@ -733,58 +760,86 @@ __global__ __launch_bounds__(256, 4) void thin_kernel(Args A) {
     }
     float tot[2][4] = {}, off[2][4] = {};
     const uint32_t wmis = DT == DT_Q4_K ? 0 : (uint32_t)(uintptr_t)(M.W + (row0 + min(wn0 + a, A.N - 1)) * A.rb);
-    for (int b = 0; b < A.nb; b++) {
+    const int ng = C::K32 ? (A.nb + 7) / 8 : A.nb;
+    for (int b = 0; b < ng; b++) {
         wait_vmcnt<0>();
         lds_barrier();
         const uint8_t* buf = smem + C::WBYTES + (b & 1) * C::BUF;
-        ThinGroup<DT> grp;
+        std::conditional_t<C::K32, ThinGroupQ8<AL>, ThinGroup<DT>> grp;
         if constexpr (C::LINES) grp.read(smem + C::WWAVE * cp.wave, (uint32_t)(128 * a + 16 * ((a >> 1) & 7)), b, g);
-        else grp.read(smem + C::WWAVE * cp.wave + a * C::WSLOT + ((wmis + (uint32_t)b * C::GROUP) & 15u), g);
-        if (b + 1 < A.nb) {
+        else grp.read(smem + C::WWAVE * cp.wave + a * C::WSLOT + (AL ? 0 : (wmis + (uint32_t)b * C::GROUP) & 15u), g);
+        if (b + 1 < ng) {
             cp.activations(b + 1, lds0 + C::WBYTES + ((b + 1) & 1) * C::BUF);
             wait_lgkm0();
             cp.weights(b + 1, lds0);
         }
-        v4i acc[2][2];
-#pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            v4i pH, pL;
-            grp.planes(ks, g, pH, pL);
-            const v4i z = {};
+        if constexpr (C::K32) {
+            // d*dx of four blocks at a time as outer products (lanes g hold
+            // block 4 q + g's scales)
+            const float* dl = (const float*)(buf + C::ABYTES);
+            const int nk = min(8, A.nb - 8 * b);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const v4i av = *(const v4i*)(buf + (16 * i + a) * 256 + 16 * ((4 * ks + g) ^ a));
-                acc[0][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pH, ks ? acc[0][i] : z, 0, 0, 0);
-                acc[1][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pL, ks ? acc[1][i] : z, 0, 0, 0);
+                if (16 * i >= tile.m) break;
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const v16f zf = {};
+                    const v16f dd = __builtin_amdgcn_mfma_f32_16x16x1f32(dl[8 * (16 * i + a) + 4 * q + g], grp.d[q], zf, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int ks = 4 * q + k;
+                        if (ks < nk) {
+                            const long av = *(const long*)(buf + (16 * i + a) * 256 + 16 * ((2 * ks + (g >> 1)) ^ a) + 8 * (g & 1));
+                            const v4i z = {};
+                            const v4i S = __builtin_amdgcn_mfma_i32_16x16x32_i8(av, grp.block(ks), z, 0, 0, 0);
+#pragma unroll
+                            for (int r = 0; r < 4; r++) tot[i][r] = __builtin_fmaf((float)S[r], dd[4 * k + r], tot[i][r]);
+                        }
+                    }
+                }
             }
-        }
-        const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
+        } else {
+            v4i acc[2][2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float4 dx = *(const float4*)(dl + 16 * i + 4 * g);
-            const float dv[4] = {dx.x, dx.y, dx.z, dx.w};
-            if constexpr (DT == DT_Q4_K) {
-                // (k 16 .. 31 of the mins' product are zeros: lanes g = 2, 3)
-                v8h bm = {};
-                if (g < 2) {
-                    Group<DT_Q4_K> full;
-                    full.s.m = grp.m;
-                    bm = full.mins(g);
+            for (int ks = 0; ks < 4; ks++) {
+                v4i pH, pL;
+                grp.planes(ks, g, pH, pL);
+                const v4i z = {};
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const v4i av = *(const v4i*)(buf + (16 * i + a) * 256 + 16 * ((4 * ks + g) ^ a));
+                    acc[0][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pH, ks ? acc[0][i] : z, 0, 0, 0);
+                    acc[1][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pL, ks ? acc[1][i] : z, 0, 0, 0);
                 }
-                const v8h v = *(const v8h*)(buf + C::ABYTES + 32 * (16 * i + a) + 16 * (g & 1));
-                v4f Mm = {};
-                Mm = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, bm, Mm, 0, 0, 0);
+            }
+            const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int S = (acc[0][i][r] << 3) + acc[1][i][r];
-                    tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
-                    off[i][r] = __builtin_fmaf(Mm[r], grp.dmin * dv[r], off[i][r]);
-                }
-            } else {
+            for (int i = 0; i < 2; i++) {
+                const float4 dx = *(const float4*)(dl + 16 * i + 4 * g);
+                const float dv[4] = {dx.x, dx.y, dx.z, dx.w};
+                if constexpr (DT == DT_Q4_K) {
+                    // (k 16 .. 31 of the mins' product are zeros: lanes g = 2, 3)
+                    v8h bm = {};
+                    if (g < 2) {
+                        Group<DT_Q4_K> full;
+                        full.s.m = grp.m;
+                        bm = full.mins(g);
+                    }
+                    const v8h v = *(const v8h*)(buf + C::ABYTES + 32 * (16 * i + a) + 16 * (g & 1));
+                    v4f Mm = {};
+                    Mm = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, bm, Mm, 0, 0, 0);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int S = (acc[0][i][r] << 8) + acc[1][i][r];
-                    tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
+                    for (int r = 0; r < 4; r++) {
+                        const int S = (acc[0][i][r] << 3) + acc[1][i][r];
+                        tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
+                        off[i][r] = __builtin_fmaf(Mm[r], grp.dmin * dv[r], off[i][r]);
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int S = (acc[0][i][r] << 8) + acc[1][i][r];
+                        tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
+                    }
                 }
             }
         }
@@ -827,11 +882,11 @@ static hipError_t launch(const Args& A, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <uint32_t DT>
+template <uint32_t DT, bool AL = false>
 static hipError_t launch_thin(const Args& A, hipStream_t stream) {
     const int64_t wgs = (max_tiles(A, 32) * ((A.N + 63) / 64) + 7) / 8 * 8;
     if (wgs * 256 >= (1ll << 32)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(thin_kernel<DT>, dim3((unsigned)wgs), dim3(256), 0, stream, A);
+    hipLaunchKernelGGL((thin_kernel<DT, AL>), dim3((unsigned)wgs), dim3(256), 0, stream, A);
     return hipGetLastError();
 }
 // Where they are taken, us of tiles of 32 / of 16 rows a wave (down, 8 experts,
@@ -843,13 +898,17 @@ static hipError_t launch_thin(const Args& A, hipStream_t stream) {
 static bool thin(uint32_t dt, const Args& A) {
     if (A.pairs >= 48 * (int64_t)A.experts) return false;
     const int64_t wgs = max_tiles(A, 32) * ((A.N + 127) / 128);
-    return dt == DT_Q6_K ? wgs <= 512 || A.nb <= 8 : dt == DT_Q4_K && wgs <= 192;
+    return dt == DT_Q6_K ? wgs <= 512 || A.nb <= 8 : dt == DT_Q8_0 || wgs <= 192;
 }
 
 template <uint32_t DT, bool SW>
 static hipError_t launch_dt(const Args& A, hipStream_t stream) {
-    if constexpr (!SW && DT != DT_Q8_0)
-        if (thin(DT, A)) return launch_thin<DT>(A, stream);
+    if constexpr (!SW)
+        if (thin(DT, A)) {
+            if constexpr (DT == DT_Q8_0)
+                if (A.rb % 4 == 0 && (uintptr_t)A.mat[0].W % 4 == 0) return launch_thin<DT, true>(A, stream);
+            return launch_thin<DT>(A, stream);
+        }
     // 64 pairs a workgroup where the experts have as many on average, of Q6_K
     // where they have 48, and 96 from that on (us a call in tiles of 32 / 64 / 96:
     // down 2048 x 1024, 64 experts, 32 pairs each 57.8 / 60.6 / -, 48 70.7 / 69.6 /
