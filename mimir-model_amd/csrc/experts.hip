@@ -623,7 +623,8 @@ __global__ __launch_bounds__(C::T, C::OCC) void tile_kernel(Args A) {
     }
 }
 
-// The same products with 16 weight rows a wave, on v_mfma_i32_16x16x64_i8, and 32
+// The same products with 16 weight rows a wave, on v_mfma_i32_16x16x64_i8 (Q8_0,
+// whose blocks have a sum each, on 16x16x32), and 32
 // pairs: half the unpacking a wave and twice the waves, where tiles of 32 rows a
 // wave leave SIMDs without one. Lane l holds weight row a = l % 16 and of a k step
 // of 64 the elements 16 g .. 16 g + 15, g = l / 16; of a 16 x 16 result the pairs
@@ -799,49 +800,57 @@ __global__ __launch_bounds__(256, 4) void thin_kernel(Args A) {
                 }
             }
         } else {
-            v4i acc[2][2];
+            // Q6_K: the second half of the pairs only where there are any (16
+            // tokens of 60 experts and the like 3 to 5 % faster; Q4_K loses 2 % with
+            // more pairs than that and gains 3 % below).
+            auto products = [&](auto live) __attribute__((always_inline)) {
+                constexpr int I = decltype(live)::value;
+                v4i acc[2][I];
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                v4i pH, pL;
-                grp.planes(ks, g, pH, pL);
-                const v4i z = {};
+                for (int ks = 0; ks < 4; ks++) {
+                    v4i pH, pL;
+                    grp.planes(ks, g, pH, pL);
+                    const v4i z = {};
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const v4i av = *(const v4i*)(buf + (16 * i + a) * 256 + 16 * ((4 * ks + g) ^ a));
-                    acc[0][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pH, ks ? acc[0][i] : z, 0, 0, 0);
-                    acc[1][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pL, ks ? acc[1][i] : z, 0, 0, 0);
-                }
-            }
-            const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float4 dx = *(const float4*)(dl + 16 * i + 4 * g);
-                const float dv[4] = {dx.x, dx.y, dx.z, dx.w};
-                if constexpr (DT == DT_Q4_K) {
-                    // (k 16 .. 31 of the mins' product are zeros: lanes g = 2, 3)
-                    v8h bm = {};
-                    if (g < 2) {
-                        Group<DT_Q4_K> full;
-                        full.s.m = grp.m;
-                        bm = full.mins(g);
-                    }
-                    const v8h v = *(const v8h*)(buf + C::ABYTES + 32 * (16 * i + a) + 16 * (g & 1));
-                    v4f Mm = {};
-                    Mm = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, bm, Mm, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int S = (acc[0][i][r] << 3) + acc[1][i][r];
-                        tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
-                        off[i][r] = __builtin_fmaf(Mm[r], grp.dmin * dv[r], off[i][r]);
-                    }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int S = (acc[0][i][r] << 8) + acc[1][i][r];
-                        tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
+                    for (int i = 0; i < I; i++) {
+                        const v4i av = *(const v4i*)(buf + (16 * i + a) * 256 + 16 * ((4 * ks + g) ^ a));
+                        acc[0][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pH, ks ? acc[0][i] : z, 0, 0, 0);
+                        acc[1][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, pL, ks ? acc[1][i] : z, 0, 0, 0);
                     }
                 }
-            }
+                const float* dl = (const float*)(buf + C::ABYTES + C::XBYTES);
+#pragma unroll
+                for (int i = 0; i < I; i++) {
+                    const float4 dx = *(const float4*)(dl + 16 * i + 4 * g);
+                    const float dv[4] = {dx.x, dx.y, dx.z, dx.w};
+                    if constexpr (DT == DT_Q4_K) {
+                        // (k 16 .. 31 of the mins' product are zeros: lanes g = 2, 3)
+                        v8h bm = {};
+                        if (g < 2) {
+                            Group<DT_Q4_K> full;
+                            full.s.m = grp.m;
+                            bm = full.mins(g);
+                        }
+                        const v8h v = *(const v8h*)(buf + C::ABYTES + 32 * (16 * i + a) + 16 * (g & 1));
+                        v4f Mm = {};
+                        Mm = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, bm, Mm, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int S = (acc[0][i][r] << 3) + acc[1][i][r];
+                            tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
+                            off[i][r] = __builtin_fmaf(Mm[r], grp.dmin * dv[r], off[i][r]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int S = (acc[0][i][r] << 8) + acc[1][i][r];
+                            tot[i][r] = __builtin_fmaf((float)S, grp.d * dv[r], tot[i][r]);
+                        }
+                    }
+                }
+            };
+            if (DT == DT_Q6_K && tile.m <= 16) products(std::integral_constant<int, 1>());
+            else products(std::integral_constant<int, 2>());
         }
     }
     const int n = wn0 + a, refused = flags[0];
@@ -894,7 +903,10 @@ static hipError_t launch_thin(const Args& A, hipStream_t stream) {
 // 8 tokens 113 / 109, 128 tokens 175 / 152, 160 tokens (672 tiles of 32) 180 / 185; 16
 // experts, 8192 -> 4096, 64 tokens (616) 115 / 123; short rows, 64 experts, 1024 -> 2048
 // 44.2 / 41.8, 60 experts, 1536 51.5 / 48.3. Q4_K 8192 -> 2048, 64 tokens 46.1 / 41.7,
-// 14336 -> 4096, 8 tokens 72.6 / 75.6. Weights of two groups in LDS: 1 to 3 % slower.
+// 14336 -> 4096, 8 tokens 72.6 / 75.6. Q8_0 60 experts, four a token, 1408 -> 2048,
+// 37 tokens 49.9 / 45.4, 181 57.9 / 56.3, 1440 -> 2048 54.3 / 45.6; two of 8, 14336 ->
+// 4096, 64 tokens 150 / 137. Weights of two groups in LDS: 1 to 3 % slower. Gate and
+// up this way: Q8_0 2048 x 1408 1 to 3 % faster, 4096 x 14336 and Q4_K 7 to 15 % slower.
 static bool thin(uint32_t dt, const Args& A) {
     if (A.pairs >= 48 * (int64_t)A.experts) return false;
     const int64_t wgs = max_tiles(A, 32) * ((A.N + 127) / 128);
