@@ -956,18 +956,18 @@ static bool few_pairs_swiglu(const DevWeight& w, int pairs, int experts) {
     if (pairs <= (w.dt == DT_Q8_0 ? 4 : 8) || (pairs <= 16 && experts >= 2 * pairs)) return true;
     return w.dt != DT_Q8_0 && experts >= 4 * pairs && pairs <= (w.k >= 4096 ? 48 : 24);
 }
-// down with the sum in its launch, alone / in tiles: 4096 x 14336, 8 experts, 2
-// / 4 / 8 / 16 pairs Q6_K 28 / 45 / 74 / 130 against 111 / 111 / 112 / 113, 12 /
-// 16 pairs Q4_K 66 / 82 against 73 / 74; 2048 x 1024 Q4_K, 64 experts, 8 / 16 /
-// 32 / 64 pairs 8.7 / 10.0 / 13.0 / 19.3 against 15.5 / 16.5 / 19.6 / 24.9; 2048 x
-// 1536 Q6_K, 60 experts, 32 / 48 pairs 27.1 / 35.4 against 29.8 / 35.1; Q8_0 2048 x
-// 1408, 60 experts, 16 / 32 / 64 pairs 18.1 / 28.5 / 44.2 against 26.2 / 33.8 / 47.8.
-// 128 experts, 72 / 96 / 128 pairs: 768 -> 2048 Q4_K 20.7 / 24.6 / 28.8 against 28.8 /
-// 31.6 / 34.2, Q6_K 30.8 / 37.2 / 44.7 against 35.0 / 38.2 / 41.5, Q8_0 31.8 / 37.4 /
-// 45.5 against 33.9 / 36.8 / 41.6; 1536 -> 4096 Q4_K 52 / 66 / 84 against 60 / 69 / 79,
-// Q6_K 86 / - / 142 against 83 / - / 113.
+// down with the sum in its launch, alone / in tiles: 14336 -> 4096, 8 experts, 2 /
+// 4 / 8 / 12 / 16 pairs Q6_K 28 / 45 / 75 / 102 / 131 against 70 / 72 / 88 / 98 / 105, 12 /
+// 16 pairs Q4_K 66 / 83 against 70 / 72, 8 pairs Q8_0 91 against 83; 1024 -> 2048
+// Q4_K, 64 experts, 8 / 16 / 32 / 64 pairs 8.8 / 10.1 / 13.0 / 19.6 against 15.1 /
+// 16.5 / 19.3 / 24.5; 60 experts, 32 / 48 pairs, 1536 -> 2048 Q6_K 27.2 / 35.6 against
+// 26.7 / 32.0; 1408 -> 2048 Q8_0, 16 / 32 / 48 / 64 pairs 18.3 / 28.4 / 37.0 / 44.3 against
+// 19.8 / 29.7 / 34.0 / 37.4. 128 experts, 72 / 96 / 128 pairs: 768 -> 2048 Q4_K 20.7 /
+// 24.6 / 28.8 against 28.8 / 31.6 / 34.2, 1536 -> 4096 52 / 66 / 84 against 60 / 69 / 79.
 static bool few_pairs_combine(uint32_t dt, int pairs, int experts) {
-    return pairs <= 8 || (pairs <= (dt == DT_Q4_K ? 128 : 64) && experts >= pairs);
+    if (pairs <= (dt == DT_Q8_0 ? 4 : 8)) return true;
+    if (dt == DT_Q4_K) return pairs <= 128 && experts >= pairs;
+    return pairs <= 32 ? 2 * experts >= 3 * pairs : pairs <= 64 && experts >= 2 * pairs;
 }
 
 bool experts_ok(const DevWeight& w) {

@@ -15,7 +15,7 @@
 // ones. In tiles, whose rows of 32 pairs are mostly empty here, a workgroup
 // reads its rows group after group. One token, us a call alone / in tiles: gate
 // and up 2048 x 1408 of four choices 11.0 / 21.3, 4096 x 7168 of two 30.8 / 40.2;
-// down 2048 x 1408 9.6 / 22.0, 4096 x 14336 32.9 / 117.
+// down 2048 x 1408 9.7 / 15.6, 4096 x 14336 33 / 70.
 #include "decoder_math.hpp"
 #include "experts.hpp"
 #include "f32path.hpp"
