@@ -437,7 +437,7 @@ template <int V>
 __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ part, const float* __restrict__ weights,
                                                       const int32_t* __restrict__ expert, int top, int64_t N,
                                                       float* __restrict__ y) {
-    const int64_t t = blockIdx.x, n = ((int64_t)blockIdx.y * 256 + threadIdx.x) * V;
+    const int64_t t = blockIdx.x, n = (((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 256 + threadIdx.x) * V;
     if (n >= N) return;
     float s[V];
 #pragma unroll
@@ -545,12 +545,15 @@ hipError_t launch_experts_quantize(uint32_t dt, const float* x, int64_t rows, in
 
 hipError_t launch_experts_sum(const float* part, const float* weights, const int32_t* expert, int64_t T, int top, int64_t N,
                               float* y, hipStream_t s) {
-    if (N % 4 == 0)
-        hipLaunchKernelGGL(xr::combine_kernel<4>, dim3((unsigned)T, (unsigned)((N / 4 + 255) / 256)), dim3(256), 0, s, part,
-                           weights, expert, top, N, y);
-    else
-        hipLaunchKernelGGL(xr::combine_kernel<1>, dim3((unsigned)T, (unsigned)((N + 255) / 256)), dim3(256), 0, s, part,
-                           weights, expert, top, N, y);
+    // (a grid has at most 65535 workgroups in y, and less than 2^32 threads)
+    const int64_t wgs = ((N % 4 ? N : N / 4) + 255) / 256, layers = (wgs + 65534) / 65535;
+    const int64_t most = ((1ll << 24) - 1) / ((wgs + layers - 1) / layers * layers);  // tokens of a launch
+    for (int64_t t = 0; t < T; t += most) {
+        const dim3 grid((unsigned)(T - t < most ? T - t : most), (unsigned)((wgs + layers - 1) / layers), (unsigned)layers);
+        const float *p = part + t * top * N, *w = weights + t * top;
+        if (N % 4 == 0) hipLaunchKernelGGL(xr::combine_kernel<4>, grid, dim3(256), 0, s, p, w, expert + t * top, top, N, y + t * N);
+        else hipLaunchKernelGGL(xr::combine_kernel<1>, grid, dim3(256), 0, s, p, w, expert + t * top, top, N, y + t * N);
+    }
     return hipGetLastError();
 }
 

@@ -1,0 +1,53 @@
+"""Experts of so many rows that a launch of one workgroup for every few of them
+passes the sizes that a grid may have: the same rows over and over, each result
+as that of a matrix of these rows alone."""
+import numpy as np
+import pytest
+
+import experts_ref as ref
+from test_gpu_experts import Q4_K, Q8_0, acts_for, bits, run_combine, run_swiglu, rt  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+class Repeated:
+    """`experts` experts of n rows each, all of them `period` rows over and over
+    (written on the device); alone: one expert of these rows."""
+
+    def __init__(self, gpu, rt, oracle, dt, experts, n, period, k, seed):
+        self.dt, self.experts, self.n, self.k = dt, experts, n, k
+        raw = oracle.synthetic_weight(dt, period, k, seed=seed, scale=1 / np.sqrt(k)).reshape(-1)
+        assert n % period == 0
+        whole, s, at = rt.DeviceBuffer(raw.size * (experts * n // period)), rt.Stream(), raw.size
+        whole.upload(raw)
+        while at < whole.nbytes:
+            rt.copy_async(whole.ptr + at, whole.ptr, min(at, whole.nbytes - at), s)
+            at *= 2
+        s.sync()
+        self.w = gpu.Weight((whole.ptr, whole.nbytes), dt, experts * n, k, device=True)
+        whole.free()
+        self.alone = type("Alone", (), dict(dt=dt, experts=1, n=period, k=k, w=gpu.Weight(raw, dt, period, k)))
+
+
+def same_rows(got, want):
+    """got [rows, n] is want [rows, period] over and over, bit for bit."""
+    for g, w in zip(got, want):
+        assert (bits(g).reshape(-1, w.size) == bits(w)[None]).all()
+
+
+def test_the_sum_over_rows_past_a_grid(gpu, rt, oracle):  # noqa: F811
+    """Odd rows, so that a thread of the sum has one: 65538 workgroups of 256."""
+    down = Repeated(gpu, rt, oracle, Q8_0, 1, 255 * 65795, 255, 32, 1)
+    assert down.n % 4 and down.n > 65536 * 256
+    h, ids = acts_for(2, 5, 32), np.zeros((5, 1), np.int32)
+    weights = np.random.default_rng(3).random((5, 1), np.float32)
+    same_rows(run_combine(gpu, rt, down, h, weights, ids), run_combine(gpu, rt, down.alone, h, weights, ids))
+
+
+def test_the_sum_of_tokens_past_a_grid(gpu, rt, oracle):  # noqa: F811
+    """270 tokens of 65538 workgroups each, more than 2^32 threads together."""
+    T, n = 270, 255 * 65795
+    down = Repeated(gpu, rt, oracle, Q8_0, 1, n, 255, 32, 4)
+    h, ids = acts_for(5, T, 32), np.zeros((T, 1), np.int32)
+    weights = np.random.default_rng(6).random((T, 1), np.float32)
+    same_rows(run_combine(gpu, rt, down, h, weights, ids), run_combine(gpu, rt, down.alone, h, weights, ids))
