@@ -1015,12 +1015,12 @@ static hipError_t launch_tiles(const DevWeight* const* ws, int nmat, int experts
 hipError_t launch_experts_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, void* parts,
                                  const float* x, int64_t T, int top, const int32_t* plan, float* h, hipStream_t stream) {
     const int pairs = (int)(T * top);
-    if (few_pairs_swiglu(gate, pairs, experts) && gemv_experts_swiglu_ok(gate, experts)) {
+    if (few_pairs_swiglu(gate, pairs, experts) && gemv_experts_swiglu_ok(gate, experts, pairs)) {
         const hipError_t e = launch_quantize_act(x, T, gate.k, 256, a, stream);
         if (e != hipSuccess) return e;
         return launch_gemv_experts_swiglu(gate, up, experts, a, x, T, top, plan + plan_layout(pairs, experts).expert, h, stream);
     }
-    if (few_pairs_swiglu(gate, pairs, experts) && gemv_experts_q8_ok(gate, 2)) {
+    if (few_pairs_swiglu(gate, pairs, experts) && gemv_experts_q8_ok(gate, experts, 2, pairs)) {
         const hipError_t e = launch_quantize_act(x, T, gate.k, 32, a, stream);
         if (e != hipSuccess) return e;
         return launch_gemv_experts_q8_swiglu(gate, up, experts, a, x, T, top, plan + plan_layout(pairs, experts).expert, h, stream);
@@ -1034,11 +1034,11 @@ hipError_t launch_experts_combine(const DevWeight& w, int experts, const ActPtrs
                                   hipStream_t stream) {
     const int pairs = (int)(T * top);
     const int32_t* expert = plan + plan_layout(pairs, experts).expert;
-    if (few_pairs_combine(w.dt, pairs, experts) && gemv_experts_sum_ok(w, experts, top)) {
+    if (few_pairs_combine(w.dt, pairs, experts) && gemv_experts_sum_ok(w, experts, T, top)) {
         const hipError_t e = launch_quantize_act(h, pairs, w.k, 256, a, stream);
         return e != hipSuccess ? e : launch_gemv_experts_sum(w, experts, a, h, weights, T, top, expert, y, stream);
     }
-    if (few_pairs_combine(w.dt, pairs, experts) && gemv_experts_q8_ok(w, top)) {
+    if (few_pairs_combine(w.dt, pairs, experts) && gemv_experts_q8_ok(w, experts, top, T)) {
         const hipError_t e = launch_quantize_act(h, pairs, w.k, 32, a, stream);
         return e != hipSuccess ? e : launch_gemv_experts_q8_sum(w, experts, a, h, weights, T, top, expert, y, stream);
     }

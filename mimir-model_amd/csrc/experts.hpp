@@ -26,6 +26,10 @@ __host__ __device__ __forceinline__ PlanLayout plan_layout(int64_t pairs, int ex
     return l;
 }
 
+// Whether a workgroup of 256 for every four rows of an expert, `groups` times
+// over, is a grid (less than 2^32 threads).
+inline bool experts_gemv_grid(int64_t n, int64_t groups) { return (n + 3) / 4 * groups < (1ll << 24); }
+
 // A pair's expert as the plan has it, held to the call's own experts: a plan of
 // another call gives wrong results, and no access elsewhere.
 __device__ __forceinline__ int plan_expert(const int32_t* expert, int64_t pair, int experts) {

@@ -147,7 +147,10 @@ static Args args(const DevWeight& w, int experts, const ActPtrs& a, const float*
 }  // namespace xq
 
 // (the table within 60 KB of LDS)
-bool gemv_experts_q8_ok(const DevWeight& w, int sets) { return w.dt == DT_Q8_0 && xq::lds_bytes(sets, w.k / 32) <= 60 * 1024; }
+bool gemv_experts_q8_ok(const DevWeight& w, int experts, int sets, int64_t groups) {
+    static_assert(xq::ROWS == 4, "rows of a workgroup");
+    return w.dt == DT_Q8_0 && xq::lds_bytes(sets, w.k / 32) <= 60 * 1024 && experts_gemv_grid(w.n / experts, groups);
+}
 
 hipError_t launch_gemv_experts_q8_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, const float* x,
                                          int64_t T, int top, const int32_t* expert, float* h, hipStream_t stream) {

@@ -575,9 +575,10 @@ __global__ __launch_bounds__(256) void gemv_experts_sum_kernel(GemvArgs A, const
     }
 }
 
-// Shapes that both kernels take.
-static bool gemv_experts_ok(const DevWeight& w, int experts) {
-    return (w.dt == DT_Q4_K || w.dt == DT_Q6_K) && w.k % 256 == 0 && w.n / experts <= (1 << 30);
+// Shapes that both kernels take, in `groups` rows of workgroups.
+static bool gemv_experts_ok(const DevWeight& w, int experts, int64_t groups) {
+    static_assert(PAIRS_U == 4, "rows of a workgroup");
+    return (w.dt == DT_Q4_K || w.dt == DT_Q6_K) && w.k % 256 == 0 && experts_gemv_grid(w.n / experts, groups);
 }
 
 static GemvArgs experts_args(const DevWeight& w, int experts, const ActPtrs& a, const float* x) {
@@ -597,8 +598,8 @@ static GemvArgs experts_args(const DevWeight& w, int experts, const ActPtrs& a, 
     return A;
 }
 
-bool gemv_experts_swiglu_ok(const DevWeight& w, int experts) {
-    return gemv_experts_ok(w, experts) && w.k <= 65536 && w.n / experts % PAIRS_U == 0;
+bool gemv_experts_swiglu_ok(const DevWeight& w, int experts, int pairs) {
+    return gemv_experts_ok(w, experts, pairs) && w.k <= 65536 && w.n / experts % PAIRS_U == 0;
 }
 
 hipError_t launch_gemv_experts_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, const float* x,
@@ -620,8 +621,8 @@ hipError_t launch_gemv_experts_swiglu(const DevWeight& gate, const DevWeight& up
     return hipGetLastError();
 }
 
-bool gemv_experts_sum_ok(const DevWeight& w, int experts, int top) {
-    return gemv_experts_ok(w, experts) && w.n * w.row_bytes + WEIGHT_PAD < (1ll << 32) && top * PAIRS_U <= 256 && (int64_t)top * PAIRS_U * (w.k / 256) * 16 <= 48 * 1024;
+bool gemv_experts_sum_ok(const DevWeight& w, int experts, int64_t T, int top) {
+    return gemv_experts_ok(w, experts, T) && w.n * w.row_bytes + WEIGHT_PAD < (1ll << 32) && top * PAIRS_U <= 256 && (int64_t)top * PAIRS_U * (w.k / 256) * 16 <= 48 * 1024;
 }
 
 hipError_t launch_gemv_experts_sum(const DevWeight& w, int experts, const ActPtrs& a, const float* x, const float* weights,

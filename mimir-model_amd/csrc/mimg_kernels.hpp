@@ -260,15 +260,16 @@ hipError_t launch_experts_swiglu(const DevWeight& gate, const DevWeight& up, int
 hipError_t launch_experts_quantize(uint32_t dt, const float* x, int64_t rows, int64_t K, const ActPtrs& a, void* parts,
                                    hipStream_t s);
 // The same for few pairs, each with a row of workgroups of its own (gemv_kquant.hip).
-bool gemv_experts_swiglu_ok(const DevWeight& w, int experts);
+bool gemv_experts_swiglu_ok(const DevWeight& w, int experts, int pairs);
 hipError_t launch_gemv_experts_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, const float* x,
                                       int64_t T, int top, const int32_t* expert, float* h, hipStream_t s);
 // The products of the pairs with the weighted sum in the same launch.
-bool gemv_experts_sum_ok(const DevWeight& w, int experts, int top);
+bool gemv_experts_sum_ok(const DevWeight& w, int experts, int64_t T, int top);
 hipError_t launch_gemv_experts_sum(const DevWeight& w, int experts, const ActPtrs& a, const float* x, const float* weights,
                                    int64_t T, int top, const int32_t* expert, float* y, hipStream_t s);
-// Both for Q8_0 (experts_q8.hip); sets: 2 (gate and up), or top.
-bool gemv_experts_q8_ok(const DevWeight& w, int sets);
+// Both for Q8_0 (experts_q8.hip); sets: 2 (gate and up), or top; groups: the pairs,
+// or the tokens.
+bool gemv_experts_q8_ok(const DevWeight& w, int experts, int sets, int64_t groups);
 hipError_t launch_gemv_experts_q8_swiglu(const DevWeight& gate, const DevWeight& up, int experts, const ActPtrs& a, const float* x,
                                          int64_t T, int top, const int32_t* expert, float* h, hipStream_t s);
 hipError_t launch_gemv_experts_q8_sum(const DevWeight& w, int experts, const ActPtrs& a, const float* x, const float* weights,
