@@ -41,6 +41,7 @@
 //
 // Rows of x the quantizer refused and weight rows with a non-finite block
 // scale take the float32 path (f32path.hpp) at the end.
+#include <algorithm>
 #include <type_traits>
 
 #include "decoder_math.hpp"
@@ -71,6 +72,7 @@ struct Args {
     const int32_t* plan;
     int64_t rb, K;
     int64_t wbytes;       // bytes of a matrix of all experts
+    int64_t wg0;          // workgroups of the launches before this one
     int N, nb, experts, pairs;  // nb: blocks (of 256; of 32 for Q8_0) of a row
     int rowdiv;           // a pair's activation row is pair / rowdiv
     ActPtrs act;
@@ -158,7 +160,7 @@ __device__ __forceinline__ bool find_tile_of(const Args& A, int ntn, int BM, Til
         total = __builtin_amdgcn_readlane(upto[i], 63);
     }
     const int64_t all = (int64_t)total * ntn, per = (all + 7) / 8;
-    const int64_t wg = blockIdx.x, idx = (wg & 7) * per + (wg >> 3);
+    const int64_t wg = A.wg0 + blockIdx.x, idx = (wg & 7) * per + (wg >> 3);
     if ((wg >> 3) >= per || idx >= all) return false;
     const int u = (int)(idx / ntn);
 #pragma unroll
@@ -881,22 +883,27 @@ static int64_t max_tiles(const Args& A, int BM) {
     return (A.pairs + some * (BM - 1)) / BM;
 }
 
+// A workgroup for every tile of BM pairs and BN weight rows, in launches of 2^31
+// threads (a grid has less than 2^32): 512 experts of a pair each reach the second
+// one at 2^20 rows of 64 a tile.
+static hipError_t launch_grid(void (*kernel)(Args), Args A, int BM, int BN, hipStream_t stream) {
+    constexpr int64_t MOST = 1 << 23;
+    const int64_t wgs = (max_tiles(A, BM) * ((A.N + BN - 1) / BN) + 7) / 8 * 8;
+    for (A.wg0 = 0; A.wg0 < wgs; A.wg0 += MOST)
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(wgs - A.wg0, MOST)), dim3(256), 0, stream, A);
+    return hipGetLastError();
+}
+
 template <uint32_t DT, int MT, bool SW, bool AL = false>
 static hipError_t launch(const Args& A, hipStream_t stream) {
     using C = Cfg<DT, MT, AL>;
-    const int BN = SW ? 64 : 128;
-    const int64_t wgs = (max_tiles(A, C::BM) * ((A.N + BN - 1) / BN) + 7) / 8 * 8;
-    if (wgs * C::T >= (1ll << 32)) return hipErrorInvalidValue;  // (275 GB of results)
-    hipLaunchKernelGGL((tile_kernel<DT, C, SW>), dim3((unsigned)wgs), dim3(C::T), 0, stream, A);
-    return hipGetLastError();
+    static_assert(C::T == 256, "threads of a workgroup");
+    return launch_grid(tile_kernel<DT, C, SW>, A, C::BM, SW ? 64 : 128, stream);
 }
 
 template <uint32_t DT, bool AL = false>
 static hipError_t launch_thin(const Args& A, hipStream_t stream) {
-    const int64_t wgs = (max_tiles(A, 32) * ((A.N + 63) / 64) + 7) / 8 * 8;
-    if (wgs * 256 >= (1ll << 32)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((thin_kernel<DT, AL>), dim3((unsigned)wgs), dim3(256), 0, stream, A);
-    return hipGetLastError();
+    return launch_grid(thin_kernel<DT, AL>, A, 32, 64, stream);
 }
 // Where they are taken, us of tiles of 32 / of 16 rows a wave (down, 8 experts,
 // two a token): Q6_K 8192 -> 2048, 8 tokens 67.3 / 46.7, 64 69.3 / 50.6, 14336 -> 4096,

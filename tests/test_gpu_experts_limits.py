@@ -61,3 +61,19 @@ def test_few_pairs_of_rows_past_a_grid(gpu, rt, oracle, dt, k, n, T):  # noqa: F
     same_rows(run_swiglu(gpu, rt, w, w, x, ids), run_swiglu(gpu, rt, w.alone, w.alone, x, ids))
     weights = np.random.default_rng(9).random((T, 1), np.float32)
     same_rows(run_combine(gpu, rt, w, x, weights, ids), run_combine(gpu, rt, w.alone, x, weights, ids))
+
+
+def test_tiles_past_a_grid(gpu, rt, oracle):  # noqa: F811
+    """A pair for each of 512 experts of 2^21 rows and more: more than 2^24 tiles
+    of 64 rows, 36 GB of weights."""
+    n = 96 * ((1 << 21) // 96 + 3)
+    w = Repeated(gpu, rt, oracle, Q8_0, 512, n, 96, 32, 10)
+    assert n * 512 > 64 << 24
+    x = np.tile(acts_for(11, 16, 32), (32, 1))
+    ids = np.random.default_rng(12).permutation(512).astype(np.int32)[:, None]
+    alone = np.zeros((16, 1), np.int32)
+    want = run_swiglu(gpu, rt, w.alone, w.alone, x[:16], alone)
+    same_rows(run_swiglu(gpu, rt, w, w, x, ids), np.tile(want, (32, 1)))
+    weights = np.tile(np.random.default_rng(13).random((16, 1), np.float32), (32, 1))
+    want = run_combine(gpu, rt, w.alone, x[:16], weights[:16], alone)
+    same_rows(run_combine(gpu, rt, w, x, weights, ids), np.tile(want, (32, 1)))
