@@ -658,7 +658,8 @@ int mimg_experts_route_dev(const float *x, const float *router, int64_t T, int64
  * be of the same T, top and experts. ws:
  * mimg_experts_swiglu_workspace_bytes, 256-byte aligned. Returns
  * MIMG_NOT_HANDLED (nothing launched) for weights of different dtypes or of
- * one without such a product. */
+ * one without such a product, of 2^31 rows or more, of more than 2^30 an expert,
+ * or of rows of 64 MiB. */
 uint64_t mimg_experts_swiglu_workspace_bytes(int64_t T, int top, int64_t n, int64_t k);
 int mimg_experts_swiglu_a8_dev(uint64_t gate, uint64_t up, int experts, const float *x, int64_t T, int top, const void *plan,
                                uint64_t plan_bytes, float *h, void *ws, uint64_t ws_bytes, void *stream);

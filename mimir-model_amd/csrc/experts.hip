@@ -977,10 +977,11 @@ static bool few_pairs_combine(uint32_t dt, int pairs, int experts) {
     return pairs <= 32 ? 2 * experts >= 3 * pairs : pairs <= 64 && experts >= 2 * pairs;
 }
 
-bool experts_ok(const DevWeight& w) {
+// (rows of an expert are counted in 32 bits, with a tile's past the last one)
+bool experts_ok(const DevWeight& w, int experts) {
     const bool k256 = w.dt == DT_Q4_K || w.dt == DT_Q6_K;
     return (k256 || w.dt == DT_Q8_0) && w.k % (k256 ? 256 : 32) == 0 && (uintptr_t)w.data % (w.dt == DT_Q4_K ? 16 : 2) == 0 &&
-           w.n <= (1ll << 31) - 1 && w.row_bytes < (1 << 26);
+           w.n <= (1ll << 31) - 1 && w.n / experts <= (1ll << 30) && w.row_bytes < (1 << 26);
 }
 
 // The tiles' products of ws[0], or swiglu of those of ws[0] and ws[1].

@@ -1754,9 +1754,9 @@ static int check_experts_product(const char* what, const Weight* w, const Weight
     const DevWeight& d = w->dw;
     if (d.n % experts) return fail(MIMG_ERR_ARG, "%s: %lld rows are not those of %d experts", what, (long long)d.n, experts);
     if (other && (other->dw.n != d.n || other->dw.k != d.k)) return fail(MIMG_ERR_ARG, "%s: gate and up must have one shape", what);
-    if ((other && other->dw.dt != d.dt) || !experts_ok(d) || (other && !experts_ok(other->dw)))
-        return fail(MIMG_NOT_HANDLED, "%s: no product for %s%s%s weights of K = %lld", what, dt_name(d.dt), other ? " and " : "",
-                    other ? dt_name(other->dw.dt) : "", (long long)d.k);
+    if ((other && other->dw.dt != d.dt) || !experts_ok(d, experts) || (other && !experts_ok(other->dw, experts)))
+        return fail(MIMG_NOT_HANDLED, "%s: no product for %s%s%s weights of K = %lld, %d experts of %lld rows", what, dt_name(d.dt),
+                    other ? " and " : "", other ? dt_name(other->dw.dt) : "", (long long)d.k, experts, (long long)(d.n / experts));
     *n = d.n / experts;
     *k = d.k;
     if (T == 0) return MIMG_OK;

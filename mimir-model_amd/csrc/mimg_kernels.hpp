@@ -245,7 +245,7 @@ uint64_t experts_route_ws_bytes(int64_t T, int experts);
 hipError_t launch_experts_route(const float* x, const float* router, int64_t T, int64_t K, int experts, int top, int normalize,
                                 int32_t* ids, float* weights, int32_t* plan, double* logits, hipStream_t s);
 hipError_t launch_experts_plan(const int32_t* ids, int64_t T, int top, int experts, int32_t* plan, hipStream_t s);
-bool experts_ok(const DevWeight& w);
+bool experts_ok(const DevWeight& w, int experts);
 // The weighted sum of each token's products (mimg_experts_combine_a8_dev): product
 // [T * top, N] is scratch.
 hipError_t launch_experts_combine(const DevWeight& w, int experts, const ActPtrs& a, void* parts, const float* h,

@@ -77,3 +77,14 @@ def test_tiles_past_a_grid(gpu, rt, oracle):  # noqa: F811
     weights = np.tile(np.random.default_rng(13).random((16, 1), np.float32), (32, 1))
     want = run_combine(gpu, rt, w.alone, x[:16], weights[:16], alone)
     same_rows(run_combine(gpu, rt, w, x, weights, ids), np.tile(want, (32, 1)))
+
+
+def test_experts_of_too_many_rows_are_not_handled(gpu, rt, oracle):  # noqa: F811
+    """2^30 rows are an expert's most; nothing is launched."""
+    n = (1 << 30) + 128
+    w = Repeated(gpu, rt, oracle, Q8_0, 1, n, 128, 32, 14)
+    L, B = gpu.load(), rt.DeviceBuffer
+    x, weights, y, plan, ws = B(128), B(4), B(n * 4), B(1 << 12), B(n * 4 + (1 << 16))
+    nb = gpu.experts_plan_bytes(1, 1, 1)
+    assert L.mimg_experts_swiglu_a8_dev(w.w.handle, w.w.handle, 1, x.ptr, 1, 1, plan.ptr, nb, y.ptr, ws.ptr, ws.nbytes, None) == 1
+    assert L.mimg_experts_combine_a8_dev(w.w.handle, 1, x.ptr, weights.ptr, 1, 1, plan.ptr, nb, y.ptr, ws.ptr, ws.nbytes, None) == 1
