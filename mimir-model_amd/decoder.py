@@ -92,6 +92,13 @@ def config_from_metadata(md, context=0):
         if arch != "llama":
             raise ValueError(f"experts in an architecture {arch!r}: only \"llama\" graphs have them")
         c["experts"], c["experts_used"] = req("expert_count"), req("expert_used_count")
+        # what a file may ask for beyond a softmax normalized over the chosen
+        # experts (gating function 1), each value with those that mean no more
+        for key, plain in (("expert_shared_count", (0,)), ("expert_weights_norm", (True,)), ("expert_weights_scale", (0, 1)),
+                           ("expert_gating_func", (0, 1)), ("expert_group_count", (0, 1))):
+            v = md.get(f"{arch}.{key}", plain[0])
+            if v not in plain:
+                raise ValueError(f"metadata {arch}.{key} = {v!r} is not supported yet")
     # the importer stores f32 metadata widened to f64; the graph's rms_norm
     # attribute keeps it, and rms_norm.v1 rounds it to f32
     c["norm_eps"] = eps
@@ -243,6 +250,10 @@ class Decoder:
                     raise ValueError(f"{p}{name}.weight: quantized [{n}, {rows // n}, {k}] is wanted")
             if self.w[p + "ffn_gate_exps.weight"].dt != self.w[p + "ffn_up_exps.weight"].dt:
                 raise ValueError(f"{p}: gate and up experts of two dtypes")
+            # shared experts, and biases of the router, of its choice or of the experts
+            extra = [n for n in tensors if n.startswith(p) and ("_shexp." in n or n.endswith(("_inp.bias", "_exps.bias")) or "exp_probs_b" in n)]
+            if extra:
+                raise ValueError(f"{extra[0]}: not handled")
 
     # ---- the graph's ops ---------------------------------------------------
 

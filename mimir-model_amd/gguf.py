@@ -243,10 +243,11 @@ class GGUFFile:
         sec = mimg.WeightsSection(np.frombuffer(self.buf[self.data_start:self.data_start + end], np.uint8))
         tensors = {}
         for t in self.tensors:
-            # (an expert tensor is a matrix of all experts' rows)
+            # (an expert tensor is a matrix of all experts' rows; their biases for
+            # the decoder to turn away)
             if t.dtype in (64, 66, 67) and len(t.shape) == (3 if "_exps." in t.name else 2):
                 rows = int(np.prod(t.shape[:-1]))
                 tensors[t.name] = (t.dtype, t.shape, sec.view(t.offset, t.length, t.dtype, rows, t.shape[-1]))
-            elif t.dtype == 1 and (len(t.shape) == 1 or t.name.endswith(".ffn_gate_inp.weight")):
+            elif t.dtype == 1 and (len(t.shape) == 1 or t.name.endswith((".ffn_gate_inp.weight", "_exps.bias"))):
                 tensors[t.name] = (1, t.shape, np.frombuffer(self.tensor_bytes(t.name), np.float32).copy())
         return sec, tensors
