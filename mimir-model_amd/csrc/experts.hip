@@ -31,13 +31,16 @@
 // are in order by expert, weight rows, pairs, dealt to the XCDs in eight runs, so
 // that the tiles that share weights meet in one L2.
 //
-// Bounds. Few pairs an expert: the weights' way into LDS. 64 tokens, two of 8
-// experts, 4096 x 14336 Q4_K gate and up 118 us: 537 MB at 4.6 TB/s, where the
-// copies alone take 108 to 117 us and the instructions alone 100; 181 tokens, four of
-// 60, 2048 x 1408 Q8_0 81 us: 373 MB at 4.6 TB/s. Many: vector instructions beside
-// the matrix cores. 2048 tokens, two of 8: gate and up 1250 us, 0.77 POP/s of
-// products and 1.54 of the planes' (the matrix cores at work 42 % of the cycles,
-// vector instructions 65 %), down 4096 x 14336 Q6_K 675 us, 0.71 and 1.42 POP/s.
+// Bounds (calls one after another, with their quantizer). Few pairs an expert: the
+// weights' way into LDS. 64 tokens, two of 8 experts, 4096 x 14336 Q4_K gate and up
+// 121 to 133 us: 537 MB at 4.0 to 4.4 TB/s, where the copies alone take 108 to 117 us
+// and the instructions alone 100; 181 tokens, four of 60, 2048 x 1408 Q8_0 85 us: 373
+// MB at 4.4 TB/s. Many: vector instructions beside the matrix cores. 2048 tokens,
+// two of 8: gate and up 1375 us, 0.70 POP/s of products and 1.4 of the planes' (the
+// matrix cores at work 42 % of the cycles, vector instructions 66 %; a library
+// product of 8192^3 on the same card 1.95), down 4096 x 14336 Q6_K 740 us for the tiles
+// alone, 0.65 and 1.3 POP/s (38 and 66 %, conflicts of the LDS 20 %). Q8_0 has one
+// plane, but a float step every 32 weights: gate and up 1880 us (23 and 60 %).
 //
 // Rows of x the quantizer refused and weight rows with a non-finite block
 // scale take the float32 path (f32path.hpp) at the end.
@@ -957,8 +960,14 @@ static hipError_t launch_dt(const Args& A, hipStream_t stream) {
 // 31.5 / 37.7.
 // Of many more experts (Q4_K): 2048 x 768, 128 experts, 24 / 32 / 64 pairs 17.8 /
 // 22.1 / 34.5 against 19.7 / 21.0 / 28.2; 4096 x 1536, 128 experts, 32 pairs 42
-// against 49 (Q6_K 69 against 81), 256 experts, 48 / 64 pairs 63 / 81 against 76 / 91;
-// Q8_0 2048 x 1408, 160 experts, 24 pairs 36.7 against 33.9.
+// against 49 (Q6_K 69 against 81), 256 experts, 48 / 56 / 64 pairs 68 / 73 / 85 against
+// 81 / 85 / 97 (the bound of 48 leaves that gain; other sizes are not measured above
+// it); Q8_0 2048 x 1408, 160 experts, 24 pairs 36.7 against 33.9. Q6_K below K = 4096:
+// 2048 x 768, 128 experts, 24 / 32 / 64 pairs 27.2 / 33.0 / 56.3 against 26.7 / 31.1 / 44.6,
+// 2048 x 1024, 64 experts, 8 / 16 / 32 pairs 14.8 / 24.6 / 40.1 against 21.1 / 23.6 / 31.9. The
+// step at K = 4096 lies between the two widths measured on either side (Q4_K, 32
+// pairs of 128 experts: 1024 x 1024 24.3 against 16.3, 3584 x 1536 42.6 against 48.8, 4096 x 1536
+// 44.4 against 52.5).
 static bool few_pairs_swiglu(const DevWeight& w, int pairs, int experts) {
     if (pairs <= (w.dt == DT_Q8_0 ? 4 : 8) || (pairs <= 16 && experts >= 2 * pairs)) return true;
     return w.dt != DT_Q8_0 && experts >= 4 * pairs && pairs <= (w.k >= 4096 ? 48 : 24);
@@ -970,7 +979,10 @@ static bool few_pairs_swiglu(const DevWeight& w, int pairs, int experts) {
 // 16.5 / 19.3 / 24.5; 60 experts, 32 / 48 pairs, 1536 -> 2048 Q6_K 27.2 / 35.6 against
 // 26.7 / 32.0; 1408 -> 2048 Q8_0, 16 / 32 / 48 / 64 pairs 18.3 / 28.4 / 37.0 / 44.3 against
 // 19.8 / 29.7 / 34.0 / 37.4. 128 experts, 72 / 96 / 128 pairs: 768 -> 2048 Q4_K 20.7 /
-// 24.6 / 28.8 against 28.8 / 31.6 / 34.2, 1536 -> 4096 52 / 66 / 84 against 60 / 69 / 79.
+// 24.6 / 28.8 against 28.8 / 31.6 / 34.2, 1536 -> 4096 52 / 66 / 84 against 60 / 69 / 79;
+// 32 / 40 / 64 / 96 pairs: 768 -> 2048 Q6_K 17.4 / 20.4 / 27.4 / 37.1 against 22.0 / 24.8 / 29.5 /
+// 35.5, 40 / 64 pairs 1536 -> 4096 54.0 / 79.0 against 54.8 / 75.9, 48 / 64 / 96 pairs 1408 ->
+// 2048 Q8_0 38.7 / 48.0 / 64.6 against 39.6 / 45.1 / 54.7.
 static bool few_pairs_combine(uint32_t dt, int pairs, int experts) {
     if (pairs <= (dt == DT_Q8_0 ? 4 : 8)) return true;
     if (dt == DT_Q4_K) return pairs <= 128 && experts >= pairs;

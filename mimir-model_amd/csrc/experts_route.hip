@@ -11,10 +11,12 @@
 // to float32 a token whose experts are nearly alike would go to another one
 // whenever the order of the sum changes (with the batch, say). Products of two
 // float32 are exact in float64 and their sum is kept there, on
-// v_mfma_f64_16x16x4: 2 T E K operations, which bound it for many tokens (2048
-// of 128 experts, K = 4096: 30 us at the rate a float64 product reaches, x and r
-// are read in 5; the logits take 39 to 42, choices 5 and plan 5). Few tokens are
-// bound by launches (181 of 60 experts, K = 2048: 5.2, 3.5 and 2.8 us).
+// v_mfma_f64_16x16x4: 2 T E K operations (2048 tokens of 128 experts, K = 4096: 32
+// us at the 66 TFLOP/s that a float64 product of 8192^3 reaches, x and r are read
+// in 5; the logits take 42 to 43, choices 5 and plan 5). There the matrix cores are
+// at work 59 % of the cycles and vector instructions 14 %: two waves a SIMD, waiting
+// for loads a quarter of their time. Few tokens are
+// bound by launches (181 of 60 experts, K = 2048: 5.1, 3.5 and 3.0 us).
 #include "decoder_math.hpp"
 #include "experts.hpp"
 #include "mimg_device.hpp"
@@ -408,7 +410,8 @@ __global__ __launch_bounds__(PLAN_T) void plan_kernel(const int32_t* __restrict_
 // The quantizer of the tiles' activations: a row by one workgroup, CPW chunks
 // of 256 a wave with their loads in flight together, only what the tiles read
 // (q, scales, Q4_K's sums in the form of its f16 operand, ok): 4096 rows of
-// 14336 take 74 us (4.0 TB/s) against 84 with every array of the other products.
+// 14336 take 74 to 78 us (3.9 TB/s; Q4_K 85), 84 with every array of the other
+// products where this took 74.
 template <int BLOCK, int OUT, int CPW>
 __global__ __launch_bounds__(1024) void quantize_kernel(const float* __restrict__ x, int64_t K, ActPtrs a, _Float16* parts) {
     const int64_t row = blockIdx.x, nch = (K + 255) / 256;
