@@ -892,9 +892,12 @@ static int64_t max_tiles(const Args& A, int BM) {
 static hipError_t launch_grid(void (*kernel)(Args), Args A, int BM, int BN, hipStream_t stream) {
     constexpr int64_t MOST = 1 << 23;
     const int64_t wgs = (max_tiles(A, BM) * ((A.N + BN - 1) / BN) + 7) / 8 * 8;
-    for (A.wg0 = 0; A.wg0 < wgs; A.wg0 += MOST)
+    for (A.wg0 = 0; A.wg0 < wgs; A.wg0 += MOST) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(wgs - A.wg0, MOST)), dim3(256), 0, stream, A);
-    return hipGetLastError();
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 template <uint32_t DT, int MT, bool SW, bool AL = false>

@@ -556,8 +556,10 @@ hipError_t launch_experts_sum(const float* part, const float* weights, const int
         const float *p = part + t * top * N, *w = weights + t * top;
         if (N % 4 == 0) hipLaunchKernelGGL(xr::combine_kernel<4>, grid, dim3(256), 0, s, p, w, expert + t * top, top, N, y + t * N);
         else hipLaunchKernelGGL(xr::combine_kernel<1>, grid, dim3(256), 0, s, p, w, expert + t * top, top, N, y + t * N);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace mimg

@@ -4,7 +4,6 @@ as that of a matrix of these rows alone."""
 import numpy as np
 import pytest
 
-import experts_ref as ref
 from test_gpu_experts import Q4_K, Q8_0, acts_for, bits, run_combine, run_swiglu, rt  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -53,10 +52,12 @@ def test_the_sum_of_tokens_past_a_grid(gpu, rt, oracle):  # noqa: F811
     same_rows(run_combine(gpu, rt, down, h, weights, ids), run_combine(gpu, rt, down.alone, h, weights, ids))
 
 
-@pytest.mark.parametrize("dt,k,n,T", [(Q8_0, 32, 1 << 26, 1), (Q8_0, 32, 1 << 24, 4), (Q4_K, 256, 1 << 26, 1), (Q4_K, 256, 3 << 22, 6)])
+@pytest.mark.parametrize("dt,k,n,T", [(Q8_0, 32, 1020 * 65794, 1), (Q8_0, 32, 1020 * 16449, 4), (Q4_K, 256, 1020 * 65794, 1),
+                                       (Q4_K, 256, 1020 * 12337, 6)])
 def test_few_pairs_of_rows_past_a_grid(gpu, rt, oracle, dt, k, n, T):  # noqa: F811
     """2^24 workgroups of 256 and more, where a pair runs its expert by itself."""
-    w = Repeated(gpu, rt, oracle, dt, 1, n, 128, k, 7)
+    assert n // 4 * T >= 1 << 24
+    w = Repeated(gpu, rt, oracle, dt, 1, n, 1020, k, 7)
     x, ids = acts_for(8, T, k), np.zeros((T, 1), np.int32)
     same_rows(run_swiglu(gpu, rt, w, w, x, ids), run_swiglu(gpu, rt, w.alone, w.alone, x, ids))
     weights = np.random.default_rng(9).random((T, 1), np.float32)
